@@ -273,11 +273,13 @@ def _linear_plain(s):
 def _encode(a, shift, top, least):
     """Codes and block scales of the log-linear 8-bit code: the magnitude's
     share of its block's largest, rounded (to even) to the bits of a float32
-    above `shift`, counted down from `top` (1.0)."""
+    above `shift`, counted down from `top` (1.0).  A block whose largest is
+    below the smallest normal number is stored as zero."""
     a = a.view(-1, BLOCK)
     size = a.abs()
     scale = size.amax(1, keepdim=True)
-    bits = (size / scale).view(torch.int32)
+    scale = torch.where(scale < 2.0 ** -126, 0.0, scale)
+    bits = (size * (1 / scale)).view(torch.int32)
     code = ((bits + ((1 << (shift - 1)) - 1) + ((bits >> shift) & 1)) >> shift) - (ONE_BITS >> shift) + top
     code = torch.where(size > 0, code.clamp(least, top), 0)
     return torch.where(a < 0, -code, code), scale
