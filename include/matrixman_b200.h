@@ -343,6 +343,98 @@ int mm_nll_loss_backward(const mm_tensor_t* grad_output, const mm_tensor_t* inpu
                          int64_t ignore_index, const mm_tensor_t* total_weight,
                          const mm_tensor_t* grad_input, void* stream);
 
+/* Layer norm over the rows of x [rows, width] (dense rows, any row stride):
+ * y = (x - mean) * rstd * weight + bias with rstd = 1 / sqrt(var + eps), var the
+ * mean squared distance from the row's mean.  weight and bias [width] may be
+ * NULL; y is dense; mean and rstd [rows] are kept for the backward pass.  No
+ * counterpart in the reference, whose only normalisation is eval BatchNorm. */
+int mm_layer_norm(const mm_tensor_t* x, const mm_tensor_t* weight, const mm_tensor_t* bias, double eps,
+                  const mm_tensor_t* y, const mm_tensor_t* mean, const mm_tensor_t* rstd, void* stream);
+
+/* Gradients of mm_layer_norm: with xh = (x - mean) * rstd and g = dy * weight,
+ * dx = rstd * (g - mean(g) - xh * mean(g * xh)), dweight = sum over rows of
+ * dy * xh, dbias = sum over rows of dy.  dx, dweight and dbias may be NULL.
+ * workspace: device memory, 16-byte aligned, of
+ * mm_layer_norm_backward_workspace_size bytes (it holds partial column sums;
+ * unused, and may be NULL, when dweight and dbias are NULL).  The sums are
+ * added in a fixed order: equal inputs give equal bits. */
+int mm_layer_norm_backward(const mm_tensor_t* dy, const mm_tensor_t* x, const mm_tensor_t* mean,
+                           const mm_tensor_t* rstd, const mm_tensor_t* weight, const mm_tensor_t* dx,
+                           const mm_tensor_t* dweight, const mm_tensor_t* dbias, void* workspace,
+                           size_t workspace_bytes, void* stream);
+int mm_layer_norm_backward_workspace_size(int64_t rows, int64_t width, size_t* bytes);
+
+typedef enum mm_linear_act {
+  MM_LINEAR_NONE = 0,
+  MM_LINEAR_RELU = 1,
+  MM_LINEAR_SILU = 2,
+  MM_LINEAR_SIGMOID = 3,
+  MM_LINEAR_GELU = 4,      /* z * Phi(z), by erfc */
+  MM_LINEAR_GELU_TANH = 5  /* 0.5 z (1 + tanh(sqrt(2/pi) (z + 0.044715 z^3))) */
+} mm_linear_act_t;
+
+/* y = act(x w^T + bias) + residual, or act(x w^T + bias + residual) when
+ * residual_before_act: x [m, k] and w [n, k] of any strides, bias [n] and
+ * residual [m, n] (dense rows) or NULL, y [m, n] dense.  z (dense [m, n] or
+ * NULL) receives the values that the activation is applied to, which the
+ * backward pass needs.  float32 accuracy throughout.  workspace: device memory,
+ * 256-byte aligned, of mm_linear_workspace_size(m, n, k, 0) bytes.  Extends
+ * mm_gemm (which has no residual, GELU or gradient). */
+int mm_linear(const mm_tensor_t* x, const mm_tensor_t* w, const mm_tensor_t* bias, const mm_tensor_t* residual,
+              int act, int residual_before_act, const mm_tensor_t* y, const mm_tensor_t* z, void* workspace,
+              size_t workspace_bytes, void* stream);
+
+/* Gradients of mm_linear from dy [m, n] (dense rows) and the z it wrote (any z,
+ * or NULL, without an activation; y serves as z for ReLU without a residual):
+ * dz = dy * act'(z), dx = dz w, dw = dz^T x, db = sum over rows of dz.  Every
+ * output is dense and may be NULL.  workspace:
+ * mm_linear_workspace_size(m, n, k, 1) bytes, 256-byte aligned.  Sums are added
+ * in a fixed order: equal inputs give equal bits. */
+int mm_linear_backward(const mm_tensor_t* dy, const mm_tensor_t* x, const mm_tensor_t* w, const mm_tensor_t* z,
+                       int act, const mm_tensor_t* dx, const mm_tensor_t* dw, const mm_tensor_t* db,
+                       const mm_tensor_t* dz, void* workspace, size_t workspace_bytes, void* stream);
+int mm_linear_workspace_size(int64_t m, int64_t n, int64_t k, int backward, size_t* bytes);
+
+/* One tensor of an optimiser step, numel consecutive float32 elements.  With
+ * 32-bit states exp_avg and exp_avg_sq point to float32 and the scales are
+ * NULL; with 8-bit states they point to one code byte per element (8-byte
+ * aligned, whole blocks of 256) and the scales to one float32 per block. */
+typedef struct mm_adamw_tensor {
+  float* param;
+  const float* grad;
+  void* exp_avg;
+  void* exp_avg_sq;
+  float* exp_avg_scale;
+  float* exp_avg_sq_scale;
+  float* step;     /* device, one value: steps taken so far */
+  int64_t numel;
+} mm_adamw_tensor_t;
+
+/* One AdamW (decoupled = 1) or Adam (0: weight_decay * param joins the gradient)
+ * step over `count` tensors: m = b1 m + (1 - b1) g, v = b2 v + (1 - b2) g^2,
+ * p = p (1 - lr wd) - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps).
+ * t is *step, after adding 1 to it when `advance` (each tensor then needs a step
+ * of its own).  state_bits 32 or 8.  8-bit states: a block of 256 elements has
+ * one scale, the largest magnitude; m is held as sign and 7-bit code (8 steps
+ * per power of two over 16 powers of two, code 0 is zero), v as an 8-bit code of
+ * its square root (16 steps; at least code 1 unless v is 0).  A non-finite
+ * gradient makes the states of its whole block NaN.  workspace: 8 bytes per
+ * tensor (mm_adamw_workspace_size).  Does the work of the reference's
+ * lerp_ / addcmul_ / addcdiv_ sequence (backends/opengl/dispatch.py:171-179,
+ * :264-290) in one pass. */
+int mm_adamw(const mm_adamw_tensor_t* tensors, int count, int state_bits, double lr, double beta1, double beta2,
+             double eps, double weight_decay, int decoupled, int maximize, int advance, void* workspace,
+             size_t workspace_bytes, void* stream);
+int mm_adamw_workspace_size(int count, size_t* bytes);
+
+/* 8-bit states of numel dense float32 moments, and the values that 8-bit states
+ * stand for (decoding what was encoded and encoding it again gives the same
+ * codes). */
+int mm_adamw_encode(const float* exp_avg, const float* exp_avg_sq, int64_t numel, uint8_t* exp_avg_code,
+                    float* exp_avg_scale, uint8_t* exp_avg_sq_code, float* exp_avg_sq_scale, void* stream);
+int mm_adamw_decode(const uint8_t* exp_avg_code, const float* exp_avg_scale, const uint8_t* exp_avg_sq_code,
+                    const float* exp_avg_sq_scale, int64_t numel, float* exp_avg, float* exp_avg_sq, void* stream);
+
 /* Generic 2-D max pooling over dims (2,3) of a rank-4 tensor, -inf padding,
  * NaN-propagating like torch.  Replaces max_pool2d_5x5_s1_p2 (gpumatrix.py:74)
  * and CudaBackend.max_pool2d (cuda/backend.py:1351-1393), which only accepted

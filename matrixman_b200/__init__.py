@@ -35,6 +35,8 @@ from .api import (
 from .pipeline import infer, infer_stream
 from .detect import postprocess_detections
 from .frames import preprocess_frames
+from . import optim
+from .fused_linear import linear
 from .preparation import auto_prepare, prepare, prepare_cuda, prepare_opengl
 from .tensor import Gm45Tensor, MatrixManTensor, install_tensor_method, is_matrixman_tensor
 
@@ -101,6 +103,8 @@ sys.modules[__name__].__class__ = _MatrixManModule
 __all__ = [
     "infer",
     "infer_stream",
+    "linear",
+    "optim",
     "postprocess_detections",
     "preprocess_frames",
     "MatrixManTensor", "Gm45Tensor", "auto_prepare", "config", "debug_enabled", "device_count",

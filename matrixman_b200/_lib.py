@@ -35,6 +35,7 @@ ACT_NONE, ACT_RELU, ACT_SILU, ACT_SIGMOID = 0, 1, 2, 3
 (UNARY_COPY, UNARY_SILU, UNARY_RELU, UNARY_SIGMOID, UNARY_ADD_SCALAR, UNARY_MUL_SCALAR,
  UNARY_DIV_SCALAR, UNARY_NEG, UNARY_CLAMP) = range(9)
 BINARY_ADD, BINARY_SUB, BINARY_MUL, BINARY_DIV = range(4)
+LINEAR_ACTS = {"none": 0, "relu": 1, "silu": 2, "sigmoid": 3, "gelu": 4, "gelu_tanh": 5}
 PW3_THRESHOLD_BACKWARD, PW3_ADDCMUL, PW3_ADDCDIV, PW3_LERP, PW3_SQRT = range(5)
 
 LIB_DIR = Path(__file__).resolve().parent / "_lib"
@@ -197,6 +198,16 @@ SIGNATURES = {
     "mm_log_softmax_backward": [_T, _T, _i, _T, _vp],
     "mm_nll_loss": [_T, _T, _T, _i, _i64, _T, _T, _vp],
     "mm_nll_loss_backward": [_T, _T, _T, _T, _i, _i64, _T, _T, _vp],
+    "mm_layer_norm": [_T, _T, _T, _d, _T, _T, _T, _vp],
+    "mm_layer_norm_backward": [_T, _T, _T, _T, _T, _T, _T, _T, _vp, _sz, _vp],
+    "mm_layer_norm_backward_workspace_size": [_i64, _i64, ctypes.POINTER(_sz)],
+    "mm_linear": [_T, _T, _T, _T, _i, _i, _T, _T, _vp, _sz, _vp],
+    "mm_linear_backward": [_T, _T, _T, _T, _i, _T, _T, _T, _T, _vp, _sz, _vp],
+    "mm_linear_workspace_size": [_i64, _i64, _i64, _i, ctypes.POINTER(_sz)],
+    "mm_adamw": [_vp, _i, _i, _d, _d, _d, _d, _d, _i, _i, _i, _vp, _sz, _vp],
+    "mm_adamw_workspace_size": [_i, ctypes.POINTER(_sz)],
+    "mm_adamw_encode": [_fp, _fp, _i64, _vp, _fp, _vp, _fp, _vp],
+    "mm_adamw_decode": [_vp, _fp, _vp, _fp, _i64, _fp, _fp, _vp],
 }
 
 

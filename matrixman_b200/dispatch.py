@@ -585,6 +585,66 @@ def _bn_legit_no_training(x, weight, bias, running_mean, running_var, momentum, 
     return out, empty, empty
 
 
+@_register(aten.native_layer_norm.default)
+def _native_layer_norm(x, normalized_shape, weight, bias, eps):
+    return ops.layer_norm(x, normalized_shape, weight, bias, eps)
+
+
+@_register(aten.native_layer_norm_backward.default)
+def _native_layer_norm_backward(grad_out, x, normalized_shape, mean, rstd, weight, bias, output_mask):
+    return ops.layer_norm_backward(grad_out, x, normalized_shape, mean, rstd, weight, bias, output_mask)
+
+
+# -- torch.optim.AdamW / Adam with fused=True ---------------------------------
+
+@_register(aten._foreach_add_.Scalar)
+def _foreach_add_(tensors, scalar):
+    for t in tensors:
+        ops.binary("add", t, scalar, out=t)
+
+
+def _fused_adam(decoupled, params, grads, exp_avgs, exp_avg_sqs, max_exp_avg_sqs, state_steps, *, lr, beta1, beta2,
+                weight_decay, eps, amsgrad, maximize, grad_scale=None, found_inf=None):
+    from . import optim
+    if amsgrad or max_exp_avg_sqs:
+        raise NotImplementedError("MatrixMan/CUDA: fused Adam does not implement amsgrad")
+    if grad_scale is not None or found_inf is not None:
+        raise NotImplementedError("MatrixMan/CUDA: fused Adam does not implement gradient scaling")
+    if not params:
+        return
+    lists = (grads, exp_avgs, exp_avg_sqs, state_steps)
+    if any(len(v) != len(params) for v in lists):
+        raise RuntimeError("MatrixMan/CUDA: fused Adam needs lists of one length")
+    rt = ops._runtime_of(*params)
+    rows, held = [], []
+    for p, g, m, v, step in zip(params, *lists):
+        for t, name in ((p, "parameter"), (m, "exp_avg"), (v, "exp_avg_sq")):
+            optim._check_storage(t, f"fused Adam {name}")
+        for t, name in ((g, "gradient"), (step, "step")):
+            ops.require_f32(ops.require_mm(t, f"fused Adam {name}"), f"fused Adam {name}")
+        ops._runtime_of(p, g, m, v, step)
+        if any(tuple(t.shape) != tuple(p.shape) for t in (g, m, v)):
+            raise RuntimeError("MatrixMan/CUDA: fused Adam needs equal shapes of parameter, gradient and states")
+        if not (optim._same_order(m, p) and optim._same_order(v, p)):
+            raise NotImplementedError("MatrixMan/CUDA: fused Adam states must have their parameter's strides")
+        g = optim._in_order(g, p)
+        held.append(g)
+        rows.append((optim._pointer(p), optim._pointer(g), optim._pointer(m), optim._pointer(v), 0, 0,
+                     optim._pointer(step), p.numel()))
+    optim.run_adamw(rt, rows, 32, lr=float(lr), beta1=beta1, beta2=beta2, eps=eps, weight_decay=weight_decay,
+                    decoupled=decoupled, maximize=bool(maximize), advance=False)
+
+
+@_register(aten._fused_adamw_.default)
+def _fused_adamw_(params, *args, **kwargs):
+    _fused_adam(True, params, *args, **kwargs)
+
+
+@_register(aten._fused_adam_.default)
+def _fused_adam_(params, *args, **kwargs):
+    _fused_adam(False, params, *args, **kwargs)
+
+
 # ---------------------------------------------------------------------------
 # Factories reached through a MatrixMan tensor argument
 # ---------------------------------------------------------------------------

@@ -24,9 +24,11 @@ from .tensor import (
     contiguous_strides,
     dense_strides_like,
     is_channels_last,
+    is_contiguous,
     is_dense,
     numel,
     readback_tensor,
+    view_strides,
 )
 
 F32 = torch.float32
@@ -562,6 +564,108 @@ def batch_norm_eval(x, weight, bias, running_mean, running_var, eps) -> MatrixMa
             ctypes.c_void_p(var.element_ptr), ctypes.c_void_p(w.element_ptr),
             ctypes.c_void_p(b.element_ptr), float(eps), _p(y.desc()), rt.stream)
     return y
+
+
+def _norm_matrix(x: MatrixManTensor, width: int) -> MatrixManTensor:
+    """x as [rows, width] with dense rows, copied only where its strides force it."""
+    rows = numel(x.shape) // width if width else 0
+    st = x._logical_strides
+    if x.dim() == 2 and int(x.shape[1]) == width and (st[1] == 1 or width == 1):
+        return x
+    if not is_contiguous(x.shape, st):
+        flat = view_strides(x.shape, st, (rows, width))
+        if flat is not None and (flat[1] == 1 or width == 1):
+            return MatrixManTensor(x._owner, (rows, width), x._storage_offset, flat)
+        x = materialize(x)
+    return MatrixManTensor(x._owner, (rows, width), x._storage_offset, (width, 1))
+
+
+def _norm_vector(rt, value, shape, name: str) -> MatrixManTensor | None:
+    """An affine parameter as a dense vector."""
+    if value is None:
+        return None
+    t = device_operand(rt, value, f"LayerNorm {name}")
+    require_f32(t, f"LayerNorm {name}")
+    if tuple(t.shape) != shape:
+        raise RuntimeError(f"MatrixMan/CUDA: LayerNorm {name} must have the normalized shape {shape}, "
+                           f"got {tuple(t.shape)}")
+    if not is_contiguous(t.shape, t._logical_strides):
+        t = materialize(t)
+    return MatrixManTensor(t._owner, (numel(shape),), t._storage_offset, (1,))
+
+
+def _norm_shape(x: MatrixManTensor, normalized_shape) -> tuple[int, ...]:
+    shape = tuple(int(v) for v in normalized_shape)
+    if not shape or tuple(int(v) for v in x.shape[-len(shape):]) != shape:
+        raise RuntimeError(f"MatrixMan/CUDA: LayerNorm input {tuple(x.shape)} does not end in the normalized "
+                           f"shape {shape}")
+    if numel(shape) == 0:
+        raise NotImplementedError("MatrixMan/CUDA: LayerNorm over an empty normalized shape is not implemented")
+    return shape
+
+
+def layer_norm(x, normalized_shape, weight=None, bias=None, eps=1e-5):
+    """(y, mean, rstd) of native_layer_norm; mean and rstd keep the leading
+    dimensions and have size 1 in the normalized ones."""
+    x = require_mm(x, "LayerNorm")
+    require_f32(x, "LayerNorm")
+    shape = _norm_shape(x, normalized_shape)
+    rt = x.runtime
+    w = _norm_vector(rt, weight, shape, "weight")
+    b = _norm_vector(rt, bias, shape, "bias")
+    x2 = _norm_matrix(x, numel(shape))
+    rows = int(x2.shape[0])
+    lead = tuple(int(v) for v in x.shape[:x.dim() - len(shape)])
+    y = empty(rt, tuple(x.shape))
+    mean, rstd = empty(rt, (rows,)), empty(rt, (rows,))
+    y2 = MatrixManTensor(y._owner, (rows, numel(shape)), 0, (numel(shape), 1))
+    _launch("mm_layer_norm", _p(x2.desc()), _p(w.desc()) if w is not None else None,
+            _p(b.desc()) if b is not None else None, float(eps), _p(y2.desc()), _p(mean.desc()), _p(rstd.desc()),
+            rt.stream)
+    stat = lead + (1,) * len(shape)
+    return y, *(MatrixManTensor(t._owner, stat, 0, contiguous_strides(stat)) for t in (mean, rstd))
+
+
+def layer_norm_backward(dy, x, normalized_shape, mean, rstd, weight, bias, mask):
+    """(dx, dweight, dbias) of native_layer_norm_backward; None where the mask is false."""
+    x = require_mm(x, "LayerNorm backward")
+    for t in (dy, mean, rstd):
+        require_mm(t, "LayerNorm backward")
+    for t in (dy, x, mean, rstd):
+        require_f32(t, "LayerNorm backward")
+    shape = _norm_shape(x, normalized_shape)
+    if tuple(dy.shape) != tuple(x.shape):
+        raise RuntimeError("MatrixMan/CUDA: LayerNorm backward needs equal shapes of gradient and input")
+    rt = _runtime_of(dy, x, mean, rstd)
+    need_x, need_w, need_b = (bool(v) for v in mask)
+    if (need_w and not isinstance(weight, MatrixManTensor)) or (need_b and not isinstance(bias, MatrixManTensor)):
+        raise RuntimeError("MatrixMan/CUDA: LayerNorm parameters that need a gradient must be MatrixMan tensors")
+    width = numel(shape)
+    w = _norm_vector(rt, weight, shape, "weight")
+    x2, g2 = _norm_matrix(x, width), _norm_matrix(dy, width)
+    rows = int(x2.shape[0])
+    stats = []
+    for t in (mean, rstd):
+        if numel(t.shape) != rows:
+            raise RuntimeError("MatrixMan/CUDA: LayerNorm backward statistics do not match the input's rows")
+        if not is_contiguous(t.shape, t._logical_strides):
+            t = materialize(t)
+        stats.append(MatrixManTensor(t._owner, (rows,), t._storage_offset, (1,)))
+    dx = empty(rt, tuple(x.shape)) if need_x else None
+    dw = empty(rt, shape) if need_w else None
+    db = empty(rt, shape) if need_b else None
+    work, size = None, ctypes.c_size_t(0)
+    if need_w or need_b:
+        _lib.call("mm_layer_norm_backward_workspace_size", rows, width, ctypes.byref(size))
+        work = rt.new_storage(size.value, torch.uint8, _lib.POOL_SCRATCH)
+
+    def flat(t, dims):
+        return _p(MatrixManTensor(t._owner, dims, 0, contiguous_strides(dims)).desc()) if t is not None else None
+
+    _launch("mm_layer_norm_backward", _p(g2.desc()), _p(x2.desc()), _p(stats[0].desc()), _p(stats[1].desc()),
+            _p(w.desc()) if w is not None else None, flat(dx, (rows, width)), flat(dw, (width,)), flat(db, (width,)),
+            ctypes.c_void_p(work.pointer) if work is not None else None, size.value, rt.stream)
+    return dx, dw, db
 
 
 def softmax(x, dim, log=False) -> MatrixManTensor:
