@@ -40,7 +40,7 @@ NVCC_FLAGS = [
 ]
 
 SOURCES = ["mm_runtime.cu", "mm_ops.cu", "mm_conv_simt.cu", "mm_conv_tc.cu", "mm_detect.cu", "mm_frames.cu", "mm_train.cu",
-           "mm_norm.cu", "mm_linear.cu", "mm_adamw.cu"]
+           "mm_norm.cu", "mm_linear.cu", "mm_linear_tc.cu", "mm_adamw.cu"]
 
 
 def _digest(paths) -> str:

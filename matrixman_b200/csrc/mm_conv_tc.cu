@@ -64,6 +64,7 @@
 namespace mm {
 
 __device__ int g_tc_error = 0;
+int lin_kernel_error(int* code, int clear);  // the same of the linear operator's kernel
 
 constexpr int TC_BM = 128;        // pixels per tile (MMA M)
 constexpr int TC_BK = 32;         // channels per k-block (128 bytes of fp32)
@@ -1787,8 +1788,12 @@ extern "C" int mm_kernel_error(int device, int* code_out, int clear) {
     int zero = 0;
     e = cudaMemcpyToSymbol(g_tc_error, &zero, sizeof(int));
   }
+  int linear = 0;
+  const int rc = e == cudaSuccess ? lin_kernel_error(&linear, clear) : MM_OK;
   if (prev != device) cudaSetDevice(prev);
   if (e != cudaSuccess) return cuda_fail(e, "mm_kernel_error");
+  if (rc != MM_OK) return rc;
+  if (code == 0) code = linear;
   *code_out = code;
   return MM_OK;
 }

@@ -9,7 +9,7 @@
 
 #include <string>
 
-#include "mm_linear.cuh"
+#include "mm_linear_tc.cuh"
 
 namespace mm {
 
@@ -137,13 +137,143 @@ static int lin_product(const LinProduct& p, const LinEpilogue& e, cudaStream_t s
 
 constexpr int LIN_DZ_ROWS = 256;  // partial rows of the bias gradient
 
+// Whether a product of this size runs on the tensor cores.
+static bool lin_on_tensor_cores(int64_t m, int64_t n, int64_t k) { return m > 32 && k >= 32 && n >= 32; }
+
+// Workspace pieces, 256-byte aligned.
+struct LinCarve {
+  char* base;
+  size_t used;
+  void* take(int64_t bytes) {
+    void* p = base ? base + used : nullptr;
+    used += ((size_t)bytes + 255) & ~(size_t)255;
+    return p;
+  }
+};
+
+// A matrix in planes.
+struct LinStored {
+  uint16_t* planes;
+  int* flags;
+  int64_t rows, cols, ld;
+  // As a product's operand whose lines run along the stored rows, or columns.
+  LinPlanes by_rows() const { return {planes, flags, rows, cols, ld, 0}; }
+  LinPlanes by_cols() const { return {planes, flags, cols, rows, ld, 1}; }
+};
+
+// Adds the split of a [r, c] matrix to the list, stored along whichever
+// direction is dense; *turned says that it is stored transposed.
+static LinStored lin_store(LinCarve* ws, LinSplits* all, const float* src, int64_t s0, int64_t s1, int64_t r, int64_t c,
+                           bool* turned) {
+  *turned = s1 != 1 && c > 1 && (s0 == 1 || r == 1);
+  if (*turned) {
+    int64_t t = r; r = c; c = t;
+    t = s0; s0 = s1; s1 = t;
+  }
+  LinStored st;
+  st.rows = r;
+  st.cols = c;
+  st.ld = (c + 7) / 8 * 8;
+  st.planes = (uint16_t*)ws->take(lin_plane_bytes(r, c));
+  st.flags = (int*)ws->take(4 * lin_flag_words(r, c));
+  if (c == 1) s1 = 1;
+  LinSplit s = {src, s0, s1, nullptr, 0, 0, r, (int)c, st.ld, st.planes, st.flags, nullptr, nullptr, 0, 0};
+  s.vec = s1 == 1 && s0 % 4 == 0 && (uintptr_t)src % 16 == 0;
+  lin_add_split(all, s);
+  return st;
+}
+
+static int lin_forward_tc(const mm_tensor_t* x, const mm_tensor_t* w, const LinEpilogue& e, float* y, void* workspace,
+                          cudaStream_t s) {
+  const int64_t m = x->size[0], k = x->size[1], n = w->size[0];
+  LinCarve ws = {(char*)workspace, 0};
+  LinSplits all;
+  all.count = 0;
+  all.blocks = 0;
+  bool xt, wt;
+  const LinStored xs = lin_store(&ws, &all, (const float*)x->data, x->stride[0], x->stride[1], m, k, &xt);
+  const LinStored wst = lin_store(&ws, &all, (const float*)w->data, w->stride[0], w->stride[1], n, k, &wt);
+  const LinChoice c = lin_choose(m, n, k);
+  float* part = (float*)ws.take(lin_part_bytes(c));
+  int rc = lin_run_splits(all, s);
+  if (rc != MM_OK) return rc;
+  return lin_run_gemm(xt ? xs.by_cols() : xs.by_rows(), wt ? wst.by_cols() : wst.by_rows(), y, e, c, part, s);
+}
+
+static int lin_backward_tc(const mm_tensor_t* dy, const mm_tensor_t* x, const mm_tensor_t* w, const mm_tensor_t* z,
+                           int act, const mm_tensor_t* dx, const mm_tensor_t* dw, const mm_tensor_t* db,
+                           const mm_tensor_t* dz, void* workspace, cudaStream_t s) {
+  const int64_t m = x->size[0], k = x->size[1], n = w->size[0];
+  LinCarve ws = {(char*)workspace, 0};
+  LinSplits all;
+  all.count = 0;
+  all.blocks = 0;
+  bool gt, xt = false, wt = false;
+  const LinStored g = lin_store(&ws, &all, (const float*)dy->data, n > 1 ? dy->stride[0] : 1, 1, m, n, &gt);
+  LinSplit& gs = all.s[0];
+  gs.s0 = dy->stride[0];
+  if (act != MM_LINEAR_NONE) {
+    gs.z = (const float*)z->data;
+    gs.act = act;
+    gs.vec = gs.vec && n % 4 == 0 && (uintptr_t)gs.z % 16 == 0;
+  }
+  gs.out = dz ? (float*)dz->data : nullptr;
+  if (db) gs.part = (float*)ws.take(4 * lin_part_rows(m) * n);
+  LinStored wst = {}, xs = {};
+  if (dx) wst = lin_store(&ws, &all, (const float*)w->data, w->stride[0], w->stride[1], n, k, &wt);
+  if (dw) xs = lin_store(&ws, &all, (const float*)x->data, x->stride[0], x->stride[1], m, k, &xt);
+  int rc = lin_run_splits(all, s);
+  if (rc != MM_OK) return rc;
+  if (db) {
+    linear_columns_kernel<<<(unsigned)((n + 31) / 32), 256, 0, s>>>(gs.part, (int)lin_part_rows(m), (int)n,
+                                                                    (float*)db->data);
+    MM_LAUNCH_CHECK("mm_linear_backward launch");
+  }
+  const LinEpilogue none = {nullptr, nullptr, nullptr, 0, MM_LINEAR_NONE, 0};
+  if (dx) {
+    const LinChoice c = lin_choose(m, k, n);
+    float* part = (float*)ws.take(lin_part_bytes(c));
+    rc = lin_run_gemm(g.by_rows(), wt ? wst.by_rows() : wst.by_cols(), (float*)dx->data, none, c, part, s);
+    if (rc != MM_OK) return rc;
+  }
+  if (dw) {
+    const LinChoice c = lin_choose(n, k, m);
+    float* part = (float*)ws.take(lin_part_bytes(c));
+    rc = lin_run_gemm(g.by_cols(), xt ? xs.by_rows() : xs.by_cols(), (float*)dw->data, none, c, part, s);
+  }
+  return rc;
+}
+
+static size_t lin_workspace(int64_t m, int64_t n, int64_t k, bool backward) {
+  LinCarve ws = {nullptr, 0};
+  if (lin_on_tensor_cores(m, n, k)) {
+    ws.take(lin_plane_bytes(m, k));
+    ws.take(4 * lin_flag_words(m, k));
+    ws.take(lin_plane_bytes(n, k));
+    ws.take(4 * lin_flag_words(n, k));
+    if (!backward) {
+      ws.take(lin_part_bytes(lin_choose(m, n, k)));
+    } else {
+      ws.take(lin_plane_bytes(m, n));
+      ws.take(4 * lin_flag_words(m, n));
+      ws.take(4 * lin_part_rows(m) * n);
+      ws.take(lin_part_bytes(lin_choose(m, k, n)));
+      ws.take(lin_part_bytes(lin_choose(n, k, m)));
+    }
+  } else if (backward) {
+    ws.take(4 * m * n);
+    ws.take(4 * LIN_DZ_ROWS * n);
+  }
+  return ws.used;
+}
+
 }  // namespace mm
 
 using namespace mm;
 
 extern "C" int mm_linear_workspace_size(int64_t m, int64_t n, int64_t k, int backward, size_t* bytes) {
   if (bytes == nullptr || m < 0 || n < 0 || k < 0) return fail(MM_ERR_INVALID, "mm_linear_workspace_size: invalid argument");
-  *bytes = backward ? (size_t)(m * n + LIN_DZ_ROWS * n) * sizeof(float) : 0;
+  *bytes = lin_workspace(m, n, k, backward != 0);
   return MM_OK;
 }
 
@@ -168,6 +298,7 @@ extern "C" int mm_linear(const mm_tensor_t* x, const mm_tensor_t* w, const mm_te
                   w->stride[0], w->stride[1], (int)m, (int)n, (int)k};
   LinEpilogue e = {bias ? (const float*)bias->data : nullptr, residual ? (const float*)residual->data : nullptr,
                    z ? (float*)z->data : nullptr, residual ? residual->stride[0] : 0, act, residual_before_act != 0};
+  if (lin_on_tensor_cores(m, n, k)) return lin_forward_tc(x, w, e, (float*)y->data, workspace, resolve_stream(stream));
   return lin_product(p, e, resolve_stream(stream));
 }
 
@@ -199,8 +330,11 @@ extern "C" int mm_linear_backward(const mm_tensor_t* dy, const mm_tensor_t* x, c
     if (db && n > 0) MM_CUDA(cudaMemsetAsync(db->data, 0, (size_t)n * 4, s), "mm_linear_backward: zero");
     return MM_OK;
   }
-  float* g = dz ? (float*)dz->data : (float*)workspace;
-  float* part = (float*)workspace + m * n;
+  if (lin_on_tensor_cores(m, n, k)) return lin_backward_tc(dy, x, w, z, act, dx, dw, db, dz, workspace, s);
+  LinCarve ws = {(char*)workspace, 0};
+  float* own = (float*)ws.take(4 * m * n);
+  float* part = (float*)ws.take(4 * LIN_DZ_ROWS * n);
+  float* g = dz ? (float*)dz->data : own;
   const int rows = m < LIN_DZ_ROWS ? (int)m : LIN_DZ_ROWS;
   linear_dz_kernel<<<dim3((unsigned)((n + 255) / 256), rows), 256, 0, s>>>(
       (const float*)dy->data, dy->stride[0], act == MM_LINEAR_NONE ? nullptr : (const float*)z->data, act, (int)m,

@@ -1,0 +1,696 @@
+// Matrix products of the linear operator on the tensor cores, in float32
+// accuracy.
+//
+// A float32 value is the exact sum of three bf16 values: a1 = a rounded to
+// bf16, a2 = (a - a1) rounded to bf16, a3 = a - a1 - a2 (24 significant bits =
+// 3 x 8, and bf16 has float32's exponents, so nothing is scaled and no value of
+// the range is lost).  Of the nine products of pieces the six largest are
+// formed, a1 b1, a1 b2, a2 b1, a2 b2, a1 b3, a3 b1; the other three are below
+// 2^-24 of the whole.  Six bf16 products instead of one bound the rate at a
+// sixth of the bf16 rate.
+//
+//   linear_split_kernel   float32 operands -> three bf16 planes each (6 bytes
+//                         per value), with dz = dy act'(z) and the partial
+//                         sums of db on the way in the backward pass
+//   linear_gemm_kernel    C = A B^T (+ epilogue) over the planes
+//   linear_join_kernel    sums of the tiles whose reduction was divided
+//   linear_special_kernel rows and columns that hold infinities (see there)
+#include <cuda.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include <string>
+
+#include "mm_linear_tc.cuh"
+
+namespace mm {
+
+// ---------------------------------------------------------------------------
+// Splitting
+// ---------------------------------------------------------------------------
+
+constexpr int SP_ROWS = 64, SP_COLS = 128;  // values per block
+
+// Three bf16 pieces (as their float32 bits, low halves zero).  a1 is rounded to
+// nearest but stays finite; infinities and NaNs keep a2 = a3 = 0.
+__device__ __forceinline__ void split3(float a, uint32_t& h1, uint32_t& h2, uint32_t& h3) {
+  const uint32_t u = __float_as_uint(a);
+  const uint32_t mag = u & 0x7fffffffu, sign = u & 0x80000000u;
+  if (mag >= 0x7f800000u) {
+    h1 = mag > 0x7f800000u ? 0x7fc00000u : u;
+    h2 = h3 = 0u;
+    return;
+  }
+  h1 = sign | min((mag + 0x8000u) & 0xffff0000u, 0x7f7f0000u);
+  const float r = a - __uint_as_float(h1);
+  h2 = (__float_as_uint(r) + 0x8000u) & 0xffff0000u;
+  h3 = __float_as_uint(r - __uint_as_float(h2)) & 0xffff0000u;
+}
+
+// Blocks of 64 x 128 values; 16 threads x 8 values across a row, 16 rows at a
+// time.  Bound by memory: 4 bytes in and 6 out per value.
+__global__ void __launch_bounds__(256) linear_split_kernel(const __grid_constant__ LinSplits all) {
+  __shared__ float sums[16][SP_COLS + 4];
+  pdl_wait();
+  int k = 0;
+  while (k + 1 < all.count && blockIdx.x >= all.s[k + 1].first) ++k;
+  const LinSplit& s = all.s[k];
+  const int block = (int)(blockIdx.x - s.first);
+  const int bc = block % s.blocks_c, br = block / s.blocks_c;
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  const int c0 = bc * SP_COLS + tx * 8;
+  float sum[8] = {};
+  int inf = 0;
+#pragma unroll
+  for (int i = 0; i < SP_ROWS / 16; ++i) {
+    const int64_t row = (int64_t)br * SP_ROWS + i * 16 + ty;
+    if (row >= s.rows || c0 >= s.cols) continue;
+    float v[8];
+    const float* src = s.src + row * s.s0;
+    if (s.vec && c0 + 8 <= s.cols) {
+      const float4 a = *reinterpret_cast<const float4*>(src + c0), b = *reinterpret_cast<const float4*>(src + c0 + 4);
+      v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+      v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = c0 + e < s.cols ? src[(int64_t)(c0 + e) * s.s1] : 0.f;
+    }
+    if (s.z) {
+      const float* z = s.z + row * s.cols;
+      if (s.vec && c0 + 8 <= s.cols) {
+        const float4 a = *reinterpret_cast<const float4*>(z + c0), b = *reinterpret_cast<const float4*>(z + c0 + 4);
+        const float t[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] *= lin_slope(t[e], s.act);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (c0 + e < s.cols) v[e] *= lin_slope(z[c0 + e], s.act);
+      }
+    }
+    if (s.out) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (c0 + e < s.cols) s.out[row * s.cols + c0 + e] = v[e];
+    }
+    uint32_t p[3][4];
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) {
+      uint32_t a1, a2, a3, b1, b2, b3;
+      split3(v[e], a1, a2, a3);
+      split3(v[e + 1], b1, b2, b3);
+      p[0][e / 2] = a1 >> 16 | b1;
+      p[1][e / 2] = a2 >> 16 | b2;
+      p[2][e / 2] = a3 >> 16 | b3;
+    }
+#pragma unroll
+    for (int q = 0; q < 3; ++q)
+      *reinterpret_cast<uint4*>(s.planes + (q * s.rows + row) * s.ld + c0) = make_uint4(p[q][0], p[q][1], p[q][2], p[q][3]);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      sum[e] += v[e];
+      inf |= (__float_as_uint(v[e]) & 0x7fffffffu) == 0x7f800000u;
+    }
+  }
+  inf = __syncthreads_or(inf);
+  if (threadIdx.x == 0) s.flags[block] = inf;
+  if (!s.part) return;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) sums[ty][tx * 8 + e] = sum[e];
+  __syncthreads();
+  const int c = bc * SP_COLS + threadIdx.x;
+  if (threadIdx.x < SP_COLS && c < s.cols) {
+    float t = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) t += sums[i][threadIdx.x];
+    s.part[(int64_t)br * s.cols + c] = t;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Tensor-core product
+// ---------------------------------------------------------------------------
+
+__device__ int g_lin_error = 0;
+
+enum { LG_ERR_FULL = 101, LG_ERR_EMPTY = 102, LG_ERR_ACC = 103, LG_ERR_FREE = 104, LG_ERR_DRAIN = 105 };
+
+constexpr int LG_BM = 128, LG_BK = 32;
+constexpr int LG_EPI_WARPS = 8, LG_WARP_TMA = 8, LG_WARP_MMA = 9, LG_THREADS = 320;
+constexpr uint64_t LG_WAIT_NS = 200ull * 1000 * 1000;
+
+__device__ __forceinline__ uint32_t lg_smem(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+
+__device__ __forceinline__ void lg_bar_init(uint64_t* bar, uint32_t count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(lg_smem(bar)), "r"(count));
+}
+
+__device__ __forceinline__ bool lg_try(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(lg_smem(bar)), "r"(parity), "r"(1000u)
+      : "memory");
+  return ok != 0;
+}
+
+// Bounded wait.  It gives up after 200 ms, or soon after another wait did, and
+// records which one; a drain (wait for this CTA's own copies and MMAs) ignores
+// the others' errors.
+__device__ __forceinline__ bool lg_wait(uint64_t* bar, uint32_t parity, int code) {
+  if (lg_try(bar, parity)) return true;
+  uint64_t t0, t;
+  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t0));
+  for (uint32_t i = 1; i < (1u << 26); ++i) {
+    if (lg_try(bar, parity)) return true;
+    if ((i & 63) == 0) {
+      if (code != LG_ERR_DRAIN && *reinterpret_cast<volatile int*>(&g_lin_error) != 0) return false;
+      asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+      if (t - t0 > LG_WAIT_NS) break;
+    }
+  }
+  atomicCAS(&g_lin_error, 0, code);
+  return false;
+}
+
+__device__ __forceinline__ void lg_arrive(uint64_t* bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(lg_smem(bar)) : "memory");
+}
+
+__device__ __forceinline__ void lg_commit(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(lg_smem(bar))
+               : "memory");
+}
+
+__device__ __forceinline__ void lg_load(void* dst, const CUtensorMap* map, uint64_t* bar, int x, int y) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+      ::"r"(lg_smem(dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(0), "r"(lg_smem(bar))
+      : "memory");
+}
+
+__device__ __forceinline__ void lg_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+__device__ __forceinline__ bool lg_elect() {
+  uint32_t leader;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b32 l;\n\t"
+      "elect.sync l|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(leader));
+  return leader != 0;
+}
+
+__device__ __forceinline__ void lg_tmem_load32(uint32_t addr, float* v) {
+  uint32_t r[32];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(addr));
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+
+// An operand tile of ROWS rows (of C's m or n) and 32 of the reduction, three
+// planes.  K-major (the planes' rows are dense along the reduction): ROWS rows
+// of 64 bytes per plane, 64-byte swizzle, 8-row groups 512 bytes apart.
+// MN-major (dense along m or n): groups of 64 of them, 32 rows of 128 bytes per
+// plane and group, 128-byte swizzle; groups 12 KB apart, 8-row groups 1 KB.
+template <int ROWS, bool MN>
+struct LgTile {
+  static constexpr uint32_t plane = MN ? 4096u : ROWS * 64u;
+  static constexpr uint32_t bytes = ROWS * 192u;
+  static constexpr uint32_t hi = (MN ? (1024u >> 4) : (512u >> 4)) | 1u << 14 | (MN ? 2u : 4u) << 29;
+  // Descriptor of piece p (0..2), step kk (16 of the reduction) of the tile at addr.
+  static __device__ __forceinline__ uint64_t desc(uint32_t addr, int p, int kk) {
+    const uint32_t at = addr + (uint32_t)p * plane + (uint32_t)kk * (MN ? 2048u : 32u);
+    const uint32_t lo = ((at >> 4) & 0x3fffu) | ((MN ? 12288u >> 4 : 1u) << 16);
+    return (uint64_t)hi << 32 | lo;
+  }
+  static __device__ __forceinline__ void load(uint8_t* dst, const CUtensorMap* map, uint64_t* bar, int row, int k) {
+    if (MN) {
+#pragma unroll
+      for (int g = 0; g < ROWS / 64; ++g) lg_load(dst + g * 12288, map, bar, row + 64 * g, k);
+    } else {
+      lg_load(dst, map, bar, k, row);
+    }
+  }
+};
+
+template <int BN>
+constexpr int lg_stages() {
+  return BN == 256 ? 3 : BN == 128 ? 4 : 6;
+}
+
+// One unit of work: an output tile and a range of its reduction's stages.
+struct LgUnit {
+  int m0, n0, begin, end;
+  int part;  // index of its partial tile, or -1: the whole reduction
+};
+
+__device__ __forceinline__ LgUnit lg_unit(const LinGemm& a, int u, int bn) {
+  LgUnit w;
+  int tile = u, split = 0, splits = 1;
+  w.part = -1;
+  if (u >= a.full) {
+    tile = a.full + (u - a.full) / a.splits;
+    split = (u - a.full) % a.splits;
+    splits = a.splits;
+    if (splits > 1) w.part = u - a.full;
+  }
+  // Tiles in groups of eight rows of tiles, column by column, so that those
+  // running together share operand tiles in L2.
+  const int per = LIN_GROUP * a.tiles_n;
+  const int group = tile / per, in = tile - group * per;
+  const int rows = min(LIN_GROUP, a.tiles_m - group * LIN_GROUP);
+  w.m0 = (group * LIN_GROUP + in % rows) * LG_BM;
+  w.n0 = (in / rows) * bn;
+  w.begin = (int)((int64_t)a.stages * split / splits);
+  w.end = (int)((int64_t)a.stages * (split + 1) / splits);
+  return w;
+}
+
+// Persistent CTAs, one per SM.  Warps 0-7 add up and store, warp 8 loads (TMA),
+// warp 9 issues the MMAs.  The MMAs of one stage (32 of the reduction, twelve
+// products of 128 x BN x 16) go into one of two accumulators in tensor memory,
+// small products first; warps 0-7 add it to float32 totals in registers while
+// the next stage runs in the other.  The tensor core rounds its sums toward
+// zero, which over a long reduction drifts by about K 2^-24; with one stage per
+// accumulator only the two a1 b1 products of a stage are added at full size.
+template <int BN, bool AMN, bool BMN>
+__global__ void __launch_bounds__(LG_THREADS, 1) linear_gemm_kernel(const __grid_constant__ CUtensorMap ma,
+                                                                    const __grid_constant__ CUtensorMap mb,
+                                                                    const LinGemm a) {
+  using TA = LgTile<LG_BM, AMN>;
+  using TB = LgTile<BN, BMN>;
+  constexpr int S = lg_stages<BN>();
+  constexpr uint32_t stage_bytes = TA::bytes + TB::bytes;
+  constexpr uint32_t cols = 2 * BN;
+  constexpr int HALF = BN / 2;  // columns per warp
+  extern __shared__ uint8_t raw[];
+  uint8_t* smem = raw + ((1024 - (lg_smem(raw) & 1023)) & 1023);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + S * stage_bytes);
+  uint64_t *empty = full + S, *acc_full = empty + S, *acc_free = acc_full + 2, *drain = acc_free + 2;
+  uint32_t* slot = reinterpret_cast<uint32_t*>(drain + 1);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < S; ++i) {
+      lg_bar_init(&full[i], 1);
+      lg_bar_init(&empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      lg_bar_init(&acc_full[i], 1);
+      lg_bar_init(&acc_free[i], LG_EPI_WARPS);
+    }
+    lg_bar_init(drain, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == LG_WARP_MMA) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(lg_smem(slot)), "r"(cols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const uint32_t tmem = *slot;
+  pdl_wait();
+
+  if (warp == LG_WARP_TMA) {
+    int st = 0, filled = 0;
+    uint32_t par = 1;
+    bool alive = true;
+    for (int u = blockIdx.x; u < a.units && alive; u += gridDim.x) {
+      const LgUnit w = lg_unit(a, u, BN);
+      for (int k = w.begin; k < w.end; ++k) {
+        if (!__all_sync(0xffffffffu, lg_wait(&empty[st], par, LG_ERR_EMPTY))) {
+          alive = false;
+          break;
+        }
+        if (lg_elect()) {
+          asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(lg_smem(&full[st])),
+                       "r"(stage_bytes)
+                       : "memory");
+          uint8_t* dst = smem + (uint32_t)st * stage_bytes;
+          TA::load(dst, &ma, &full[st], w.m0, k * LG_BK);
+          TB::load(dst + TA::bytes, &mb, &full[st], w.n0, k * LG_BK);
+        }
+        ++filled;
+        if (++st == S) {
+          st = 0;
+          par ^= 1u;
+        }
+      }
+    }
+    // Nothing may land in shared memory after the CTA has gone: wait for the
+    // last fill of every stage (over already unless a wait gave up).
+    for (int i = max(0, filled - S); i < filled; ++i) lg_wait(&full[i % S], (uint32_t)(i / S) & 1u, LG_ERR_DRAIN);
+  } else if (warp == LG_WARP_MMA) {
+    constexpr uint32_t idesc = 1u << 4 | 1u << 7 | 1u << 10 | (AMN ? 1u << 15 : 0u) | (BMN ? 1u << 16 : 0u) |
+                               (uint32_t)(BN >> 3) << 17 | (uint32_t)(LG_BM >> 4) << 24;
+    int st = 0, buf = 0;
+    uint32_t par = 0, bpar = 1;
+    bool alive = true;
+    for (int u = blockIdx.x; u < a.units && alive; u += gridDim.x) {
+      const LgUnit w = lg_unit(a, u, BN);
+      for (int k = w.begin; k < w.end; ++k) {
+        const bool ok = lg_wait(&acc_free[buf], bpar, LG_ERR_FREE) && lg_wait(&full[st], par, LG_ERR_FULL);
+        if (!__all_sync(0xffffffffu, ok)) {
+          alive = false;
+          break;
+        }
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        if (lg_elect()) {
+          const uint32_t at = lg_smem(smem + (uint32_t)st * stage_bytes), bt = at + TA::bytes;
+          const uint32_t d = tmem + (uint32_t)(buf * BN);
+          constexpr int pa[6] = {2, 0, 1, 0, 1, 0}, pb[6] = {0, 2, 1, 1, 0, 0};
+#pragma unroll
+          for (int q = 0; q < 6; ++q)
+#pragma unroll
+            for (int kk = 0; kk < 2; ++kk)
+              lg_mma(d, TA::desc(at, pa[q], kk), TB::desc(bt, pb[q], kk), idesc, q + kk > 0 ? 1u : 0u);
+          lg_commit(&empty[st]);
+          lg_commit(&acc_full[buf]);
+        }
+        if (++st == S) {
+          st = 0;
+          par ^= 1u;
+        }
+        if (++buf == 2) {
+          buf = 0;
+          bpar ^= 1u;
+        }
+      }
+    }
+    // No MMA may still write tensor memory when it is freed.
+    __syncwarp();
+    if (lg_elect()) lg_commit(drain);
+    __syncwarp();
+    lg_wait(drain, 0u, LG_ERR_DRAIN);
+  } else {
+    const int quarter = warp & 3, half = warp >> 2;
+    const uint32_t base = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(half * HALF);
+    int buf = 0;
+    uint32_t par = 0;
+    bool alive = true;
+    for (int u = blockIdx.x; u < a.units && alive; u += gridDim.x) {
+      const LgUnit w = lg_unit(a, u, BN);
+      float acc[HALF];
+#pragma unroll
+      for (int i = 0; i < HALF; ++i) acc[i] = 0.f;
+      for (int k = w.begin; k < w.end; ++k) {
+        if (!__all_sync(0xffffffffu, lg_wait(&acc_full[buf], par, LG_ERR_ACC))) {
+          alive = false;
+          break;
+        }
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll
+        for (int j = 0; j < HALF / 32; ++j) {
+          float v[32];
+          lg_tmem_load32(base + (uint32_t)(buf * BN + 32 * j), v);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) acc[32 * j + i] += v[i];
+        }
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) lg_arrive(&acc_free[buf]);
+        if (++buf == 2) {
+          buf = 0;
+          par ^= 1u;
+        }
+      }
+      if (!alive) break;
+      const int64_t row = (int64_t)w.m0 + quarter * 32 + lane;
+      int col = w.n0 + half * HALF;
+      float* out = a.c + row * a.n;
+      float* part = w.part >= 0 ? a.part + ((int64_t)w.part * LG_BM + quarter * 32 + lane) * BN + half * HALF : nullptr;
+      // Eight columns at a time; the totals move down by eight registers per
+      // step, so that the epilogue's code is there once.
+#pragma unroll 1
+      for (int j = 0; j < HALF / 8; ++j, col += 8) {
+        if (part) {
+          reinterpret_cast<float4*>(part)[2 * j] = make_float4(acc[0], acc[1], acc[2], acc[3]);
+          reinterpret_cast<float4*>(part)[2 * j + 1] = make_float4(acc[4], acc[5], acc[6], acc[7]);
+        } else if (row < a.m && col < a.n) {
+          if (a.vec && col + 8 <= a.n) {
+            float v[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = lin_finish(a.e, acc[e], row, col + e, a.n);
+            reinterpret_cast<float4*>(out + col)[0] = make_float4(v[0], v[1], v[2], v[3]);
+            reinterpret_cast<float4*>(out + col)[1] = make_float4(v[4], v[5], v[6], v[7]);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              if (col + e < a.n) out[col + e] = lin_finish(a.e, acc[e], row, col + e, a.n);
+          }
+        }
+#pragma unroll
+        for (int i = 0; i + 8 < HALF; ++i) acc[i] = acc[i + 8];
+      }
+    }
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  if (warp == LG_WARP_MMA) {
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(cols) : "memory");
+  }
+}
+
+// Tiles whose reduction was divided: the partial tiles are added in order and
+// go through the epilogue.  One block per 8 rows of a tile.
+__global__ void __launch_bounds__(256) linear_join_kernel(const LinGemm a, int bn) {
+  pdl_wait();
+  const int tile = blockIdx.x / (LG_BM / 8), r0 = blockIdx.x % (LG_BM / 8) * 8;
+  const LgUnit w = lg_unit(a, a.full + tile * a.splits, bn);
+  const float* part = a.part + (int64_t)tile * a.splits * LG_BM * bn;
+  for (int i = threadIdx.x; i < 8 * bn; i += 256) {
+    const int r = r0 + i / bn, c = i % bn;
+    const int64_t row = w.m0 + r;
+    if (row >= a.m || w.n0 + c >= a.n) continue;
+    float v = 0.f;
+    for (int s = 0; s < a.splits; ++s) v += part[((int64_t)s * LG_BM + r) * bn + c];
+    a.c[row * a.n + w.n0 + c] = lin_finish(a.e, v, row, w.n0 + c, a.n);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Infinities.  Their pieces are (inf, 0, 0), and inf times another operand's
+// zero piece is NaN where the whole product is infinite.  linear_split_kernel
+// says which of its blocks hold an infinity; rows of A (columns of C) and rows
+// of B that do are computed again here from the pieces' sums, in float32.
+// Without any, every block reads its flags and leaves.
+// ---------------------------------------------------------------------------
+
+__device__ __forceinline__ float lin_value(const LinPlanes& p, int64_t line, int64_t k) {
+  const int64_t at = p.mn ? k * p.ld + line : line * p.ld + k;
+  const int64_t plane = p.mn ? p.k * p.ld : p.lines * p.ld;
+  float v = 0.f;
+#pragma unroll
+  for (int q = 2; q >= 0; --q) v += __uint_as_float((uint32_t)p.planes[q * plane + at] << 16);
+  return v;
+}
+
+__global__ void __launch_bounds__(256) linear_special_kernel(const LinGemm a, const LinPlanes pa, const LinPlanes pb,
+                                                             int blocks_a) {
+  pdl_wait();
+  const bool is_b = (int)blockIdx.x >= blocks_a;
+  const LinPlanes& p = is_b ? pb : pa;
+  const LinPlanes& other = is_b ? pa : pb;
+  const int block = is_b ? blockIdx.x - blocks_a : blockIdx.x;
+  // Lines of this block and the flags that speak of them.
+  const int per = p.mn ? SP_COLS : SP_ROWS;
+  const int across = (int)((p.k + (p.mn ? SP_ROWS : SP_COLS) - 1) / (p.mn ? SP_ROWS : SP_COLS));
+  const int blocks_c = (int)(((p.mn ? p.lines : p.k) + SP_COLS - 1) / SP_COLS);
+  int any = 0;
+  for (int i = threadIdx.x; i < across; i += 256) any |= p.flags[p.mn ? i * blocks_c + block : block * blocks_c + i];
+  if (!__syncthreads_or(any)) return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t end = min((int64_t)(block + 1) * per, p.lines);
+  for (int64_t line = (int64_t)block * per; line < end; ++line) {
+    int inf = 0, nan = 0;
+    for (int64_t k = threadIdx.x; k < p.k; k += 256) {
+      const float v = lin_value(p, line, k);
+      inf |= isinf(v);
+      nan |= isnan(v);
+    }
+    inf = __syncthreads_or(inf);
+    nan = __syncthreads_or(nan);
+    if (!inf || nan) continue;  // a NaN makes the whole line NaN already
+    for (int64_t o = warp; o < other.lines; o += 8) {
+      float v = 0.f;
+      for (int64_t k = lane; k < p.k; k += 32) v += lin_value(p, line, k) * lin_value(other, o, k);
+#pragma unroll
+      for (int s = 16; s > 0; s >>= 1) v += __shfl_xor_sync(0xffffffffu, v, s);
+      const int64_t row = is_b ? o : line, col = is_b ? line : o;
+      if (lane == 0) a.c[row * a.n + col] = lin_finish(a.e, v, row, (int)col, a.n);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Host side
+// ---------------------------------------------------------------------------
+
+int lin_kernel_error(int* code, int clear) {
+  cudaError_t e = cudaMemcpyFromSymbol(code, g_lin_error, sizeof(int));
+  if (e == cudaSuccess && clear && *code != 0) {
+    const int zero = 0;
+    e = cudaMemcpyToSymbol(g_lin_error, &zero, sizeof(int));
+  }
+  return e == cudaSuccess ? MM_OK : cuda_fail(e, "mm_kernel_error");
+}
+
+int64_t lin_flag_words(int64_t rows, int64_t cols) {
+  return ((rows + SP_ROWS - 1) / SP_ROWS) * ((cols + SP_ROWS - 1) / SP_ROWS);
+}
+
+int64_t lin_plane_bytes(int64_t rows, int64_t cols) { return 6 * ((rows + 7) / 8 * 8) * ((cols + 7) / 8 * 8); }
+
+int64_t lin_part_rows(int64_t m) { return (m + SP_ROWS - 1) / SP_ROWS; }
+
+void lin_add_split(LinSplits* all, const LinSplit& s) {
+  LinSplit& t = all->s[all->count];
+  t = s;
+  t.first = (uint32_t)all->blocks;
+  t.blocks_c = (s.cols + SP_COLS - 1) / SP_COLS;
+  all->blocks += (int64_t)t.blocks_c * ((s.rows + SP_ROWS - 1) / SP_ROWS);
+  ++all->count;
+}
+
+int lin_run_splits(const LinSplits& all, cudaStream_t s) {
+  if (all.blocks > INT32_MAX) return fail(MM_ERR_UNSUPPORTED, "mm_linear: operands too large");
+  cudaError_t e = launch_pdl(linear_split_kernel, dim3((unsigned)all.blocks), dim3(256), 0, s, all);
+  return e == cudaSuccess ? MM_OK : cuda_fail(e, "mm_linear split launch");
+}
+
+// Tile width and division of the reduction, by an estimate in SM clocks: a
+// stage takes 6 BN clocks of MMAs (and no less than about 500 for its loads and
+// barriers), a tile about 4,000 more to fill the pipeline and store.  Whole
+// waves of tiles run undivided; the rest is divided where that ends sooner
+// although its partial tiles are written and read once more.
+LinChoice lin_choose(int64_t m, int64_t n, int64_t k) {
+  const int sms = sm_count();
+  LinChoice best = {0, 0, 1, 0, 0, 0, 0};
+  double least = 0;
+  for (int bn : {256, 128, 64}) {
+    const int64_t tm = (m + LG_BM - 1) / LG_BM, tn = (n + bn - 1) / bn, tiles = tm * tn;
+    const int64_t stages = (k + LG_BK - 1) / LG_BK;
+    const double stage = 6.0 * bn < 500 ? 500 : 6.0 * bn, tile = 4000;
+    const int64_t full = tiles / sms * sms, rest = tiles - full;
+    const double base = (double)(full / sms) * (stages * stage + tile);
+    for (int s = 1; s <= LIN_MAX_SPLITS; ++s) {
+      if (s > 1 && (rest == 0 || s > stages || rest * s > LIN_MAX_PARTS)) break;
+      double t = base;
+      if (rest) {
+        const int64_t waves = (rest * s + sms - 1) / sms;
+        t += waves * (((stages + s - 1) / s) * stage + tile);
+        if (s > 1) t += 4000 + (double)rest * s * LG_BM * bn * 8 / 3500;  // about 3,500 bytes per clock
+      }
+      if (best.bn == 0 || t < least) {
+        least = t;
+        best = {bn, (int)full, s, (int)tm, (int)tn, (int)stages, (int)(full + rest * s)};
+      }
+    }
+  }
+  return best;
+}
+
+int64_t lin_part_bytes(const LinChoice& c) {
+  return c.splits > 1 ? (int64_t)(c.units - c.full) * LG_BM * c.bn * 4 : 0;
+}
+
+static int lin_map(const LinPlanes& p, int rows, CUtensorMap* out) {
+  using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+  static const EncodeFn encode = [] {
+    void* fn = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    const cudaError_t e = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q);
+    return e == cudaSuccess && q == cudaDriverEntryPointSuccess ? (EncodeFn)fn : nullptr;
+  }();
+  if (encode == nullptr) return fail(MM_ERR_CUDA, "mm_linear: cuTensorMapEncodeTiled entry point unavailable");
+  const cuuint64_t r = (cuuint64_t)(p.mn ? p.k : p.lines), c = (cuuint64_t)(p.mn ? p.lines : p.k);
+  const cuuint64_t dims[3] = {c, r, 3}, strides[2] = {(cuuint64_t)p.ld * 2, r * (cuuint64_t)p.ld * 2};
+  const cuuint32_t box[3] = {p.mn ? 64u : (cuuint32_t)LG_BK, p.mn ? (cuuint32_t)LG_BK : (cuuint32_t)rows, 3};
+  const cuuint32_t ones[3] = {1, 1, 1};
+  const CUresult e = encode(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, (void*)p.planes, dims, strides, box, ones,
+                            CU_TENSOR_MAP_INTERLEAVE_NONE,
+                            p.mn ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (e != CUDA_SUCCESS)
+    return fail(MM_ERR_CUDA, "mm_linear: cuTensorMapEncodeTiled failed (CUresult " + std::to_string((int)e) + ")");
+  return MM_OK;
+}
+
+template <int BN, bool AMN, bool BMN>
+static int lin_launch(const CUtensorMap& ma, const CUtensorMap& mb, const LinGemm& g, cudaStream_t s) {
+  constexpr size_t smem = 1024 + (size_t)lg_stages<BN>() * (LG_BM + BN) * 192 + 256;
+  auto kernel = linear_gemm_kernel<BN, AMN, BMN>;
+  MM_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem),
+          "mm_linear: shared memory attribute");
+  const int sms = sm_count();
+  MM_CUDA(launch_pdl(kernel, dim3((unsigned)(g.units < sms ? g.units : sms)), dim3(LG_THREADS), smem, s, ma, mb, g),
+          "mm_linear launch");
+  return MM_OK;
+}
+
+template <int BN>
+static int lin_launch_bn(bool amn, bool bmn, const CUtensorMap& ma, const CUtensorMap& mb, const LinGemm& g,
+                         cudaStream_t s) {
+  if (amn) return bmn ? lin_launch<BN, true, true>(ma, mb, g, s) : lin_launch<BN, true, false>(ma, mb, g, s);
+  return bmn ? lin_launch<BN, false, true>(ma, mb, g, s) : lin_launch<BN, false, false>(ma, mb, g, s);
+}
+
+int lin_run_gemm(const LinPlanes& pa, const LinPlanes& pb, float* c, const LinEpilogue& e, const LinChoice& ch,
+                 float* part, cudaStream_t s) {
+  LinGemm g;
+  g.m = (int)pa.lines;
+  g.n = (int)pb.lines;
+  g.stages = ch.stages;
+  g.tiles_m = ch.tiles_m;
+  g.tiles_n = ch.tiles_n;
+  g.full = ch.full;
+  g.splits = ch.splits;
+  g.units = ch.units;
+  // The epilogue's eight columns are written as two 16-byte stores.
+  g.vec = g.n % 4 == 0 && (uintptr_t)c % 16 == 0;
+  g.c = c;
+  g.part = part;
+  g.e = e;
+  CUtensorMap ma, mb;
+  int rc = lin_map(pa, LG_BM, &ma);
+  if (rc == MM_OK) rc = lin_map(pb, ch.bn, &mb);
+  if (rc != MM_OK) return rc;
+  rc = ch.bn == 256   ? lin_launch_bn<256>(pa.mn, pb.mn, ma, mb, g, s)
+       : ch.bn == 128 ? lin_launch_bn<128>(pa.mn, pb.mn, ma, mb, g, s)
+                      : lin_launch_bn<64>(pa.mn, pb.mn, ma, mb, g, s);
+  if (rc != MM_OK) return rc;
+  if (ch.splits > 1) {
+    const unsigned grid = (unsigned)((ch.units - ch.full) / ch.splits * (LG_BM / 8));
+    MM_CUDA(launch_pdl(linear_join_kernel, dim3(grid), dim3(256), 0, s, g, ch.bn), "mm_linear join launch");
+  }
+  const int per_a = pa.mn ? SP_COLS : SP_ROWS, per_b = pb.mn ? SP_COLS : SP_ROWS;
+  const int blocks_a = (int)((pa.lines + per_a - 1) / per_a), blocks_b = (int)((pb.lines + per_b - 1) / per_b);
+  MM_CUDA(launch_pdl(linear_special_kernel, dim3((unsigned)(blocks_a + blocks_b)), dim3(256), 0, s, g, pa, pb, blocks_a),
+          "mm_linear special launch");
+  return MM_OK;
+}
+
+}  // namespace mm
