@@ -343,25 +343,24 @@ int mm_nll_loss_backward(const mm_tensor_t* grad_output, const mm_tensor_t* inpu
                          int64_t ignore_index, const mm_tensor_t* total_weight,
                          const mm_tensor_t* grad_input, void* stream);
 
-/* Layer norm over the rows of x [rows, width] (dense rows, any row stride):
+/* Layer norm over the rows of x [rows, width] (dense rows x_stride apart):
  * y = (x - mean) * rstd * weight + bias with rstd = 1 / sqrt(var + eps), var the
  * mean squared distance from the row's mean.  weight and bias [width] may be
  * NULL; y is dense; mean and rstd [rows] are kept for the backward pass.  No
  * counterpart in the reference, whose only normalisation is eval BatchNorm. */
-int mm_layer_norm(const mm_tensor_t* x, const mm_tensor_t* weight, const mm_tensor_t* bias, double eps,
-                  const mm_tensor_t* y, const mm_tensor_t* mean, const mm_tensor_t* rstd, void* stream);
+int mm_layer_norm(const float* x, int64_t x_stride, int64_t rows, int64_t width, const float* weight,
+                  const float* bias, double eps, float* y, float* mean, float* rstd, void* stream);
 
 /* Gradients of mm_layer_norm: with xh = (x - mean) * rstd and g = dy * weight,
  * dx = rstd * (g - mean(g) - xh * mean(g * xh)), dweight = sum over rows of
- * dy * xh, dbias = sum over rows of dy.  dx, dweight and dbias may be NULL.
- * workspace: device memory, 16-byte aligned, of
- * mm_layer_norm_backward_workspace_size bytes (it holds partial column sums;
- * unused, and may be NULL, when dweight and dbias are NULL).  The sums are
- * added in a fixed order: equal inputs give equal bits. */
-int mm_layer_norm_backward(const mm_tensor_t* dy, const mm_tensor_t* x, const mm_tensor_t* mean,
-                           const mm_tensor_t* rstd, const mm_tensor_t* weight, const mm_tensor_t* dx,
-                           const mm_tensor_t* dweight, const mm_tensor_t* dbias, void* workspace,
-                           size_t workspace_bytes, void* stream);
+ * dy * xh, dbias = sum over rows of dy.  dx (dense), dweight and dbias may be
+ * NULL.  workspace: device memory, 16-byte aligned, of
+ * mm_layer_norm_backward_workspace_size bytes for partial column sums, or NULL
+ * to take it from the scratch pool.  The sums are added in a fixed order: equal
+ * inputs give equal bits. */
+int mm_layer_norm_backward(const float* dy, int64_t dy_stride, const float* x, int64_t x_stride, int64_t rows,
+                           int64_t width, const float* mean, const float* rstd, const float* weight, float* dx,
+                           float* dweight, float* dbias, void* workspace, size_t workspace_bytes, void* stream);
 int mm_layer_norm_backward_workspace_size(int64_t rows, int64_t width, size_t* bytes);
 
 typedef enum mm_linear_act {
@@ -374,25 +373,29 @@ typedef enum mm_linear_act {
 } mm_linear_act_t;
 
 /* y = act(x w^T + bias) + residual, or act(x w^T + bias + residual) when
- * residual_before_act: x [m, k] and w [n, k] of any strides, bias [n] and
- * residual [m, n] (dense rows) or NULL, y [m, n] dense.  z (dense [m, n] or
- * NULL) receives the values that the activation is applied to, which the
- * backward pass needs.  float32 accuracy throughout.  workspace: device memory,
- * 256-byte aligned, of mm_linear_workspace_size(m, n, k, 0) bytes.  Extends
- * mm_gemm (which has no residual, GELU or gradient). */
-int mm_linear(const mm_tensor_t* x, const mm_tensor_t* w, const mm_tensor_t* bias, const mm_tensor_t* residual,
-              int act, int residual_before_act, const mm_tensor_t* y, const mm_tensor_t* z, void* workspace,
-              size_t workspace_bytes, void* stream);
+ * residual_before_act: x [m, k] and w [n, k] with any strides (s0 between rows,
+ * s1 between columns), bias [n] or NULL, residual [m, n] (dense rows
+ * residual_stride apart) or NULL, y dense [m, n].  z (dense [m, n] or NULL)
+ * receives the values that the activation is applied to, which the backward
+ * pass needs.  float32 accuracy throughout.  workspace: device memory, 256-byte
+ * aligned, of mm_linear_workspace_size(m, n, k, 0) bytes, or NULL to take it from
+ * the scratch pool.  Extends mm_gemm (which has no residual, GELU or gradient). */
+int mm_linear(const float* x, int64_t xs0, int64_t xs1, const float* w, int64_t ws0, int64_t ws1,
+              const float* bias, const float* residual, int64_t residual_stride, int64_t m, int64_t n, int64_t k,
+              int act, int residual_before_act, float* y, float* z, void* workspace, size_t workspace_bytes,
+              void* stream);
 
-/* Gradients of mm_linear from dy [m, n] (dense rows) and the z it wrote (any z,
- * or NULL, without an activation; y serves as z for ReLU without a residual):
- * dz = dy * act'(z), dx = dz w, dw = dz^T x, db = sum over rows of dz.  Every
- * output is dense and may be NULL.  workspace:
- * mm_linear_workspace_size(m, n, k, 1) bytes, 256-byte aligned.  Sums are added
- * in a fixed order: equal inputs give equal bits. */
-int mm_linear_backward(const mm_tensor_t* dy, const mm_tensor_t* x, const mm_tensor_t* w, const mm_tensor_t* z,
-                       int act, const mm_tensor_t* dx, const mm_tensor_t* dw, const mm_tensor_t* db,
-                       const mm_tensor_t* dz, void* workspace, size_t workspace_bytes, void* stream);
+/* Gradients of mm_linear from dy [m, n] (dense rows dy_stride apart) and the z
+ * it wrote (unused without an activation; y serves as z for ReLU without a
+ * residual): dz = dy * act'(z), dx = dz w, dw = dz^T x, db = sum over rows of dz.
+ * Every output is dense and may be NULL.  workspace:
+ * mm_linear_workspace_size(m, n, k, 1) bytes, 256-byte aligned, or NULL to take
+ * it from the scratch pool.  Sums are added in a fixed order: equal inputs give
+ * equal bits. */
+int mm_linear_backward(const float* dy, int64_t dy_stride, const float* x, int64_t xs0, int64_t xs1,
+                       const float* w, int64_t ws0, int64_t ws1, const float* z, int64_t m, int64_t n, int64_t k,
+                       int act, float* dx, float* dw, float* db, float* dz, void* workspace,
+                       size_t workspace_bytes, void* stream);
 int mm_linear_workspace_size(int64_t m, int64_t n, int64_t k, int backward, size_t* bytes);
 
 /* One tensor of an optimiser step, numel consecutive float32 elements.  With
@@ -419,7 +422,8 @@ typedef struct mm_adamw_tensor {
  * per power of two over 16 powers of two, code 0 is zero), v as an 8-bit code of
  * its square root (16 steps; at least code 1 unless v is 0).  A non-finite
  * gradient makes the states of its whole block NaN.  workspace: 8 bytes per
- * tensor (mm_adamw_workspace_size).  Does the work of the reference's
+ * tensor (mm_adamw_workspace_size), 8-byte aligned, or NULL to take it from the
+ * scratch pool.  Does the work of the reference's
  * lerp_ / addcmul_ / addcdiv_ sequence (backends/opengl/dispatch.py:171-179,
  * :264-290) in one pass. */
 int mm_adamw(const mm_adamw_tensor_t* tensors, int count, int state_bits, double lr, double beta1, double beta2,

@@ -198,11 +198,13 @@ SIGNATURES = {
     "mm_log_softmax_backward": [_T, _T, _i, _T, _vp],
     "mm_nll_loss": [_T, _T, _T, _i, _i64, _T, _T, _vp],
     "mm_nll_loss_backward": [_T, _T, _T, _T, _i, _i64, _T, _T, _vp],
-    "mm_layer_norm": [_T, _T, _T, _d, _T, _T, _T, _vp],
-    "mm_layer_norm_backward": [_T, _T, _T, _T, _T, _T, _T, _T, _vp, _sz, _vp],
+    "mm_layer_norm": [_fp, _i64, _i64, _i64, _fp, _fp, _d, _fp, _fp, _fp, _vp],
+    "mm_layer_norm_backward": [_fp, _i64, _fp, _i64, _i64, _i64, _fp, _fp, _fp, _fp, _fp, _fp, _vp, _sz, _vp],
     "mm_layer_norm_backward_workspace_size": [_i64, _i64, ctypes.POINTER(_sz)],
-    "mm_linear": [_T, _T, _T, _T, _i, _i, _T, _T, _vp, _sz, _vp],
-    "mm_linear_backward": [_T, _T, _T, _T, _i, _T, _T, _T, _T, _vp, _sz, _vp],
+    "mm_linear": [_fp, _i64, _i64, _fp, _i64, _i64, _fp, _fp, _i64, _i64, _i64, _i64, _i, _i, _fp, _fp, _vp, _sz,
+                  _vp],
+    "mm_linear_backward": [_fp, _i64, _fp, _i64, _i64, _fp, _i64, _i64, _fp, _i64, _i64, _i64, _i, _fp, _fp, _fp,
+                           _fp, _vp, _sz, _vp],
     "mm_linear_workspace_size": [_i64, _i64, _i64, _i, ctypes.POINTER(_sz)],
     "mm_adamw": [_vp, _i, _i, _d, _d, _d, _d, _d, _i, _i, _i, _vp, _sz, _vp],
     "mm_adamw_workspace_size": [_i, ctypes.POINTER(_sz)],

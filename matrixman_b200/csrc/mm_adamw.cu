@@ -369,8 +369,8 @@ extern "C" int mm_adamw(const mm_adamw_tensor_t* tensors, int count, int state_b
     }
   }
   if (count == 0) return MM_OK;
-  if (workspace == nullptr || workspace_bytes < (size_t)count * sizeof(float2) || !aw_aligned(workspace, 8))
-    return fail(MM_ERR_INVALID, "mm_adamw: the workspace is missing, misaligned or too small");
+  if (workspace != nullptr && (workspace_bytes < (size_t)count * sizeof(float2) || !aw_aligned(workspace, 8)))
+    return fail(MM_ERR_INVALID, "mm_adamw: the workspace is misaligned or too small");
   AwScalars a;
   a.b1 = (float)beta1;
   a.omb1 = (float)(1.0 - beta1);
@@ -381,6 +381,12 @@ extern "C" int mm_adamw(const mm_adamw_tensor_t* tensors, int count, int state_b
   a.l2 = decoupled ? 0.f : (float)weight_decay;
   a.maximize = maximize != 0;
   cudaStream_t s = resolve_stream(stream);
+  Scratch scratch;
+  if (workspace == nullptr) {
+    const int rc = scratch.get((size_t)count * sizeof(float2), s);
+    if (rc != MM_OK) return rc;
+    workspace = scratch.data;
+  }
   float2* coef = (float2*)workspace;
   for (int at = 0; at < count; at += AW_MANY) {
     const int n = count - at < AW_MANY ? count - at : AW_MANY;

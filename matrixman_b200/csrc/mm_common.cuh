@@ -66,6 +66,23 @@ cudaError_t launch_pdl(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t s
   return cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
 }
 
+// A block of the current device's scratch pool for one call: taken when the
+// caller passes no workspace, returned to the pool (reuse ordered after the
+// work queued on `stream`) when the call has queued its kernels.
+struct Scratch {
+  void* data = nullptr;
+  cudaStream_t stream = nullptr;
+  int get(size_t bytes, cudaStream_t s) {
+    int device = 0;
+    cudaGetDevice(&device);
+    stream = s;
+    return mm_alloc(device, bytes, MM_POOL_SCRATCH, s, &data);
+  }
+  ~Scratch() {
+    if (data) mm_free(data, stream);
+  }
+};
+
 // Number of SMs of the current device (cached per device).
 int sm_count();
 

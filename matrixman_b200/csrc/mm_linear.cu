@@ -99,32 +99,11 @@ __global__ void __launch_bounds__(256) linear_columns_kernel(const float* part, 
   }
 }
 
-static int lin_matrix(const mm_tensor_t* t, const char* name, int64_t rows, int64_t cols, bool dense) {
-  int rc = validate(t, name, MM_F32);
-  if (rc != MM_OK) return rc;
-  if (t->ndim != 2 || (rows >= 0 && t->size[0] != rows) || (cols >= 0 && t->size[1] != cols))
-    return fail(MM_ERR_INVALID, std::string(name) + ": has the wrong shape");
-  if (t->size[0] > INT32_MAX / 2 || t->size[1] > INT32_MAX / 2)
-    return fail(MM_ERR_UNSUPPORTED, std::string(name) + ": dimension too large");
-  if (dense && t->size[1] > 1 && t->stride[1] != 1)
-    return fail(MM_ERR_UNSUPPORTED, std::string(name) + ": rows must be dense");
-  return MM_OK;
-}
-
-static int lin_output(const mm_tensor_t* t, const char* name, int64_t rows, int64_t cols) {
-  int rc = lin_matrix(t, name, rows, cols, true);
-  if (rc == MM_OK && rows > 1 && cols > 0 && t->stride[0] != cols)
-    return fail(MM_ERR_UNSUPPORTED, std::string(name) + ": must be dense");
-  return rc;
-}
-
-static int lin_vector(const mm_tensor_t* t, const char* name, int64_t n) {
-  int rc = validate(t, name, MM_F32);
-  if (rc != MM_OK) return rc;
-  if (t->ndim != 1 || t->size[0] != n) return fail(MM_ERR_INVALID, std::string(name) + ": has the wrong length");
-  if (n > 1 && t->stride[0] != 1) return fail(MM_ERR_UNSUPPORTED, std::string(name) + ": must be dense");
-  return MM_OK;
-}
+// A strided matrix of the call's arguments.
+struct LinMatrix {
+  const float* data;
+  int64_t s0, s1;
+};
 
 static int lin_product(const LinProduct& p, const LinEpilogue& e, cudaStream_t s) {
   if (p.m == 0 || p.n == 0) return MM_OK;
@@ -183,16 +162,15 @@ static LinStored lin_store(LinCarve* ws, LinSplits* all, const float* src, int64
   return st;
 }
 
-static int lin_forward_tc(const mm_tensor_t* x, const mm_tensor_t* w, const LinEpilogue& e, float* y, void* workspace,
-                          cudaStream_t s) {
-  const int64_t m = x->size[0], k = x->size[1], n = w->size[0];
+static int lin_forward_tc(const LinMatrix& x, const LinMatrix& w, int64_t m, int64_t n, int64_t k,
+                          const LinEpilogue& e, float* y, void* workspace, cudaStream_t s) {
   LinCarve ws = {(char*)workspace, 0};
   LinSplits all;
   all.count = 0;
   all.blocks = 0;
   bool xt, wt;
-  const LinStored xs = lin_store(&ws, &all, (const float*)x->data, x->stride[0], x->stride[1], m, k, &xt);
-  const LinStored wst = lin_store(&ws, &all, (const float*)w->data, w->stride[0], w->stride[1], n, k, &wt);
+  const LinStored xs = lin_store(&ws, &all, x.data, x.s0, x.s1, m, k, &xt);
+  const LinStored wst = lin_store(&ws, &all, w.data, w.s0, w.s1, n, k, &wt);
   const LinChoice c = lin_choose(m, n, k);
   float* part = (float*)ws.take(lin_part_bytes(c));
   int rc = lin_run_splits(all, s);
@@ -200,46 +178,43 @@ static int lin_forward_tc(const mm_tensor_t* x, const mm_tensor_t* w, const LinE
   return lin_run_gemm(xt ? xs.by_cols() : xs.by_rows(), wt ? wst.by_cols() : wst.by_rows(), y, e, c, part, s);
 }
 
-static int lin_backward_tc(const mm_tensor_t* dy, const mm_tensor_t* x, const mm_tensor_t* w, const mm_tensor_t* z,
-                           int act, const mm_tensor_t* dx, const mm_tensor_t* dw, const mm_tensor_t* db,
-                           const mm_tensor_t* dz, void* workspace, cudaStream_t s) {
-  const int64_t m = x->size[0], k = x->size[1], n = w->size[0];
+static int lin_backward_tc(const LinMatrix& dy, const LinMatrix& x, const LinMatrix& w, const float* z, int act,
+                           int64_t m, int64_t n, int64_t k, float* dx, float* dw, float* db, float* dz,
+                           void* workspace, cudaStream_t s) {
   LinCarve ws = {(char*)workspace, 0};
   LinSplits all;
   all.count = 0;
   all.blocks = 0;
   bool gt, xt = false, wt = false;
-  const LinStored g = lin_store(&ws, &all, (const float*)dy->data, n > 1 ? dy->stride[0] : 1, 1, m, n, &gt);
+  const LinStored g = lin_store(&ws, &all, dy.data, dy.s0, 1, m, n, &gt);
   LinSplit& gs = all.s[0];
-  gs.s0 = dy->stride[0];
   if (act != MM_LINEAR_NONE) {
-    gs.z = (const float*)z->data;
+    gs.z = z;
     gs.act = act;
-    gs.vec = gs.vec && n % 4 == 0 && (uintptr_t)gs.z % 16 == 0;
+    gs.vec = gs.vec && n % 4 == 0 && (uintptr_t)z % 16 == 0;
   }
-  gs.out = dz ? (float*)dz->data : nullptr;
+  gs.out = dz;
   if (db) gs.part = (float*)ws.take(4 * lin_part_rows(m) * n);
   LinStored wst = {}, xs = {};
-  if (dx) wst = lin_store(&ws, &all, (const float*)w->data, w->stride[0], w->stride[1], n, k, &wt);
-  if (dw) xs = lin_store(&ws, &all, (const float*)x->data, x->stride[0], x->stride[1], m, k, &xt);
+  if (dx) wst = lin_store(&ws, &all, w.data, w.s0, w.s1, n, k, &wt);
+  if (dw) xs = lin_store(&ws, &all, x.data, x.s0, x.s1, m, k, &xt);
   int rc = lin_run_splits(all, s);
   if (rc != MM_OK) return rc;
   if (db) {
-    linear_columns_kernel<<<(unsigned)((n + 31) / 32), 256, 0, s>>>(gs.part, (int)lin_part_rows(m), (int)n,
-                                                                    (float*)db->data);
+    linear_columns_kernel<<<(unsigned)((n + 31) / 32), 256, 0, s>>>(gs.part, (int)lin_part_rows(m), (int)n, db);
     MM_LAUNCH_CHECK("mm_linear_backward launch");
   }
   const LinEpilogue none = {nullptr, nullptr, nullptr, 0, MM_LINEAR_NONE, 0};
   if (dx) {
     const LinChoice c = lin_choose(m, k, n);
     float* part = (float*)ws.take(lin_part_bytes(c));
-    rc = lin_run_gemm(g.by_rows(), wt ? wst.by_rows() : wst.by_cols(), (float*)dx->data, none, c, part, s);
+    rc = lin_run_gemm(g.by_rows(), wt ? wst.by_rows() : wst.by_cols(), dx, none, c, part, s);
     if (rc != MM_OK) return rc;
   }
   if (dw) {
     const LinChoice c = lin_choose(n, k, m);
     float* part = (float*)ws.take(lin_part_bytes(c));
-    rc = lin_run_gemm(g.by_cols(), xt ? xs.by_rows() : xs.by_cols(), (float*)dw->data, none, c, part, s);
+    rc = lin_run_gemm(g.by_cols(), xt ? xs.by_rows() : xs.by_cols(), dw, none, c, part, s);
   }
   return rc;
 }
@@ -267,6 +242,18 @@ static size_t lin_workspace(int64_t m, int64_t n, int64_t k, bool backward) {
   return ws.used;
 }
 
+static int lin_check(const char* who, int64_t m, int64_t n, int64_t k, int act, const void* workspace,
+                     size_t workspace_bytes, size_t need) {
+  const std::string name(who);
+  if (m < 0 || n < 0 || k < 0) return fail(MM_ERR_INVALID, name + ": negative size");
+  if (m > INT32_MAX / 2 || n > INT32_MAX / 2 || k > INT32_MAX / 2)
+    return fail(MM_ERR_UNSUPPORTED, name + ": dimension too large");
+  if (act < MM_LINEAR_NONE || act > MM_LINEAR_GELU_TANH) return fail(MM_ERR_INVALID, name + ": unknown activation");
+  if (workspace != nullptr && (workspace_bytes < need || (uintptr_t)workspace % 256 != 0))
+    return fail(MM_ERR_INVALID, name + ": the workspace is misaligned or too small");
+  return MM_OK;
+}
+
 }  // namespace mm
 
 using namespace mm;
@@ -277,81 +264,72 @@ extern "C" int mm_linear_workspace_size(int64_t m, int64_t n, int64_t k, int bac
   return MM_OK;
 }
 
-extern "C" int mm_linear(const mm_tensor_t* x, const mm_tensor_t* w, const mm_tensor_t* bias,
-                         const mm_tensor_t* residual, int act, int residual_before_act, const mm_tensor_t* y,
-                         const mm_tensor_t* z, void* workspace, size_t workspace_bytes, void* stream) {
-  int rc;
-  if (act < MM_LINEAR_NONE || act > MM_LINEAR_GELU_TANH) return fail(MM_ERR_INVALID, "mm_linear: unknown activation");
-  if ((rc = lin_matrix(x, "mm_linear input", -1, -1, false)) != MM_OK) return rc;
-  const int64_t m = x->size[0], k = x->size[1];
-  if ((rc = lin_matrix(w, "mm_linear weight", -1, k, false)) != MM_OK) return rc;
-  const int64_t n = w->size[0];
-  if (bias && (rc = lin_vector(bias, "mm_linear bias", n)) != MM_OK) return rc;
-  if (residual && (rc = lin_matrix(residual, "mm_linear residual", m, n, true)) != MM_OK) return rc;
-  if ((rc = lin_output(y, "mm_linear output", m, n)) != MM_OK) return rc;
-  if (z && (rc = lin_output(z, "mm_linear pre-activation", m, n)) != MM_OK) return rc;
-  size_t need = 0;
-  if ((rc = mm_linear_workspace_size(m, n, k, 0, &need)) != MM_OK) return rc;
-  if (need > 0 && (workspace == nullptr || workspace_bytes < need || (uintptr_t)workspace % 256 != 0))
-    return fail(MM_ERR_INVALID, "mm_linear: the workspace is missing, misaligned or too small");
-  LinProduct p = {(const float*)x->data, (const float*)w->data, (float*)y->data, x->stride[0], x->stride[1],
-                  w->stride[0], w->stride[1], (int)m, (int)n, (int)k};
-  LinEpilogue e = {bias ? (const float*)bias->data : nullptr, residual ? (const float*)residual->data : nullptr,
-                   z ? (float*)z->data : nullptr, residual ? residual->stride[0] : 0, act, residual_before_act != 0};
-  if (lin_on_tensor_cores(m, n, k)) return lin_forward_tc(x, w, e, (float*)y->data, workspace, resolve_stream(stream));
-  return lin_product(p, e, resolve_stream(stream));
+extern "C" int mm_linear(const float* x, int64_t xs0, int64_t xs1, const float* w, int64_t ws0, int64_t ws1,
+                         const float* bias, const float* residual, int64_t residual_stride, int64_t m, int64_t n,
+                         int64_t k, int act, int residual_before_act, float* y, float* z, void* workspace,
+                         size_t workspace_bytes, void* stream) {
+  const size_t need = m < 0 || n < 0 || k < 0 ? 0 : lin_workspace(m, n, k, false);
+  int rc = lin_check("mm_linear", m, n, k, act, workspace, workspace_bytes, need);
+  if (rc != MM_OK) return rc;
+  if (xs0 < 0 || xs1 < 0 || ws0 < 0 || ws1 < 0 || residual_stride < 0)
+    return fail(MM_ERR_INVALID, "mm_linear: negative stride");
+  if (m == 0 || n == 0) return MM_OK;
+  if (!y || (k > 0 && (!x || !w))) return fail(MM_ERR_INVALID, "mm_linear: null data pointer");
+  cudaStream_t s = resolve_stream(stream);
+  const LinEpilogue e = {bias, residual, z, residual_stride, act, residual_before_act != 0};
+  if (!lin_on_tensor_cores(m, n, k))
+    return lin_product({x, w, y, xs0, xs1, ws0, ws1, (int)m, (int)n, (int)k}, e, s);
+  Scratch scratch;
+  if (workspace == nullptr) {
+    if ((rc = scratch.get(need, s)) != MM_OK) return rc;
+    workspace = scratch.data;
+  }
+  return lin_forward_tc({x, xs0, xs1}, {w, ws0, ws1}, m, n, k, e, y, workspace, s);
 }
 
-extern "C" int mm_linear_backward(const mm_tensor_t* dy, const mm_tensor_t* x, const mm_tensor_t* w,
-                                  const mm_tensor_t* z, int act, const mm_tensor_t* dx, const mm_tensor_t* dw,
-                                  const mm_tensor_t* db, const mm_tensor_t* dz, void* workspace,
+extern "C" int mm_linear_backward(const float* dy, int64_t dy_stride, const float* x, int64_t xs0, int64_t xs1,
+                                  const float* w, int64_t ws0, int64_t ws1, const float* z, int64_t m, int64_t n,
+                                  int64_t k, int act, float* dx, float* dw, float* db, float* dz, void* workspace,
                                   size_t workspace_bytes, void* stream) {
-  int rc;
-  if (act < MM_LINEAR_NONE || act > MM_LINEAR_GELU_TANH)
-    return fail(MM_ERR_INVALID, "mm_linear_backward: unknown activation");
-  if ((rc = lin_matrix(x, "mm_linear_backward input", -1, -1, false)) != MM_OK) return rc;
-  const int64_t m = x->size[0], k = x->size[1];
-  if ((rc = lin_matrix(w, "mm_linear_backward weight", -1, k, false)) != MM_OK) return rc;
-  const int64_t n = w->size[0];
-  if ((rc = lin_matrix(dy, "mm_linear_backward output gradient", m, n, true)) != MM_OK) return rc;
-  if (act != MM_LINEAR_NONE && (rc = lin_output(z, "mm_linear_backward pre-activation", m, n)) != MM_OK) return rc;
-  if (dx && (rc = lin_output(dx, "mm_linear_backward input gradient", m, k)) != MM_OK) return rc;
-  if (dw && (rc = lin_output(dw, "mm_linear_backward weight gradient", n, k)) != MM_OK) return rc;
-  if (db && (rc = lin_vector(db, "mm_linear_backward bias gradient", n)) != MM_OK) return rc;
-  if (dz && (rc = lin_output(dz, "mm_linear_backward pre-activation gradient", m, n)) != MM_OK) return rc;
-  size_t need = 0;
-  if ((rc = mm_linear_workspace_size(m, n, k, 1, &need)) != MM_OK) return rc;
-  if (need > 0 && (workspace == nullptr || workspace_bytes < need || (uintptr_t)workspace % 256 != 0))
-    return fail(MM_ERR_INVALID, "mm_linear_backward: the workspace is missing, misaligned or too small");
+  const size_t need = m < 0 || n < 0 || k < 0 ? 0 : lin_workspace(m, n, k, true);
+  int rc = lin_check("mm_linear_backward", m, n, k, act, workspace, workspace_bytes, need);
+  if (rc != MM_OK) return rc;
+  if (dy_stride < 0 || xs0 < 0 || xs1 < 0 || ws0 < 0 || ws1 < 0)
+    return fail(MM_ERR_INVALID, "mm_linear_backward: negative stride");
+  if (!dx && !dw && !db && !dz) return MM_OK;
+  if (m > 0 && n > 0 && (!dy || (act != MM_LINEAR_NONE && !z) || (k > 0 && ((dx && !w) || (dw && !x)))))
+    return fail(MM_ERR_INVALID, "mm_linear_backward: null data pointer");
   cudaStream_t s = resolve_stream(stream);
   if (m == 0 || n == 0) {
-    if (dx && m * k > 0) MM_CUDA(cudaMemsetAsync(dx->data, 0, (size_t)(m * k) * 4, s), "mm_linear_backward: zero");
-    if (dw && n * k > 0) MM_CUDA(cudaMemsetAsync(dw->data, 0, (size_t)(n * k) * 4, s), "mm_linear_backward: zero");
-    if (db && n > 0) MM_CUDA(cudaMemsetAsync(db->data, 0, (size_t)n * 4, s), "mm_linear_backward: zero");
+    if (dx && m * k > 0) MM_CUDA(cudaMemsetAsync(dx, 0, (size_t)(m * k) * 4, s), "mm_linear_backward: zero");
+    if (dw && n * k > 0) MM_CUDA(cudaMemsetAsync(dw, 0, (size_t)(n * k) * 4, s), "mm_linear_backward: zero");
+    if (db && n > 0) MM_CUDA(cudaMemsetAsync(db, 0, (size_t)n * 4, s), "mm_linear_backward: zero");
     return MM_OK;
   }
-  if (lin_on_tensor_cores(m, n, k)) return lin_backward_tc(dy, x, w, z, act, dx, dw, db, dz, workspace, s);
+  Scratch scratch;
+  if (workspace == nullptr && need > 0) {
+    if ((rc = scratch.get(need, s)) != MM_OK) return rc;
+    workspace = scratch.data;
+  }
+  if (lin_on_tensor_cores(m, n, k))
+    return lin_backward_tc({dy, dy_stride, 1}, {x, xs0, xs1}, {w, ws0, ws1}, z, act, m, n, k, dx, dw, db, dz,
+                           workspace, s);
   LinCarve ws = {(char*)workspace, 0};
   float* own = (float*)ws.take(4 * m * n);
   float* part = (float*)ws.take(4 * LIN_DZ_ROWS * n);
-  float* g = dz ? (float*)dz->data : own;
+  float* g = dz ? dz : own;
   const int rows = m < LIN_DZ_ROWS ? (int)m : LIN_DZ_ROWS;
   linear_dz_kernel<<<dim3((unsigned)((n + 255) / 256), rows), 256, 0, s>>>(
-      (const float*)dy->data, dy->stride[0], act == MM_LINEAR_NONE ? nullptr : (const float*)z->data, act, (int)m,
-      (int)n, g, part);
+      dy, dy_stride, act == MM_LINEAR_NONE ? nullptr : z, act, (int)m, (int)n, g, part);
   MM_LAUNCH_CHECK("mm_linear_backward launch");
   if (db) {
-    linear_columns_kernel<<<(unsigned)((n + 31) / 32), 256, 0, s>>>(part, rows, (int)n, (float*)db->data);
+    linear_columns_kernel<<<(unsigned)((n + 31) / 32), 256, 0, s>>>(part, rows, (int)n, db);
     MM_LAUNCH_CHECK("mm_linear_backward launch");
   }
   const LinEpilogue none = {nullptr, nullptr, nullptr, 0, MM_LINEAR_NONE, 0};
   if (dx) {
-    LinProduct p = {g, (const float*)w->data, (float*)dx->data, n, 1, w->stride[1], w->stride[0], (int)m, (int)k, (int)n};
-    if ((rc = lin_product(p, none, s)) != MM_OK) return rc;
+    rc = lin_product({g, w, dx, n, 1, ws1, ws0, (int)m, (int)k, (int)n}, none, s);
+    if (rc != MM_OK) return rc;
   }
-  if (dw) {
-    LinProduct p = {g, (const float*)x->data, (float*)dw->data, 1, n, x->stride[1], x->stride[0], (int)n, (int)k, (int)m};
-    if ((rc = lin_product(p, none, s)) != MM_OK) return rc;
-  }
-  return MM_OK;
+  return dw ? lin_product({g, x, dw, 1, n, xs1, xs0, (int)n, (int)k, (int)m}, none, s) : MM_OK;
 }

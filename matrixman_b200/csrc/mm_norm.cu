@@ -420,79 +420,44 @@ static void ln_backward_vec(const LnPlan& p, const LnArgs& a, int blocks, bool c
 }
 #undef LN_CASE
 
-// ---------------------------------------------------------------------------
-// Arguments
-// ---------------------------------------------------------------------------
-
-// A [rows, width] operand whose rows are dense.
-static int ln_matrix(const mm_tensor_t* t, const char* name, int64_t rows, int64_t width, int64_t* stride) {
-  int rc = validate(t, name, MM_F32);
-  if (rc != MM_OK) return rc;
-  if (t->ndim != 2 || t->size[0] != rows || t->size[1] != width)
-    return fail(MM_ERR_INVALID, std::string(name) + ": must be [rows, width] like x");
-  if (width > 1 && t->stride[1] != 1)
-    return fail(MM_ERR_UNSUPPORTED, std::string(name) + ": rows must be dense");
-  *stride = t->stride[0];
-  return MM_OK;
-}
-
-static int ln_dense(const mm_tensor_t* t, const char* name, int64_t n) {
-  int rc = validate(t, name, MM_F32);
-  if (rc != MM_OK) return rc;
-  if (t->ndim != 1 || t->size[0] != n) return fail(MM_ERR_INVALID, std::string(name) + ": has the wrong length");
-  if (n > 1 && t->stride[0] != 1) return fail(MM_ERR_UNSUPPORTED, std::string(name) + ": must be dense");
-  return MM_OK;
-}
-
-static int ln_output(const mm_tensor_t* t, const char* name, int64_t rows, int64_t width) {
-  int64_t stride;
-  int rc = ln_matrix(t, name, rows, width, &stride);
-  if (rc == MM_OK && rows > 1 && stride != width)
-    return fail(MM_ERR_UNSUPPORTED, std::string(name) + ": must be dense");
-  return rc;
-}
-
-static int ln_setup(const mm_tensor_t* x, const mm_tensor_t* w, const mm_tensor_t* mean, const mm_tensor_t* rstd,
-                    LnArgs* a, const char* who) {
+// Fills what both passes share; the Python layer hands over rows that are dense.
+static int ln_setup(const char* who, const float* x, int64_t xs, int64_t rows, int64_t width, const float* w,
+                    float* mean, float* rstd, LnArgs* a) {
   const std::string name(who);
-  int rc = validate(x, (name + " input").c_str(), MM_F32);
-  if (rc != MM_OK) return rc;
-  if (x->ndim != 2) return fail(MM_ERR_UNSUPPORTED, name + ": input must be [rows, width]");
-  const int64_t rows = x->size[0], width = x->size[1];
-  if (width > INT32_MAX / 2) return fail(MM_ERR_UNSUPPORTED, name + ": rows are too wide");
-  if (rows > INT32_MAX) return fail(MM_ERR_UNSUPPORTED, name + ": too many rows");
-  if ((rc = ln_matrix(x, (name + " input").c_str(), rows, width, &a->xs)) != MM_OK) return rc;
-  if (w && (rc = ln_dense(w, (name + " weight").c_str(), width)) != MM_OK) return rc;
-  if ((rc = ln_dense(mean, (name + " mean").c_str(), rows)) != MM_OK) return rc;
-  if ((rc = ln_dense(rstd, (name + " rstd").c_str(), rows)) != MM_OK) return rc;
-  a->x = (const float*)x->data;
-  a->w = w ? (const float*)w->data : nullptr;
-  a->b = a->dy = nullptr;
-  a->y = a->part = nullptr;
-  a->mean = (float*)mean->data;
-  a->rstd = (float*)rstd->data;
+  if (rows < 0 || width < 0 || xs < 0) return fail(MM_ERR_INVALID, name + ": negative size or stride");
+  if (width > INT32_MAX / 2 || rows > INT32_MAX) return fail(MM_ERR_UNSUPPORTED, name + ": too many rows or columns");
+  if (rows > 0 && width > 0 && (!x || !mean || !rstd)) return fail(MM_ERR_INVALID, name + ": null data pointer");
+  *a = {};
+  a->x = x;
+  a->w = w;
+  a->mean = mean;
+  a->rstd = rstd;
   a->rows = rows;
-  a->dys = 0;
+  a->xs = xs;
   a->width = (int)width;
-  a->eps = 0.f;
   return MM_OK;
+}
+
+// Partial rows a backward call of this size may need, whichever kernel it runs.
+static int64_t ln_partial_rows(int64_t rows) {
+  const int64_t most = (int64_t)sm_count() * LN_MAX_BLOCKS_PER_SM;
+  return rows < 1 ? 1 : rows < most ? rows : most;
 }
 
 }  // namespace mm
 
 using namespace mm;
 
-extern "C" int mm_layer_norm(const mm_tensor_t* x, const mm_tensor_t* weight, const mm_tensor_t* bias, double eps,
-                             const mm_tensor_t* y, const mm_tensor_t* mean, const mm_tensor_t* rstd, void* stream) {
+extern "C" int mm_layer_norm(const float* x, int64_t x_stride, int64_t rows, int64_t width, const float* weight,
+                             const float* bias, double eps, float* y, float* mean, float* rstd, void* stream) {
   LnArgs a;
-  int rc = ln_setup(x, weight, mean, rstd, &a, "mm_layer_norm");
+  int rc = ln_setup("mm_layer_norm", x, x_stride, rows, width, weight, mean, rstd, &a);
   if (rc != MM_OK) return rc;
-  if (bias && (rc = ln_dense(bias, "mm_layer_norm bias", a.width)) != MM_OK) return rc;
-  if ((rc = ln_output(y, "mm_layer_norm output", a.rows, a.width)) != MM_OK) return rc;
-  if (a.rows == 0) return MM_OK;
-  if (a.width == 0) return fail(MM_ERR_UNSUPPORTED, "mm_layer_norm: rows are empty");
-  a.b = bias ? (const float*)bias->data : nullptr;
-  a.y = (float*)y->data;
+  if (rows == 0) return MM_OK;
+  if (width == 0) return fail(MM_ERR_UNSUPPORTED, "mm_layer_norm: rows are empty");
+  if (!y) return fail(MM_ERR_INVALID, "mm_layer_norm: null data pointer");
+  a.b = bias;
+  a.y = y;
   a.eps = (float)eps;
   cudaStream_t s = resolve_stream(stream);
   const LnPlan p = ln_plan(a, false);
@@ -508,12 +473,6 @@ extern "C" int mm_layer_norm(const mm_tensor_t* x, const mm_tensor_t* weight, co
   return MM_OK;
 }
 
-// Partial rows a backward call of this size may need, whichever kernel it runs.
-static int64_t ln_partial_rows(int64_t rows) {
-  const int64_t most = (int64_t)sm_count() * LN_MAX_BLOCKS_PER_SM;
-  return rows < 1 ? 1 : rows < most ? rows : most;
-}
-
 extern "C" int mm_layer_norm_backward_workspace_size(int64_t rows, int64_t width, size_t* bytes) {
   if (bytes == nullptr || rows < 0 || width < 0)
     return fail(MM_ERR_INVALID, "mm_layer_norm_backward_workspace_size: invalid argument");
@@ -521,37 +480,42 @@ extern "C" int mm_layer_norm_backward_workspace_size(int64_t rows, int64_t width
   return MM_OK;
 }
 
-extern "C" int mm_layer_norm_backward(const mm_tensor_t* dy, const mm_tensor_t* x, const mm_tensor_t* mean,
-                                      const mm_tensor_t* rstd, const mm_tensor_t* weight, const mm_tensor_t* dx,
-                                      const mm_tensor_t* dweight, const mm_tensor_t* dbias, void* workspace,
+extern "C" int mm_layer_norm_backward(const float* dy, int64_t dy_stride, const float* x, int64_t x_stride,
+                                      int64_t rows, int64_t width, const float* mean, const float* rstd,
+                                      const float* weight, float* dx, float* dweight, float* dbias, void* workspace,
                                       size_t workspace_bytes, void* stream) {
   LnArgs a;
-  int rc = ln_setup(x, weight, mean, rstd, &a, "mm_layer_norm_backward");
+  int rc = ln_setup("mm_layer_norm_backward", x, x_stride, rows, width, weight, const_cast<float*>(mean),
+                    const_cast<float*>(rstd), &a);
   if (rc != MM_OK) return rc;
-  if ((rc = ln_matrix(dy, "mm_layer_norm_backward output gradient", a.rows, a.width, &a.dys)) != MM_OK) return rc;
-  if (dx && (rc = ln_output(dx, "mm_layer_norm_backward input gradient", a.rows, a.width)) != MM_OK) return rc;
-  if (dweight && (rc = ln_dense(dweight, "mm_layer_norm_backward weight gradient", a.width)) != MM_OK) return rc;
-  if (dbias && (rc = ln_dense(dbias, "mm_layer_norm_backward bias gradient", a.width)) != MM_OK) return rc;
   const bool cols = dweight != nullptr || dbias != nullptr;
-  if ((!dx && !cols) || a.width == 0) return MM_OK;
-  cudaStream_t s = resolve_stream(stream);
-  if (a.rows == 0) {
-    for (const mm_tensor_t* t : {dweight, dbias})
-      if (t) MM_CUDA(cudaMemsetAsync(t->data, 0, (size_t)a.width * sizeof(float), s), "mm_layer_norm_backward: zero");
+  if ((!dx && !cols) || width == 0) return MM_OK;
+  if (rows > 0 && (!dy || dy_stride < 0)) return fail(MM_ERR_INVALID, "mm_layer_norm_backward: invalid gradient");
+  if (rows == 0) {
+    cudaStream_t s = resolve_stream(stream);
+    for (float* t : {dweight, dbias})
+      if (t) MM_CUDA(cudaMemsetAsync(t, 0, (size_t)width * sizeof(float), s), "mm_layer_norm_backward: zero");
     return MM_OK;
   }
   size_t need = 0;
-  mm_layer_norm_backward_workspace_size(a.rows, a.width, &need);
-  if (cols && (workspace == nullptr || workspace_bytes < need || (uintptr_t)workspace % 16 != 0))
-    return fail(MM_ERR_INVALID, "mm_layer_norm_backward: the workspace is missing, misaligned or too small");
-  a.dy = (const float*)dy->data;
-  a.y = dx ? (float*)dx->data : nullptr;
+  mm_layer_norm_backward_workspace_size(rows, width, &need);
+  if (cols && workspace != nullptr && (workspace_bytes < need || (uintptr_t)workspace % 16 != 0))
+    return fail(MM_ERR_INVALID, "mm_layer_norm_backward: the workspace is misaligned or too small");
+  cudaStream_t s = resolve_stream(stream);
+  Scratch scratch;
+  if (cols && workspace == nullptr) {
+    if ((rc = scratch.get(need, s)) != MM_OK) return rc;
+    workspace = scratch.data;
+  }
+  a.dy = dy;
+  a.dys = dy_stride;
+  a.y = dx;
   a.part = (float*)workspace;
   const LnPlan p = ln_plan(a, true);
   int blocks = ln_blocks(a, p);
   if (p.group == 0) {
-    blocks = (int)ln_partial_rows(a.rows);
-    if (dx) ln_backward_wide_kernel<<<(unsigned)a.rows, 1024, 0, s>>>(a);
+    blocks = (int)ln_partial_rows(rows);
+    if (dx) ln_backward_wide_kernel<<<(unsigned)rows, 1024, 0, s>>>(a);
     if (cols) ln_columns_kernel<<<dim3((a.width + 255) / 256, blocks), 256, 0, s>>>(a);
   } else if (p.vec == 4) {
     ln_backward_vec<4>(p, a, blocks, cols, s);
@@ -562,9 +526,7 @@ extern "C" int mm_layer_norm_backward(const mm_tensor_t* dy, const mm_tensor_t* 
   }
   MM_LAUNCH_CHECK("mm_layer_norm_backward launch");
   if (cols) {
-    ln_finish_kernel<<<dim3((a.width + 31) / 32, 2), 256, 0, s>>>(a.part, blocks, a.width,
-                                                                 dweight ? (float*)dweight->data : nullptr,
-                                                                 dbias ? (float*)dbias->data : nullptr);
+    ln_finish_kernel<<<dim3((a.width + 31) / 32, 2), 256, 0, s>>>(a.part, blocks, a.width, dweight, dbias);
     MM_LAUNCH_CHECK("mm_layer_norm_backward columns launch");
   }
   return MM_OK;

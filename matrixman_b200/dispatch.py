@@ -124,7 +124,7 @@ def _copy_(dst, src, non_blocking=False):
 
 @_register(aten.detach.default, aten.alias.default, aten.lift_fresh.default)
 def _detach(x):
-    return _view(x, tuple(x.shape), x._logical_strides)
+    return MatrixManTensor._wrap(x._owner, tuple(x.shape), x._storage_offset, x._logical_strides)
 
 
 # ---------------------------------------------------------------------------

@@ -9,74 +9,69 @@ its backward pass computes the gradients of all four operands.
 
 from __future__ import annotations
 
-import ctypes
-
 import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib, ops
-from .tensor import MatrixManTensor, contiguous_strides, is_contiguous, numel, view_strides
+from .tensor import MatrixManTensor, is_contiguous, numel, view_strides
 
 ACTIVATIONS = _lib.LINEAR_ACTS
+_RELU = ACTIVATIONS["relu"]
+pointer = ops.pointer
 
 
-def _matrix(t: MatrixManTensor, name: str) -> MatrixManTensor:
-    """[..., n] as [rows, n] without a copy where the strides allow it."""
-    if t.dim() == 2:
-        return t
+def _matrix(t: MatrixManTensor) -> tuple[MatrixManTensor, int, tuple]:
+    """[..., n] as a matrix of rows: a tensor, the number of rows, and the two
+    strides; copied only where the strides force it."""
+    st = t._logical_strides
+    if len(st) == 2:
+        return t, int(t.shape[0]), st
+    shape = tuple(t.shape)
+    n = shape[-1]
+    rows = numel(shape[:-1])
+    if rows == 0 or n == 0 or is_contiguous(shape, st):
+        return t, rows, (n, 1)
+    flat = view_strides(shape, st, (rows, n))
+    if flat is not None:
+        return t, rows, flat
+    return ops.materialize(t), rows, (n, 1)
+
+
+def _dense_rows(t: MatrixManTensor) -> tuple[MatrixManTensor, int]:
+    """The same with dense rows: a tensor and the rows' distance."""
+    m, _, st = _matrix(t)
     n = int(t.shape[-1])
-    rows = numel(t.shape[:-1])
-    if rows == 0 or n == 0 or is_contiguous(t.shape, t._logical_strides):
-        return MatrixManTensor(t._owner, (rows, n), t._storage_offset, (n, 1))
-    strides = view_strides(t.shape, t._logical_strides, (rows, n))
-    if strides is None:
-        t = ops.materialize(t)
-        strides = (n, 1)
-    return MatrixManTensor(t._owner, (rows, n), t._storage_offset, strides)
-
-
-def _dense_rows(t: MatrixManTensor) -> MatrixManTensor:
-    if int(t.shape[1]) > 1 and t._logical_strides[1] != 1:
-        return ops.materialize(t)
-    return t
-
-
-def _workspace(rt, m: int, n: int, k: int, backward: bool):
-    size = ctypes.c_size_t(0)
-    _lib.call("mm_linear_workspace_size", m, n, k, 1 if backward else 0, ctypes.byref(size))
-    return rt.new_storage(size.value, torch.uint8, _lib.POOL_SCRATCH) if size.value else None, size.value
-
-
-def _ref(t):
-    return ops._p(t.desc()) if t is not None else None
+    if n > 1 and st[1] != 1:
+        return ops.materialize(t), n
+    return m, st[0]
 
 
 def _forward(x, weight, bias, residual, act: int, first: bool, keep: bool):
-    """(y, z): z is what the activation was applied to (None unless kept)."""
+    """(y, z) of the output's shape: z is what the activation was applied to
+    (None unless kept)."""
     rt = x.runtime
-    m, k = (int(v) for v in x.shape)
-    n = int(weight.shape[0])
-    y = ops.empty(rt, (m, n))
-    z = ops.empty(rt, (m, n)) if keep else None
-    work, size = _workspace(rt, m, n, k, False)
-    ops._launch("mm_linear", _ref(x), _ref(weight), _ref(bias), _ref(residual), act, 1 if first else 0, _ref(y),
-                _ref(z), ctypes.c_void_p(work.pointer) if work else None, size, rt.stream)
+    x2, m, xs = _matrix(x)
+    n, k = weight.shape
+    ws = weight._logical_strides
+    r2, rs = (None, 0) if residual is None else _dense_rows(residual)
+    shape = tuple(x.shape[:-1]) + (n,)
+    y = ops.new_dense(rt, shape)
+    z = ops.new_dense(rt, shape) if keep else None
+    ops._launch("mm_linear", pointer(x2), xs[0], xs[1], pointer(weight), ws[0], ws[1],
+                None if bias is None else pointer(bias), None if r2 is None else pointer(r2), rs, m, n, k, act,
+                first, y._owner.pointer, None if z is None else z._owner.pointer, None, 0, rt.stream)
     return y, z
 
 
 class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, act, first):
-        x2 = _matrix(x, "input")
-        r2 = _dense_rows(_matrix(residual, "residual")) if residual is not None else None
         # ReLU's slope can be read off its own output where nothing is added to it.
-        own_output = act == ACTIVATIONS["relu"] and residual is None
-        y, z = _forward(x2, weight, bias, r2, act, first, act != 0 and not own_output)
-        shape = tuple(int(v) for v in x.shape[:-1]) + (int(weight.shape[0]),)
-        out = y if x.dim() == 2 else MatrixManTensor(y._owner, shape, 0, contiguous_strides(shape))
-        ctx.act, ctx.first, ctx.own_output = act, first, own_output
-        ctx.save_for_backward(x, weight, out if own_output else z)
-        return out
+        own_output = act == _RELU and residual is None
+        y, z = _forward(x, weight, bias, residual, act, first, act != 0 and not own_output)
+        ctx.act, ctx.first = act, first
+        ctx.save_for_backward(x, weight, y if own_output else z)
+        return y
 
     @staticmethod
     @once_differentiable
@@ -85,27 +80,34 @@ class _Linear(torch.autograd.Function):
         need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
         dy = ops.require_mm(dy, "linear gradient")
         rt = dy.runtime
-        g = _dense_rows(_matrix(dy, "gradient"))
-        x2 = _matrix(x, "input")
-        m, k = (int(v) for v in x2.shape)
-        n = int(weight.shape[0])
-        want_dz = need_r and ctx.first
-        dx = ops.empty(rt, (m, k)) if need_x else None
-        dw = ops.empty(rt, (n, k)) if need_w else None
-        db = ops.empty(rt, (n,)) if need_b else None
-        dz = ops.empty(rt, (m, n)) if want_dz else None
-        if need_x or need_w or need_b or want_dz:
-            z2 = _matrix(z, "pre-activation") if z is not None else None
-            work, size = _workspace(rt, m, n, k, True)
-            ops._launch("mm_linear_backward", _ref(g), _ref(x2), _ref(weight), _ref(z2), ctx.act, _ref(dx), _ref(dw),
-                        _ref(db), _ref(dz), ctypes.c_void_p(work.pointer) if work else None, size, rt.stream)
-        if dx is not None:
-            dx = MatrixManTensor(dx._owner, tuple(x.shape), 0, contiguous_strides(tuple(x.shape)))
+        n, k = weight.shape
+        dx = ops.new_dense(rt, tuple(x.shape)) if need_x else None
+        dw = ops.new_dense(rt, (n, k)) if need_w else None
+        db = ops.new_dense(rt, (n,)) if need_b else None
+        dz = ops.new_dense(rt, tuple(dy.shape)) if need_r and ctx.first else None
+        if need_x or need_w or need_b or dz is not None:
+            g, gs = _dense_rows(dy)
+            x2, m, xs = _matrix(x)
+            ws = weight._logical_strides
+            ops._launch("mm_linear_backward", pointer(g), gs, pointer(x2), xs[0], xs[1], pointer(weight), ws[0], ws[1],
+                        None if z is None else pointer(z), m, n, k, ctx.act,
+                        *(None if t is None else t._owner.pointer for t in (dx, dw, db, dz)), None, 0, rt.stream)
         dr = None
         if need_r:
-            dr = dy if not ctx.first else MatrixManTensor(dz._owner, tuple(dy.shape), 0,
-                                                          contiguous_strides(tuple(dy.shape)))
+            dr = dz if ctx.first else dy
         return dx, dw, db, dr, None, None
+
+
+def _operand(x, t, name: str, grad: bool) -> MatrixManTensor:
+    if isinstance(t, MatrixManTensor):
+        if t.runtime is not x.runtime:
+            raise RuntimeError(f"MatrixMan/CUDA: linear {name} is on another matrixman device")
+    else:
+        if grad and isinstance(t, torch.Tensor) and t.requires_grad:
+            raise RuntimeError(f"MatrixMan/CUDA: linear {name} needs a gradient and must be a MatrixMan tensor")
+        t = ops.device_operand(x.runtime, t, f"linear {name}")
+    ops.require_f32(t, f"linear {name}")
+    return t
 
 
 def linear(x, weight, bias=None, *, activation: str | None = None, residual=None,
@@ -121,50 +123,39 @@ def linear(x, weight, bias=None, *, activation: str | None = None, residual=None
     operators) when they need no gradient."""
     x = ops.require_mm(x, "linear")
     ops.require_f32(x, "linear")
-    act = ACTIVATIONS.get("none" if activation is None else activation)
+    act = ACTIVATIONS.get(activation) if activation is not None else 0
     if act is None:
         raise ValueError(f"MatrixMan/CUDA: linear activation must be one of {sorted(ACTIVATIONS)}, "
                          f"got {activation!r}")
-    rt = x.runtime
     grad = torch.is_grad_enabled()
-    operands = []
-    for name, t in (("weight", weight), ("bias", bias)):
-        if t is not None and not isinstance(t, MatrixManTensor):
-            if grad and isinstance(t, torch.Tensor) and t.requires_grad:
-                raise RuntimeError(f"MatrixMan/CUDA: linear {name} needs a gradient and must be a MatrixMan tensor")
-            t = ops.device_operand(rt, t, f"linear {name}")
-        if t is not None:
-            ops.require_f32(t, f"linear {name}")
-        operands.append(t)
-    weight, bias = operands
-    if weight is None or weight.dim() != 2:
+    weight = _operand(x, weight, "weight", grad)
+    if bias is not None:
+        bias = _operand(x, bias, "bias", grad)
+    if weight.dim() != 2:
         raise ValueError("MatrixMan/CUDA: linear weight must be [n, k]")
-    n, k = (int(v) for v in weight.shape)
-    if x.dim() < 1 or int(x.shape[-1]) != k:
+    n, k = weight.shape
+    if x.dim() < 1 or x.shape[-1] != k:
         raise ValueError(f"MatrixMan/CUDA: linear input {tuple(x.shape)} does not end in the weight's {k}")
     if bias is not None:
         if tuple(bias.shape) != (n,):
             raise ValueError(f"MatrixMan/CUDA: linear bias must be [{n}], got {tuple(bias.shape)}")
+        if bias._logical_strides[0] != 1 and n > 1:
+            bias = bias.clone(memory_format=torch.contiguous_format)
     if residual is not None:
         residual = ops.require_mm(residual, "linear residual")
         ops.require_f32(residual, "linear residual")
         if tuple(residual.shape) != tuple(x.shape[:-1]) + (n,):
             raise ValueError("MatrixMan/CUDA: linear residual must have the output's shape "
                              f"{tuple(x.shape[:-1]) + (n,)}, got {tuple(residual.shape)}")
-    ops._runtime_of(x, weight, bias, residual)
+        if residual.runtime is not x.runtime:
+            raise RuntimeError("MatrixMan/CUDA: linear residual is on another matrixman device")
     if x.dim() == 1:
         out = linear(x.unsqueeze(0), weight, bias, activation=activation,
                      residual=None if residual is None else residual.unsqueeze(0),
                      residual_before_act=residual_before_act)
         return out.squeeze(0)
-    if bias is not None and bias._logical_strides[0] != 1 and n > 1:
-        bias = bias.contiguous() if not bias.requires_grad else bias.clone(memory_format=torch.contiguous_format)
-    if grad and any(t is not None and t.requires_grad for t in (x, weight, bias, residual)):
-        return _Linear.apply(x, weight, bias, residual, act, bool(residual_before_act))
-    x2 = _matrix(x, "input")
-    r2 = _dense_rows(_matrix(residual, "residual")) if residual is not None else None
-    y, _ = _forward(x2, weight, bias, r2, act, bool(residual_before_act), False)
-    if x.dim() == 2:
-        return y
-    shape = tuple(int(v) for v in x.shape[:-1]) + (n,)
-    return MatrixManTensor(y._owner, shape, 0, contiguous_strides(shape))
+    first = bool(residual_before_act)
+    if grad and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad) or
+                 (residual is not None and residual.requires_grad)):
+        return _Linear.apply(x, weight, bias, residual, act, first)
+    return _forward(x, weight, bias, residual, act, first, False)[0]

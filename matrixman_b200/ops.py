@@ -566,22 +566,38 @@ def batch_norm_eval(x, weight, bias, running_mean, running_var, eps) -> MatrixMa
     return y
 
 
-def _norm_matrix(x: MatrixManTensor, width: int) -> MatrixManTensor:
-    """x as [rows, width] with dense rows, copied only where its strides force it."""
-    rows = numel(x.shape) // width if width else 0
+def pointer(t: MatrixManTensor) -> int:
+    """Address of a float32 tensor's first element."""
+    return t._owner.pointer + 4 * t._storage_offset
+
+
+def new_dense(rt: DeviceRuntime, shape: tuple) -> MatrixManTensor:
+    """A new contiguous float32 tensor; shape is a tuple of ints."""
+    n = 1
+    strides = []
+    for s in reversed(shape):
+        strides.append(n)
+        n *= s if s > 1 else 1
+    owner = rt.new_storage(numel(shape))
+    return MatrixManTensor._wrap(owner, shape, 0, tuple(reversed(strides)))
+
+
+def _norm_rows(x: MatrixManTensor, shape: tuple, width: int) -> tuple[MatrixManTensor, int]:
+    """A tensor whose last dimensions are dense rows of `width`, and the rows'
+    distance; copied only where the strides force it."""
     st = x._logical_strides
-    if x.dim() == 2 and int(x.shape[1]) == width and (st[1] == 1 or width == 1):
-        return x
+    if len(st) == 2 and len(shape) == 1 and (st[1] == 1 or width == 1):
+        return x, st[0]
     if not is_contiguous(x.shape, st):
-        flat = view_strides(x.shape, st, (rows, width))
+        flat = view_strides(x.shape, st, (numel(x.shape) // width, width))
         if flat is not None and (flat[1] == 1 or width == 1):
-            return MatrixManTensor(x._owner, (rows, width), x._storage_offset, flat)
+            return x, flat[0]
         x = materialize(x)
-    return MatrixManTensor(x._owner, (rows, width), x._storage_offset, (width, 1))
+    return x, width
 
 
 def _norm_vector(rt, value, shape, name: str) -> MatrixManTensor | None:
-    """An affine parameter as a dense vector."""
+    """An affine parameter whose elements are dense."""
     if value is None:
         return None
     t = device_operand(rt, value, f"LayerNorm {name}")
@@ -589,14 +605,12 @@ def _norm_vector(rt, value, shape, name: str) -> MatrixManTensor | None:
     if tuple(t.shape) != shape:
         raise RuntimeError(f"MatrixMan/CUDA: LayerNorm {name} must have the normalized shape {shape}, "
                            f"got {tuple(t.shape)}")
-    if not is_contiguous(t.shape, t._logical_strides):
-        t = materialize(t)
-    return MatrixManTensor(t._owner, (numel(shape),), t._storage_offset, (1,))
+    return t if is_contiguous(shape, t._logical_strides) else materialize(t)
 
 
 def _norm_shape(x: MatrixManTensor, normalized_shape) -> tuple[int, ...]:
-    shape = tuple(int(v) for v in normalized_shape)
-    if not shape or tuple(int(v) for v in x.shape[-len(shape):]) != shape:
+    shape = tuple(normalized_shape)
+    if not shape or tuple(x.shape[-len(shape):]) != shape:
         raise RuntimeError(f"MatrixMan/CUDA: LayerNorm input {tuple(x.shape)} does not end in the normalized "
                            f"shape {shape}")
     if numel(shape) == 0:
@@ -610,61 +624,55 @@ def layer_norm(x, normalized_shape, weight=None, bias=None, eps=1e-5):
     x = require_mm(x, "LayerNorm")
     require_f32(x, "LayerNorm")
     shape = _norm_shape(x, normalized_shape)
+    width = numel(shape)
     rt = x.runtime
     w = _norm_vector(rt, weight, shape, "weight")
     b = _norm_vector(rt, bias, shape, "bias")
-    x2 = _norm_matrix(x, numel(shape))
-    rows = int(x2.shape[0])
-    lead = tuple(int(v) for v in x.shape[:x.dim() - len(shape)])
-    y = empty(rt, tuple(x.shape))
-    mean, rstd = empty(rt, (rows,)), empty(rt, (rows,))
-    y2 = MatrixManTensor(y._owner, (rows, numel(shape)), 0, (numel(shape), 1))
-    _launch("mm_layer_norm", _p(x2.desc()), _p(w.desc()) if w is not None else None,
-            _p(b.desc()) if b is not None else None, float(eps), _p(y2.desc()), _p(mean.desc()), _p(rstd.desc()),
-            rt.stream)
+    full = tuple(x.shape)
+    lead = full[:len(full) - len(shape)]
+    rows = numel(lead)
+    xr, stride = _norm_rows(x, shape, width)
+    y = new_dense(rt, full)
     stat = lead + (1,) * len(shape)
-    return y, *(MatrixManTensor(t._owner, stat, 0, contiguous_strides(stat)) for t in (mean, rstd))
+    strides = contiguous_strides(stat)
+    stats = rt.new_storage(2 * rows)  # mean, then rstd
+    mean, rstd = (MatrixManTensor._wrap(stats, stat, at, strides) for at in (0, rows))
+    _launch("mm_layer_norm", pointer(xr), stride, rows, width, None if w is None else pointer(w),
+            None if b is None else pointer(b), eps, y._owner.pointer, stats.pointer, stats.pointer + 4 * rows, rt.stream)
+    return y, mean, rstd
 
 
 def layer_norm_backward(dy, x, normalized_shape, mean, rstd, weight, bias, mask):
     """(dx, dweight, dbias) of native_layer_norm_backward; None where the mask is false."""
-    x = require_mm(x, "LayerNorm backward")
-    for t in (dy, mean, rstd):
-        require_mm(t, "LayerNorm backward")
     for t in (dy, x, mean, rstd):
-        require_f32(t, "LayerNorm backward")
+        require_f32(require_mm(t, "LayerNorm backward"), "LayerNorm backward")
     shape = _norm_shape(x, normalized_shape)
     if tuple(dy.shape) != tuple(x.shape):
         raise RuntimeError("MatrixMan/CUDA: LayerNorm backward needs equal shapes of gradient and input")
     rt = _runtime_of(dy, x, mean, rstd)
-    need_x, need_w, need_b = (bool(v) for v in mask)
+    need_x, need_w, need_b = mask
     if (need_w and not isinstance(weight, MatrixManTensor)) or (need_b and not isinstance(bias, MatrixManTensor)):
         raise RuntimeError("MatrixMan/CUDA: LayerNorm parameters that need a gradient must be MatrixMan tensors")
     width = numel(shape)
     w = _norm_vector(rt, weight, shape, "weight")
-    x2, g2 = _norm_matrix(x, width), _norm_matrix(dy, width)
-    rows = int(x2.shape[0])
-    stats = []
-    for t in (mean, rstd):
-        if numel(t.shape) != rows:
-            raise RuntimeError("MatrixMan/CUDA: LayerNorm backward statistics do not match the input's rows")
-        if not is_contiguous(t.shape, t._logical_strides):
-            t = materialize(t)
-        stats.append(MatrixManTensor(t._owner, (rows,), t._storage_offset, (1,)))
-    dx = empty(rt, tuple(x.shape)) if need_x else None
-    dw = empty(rt, shape) if need_w else None
-    db = empty(rt, shape) if need_b else None
-    work, size = None, ctypes.c_size_t(0)
+    full = tuple(x.shape)
+    rows = numel(full) // width
+    xr, xs = _norm_rows(x, shape, width)
+    gr, gs = _norm_rows(dy, shape, width)
+    if numel(mean.shape) != rows or numel(rstd.shape) != rows:
+        raise RuntimeError("MatrixMan/CUDA: LayerNorm backward statistics do not match the input's rows")
+    mean, rstd = (t if is_contiguous(t.shape, t._logical_strides) else materialize(t) for t in (mean, rstd))
+    dx = new_dense(rt, full) if need_x else None
+    dw = db = None
     if need_w or need_b:
-        _lib.call("mm_layer_norm_backward_workspace_size", rows, width, ctypes.byref(size))
-        work = rt.new_storage(size.value, torch.uint8, _lib.POOL_SCRATCH)
-
-    def flat(t, dims):
-        return _p(MatrixManTensor(t._owner, dims, 0, contiguous_strides(dims)).desc()) if t is not None else None
-
-    _launch("mm_layer_norm_backward", _p(g2.desc()), _p(x2.desc()), _p(stats[0].desc()), _p(stats[1].desc()),
-            _p(w.desc()) if w is not None else None, flat(dx, (rows, width)), flat(dw, (width,)), flat(db, (width,)),
-            ctypes.c_void_p(work.pointer) if work is not None else None, size.value, rt.stream)
+        each = (width + 63) // 64 * 64  # both start at a 256-byte boundary of one block
+        owner = rt.new_storage(2 * each)
+        strides = contiguous_strides(shape)
+        dw = MatrixManTensor._wrap(owner, shape, 0, strides) if need_w else None
+        db = MatrixManTensor._wrap(owner, shape, each, strides) if need_b else None
+    _launch("mm_layer_norm_backward", pointer(gr), gs, pointer(xr), xs, rows, width, pointer(mean), pointer(rstd),
+            None if w is None else pointer(w), *(None if t is None else pointer(t) for t in (dx, dw, db)), None, 0,
+            rt.stream)
     return dx, dw, db
 
 

@@ -9,7 +9,6 @@ The reference steps Adam through element-wise operators, tensor by tensor
 from __future__ import annotations
 
 import array
-import ctypes
 
 import torch
 
@@ -17,11 +16,10 @@ from . import _lib, ops
 from .tensor import MatrixManTensor, contiguous_strides, is_dense, numel
 
 BLOCK = 256  # elements that share a scale of the 8-bit states
+_CODES = ("exp_avg_code", "exp_avg_scale", "exp_avg_sq_code", "exp_avg_sq_scale")
 
 
-def _pointer(t: MatrixManTensor) -> int:
-    """Address of a float32 tensor's first element."""
-    return t._owner.pointer + 4 * t._storage_offset
+_pointer = ops.pointer
 
 
 def _check_storage(t, name: str) -> MatrixManTensor:
@@ -49,15 +47,9 @@ def run_adamw(rt, rows: list, state_bits: int, *, lr: float, beta1: float, beta2
     out as mm_adamw_tensor_t."""
     if not rows:
         return
-    table = array.array("q")
-    for row in rows:
-        table.extend(row)
-    size = ctypes.c_size_t(0)
-    _lib.call("mm_adamw_workspace_size", len(rows), ctypes.byref(size))
-    work = rt.new_storage(size.value, torch.uint8, _lib.POOL_SCRATCH)
-    ops._launch("mm_adamw", ctypes.c_void_p(table.buffer_info()[0]), len(rows), state_bits, lr, beta1, beta2, eps,
-                weight_decay, 1 if decoupled else 0, 1 if maximize else 0, 1 if advance else 0,
-                ctypes.c_void_p(work.pointer), size.value, rt.stream)
+    table = array.array("q", [v for row in rows for v in row])
+    ops._launch("mm_adamw", table.buffer_info()[0], len(rows), state_bits, lr, beta1, beta2, eps, weight_decay,
+                decoupled, maximize, advance, None, 0, rt.stream)
 
 
 class AdamW(torch.optim.Optimizer):
@@ -191,12 +183,9 @@ class AdamW(torch.optim.Optimizer):
         state = self._state_of(p)
         if self.state_bits == 32:
             return ops.clone(state["exp_avg"]), ops.clone(state["exp_avg_sq"])
-        m = ops.empty(p.runtime, p.shape, p._logical_strides)
-        v = ops.empty(p.runtime, p.shape, p._logical_strides)
-        pointers = [ctypes.c_void_p(_pointer(state[k])) for k in ("exp_avg_code", "exp_avg_scale", "exp_avg_sq_code",
-                                                                  "exp_avg_sq_scale")]
-        ops._launch("mm_adamw_decode", *pointers, numel(p.shape), ctypes.c_void_p(_pointer(m)),
-                    ctypes.c_void_p(_pointer(v)), p.runtime.stream)
+        rt, n, shape = p.runtime, numel(p.shape), tuple(p.shape)
+        m, v = (MatrixManTensor._wrap(rt.new_storage(n), shape, 0, p._logical_strides) for _ in range(2))
+        ops._launch("mm_adamw_decode", *(_pointer(state[k]) for k in _CODES), n, _pointer(m), _pointer(v), rt.stream)
         return m, v
 
     @torch.no_grad()
@@ -222,10 +211,8 @@ class AdamW(torch.optim.Optimizer):
                 ops.copy_into(t, state[name])
         else:
             m, v = (_in_order(t, p) for t in given)
-            pointers = [ctypes.c_void_p(_pointer(state[k])) for k in ("exp_avg_code", "exp_avg_scale",
-                                                                      "exp_avg_sq_code", "exp_avg_sq_scale")]
-            ops._launch("mm_adamw_encode", ctypes.c_void_p(_pointer(m)), ctypes.c_void_p(_pointer(v)),
-                        numel(p.shape), *pointers, rt.stream)
+            ops._launch("mm_adamw_encode", _pointer(m), _pointer(v), numel(p.shape),
+                        *(_pointer(state[k]) for k in _CODES), rt.stream)
         if step is not None:
             ops.fill_(state["step"], float(step))
 

@@ -244,6 +244,18 @@ class MatrixManTensor(torch.Tensor):
             logical_strides if logical_strides is not None else contiguous_strides(shape)))
 
     @staticmethod
+    def _wrap(owner, shape, storage_offset, strides):
+        """A view whose shape and strides are tuples of ints known to lie inside
+        the owner's storage (no conversion, no check: a third of the cost)."""
+        t = torch.Tensor._make_wrapper_subclass(
+            MatrixManTensor, shape, strides=strides, storage_offset=storage_offset, dtype=owner.dtype,
+            layout=torch.strided, device=device_for(owner.device_index), requires_grad=False)
+        t._owner = owner
+        t._storage_offset = storage_offset
+        t._logical_strides = strides
+        return t
+
+    @staticmethod
     def _from_owner(owner, shape, storage_offset=0, logical_strides=None):
         shape = tuple(int(s) for s in shape)
         strides = tuple(int(s) for s in (logical_strides if logical_strides is not None

@@ -9,36 +9,22 @@ from matrixman_b200 import _lib
 FAKE = 1 << 20
 
 
-def t(shape, strides=None, dtype=_lib.MM_F32, ptr=FAKE):
-    if strides is None:
-        strides, acc = [], 1
-        for s in reversed(shape):
-            strides.insert(0, acc)
-            acc *= s
-    return ctypes.byref(_lib.make_tensor(ptr, shape, strides, dtype))
-
-
 def test_layer_norm_checks():
     f = _lib.load().mm_layer_norm
-    ok = dict(x=t((4, 8)), w=t((8,)), b=t((8,)), y=t((4, 8)), mean=t((4,)), rstd=t((4,)))
+    ok = dict(x=FAKE, xs=8, rows=4, width=8, w=FAKE, b=FAKE, y=FAKE, mean=FAKE, rstd=FAKE)
 
     def call(**kw):
         a = {**ok, **kw}
-        return f(a["x"], a["w"], a["b"], 1e-5, a["y"], a["mean"], a["rstd"], None)
+        return f(a["x"], a["xs"], a["rows"], a["width"], a["w"], a["b"], 1e-5, a["y"], a["mean"], a["rstd"], None)
 
-    assert call(x=t((4, 8, 2))) == _lib.MM_ERR_UNSUPPORTED
-    assert call(x=t((4, 8), dtype=_lib.MM_I64)) == _lib.MM_ERR_UNSUPPORTED
-    assert call(x=t((4, 8), (1, 4))) == _lib.MM_ERR_UNSUPPORTED
-    assert call(x=t((4, 8), ptr=0)) == _lib.MM_ERR_INVALID
-    assert call(w=t((7,))) == _lib.MM_ERR_INVALID
-    assert call(w=t((8,), (2,))) == _lib.MM_ERR_UNSUPPORTED
-    assert call(b=t((9,))) == _lib.MM_ERR_INVALID
-    assert call(y=t((4, 9))) == _lib.MM_ERR_INVALID
-    assert call(y=t((4, 8), (16, 1))) == _lib.MM_ERR_UNSUPPORTED
-    assert call(mean=t((5,))) == _lib.MM_ERR_INVALID
-    assert call(x=None) == _lib.MM_ERR_INVALID
-    assert call(x=t((0, 8)), y=t((0, 8)), mean=t((0,)), rstd=t((0,))) == _lib.MM_OK
-    assert call(x=t((4, 0)), w=None, b=None, y=t((4, 0))) == _lib.MM_ERR_UNSUPPORTED
+    for name in ("x", "y", "mean", "rstd"):
+        assert call(**{name: None}) == _lib.MM_ERR_INVALID
+    for name in ("xs", "rows", "width"):
+        assert call(**{name: -1}) == _lib.MM_ERR_INVALID
+    assert call(rows=1 << 31) == _lib.MM_ERR_UNSUPPORTED
+    assert call(width=1 << 31) == _lib.MM_ERR_UNSUPPORTED
+    assert call(width=0) == _lib.MM_ERR_UNSUPPORTED
+    assert call(rows=0) == _lib.MM_OK
 
 
 def test_layer_norm_backward_checks():
@@ -47,18 +33,18 @@ def test_layer_norm_backward_checks():
     assert _lib.load().mm_layer_norm_backward_workspace_size(4, 8, ctypes.byref(size)) == _lib.MM_OK
     assert size.value == 2 * 4 * 8 * 4
     assert _lib.load().mm_layer_norm_backward_workspace_size(-1, 8, ctypes.byref(size)) == _lib.MM_ERR_INVALID
-    ok = dict(dy=t((4, 8)), x=t((4, 8)), mean=t((4,)), rstd=t((4,)), w=t((8,)), dx=t((4, 8)), dw=t((8,)), db=t((8,)),
+    ok = dict(dy=FAKE, dys=8, x=FAKE, xs=8, rows=4, width=8, mean=FAKE, rstd=FAKE, dx=FAKE, dw=FAKE, db=FAKE,
               work=FAKE, n=1 << 16)
 
     def call(**kw):
         a = {**ok, **kw}
-        return f(a["dy"], a["x"], a["mean"], a["rstd"], a["w"], a["dx"], a["dw"], a["db"], a["work"], a["n"], None)
+        return f(a["dy"], a["dys"], a["x"], a["xs"], a["rows"], a["width"], a["mean"], a["rstd"], FAKE, a["dx"],
+                 a["dw"], a["db"], a["work"], a["n"], None)
 
-    assert call(dy=t((3, 8))) == _lib.MM_ERR_INVALID
-    assert call(dx=t((4, 7))) == _lib.MM_ERR_INVALID
-    assert call(dw=t((9,))) == _lib.MM_ERR_INVALID
-    assert call(db=t((8,), (3,))) == _lib.MM_ERR_UNSUPPORTED
-    assert call(work=None) == _lib.MM_ERR_INVALID
+    for name in ("dy", "x", "mean", "rstd"):
+        assert call(**{name: None}) == _lib.MM_ERR_INVALID
+    for name in ("dys", "xs", "rows", "width"):
+        assert call(**{name: -1}) == _lib.MM_ERR_INVALID
     assert call(n=16) == _lib.MM_ERR_INVALID
     assert call(work=FAKE + 4) == _lib.MM_ERR_INVALID
     assert call(dx=None, dw=None, db=None) == _lib.MM_OK
@@ -67,39 +53,40 @@ def test_layer_norm_backward_checks():
 def test_linear_checks():
     lib = _lib.load()
     big = 1 << 30
-    ok = dict(x=t((4, 8)), w=t((6, 8)), b=t((6,)), r=t((4, 6)), act=0, y=t((4, 6)), z=None, work=FAKE, n=big)
+    ok = dict(x=FAKE, xs0=8, xs1=1, w=FAKE, ws0=8, ws1=1, rs=6, m=4, n=6, k=8, act=0, y=FAKE, work=FAKE, size=big)
 
     def call(**kw):
         a = {**ok, **kw}
-        return lib.mm_linear(a["x"], a["w"], a["b"], a["r"], a["act"], 0, a["y"], a["z"], a["work"], a["n"], None)
+        return lib.mm_linear(a["x"], a["xs0"], a["xs1"], a["w"], a["ws0"], a["ws1"], FAKE, FAKE, a["rs"], a["m"],
+                             a["n"], a["k"], a["act"], 0, a["y"], None, a["work"], a["size"], None)
 
     assert call(act=6) == _lib.MM_ERR_INVALID and call(act=-1) == _lib.MM_ERR_INVALID
-    assert call(w=t((6, 9))) == _lib.MM_ERR_INVALID
-    assert call(b=t((5,))) == _lib.MM_ERR_INVALID
-    assert call(r=t((4, 7))) == _lib.MM_ERR_INVALID
-    assert call(r=t((4, 6), (1, 4))) == _lib.MM_ERR_UNSUPPORTED
-    assert call(y=t((4, 6), (12, 1))) == _lib.MM_ERR_UNSUPPORTED
-    assert call(z=t((4, 5))) == _lib.MM_ERR_INVALID
-    assert call(x=t((1 << 31, 8))) == _lib.MM_ERR_UNSUPPORTED
-    assert call(x=t((4, 8), dtype=_lib.MM_I64)) == _lib.MM_ERR_UNSUPPORTED
+    for name in ("m", "n", "k", "xs0", "xs1", "ws0", "ws1", "rs"):
+        assert call(**{name: -1}) == _lib.MM_ERR_INVALID
+    for name in ("x", "w", "y"):
+        assert call(**{name: None}) == _lib.MM_ERR_INVALID
+    assert call(m=1 << 31) == _lib.MM_ERR_UNSUPPORTED
+    assert call(work=FAKE + 4) == _lib.MM_ERR_INVALID
+    assert call(m=512, n=512, k=512, size=8) == _lib.MM_ERR_INVALID
+    assert call(m=0) == _lib.MM_OK and call(n=0) == _lib.MM_OK
 
-    ok = dict(dy=t((4, 6)), x=t((4, 8)), w=t((6, 8)), z=t((4, 6)), act=4, dx=t((4, 8)), dw=t((6, 8)), db=t((6,)),
-              dz=None, work=FAKE, n=big)
+    ok = dict(dy=FAKE, dys=6, x=FAKE, xs0=8, xs1=1, w=FAKE, ws0=8, ws1=1, z=FAKE, m=4, n=6, k=8, act=4, dx=FAKE,
+              dw=FAKE, db=FAKE, dz=None, work=FAKE, size=big)
 
     def back(**kw):
         a = {**ok, **kw}
-        return lib.mm_linear_backward(a["dy"], a["x"], a["w"], a["z"], a["act"], a["dx"], a["dw"], a["db"], a["dz"],
-                                      a["work"], a["n"], None)
+        return lib.mm_linear_backward(a["dy"], a["dys"], a["x"], a["xs0"], a["xs1"], a["w"], a["ws0"], a["ws1"],
+                                      a["z"], a["m"], a["n"], a["k"], a["act"], a["dx"], a["dw"], a["db"], a["dz"],
+                                      a["work"], a["size"], None)
 
-    assert back(z=None) == _lib.MM_ERR_INVALID
-    assert back(dy=t((4, 5))) == _lib.MM_ERR_INVALID
-    assert back(dx=t((4, 9))) == _lib.MM_ERR_INVALID
-    assert back(dw=t((8, 6))) == _lib.MM_ERR_INVALID
-    assert back(db=t((7,))) == _lib.MM_ERR_INVALID
-    assert back(dz=t((4, 7))) == _lib.MM_ERR_INVALID
-    assert back(work=None) == _lib.MM_ERR_INVALID
-    assert back(n=8) == _lib.MM_ERR_INVALID
+    for name in ("dy", "x", "w", "z"):
+        assert back(**{name: None}) == _lib.MM_ERR_INVALID
+    for name in ("m", "n", "k", "dys", "xs0", "xs1", "ws0", "ws1"):
+        assert back(**{name: -1}) == _lib.MM_ERR_INVALID
+    assert back(size=8) == _lib.MM_ERR_INVALID
+    assert back(work=FAKE + 8) == _lib.MM_ERR_INVALID
     assert back(act=9) == _lib.MM_ERR_INVALID
+    assert back(dx=None, dw=None, db=None) == _lib.MM_OK
 
 
 def test_adamw_checks():
@@ -112,7 +99,7 @@ def test_adamw_checks():
     assert call(bits=16) == _lib.MM_ERR_UNSUPPORTED
     assert call(b1=1.0) == _lib.MM_ERR_INVALID and call(b2=-0.1) == _lib.MM_ERR_INVALID
     assert call(count=-1) == _lib.MM_ERR_INVALID and call(tensors=None) == _lib.MM_ERR_INVALID
-    assert call(work=None) == _lib.MM_ERR_INVALID and call(n=7) == _lib.MM_ERR_INVALID
+    assert call(work=FAKE + 4) == _lib.MM_ERR_INVALID and call(n=7) == _lib.MM_ERR_INVALID
     assert call(count=0) == _lib.MM_OK
     for i in (0, 1, 2, 3, 6):
         bad = (ctypes.c_int64 * 8)(*row)
