@@ -21,49 +21,189 @@ struct LinProduct {
   int m, n, k;
 };
 
-constexpr int LS_T = 64, LS_K = 16, LS_PAD = 4;
+// ---------------------------------------------------------------------------
+// Small products: 32 x 32 outputs per block, the reduction in chunks of 64
+// shared by eight warps (each takes eight of a chunk), whose sums are added in
+// order at the end.  A lane holds 4 x 8 outputs and reads its lines of A and B
+// in 16-byte pieces along the reduction: 12 such reads feed 128 multiply-adds.
+// Used where a product is so small that latency bounds it: many blocks with a
+// short walk each, one launch, no workspace.
+// ---------------------------------------------------------------------------
 
-// 64 x 64 outputs per block, 4 x 4 per thread, 16 of k at a time through
-// shared memory.
-__global__ void __launch_bounds__(256) linear_simt_kernel(LinProduct p, LinEpilogue e) {
-  __shared__ float as[LS_K][LS_T + LS_PAD], bs[LS_K][LS_T + LS_PAD];
-  const int m0 = blockIdx.y * LS_T, n0 = blockIdx.x * LS_T;
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  float acc[4][4] = {};
-  // Neighbouring threads load along whichever direction is dense.
-  const bool ak = p.as1 <= p.as0, bk = p.bs1 <= p.bs0;
-  for (int k0 = 0; k0 < p.k; k0 += LS_K) {
+constexpr int LS_T = 32, LS_K = 64, LS_ROW = LS_K + 4;  // + 4: 16-byte reads of neighbouring lines hit other banks
+
+// How an operand's tile is read: 16 bytes along the reduction, along the lines,
+// or value by value.
+enum { LS_ALONG_K = 0, LS_ALONG_LINES = 1, LS_SINGLE = 2 };
+
+// The eight values of a 32 x 64 tile that a thread brings in.
+__device__ __forceinline__ void ls_fetch(const float* p, int64_t s0, int64_t s1, int lines, int k, int l0, int k0,
+                                         int mode, float (&v)[8]) {
+  const int t = threadIdx.x;
 #pragma unroll
-    for (int i = 0; i < LS_T * LS_K / 256; ++i) {
-      const int at = i * 256 + threadIdx.x;
-      const int ar = ak ? at / LS_K : at % LS_T, ac = ak ? at % LS_K : at / LS_T;
-      const int br = bk ? at / LS_K : at % LS_T, bc = bk ? at % LS_K : at / LS_T;
-      as[ac][ar] = m0 + ar < p.m && k0 + ac < p.k ? p.a[(m0 + ar) * p.as0 + (k0 + ac) * p.as1] : 0.f;
-      bs[bc][br] = n0 + br < p.n && k0 + bc < p.k ? p.b[(n0 + br) * p.bs0 + (k0 + bc) * p.bs1] : 0.f;
-    }
-    __syncthreads();
+  for (int i = 0; i < 2; ++i) {
+    const int line = mode == LS_ALONG_LINES ? (t & 7) * 4 : i * 16 + (t >> 4);
+    const int kk = mode == LS_ALONG_LINES ? i * 32 + (t >> 3) : (t & 15) * 4;
+    const int l = l0 + line, kg = k0 + kk;
+    if (mode == LS_ALONG_K && l < lines && kg + 4 <= k) {
+      const float4 q = *reinterpret_cast<const float4*>(p + l * s0 + kg);
+      v[4 * i] = q.x; v[4 * i + 1] = q.y; v[4 * i + 2] = q.z; v[4 * i + 3] = q.w;
+    } else if (mode == LS_ALONG_LINES && l + 4 <= lines && kg < k) {
+      const float4 q = *reinterpret_cast<const float4*>(p + kg * s1 + l);
+      v[4 * i] = q.x; v[4 * i + 1] = q.y; v[4 * i + 2] = q.z; v[4 * i + 3] = q.w;
+    } else {
 #pragma unroll
-    for (int kk = 0; kk < LS_K; ++kk) {
-      float av[4], bv[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        av[i] = as[kk][ty * 4 + i];
-        bv[i] = bs[kk][tx * 4 + i];
+      for (int e = 0; e < 4; ++e) {
+        const int le = mode == LS_ALONG_LINES ? l + e : l, ke = mode == LS_ALONG_LINES ? kg : kg + e;
+        v[4 * i + e] = le < lines && ke < k ? p[le * s0 + ke * s1] : 0.f;
       }
+    }
+  }
+}
+
+__device__ __forceinline__ void ls_put(float* tile, int mode, const float (&v)[8]) {
+  const int t = threadIdx.x;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    if (mode == LS_ALONG_LINES) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) tile[((t & 7) * 4 + e) * LS_ROW + i * 32 + (t >> 3)] = v[4 * i + e];
+    } else {
+      *reinterpret_cast<float4*>(tile + (i * 16 + (t >> 4)) * LS_ROW + (t & 15) * 4) =
+          make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+    }
+  }
+}
+
+__global__ void __launch_bounds__(256) linear_small_kernel(LinProduct p, LinEpilogue e, int tiles_n, int amode,
+                                                           int bmode, int vec) {
+  __shared__ float4 mem[2 * 2 * LS_T * LS_ROW / 4];
+  float* tiles = reinterpret_cast<float*>(mem);
+  const int m0 = (int)(blockIdx.x / tiles_n) * LS_T, n0 = (int)(blockIdx.x % tiles_n) * LS_T;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int ga = lane >> 2, gb = lane & 3;  // A lines 4 ga + i, B lines gb + 4 j
+  float acc[4][8] = {};
+  float av[8], bv[8];
+  pdl_wait();
+  ls_fetch(p.a, p.as0, p.as1, p.m, p.k, m0, 0, amode, av);
+  ls_fetch(p.b, p.bs0, p.bs1, p.n, p.k, n0, 0, bmode, bv);
+  int buf = 0;
+  for (int k0 = 0; k0 < p.k; k0 += LS_K, buf ^= 1) {
+    float* ta = tiles + buf * 2 * LS_T * LS_ROW;
+    float* tb = ta + LS_T * LS_ROW;
+    ls_put(ta, amode, av);
+    ls_put(tb, bmode, bv);
+    __syncthreads();  // also: every warp has finished with this buffer's last chunk
+    if (k0 + LS_K < p.k) {
+      ls_fetch(p.a, p.as0, p.as1, p.m, p.k, m0, k0 + LS_K, amode, av);
+      ls_fetch(p.b, p.bs0, p.bs1, p.n, p.k, n0, k0 + LS_K, bmode, bv);
+    }
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      const int kk = warp * 8 + q * 4;
+      float4 a[4], b[8];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) a[i] = *reinterpret_cast<const float4*>(ta + (ga * 4 + i) * LS_ROW + kk);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) b[j] = *reinterpret_cast<const float4*>(tb + (gb + 4 * j) * LS_ROW + kk);
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] += av[i] * bv[j];
+        for (int j = 0; j < 8; ++j) {
+          acc[i][j] += a[i].x * b[j].x;
+          acc[i][j] += a[i].y * b[j].y;
+          acc[i][j] += a[i].z * b[j].z;
+          acc[i][j] += a[i].w * b[j].w;
+        }
     }
-    __syncthreads();
   }
+  __syncthreads();
+  // The warps' sums, [8][32][33] floats, fit where the tiles were.
+  float* red = tiles;
 #pragma unroll
   for (int i = 0; i < 4; ++i)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int row = m0 + ty * 4 + i, col = n0 + tx * 4 + j;
-      if (row < p.m && col < p.n) p.c[(int64_t)row * p.n + col] = lin_finish(e, acc[i][j], row, col, p.n);
+    for (int j = 0; j < 8; ++j) red[(warp * LS_T + ga * 4 + i) * 33 + gb + 4 * j] = acc[i][j];
+  __syncthreads();
+  const int r = threadIdx.x >> 3, c = (threadIdx.x & 7) * 4;
+  const int row = m0 + r, col = n0 + c;
+  if (row >= p.m || col >= p.n) return;
+  float v[4] = {};
+#pragma unroll
+  for (int w = 0; w < 8; ++w)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] += red[(w * LS_T + r) * 33 + c + j];
+  lin_finish_row<4>(e, v, p.c, row, col, p.n, vec);
+}
+
+// ---------------------------------------------------------------------------
+// A few rows (tokens) times a weight with dense rows: bound by reading the
+// weight once.  A group of KW warps computes CN columns for MT rows, each warp
+// every KW-th piece of the reduction, 32 lanes x VEC values at a time.
+// ---------------------------------------------------------------------------
+
+template <int MT, int CN, int VEC>
+__global__ void __launch_bounds__(256) linear_tokens_kernel(LinProduct p, LinEpilogue e, int kw) {
+  __shared__ float red[8][MT * CN];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int part = warp % kw;
+  const int n0 = (int)(blockIdx.x * (8 / kw) + warp / kw) * CN;
+  const int m0 = blockIdx.y * MT;
+  float acc[MT][CN] = {};
+  pdl_wait();
+  const float* wp[CN];
+#pragma unroll
+  for (int j = 0; j < CN; ++j) wp[j] = p.b + (int64_t)min(n0 + j, p.n - 1) * p.bs0;
+  const float* xp[MT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i) xp[i] = p.a + (int64_t)min(m0 + i, p.m - 1) * p.as0;
+  const int step = 32 * VEC * kw;
+#pragma unroll 4
+  for (int k = (part * 32 + lane) * VEC; k < p.k; k += step) {
+    float w[CN][VEC], x[MT][VEC];
+#pragma unroll
+    for (int j = 0; j < CN; ++j) {
+      if (VEC == 4) {
+        const float4 t = __ldcs(reinterpret_cast<const float4*>(wp[j] + k));
+        w[j][0] = t.x; w[j][VEC > 1 ? 1 : 0] = t.y; w[j][VEC > 2 ? 2 : 0] = t.z; w[j][VEC > 3 ? 3 : 0] = t.w;
+      } else {
+        w[j][0] = __ldcs(wp[j] + k);
+      }
     }
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      if (VEC == 4) {
+        const float4 t = *reinterpret_cast<const float4*>(xp[i] + k);
+        x[i][0] = t.x; x[i][VEC > 1 ? 1 : 0] = t.y; x[i][VEC > 2 ? 2 : 0] = t.z; x[i][VEC > 3 ? 3 : 0] = t.w;
+      } else {
+        x[i][0] = xp[i][k];
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int j = 0; j < CN; ++j)
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) acc[i][j] += x[i][v] * w[j][v];
+  }
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < CN; ++j) {
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) acc[i][j] += __shfl_xor_sync(0xffffffffu, acc[i][j], o);
+      if (lane == 0) red[warp][i * CN + j] = acc[i][j];
+    }
+  __syncthreads();
+  // One thread per output of the block: (8 / kw) groups x MT x CN.
+  for (int t = threadIdx.x; t < 8 / kw * MT * CN; t += 256) {
+    const int g = t / (MT * CN), o = t % (MT * CN);
+    const int row = m0 + o / CN, col = (int)(blockIdx.x * (8 / kw) + g) * CN + o % CN;
+    if (row >= p.m || col >= p.n) continue;
+    float v = 0.f;
+    for (int q = 0; q < kw; ++q) v += red[g * kw + q][o];
+    p.c[(int64_t)row * p.n + col] = lin_finish(e, v, row, col, p.n);
+  }
 }
 
 // dz = dy act'(z), dense [m, n], and the partial sums of its columns over the
@@ -74,10 +214,13 @@ __global__ void __launch_bounds__(256) linear_dz_kernel(const float* dy, int64_t
   if (c >= n) return;
   float s = 0.f;
   for (int64_t row = blockIdx.y; row < m; row += gridDim.y) {
-    float g = dy[row * dys + c];
-    if (z) g *= lin_slope(z[row * n + c], act);
-    dz[row * n + c] = g;
-    s += g;
+    float g[1] = {dy[row * dys + c]};
+    if (z) {
+      const float zv[1] = {z[row * n + c]};
+      lin_times_slope<1>(g, zv, act);
+    }
+    dz[row * n + c] = g[0];
+    s += g[0];
   }
   part[(int64_t)blockIdx.y * n + c] = s;
 }
@@ -105,19 +248,81 @@ struct LinMatrix {
   int64_t s0, s1;
 };
 
+constexpr int LIN_TOKENS = 8;  // rows up to which a product is a walk over the weight
+
+static bool lin_aligned(const float* p, int64_t stride) { return (uintptr_t)p % 16 == 0 && stride % 4 == 0; }
+
+template <int MT, int CN>
+static void lin_tokens(const LinProduct& p, const LinEpilogue& e, cudaStream_t s) {
+  // Warps per column group: as many as keep the GPU's warp slots busy, with at
+  // least one 16-byte piece per lane.
+  const int64_t groups = (int64_t)((p.n + CN - 1) / CN) * ((p.m + MT - 1) / MT);
+  int kw = 1;
+  while (kw < 8 && groups * kw * 2 <= (int64_t)sm_count() * 32 && p.k >= kw * 2 * 128) kw *= 2;
+  const int per = 8 / kw * CN;
+  const dim3 grid((unsigned)((p.n + per - 1) / per), (unsigned)((p.m + MT - 1) / MT));
+  if (lin_aligned(p.a, p.m > 1 ? p.as0 : 0) && lin_aligned(p.b, p.n > 1 ? p.bs0 : 0) && p.k % 4 == 0)
+    launch_pdl(linear_tokens_kernel<MT, CN, 4>, grid, dim3(256), 0, s, p, e, kw);
+  else
+    launch_pdl(linear_tokens_kernel<MT, CN, 1>, grid, dim3(256), 0, s, p, e, kw);
+}
+
+static int ls_mode(const float* p, int64_t s0, int64_t s1) {
+  if (s1 == 1 && lin_aligned(p, s0)) return LS_ALONG_K;
+  if (s0 == 1 && lin_aligned(p, s1)) return LS_ALONG_LINES;
+  return LS_SINGLE;
+}
+
+// A product on the multiply-add units.
 static int lin_product(const LinProduct& p, const LinEpilogue& e, cudaStream_t s) {
   if (p.m == 0 || p.n == 0) return MM_OK;
-  const dim3 grid((p.n + LS_T - 1) / LS_T, (p.m + LS_T - 1) / LS_T);
-  if (grid.y > 65535) return fail(MM_ERR_UNSUPPORTED, "mm_linear: too many rows");
-  linear_simt_kernel<<<grid, 256, 0, s>>>(p, e);
+  if (p.m <= LIN_TOKENS && p.as1 == 1 && p.bs1 == 1 && p.k > 0) {
+    if (p.m == 1)
+      lin_tokens<1, 2>(p, e, s);
+    else if (p.m == 2)
+      lin_tokens<2, 2>(p, e, s);
+    else if (p.m <= 4)
+      lin_tokens<4, 4>(p, e, s);
+    else
+      lin_tokens<8, 4>(p, e, s);
+  } else {
+    const int tiles_n = (p.n + LS_T - 1) / LS_T;
+    const int64_t tiles = (int64_t)tiles_n * ((p.m + LS_T - 1) / LS_T);
+    if (tiles > INT32_MAX) return fail(MM_ERR_UNSUPPORTED, "mm_linear: output too large");
+    const int vec = p.n % 4 == 0 && (uintptr_t)p.c % 16 == 0;
+    launch_pdl(linear_small_kernel, dim3((unsigned)tiles), dim3(256), 0, s, p, e, tiles_n, ls_mode(p.a, p.as0, p.as1),
+               ls_mode(p.b, p.bs0, p.bs1), vec);
+  }
   MM_LAUNCH_CHECK("mm_linear launch");
   return MM_OK;
 }
 
 constexpr int LIN_DZ_ROWS = 256;  // partial rows of the bias gradient
 
-// Whether a product of this size runs on the tensor cores.
-static bool lin_on_tensor_cores(int64_t m, int64_t n, int64_t k) { return m > 32 && k >= 32 && n >= 32; }
+// Clocks of a small product: 148 blocks at a time, a chunk of 64 of the
+// reduction in about 600 (latency with one block per SM, multiply-adds with
+// several), 1,500 to start and end each, and 3,000 once.
+static double lin_small_clocks(int64_t m, int64_t n, int64_t k) {
+  const int64_t tiles = ((m + LS_T - 1) / LS_T) * ((n + LS_T - 1) / LS_T);
+  const int64_t waves = (tiles + sm_count() - 1) / sm_count();
+  return 3000.0 + waves * (1500.0 + 600.0 * ((k + LS_K - 1) / LS_K));
+}
+
+// Whether a call runs on the tensor cores: where the estimate of its products,
+// with 10 bytes per value to split the operands (about 3,400 bytes per clock)
+// and 5,000 clocks for the launches this takes, is below the small kernels'.
+static bool lin_on_tensor_cores(int64_t m, int64_t n, int64_t k, bool backward) {
+  if ((m <= LIN_TOKENS && !backward) || m == 0 || n < 32 || k < 32) return false;
+  double small, tensor = 5000;
+  if (backward) {
+    small = lin_small_clocks(m, k, n) + lin_small_clocks(n, k, m);
+    tensor += lin_choose(m, k, n).clocks + lin_choose(n, k, m).clocks + 10.0 * (m * n + m * k + n * k) / 3400;
+  } else {
+    small = lin_small_clocks(m, n, k);
+    tensor += lin_choose(m, n, k).clocks + 10.0 * (m * k + n * k) / 3400;
+  }
+  return tensor < small;
+}
 
 // Workspace pieces, 256-byte aligned.
 struct LinCarve {
@@ -204,7 +409,7 @@ static int lin_backward_tc(const LinMatrix& dy, const LinMatrix& x, const LinMat
     linear_columns_kernel<<<(unsigned)((n + 31) / 32), 256, 0, s>>>(gs.part, (int)lin_part_rows(m), (int)n, db);
     MM_LAUNCH_CHECK("mm_linear_backward launch");
   }
-  const LinEpilogue none = {nullptr, nullptr, nullptr, 0, MM_LINEAR_NONE, 0};
+  const LinEpilogue none = lin_epilogue(nullptr, nullptr, 0, nullptr, MM_LINEAR_NONE, false);
   if (dx) {
     const LinChoice c = lin_choose(m, k, n);
     float* part = (float*)ws.take(lin_part_bytes(c));
@@ -221,7 +426,7 @@ static int lin_backward_tc(const LinMatrix& dy, const LinMatrix& x, const LinMat
 
 static size_t lin_workspace(int64_t m, int64_t n, int64_t k, bool backward) {
   LinCarve ws = {nullptr, 0};
-  if (lin_on_tensor_cores(m, n, k)) {
+  if (lin_on_tensor_cores(m, n, k, backward)) {
     ws.take(lin_plane_bytes(m, k));
     ws.take(4 * lin_flag_words(m, k));
     ws.take(lin_plane_bytes(n, k));
@@ -276,8 +481,8 @@ extern "C" int mm_linear(const float* x, int64_t xs0, int64_t xs1, const float* 
   if (m == 0 || n == 0) return MM_OK;
   if (!y || (k > 0 && (!x || !w))) return fail(MM_ERR_INVALID, "mm_linear: null data pointer");
   cudaStream_t s = resolve_stream(stream);
-  const LinEpilogue e = {bias, residual, z, residual_stride, act, residual_before_act != 0};
-  if (!lin_on_tensor_cores(m, n, k))
+  const LinEpilogue e = lin_epilogue(bias, residual, residual_stride, z, act, residual_before_act != 0);
+  if (!lin_on_tensor_cores(m, n, k, false))
     return lin_product({x, w, y, xs0, xs1, ws0, ws1, (int)m, (int)n, (int)k}, e, s);
   Scratch scratch;
   if (workspace == nullptr) {
@@ -311,7 +516,7 @@ extern "C" int mm_linear_backward(const float* dy, int64_t dy_stride, const floa
     if ((rc = scratch.get(need, s)) != MM_OK) return rc;
     workspace = scratch.data;
   }
-  if (lin_on_tensor_cores(m, n, k))
+  if (lin_on_tensor_cores(m, n, k, true))
     return lin_backward_tc({dy, dy_stride, 1}, {x, xs0, xs1}, {w, ws0, ws1}, z, act, m, n, k, dx, dw, db, dz,
                            workspace, s);
   LinCarve ws = {(char*)workspace, 0};
@@ -326,7 +531,7 @@ extern "C" int mm_linear_backward(const float* dy, int64_t dy_stride, const floa
     linear_columns_kernel<<<(unsigned)((n + 31) / 32), 256, 0, s>>>(part, rows, (int)n, db);
     MM_LAUNCH_CHECK("mm_linear_backward launch");
   }
-  const LinEpilogue none = {nullptr, nullptr, nullptr, 0, MM_LINEAR_NONE, 0};
+  const LinEpilogue none = lin_epilogue(nullptr, nullptr, 0, nullptr, MM_LINEAR_NONE, false);
   if (dx) {
     rc = lin_product({g, w, dx, n, 1, ws1, ws0, (int)m, (int)k, (int)n}, none, s);
     if (rc != MM_OK) return rc;

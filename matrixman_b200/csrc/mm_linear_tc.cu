@@ -14,7 +14,6 @@
 //                         sums of db on the way in the backward pass
 //   linear_gemm_kernel    C = A B^T (+ epilogue) over the planes
 //   linear_join_kernel    sums of the tiles whose reduction was divided
-//   linear_special_kernel rows and columns that hold infinities (see there)
 #include <cuda.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -47,52 +46,46 @@ __device__ __forceinline__ void split3(float a, uint32_t& h1, uint32_t& h2, uint
   h3 = __float_as_uint(r - __uint_as_float(h2)) & 0xffff0000u;
 }
 
-// Blocks of 64 x 128 values; 16 threads x 8 values across a row, 16 rows at a
-// time.  Bound by memory: 4 bytes in and 6 out per value.
+// Blocks of 64 x 128 values: 16 threads x 8 values across a row, 16 rows at a
+// time, the next rows' values on their way meanwhile.  Bound by memory (4 bytes
+// in, with z 8, and 6 out per value) but for GELU's slope.
 __global__ void __launch_bounds__(256) linear_split_kernel(const __grid_constant__ LinSplits all) {
   __shared__ float sums[16][SP_COLS + 4];
-  pdl_wait();
   int k = 0;
   while (k + 1 < all.count && blockIdx.x >= all.s[k + 1].first) ++k;
   const LinSplit& s = all.s[k];
   const int block = (int)(blockIdx.x - s.first);
   const int bc = block % s.blocks_c, br = block / s.blocks_c;
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  const int c0 = bc * SP_COLS + tx * 8;
-  float sum[8] = {};
+  const int c0 = bc * SP_COLS + tx * 8, left = s.cols - c0;
+  const int64_t end = min((int64_t)(br + 1) * SP_ROWS, s.rows);
+  int64_t row = (int64_t)br * SP_ROWS + ty;
+  float sum[8] = {}, next[8], znext[8] = {};
   int inf = 0;
-#pragma unroll
-  for (int i = 0; i < SP_ROWS / 16; ++i) {
-    const int64_t row = (int64_t)br * SP_ROWS + i * 16 + ty;
-    if (row >= s.rows || c0 >= s.cols) continue;
-    float v[8];
-    const float* src = s.src + row * s.s0;
-    if (s.vec && c0 + 8 <= s.cols) {
-      const float4 a = *reinterpret_cast<const float4*>(src + c0), b = *reinterpret_cast<const float4*>(src + c0 + 4);
-      v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-      v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+  pdl_wait();
+  const bool any = left > 0;
+  auto fetch = [&](int64_t r) {
+    const float* src = s.src + r * s.s0;
+    if (s.s1 == 1) {
+      lin_load_row<8>(src + c0, left, s.vec, next);
     } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = c0 + e < s.cols ? src[(int64_t)(c0 + e) * s.s1] : 0.f;
+      for (int e = 0; e < 8; ++e) next[e] = e < left ? src[(int64_t)(c0 + e) * s.s1] : 0.f;
     }
-    if (s.z) {
-      const float* z = s.z + row * s.cols;
-      if (s.vec && c0 + 8 <= s.cols) {
-        const float4 a = *reinterpret_cast<const float4*>(z + c0), b = *reinterpret_cast<const float4*>(z + c0 + 4);
-        const float t[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+    if (s.z) lin_load_row<8>(s.z + r * s.cols + c0, left, s.vec, znext);
+  };
+  if (any && row < end) fetch(row);
+#pragma unroll 1
+  for (; any && row < end; row += 16) {
+    float v[8], z[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] *= lin_slope(t[e], s.act);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (c0 + e < s.cols) v[e] *= lin_slope(z[c0 + e], s.act);
-      }
+    for (int e = 0; e < 8; ++e) {
+      v[e] = next[e];
+      z[e] = znext[e];
     }
-    if (s.out) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (c0 + e < s.cols) s.out[row * s.cols + c0 + e] = v[e];
-    }
+    if (row + 16 < end) fetch(row + 16);
+    if (s.z) lin_times_slope<8>(v, z, s.act);
+    if (s.out) lin_store_row<8>(s.out + row * s.cols + c0, left, false, v);
     uint32_t p[3][4];
 #pragma unroll
     for (int e = 0; e < 8; e += 2) {
@@ -285,6 +278,74 @@ __device__ __forceinline__ LgUnit lg_unit(const LinGemm& a, int u, int bn) {
   return w;
 }
 
+// ---------------------------------------------------------------------------
+// Infinities.  Their pieces are (inf, 0, 0), and inf times another operand's
+// zero piece is NaN where the whole product is infinite.  linear_split_kernel
+// says which of its blocks hold an infinity; a tile's rows of A and of B (rows
+// and columns of C) that hold one and no NaN are computed again, from the
+// pieces' sums in float32, by the block that has stored the tile.
+// ---------------------------------------------------------------------------
+
+__device__ __forceinline__ float lin_value(const LinPlanes& p, int64_t line, int64_t k) {
+  const int64_t at = p.mn ? k * p.ld + line : line * p.ld + k;
+  const int64_t plane = p.mn ? p.k * p.ld : p.lines * p.ld;
+  float v = 0.f;
+#pragma unroll
+  for (int q = 2; q >= 0; --q) v += __uint_as_float((uint32_t)p.planes[q * plane + at] << 16);
+  return v;
+}
+
+// Whether any flag of the blocks of lines [l0, l1) is set, for the whole thread
+// block (every thread calls).
+__device__ __forceinline__ bool lin_flagged(const LinPlanes& p, int l0, int l1) {
+  const int per = p.mn ? SP_COLS : SP_ROWS;
+  const int across = (int)((p.k + (p.mn ? SP_ROWS : SP_COLS) - 1) / (p.mn ? SP_ROWS : SP_COLS));
+  const int blocks_c = (int)(((p.mn ? p.lines : p.k) + SP_COLS - 1) / SP_COLS);
+  const int b0 = l0 / per, b1 = (l1 + per - 1) / per;
+  int any = 0;
+  for (int i = threadIdx.x; i < (b1 - b0) * across; i += blockDim.x) {
+    const int block = b0 + i / across, at = i % across;
+    any |= p.flags[p.mn ? at * blocks_c + block : block * blocks_c + at];
+  }
+  return __syncthreads_or(any) != 0;
+}
+
+template <bool B>
+__device__ __noinline__ void lin_fix_lines(const LinGemm& a, int m0, int m1, int n0, int n1) {
+  const LinPlanes& p = B ? a.pb : a.pa;
+  const LinPlanes& other = B ? a.pa : a.pb;
+  const int l0 = B ? n0 : m0, l1 = B ? n1 : m1, o0 = B ? m0 : n0, o1 = B ? m1 : n1;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+  for (int line = l0; line < l1; ++line) {
+    int inf = 0, nan = 0;
+    for (int64_t k = threadIdx.x; k < p.k; k += blockDim.x) {
+      const float v = lin_value(p, line, k);
+      inf |= isinf(v);
+      nan |= isnan(v);
+    }
+    inf = __syncthreads_or(inf);
+    nan = __syncthreads_or(nan);
+    if (!inf || nan) continue;  // a NaN makes the whole line NaN already
+    for (int o = o0 + warp; o < o1; o += warps) {
+      float v = 0.f;
+      for (int64_t k = lane; k < p.k; k += 32) v += lin_value(p, line, k) * lin_value(other, o, k);
+#pragma unroll
+      for (int s = 16; s > 0; s >>= 1) v += __shfl_xor_sync(0xffffffffu, v, s);
+      const int row = B ? o : line, col = B ? line : o;
+      if (lane == 0) a.c[(int64_t)row * a.n + col] = lin_finish(a.e, v, row, col, a.n);
+    }
+  }
+}
+
+// Every thread of the block calls, after the tile [m0, m0 + rows) x [n0, n0 +
+// cols) has been stored and a __syncthreads.
+__device__ __forceinline__ void lin_fix(const LinGemm& a, int m0, int rows, int n0, int cols) {
+  const int m1 = min(m0 + rows, a.m), n1 = min(n0 + cols, a.n);
+  if (m0 >= m1 || n0 >= n1) return;
+  if (lin_flagged(a.pa, m0, m1)) lin_fix_lines<false>(a, m0, m1, n0, n1);
+  if (lin_flagged(a.pb, n0, n1)) lin_fix_lines<true>(a, m0, m1, n0, n1);
+}
+
 // Persistent CTAs, one per SM.  Warps 0-7 add up and store, warp 8 loads (TMA),
 // warp 9 issues the MMAs.  The MMAs of one stage (32 of the reduction, twelve
 // products of 128 x BN x 16) go into one of two accumulators in tensor memory,
@@ -307,6 +368,7 @@ __global__ void __launch_bounds__(LG_THREADS, 1) linear_gemm_kernel(const __grid
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + S * stage_bytes);
   uint64_t *empty = full + S, *acc_full = empty + S, *acc_free = acc_full + 2, *drain = acc_free + 2;
   uint32_t* slot = reinterpret_cast<uint32_t*>(drain + 1);
+  int* special = reinterpret_cast<int*>(slot + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int i = 0; i < S; ++i) {
@@ -318,6 +380,7 @@ __global__ void __launch_bounds__(LG_THREADS, 1) linear_gemm_kernel(const __grid
       lg_bar_init(&acc_free[i], LG_EPI_WARPS);
     }
     lg_bar_init(drain, 1);
+    *special = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == LG_WARP_MMA) {
@@ -408,6 +471,10 @@ __global__ void __launch_bounds__(LG_THREADS, 1) linear_gemm_kernel(const __grid
     int buf = 0;
     uint32_t par = 0;
     bool alive = true;
+    int inf = 0;  // read while the first stages are on their way
+    for (int i = threadIdx.x; i < a.flags_a; i += LG_EPI_WARPS * 32) inf |= a.pa.flags[i];
+    for (int i = threadIdx.x; i < a.flags_b; i += LG_EPI_WARPS * 32) inf |= a.pb.flags[i];
+    if (inf) *special = 1;
     for (int u = blockIdx.x; u < a.units && alive; u += gridDim.x) {
       const LgUnit w = lg_unit(a, u, BN);
       float acc[HALF];
@@ -437,7 +504,6 @@ __global__ void __launch_bounds__(LG_THREADS, 1) linear_gemm_kernel(const __grid
       if (!alive) break;
       const int64_t row = (int64_t)w.m0 + quarter * 32 + lane;
       int col = w.n0 + half * HALF;
-      float* out = a.c + row * a.n;
       float* part = w.part >= 0 ? a.part + ((int64_t)w.part * LG_BM + quarter * 32 + lane) * BN + half * HALF : nullptr;
       // Eight columns at a time; the totals move down by eight registers per
       // step, so that the epilogue's code is there once.
@@ -447,17 +513,10 @@ __global__ void __launch_bounds__(LG_THREADS, 1) linear_gemm_kernel(const __grid
           reinterpret_cast<float4*>(part)[2 * j] = make_float4(acc[0], acc[1], acc[2], acc[3]);
           reinterpret_cast<float4*>(part)[2 * j + 1] = make_float4(acc[4], acc[5], acc[6], acc[7]);
         } else if (row < a.m && col < a.n) {
-          if (a.vec && col + 8 <= a.n) {
-            float v[8];
+          float v[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = lin_finish(a.e, acc[e], row, col + e, a.n);
-            reinterpret_cast<float4*>(out + col)[0] = make_float4(v[0], v[1], v[2], v[3]);
-            reinterpret_cast<float4*>(out + col)[1] = make_float4(v[4], v[5], v[6], v[7]);
-          } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-              if (col + e < a.n) out[col + e] = lin_finish(a.e, acc[e], row, col + e, a.n);
-          }
+          for (int e = 0; e < 8; ++e) v[e] = acc[e];
+          lin_finish_row<8>(a.e, v, a.c, row, col, a.n, a.vec);
         }
 #pragma unroll
         for (int i = 0; i + 8 < HALF; ++i) acc[i] = acc[i + 8];
@@ -469,6 +528,12 @@ __global__ void __launch_bounds__(LG_THREADS, 1) linear_gemm_kernel(const __grid
   if (warp == LG_WARP_MMA) {
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(cols) : "memory");
+  }
+  if (*special) {
+    for (int u = blockIdx.x; u < a.units; u += gridDim.x) {
+      const LgUnit w = lg_unit(a, u, BN);
+      if (w.part < 0) lin_fix(a, w.m0, LG_BM, w.n0, BN);
+    }
   }
 }
 
@@ -487,60 +552,8 @@ __global__ void __launch_bounds__(256) linear_join_kernel(const LinGemm a, int b
     for (int s = 0; s < a.splits; ++s) v += part[((int64_t)s * LG_BM + r) * bn + c];
     a.c[row * a.n + w.n0 + c] = lin_finish(a.e, v, row, w.n0 + c, a.n);
   }
-}
-
-// ---------------------------------------------------------------------------
-// Infinities.  Their pieces are (inf, 0, 0), and inf times another operand's
-// zero piece is NaN where the whole product is infinite.  linear_split_kernel
-// says which of its blocks hold an infinity; rows of A (columns of C) and rows
-// of B that do are computed again here from the pieces' sums, in float32.
-// Without any, every block reads its flags and leaves.
-// ---------------------------------------------------------------------------
-
-__device__ __forceinline__ float lin_value(const LinPlanes& p, int64_t line, int64_t k) {
-  const int64_t at = p.mn ? k * p.ld + line : line * p.ld + k;
-  const int64_t plane = p.mn ? p.k * p.ld : p.lines * p.ld;
-  float v = 0.f;
-#pragma unroll
-  for (int q = 2; q >= 0; --q) v += __uint_as_float((uint32_t)p.planes[q * plane + at] << 16);
-  return v;
-}
-
-__global__ void __launch_bounds__(256) linear_special_kernel(const LinGemm a, const LinPlanes pa, const LinPlanes pb,
-                                                             int blocks_a) {
-  pdl_wait();
-  const bool is_b = (int)blockIdx.x >= blocks_a;
-  const LinPlanes& p = is_b ? pb : pa;
-  const LinPlanes& other = is_b ? pa : pb;
-  const int block = is_b ? blockIdx.x - blocks_a : blockIdx.x;
-  // Lines of this block and the flags that speak of them.
-  const int per = p.mn ? SP_COLS : SP_ROWS;
-  const int across = (int)((p.k + (p.mn ? SP_ROWS : SP_COLS) - 1) / (p.mn ? SP_ROWS : SP_COLS));
-  const int blocks_c = (int)(((p.mn ? p.lines : p.k) + SP_COLS - 1) / SP_COLS);
-  int any = 0;
-  for (int i = threadIdx.x; i < across; i += 256) any |= p.flags[p.mn ? i * blocks_c + block : block * blocks_c + i];
-  if (!__syncthreads_or(any)) return;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t end = min((int64_t)(block + 1) * per, p.lines);
-  for (int64_t line = (int64_t)block * per; line < end; ++line) {
-    int inf = 0, nan = 0;
-    for (int64_t k = threadIdx.x; k < p.k; k += 256) {
-      const float v = lin_value(p, line, k);
-      inf |= isinf(v);
-      nan |= isnan(v);
-    }
-    inf = __syncthreads_or(inf);
-    nan = __syncthreads_or(nan);
-    if (!inf || nan) continue;  // a NaN makes the whole line NaN already
-    for (int64_t o = warp; o < other.lines; o += 8) {
-      float v = 0.f;
-      for (int64_t k = lane; k < p.k; k += 32) v += lin_value(p, line, k) * lin_value(other, o, k);
-#pragma unroll
-      for (int s = 16; s > 0; s >>= 1) v += __shfl_xor_sync(0xffffffffu, v, s);
-      const int64_t row = is_b ? o : line, col = is_b ? line : o;
-      if (lane == 0) a.c[row * a.n + col] = lin_finish(a.e, v, row, (int)col, a.n);
-    }
-  }
+  __syncthreads();
+  lin_fix(a, w.m0 + r0, 8, w.n0, bn);
 }
 
 // ---------------------------------------------------------------------------
@@ -586,8 +599,7 @@ int lin_run_splits(const LinSplits& all, cudaStream_t s) {
 // although its partial tiles are written and read once more.
 LinChoice lin_choose(int64_t m, int64_t n, int64_t k) {
   const int sms = sm_count();
-  LinChoice best = {0, 0, 1, 0, 0, 0, 0};
-  double least = 0;
+  LinChoice best = {};
   for (int bn : {256, 128, 64}) {
     const int64_t tm = (m + LG_BM - 1) / LG_BM, tn = (n + bn - 1) / bn, tiles = tm * tn;
     const int64_t stages = (k + LG_BK - 1) / LG_BK;
@@ -602,10 +614,8 @@ LinChoice lin_choose(int64_t m, int64_t n, int64_t k) {
         t += waves * (((stages + s - 1) / s) * stage + tile);
         if (s > 1) t += 4000 + (double)rest * s * LG_BM * bn * 8 / 3500;  // about 3,500 bytes per clock
       }
-      if (best.bn == 0 || t < least) {
-        least = t;
-        best = {bn, (int)full, s, (int)tm, (int)tn, (int)stages, (int)(full + rest * s)};
-      }
+      if (best.bn == 0 || t < best.clocks)
+        best = {bn, (int)full, s, (int)tm, (int)tn, (int)stages, (int)(full + rest * s), t};
     }
   }
   return best;
@@ -613,6 +623,12 @@ LinChoice lin_choose(int64_t m, int64_t n, int64_t k) {
 
 int64_t lin_part_bytes(const LinChoice& c) {
   return c.splits > 1 ? (int64_t)(c.units - c.full) * LG_BM * c.bn * 4 : 0;
+}
+
+// Blocks that linear_split_kernel made of an operand.
+static int lin_flag_count(const LinPlanes& p) {
+  const int64_t r = p.mn ? p.k : p.lines, c = p.mn ? p.lines : p.k;
+  return (int)(((r + SP_ROWS - 1) / SP_ROWS) * ((c + SP_COLS - 1) / SP_COLS));
 }
 
 static int lin_map(const LinPlanes& p, int rows, CUtensorMap* out) {
@@ -674,6 +690,10 @@ int lin_run_gemm(const LinPlanes& pa, const LinPlanes& pb, float* c, const LinEp
   g.c = c;
   g.part = part;
   g.e = e;
+  g.pa = pa;
+  g.pb = pb;
+  g.flags_a = lin_flag_count(pa);
+  g.flags_b = lin_flag_count(pb);
   CUtensorMap ma, mb;
   int rc = lin_map(pa, LG_BM, &ma);
   if (rc == MM_OK) rc = lin_map(pb, ch.bn, &mb);
@@ -686,10 +706,6 @@ int lin_run_gemm(const LinPlanes& pa, const LinPlanes& pb, float* c, const LinEp
     const unsigned grid = (unsigned)((ch.units - ch.full) / ch.splits * (LG_BM / 8));
     MM_CUDA(launch_pdl(linear_join_kernel, dim3(grid), dim3(256), 0, s, g, ch.bn), "mm_linear join launch");
   }
-  const int per_a = pa.mn ? SP_COLS : SP_ROWS, per_b = pb.mn ? SP_COLS : SP_ROWS;
-  const int blocks_a = (int)((pa.lines + per_a - 1) / per_a), blocks_b = (int)((pb.lines + per_b - 1) / per_b);
-  MM_CUDA(launch_pdl(linear_special_kernel, dim3((unsigned)(blocks_a + blocks_b)), dim3(256), 0, s, g, pa, pb, blocks_a),
-          "mm_linear special launch");
   return MM_OK;
 }
 

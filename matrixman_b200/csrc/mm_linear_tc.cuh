@@ -47,6 +47,7 @@ struct LinChoice {
   int full;             // tiles that run undivided
   int splits;           // parts of the reduction of each tile behind them
   int tiles_m, tiles_n, stages, units;
+  double clocks;        // the estimate
 };
 
 struct LinGemm {
@@ -54,6 +55,8 @@ struct LinGemm {
   float* c;      // dense [m][n]
   float* part;   // partial tiles
   LinEpilogue e;
+  LinPlanes pa, pb;
+  int flags_a, flags_b;  // their numbers of flags
 };
 
 int64_t lin_flag_words(int64_t rows, int64_t cols);
