@@ -354,8 +354,6 @@ static int ln_vec(const LnArgs& a) {
   return bits % 4 == 0 ? 4 : bits % 2 == 0 ? 2 : 1;
 }
 
-constexpr int LN_MAX_BLOCKS_PER_SM = 2;
-
 struct LnPlan {
   int vec, group, each;  // elements per load, threads per row (0: too wide), elements per thread
 };
@@ -378,10 +376,16 @@ static LnPlan ln_plan(const LnArgs& a, bool backward) {
   return p;
 }
 
-// Backward blocks (= partial rows): two per SM, no more than there are rows.
+constexpr int LN_MAX_BLOCKS_PER_SM = 8;
+
+// Backward blocks (= partial rows): as many as an SM's registers hold at once
+// (64 per thread, 80 and 128 where a warp's lanes hold 8 and 16 elements), no
+// more than there are rows.  Two blocks per SM instead left too few loads in
+// flight: 32768 x 2048 took 192 us (4.2 TB/s), 65536 x 1024 283 us (2.8 TB/s).
 static int ln_blocks(const LnArgs& a, const LnPlan& p) {
   const int64_t steps = p.group == 32 ? (a.rows + LN_BWD_WARPS - 1) / LN_BWD_WARPS : a.rows;
-  const int64_t most = (int64_t)sm_count() * LN_MAX_BLOCKS_PER_SM;
+  const int per_sm = p.group == 0 ? 2 : p.group > 32 ? 1024 / p.group : p.each <= 4 ? 4 : p.each <= 8 ? 3 : 2;
+  const int64_t most = (int64_t)sm_count() * per_sm;
   return (int)(steps < 1 ? 1 : steps < most ? steps : most);
 }
 
@@ -512,9 +516,8 @@ extern "C" int mm_layer_norm_backward(const float* dy, int64_t dy_stride, const 
   a.y = dx;
   a.part = (float*)workspace;
   const LnPlan p = ln_plan(a, true);
-  int blocks = ln_blocks(a, p);
+  const int blocks = ln_blocks(a, p);
   if (p.group == 0) {
-    blocks = (int)ln_partial_rows(rows);
     if (dx) ln_backward_wide_kernel<<<(unsigned)rows, 1024, 0, s>>>(a);
     if (cols) ln_columns_kernel<<<dim3((a.width + 255) / 256, blocks), 256, 0, s>>>(a);
   } else if (p.vec == 4) {
