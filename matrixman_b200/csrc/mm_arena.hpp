@@ -114,7 +114,8 @@ class Arena {
         Block* b = it->second.back();
         it->second.pop_back();
         stats_.cached_bytes[kind] -= (int64_t)b->size;
-        if (sync_safe_ && b->has_event) be_.stream_wait(stream, b->ev);
+        // (reuse on the stream of the release is ordered already)
+        if (sync_safe_ && b->has_event && b->release_stream != stream) be_.stream_wait(stream, b->ev);
         live_[b->ptr] = b;
         account_live(b, +1);
         ++stats_.pool_hits[kind];
@@ -129,6 +130,12 @@ class Arena {
     account_live(b, +1);
     *out = b->ptr;
     return MM_OK;
+  }
+
+  // Whether ptr is a live block of this arena.
+  bool owns(void* ptr) {
+    std::lock_guard<std::mutex> g(mu_);
+    return live_.find(ptr) != live_.end();
   }
 
   int free(void* ptr, Stream stream, std::string* msg) {

@@ -308,20 +308,31 @@ static double lin_small_clocks(int64_t m, int64_t n, int64_t k) {
   return 3000.0 + waves * (1500.0 + 600.0 * ((k + LS_K - 1) / LS_K));
 }
 
-// Whether a call runs on the tensor cores: where the estimate of its products,
-// with 10 bytes per value to split the operands (about 3,400 bytes per clock)
-// and 5,000 clocks for the launches this takes, is below the small kernels'.
-static bool lin_on_tensor_cores(int64_t m, int64_t n, int64_t k, bool backward) {
-  if ((m <= LIN_TOKENS && !backward) || m == 0 || n < 32 || k < 32) return false;
+// How a call runs: on the tensor cores where the estimate of its products, with
+// 10 bytes per value to split the operands (about 3,400 bytes per clock) and
+// 5,000 clocks for the launches this takes, is below the small kernels'.
+// `first` is the forward product or dx, `second` dw.
+struct LinRoute {
+  bool tensor;
+  LinChoice first, second;
+};
+
+static LinRoute lin_route(int64_t m, int64_t n, int64_t k, bool backward) {
+  LinRoute r = {};
+  if ((m <= LIN_TOKENS && !backward) || m <= 0 || n < 32 || k < 32) return r;
   double small, tensor = 5000;
   if (backward) {
     small = lin_small_clocks(m, k, n) + lin_small_clocks(n, k, m);
-    tensor += lin_choose(m, k, n).clocks + lin_choose(n, k, m).clocks + 10.0 * (m * n + m * k + n * k) / 3400;
+    r.first = lin_choose(m, k, n);
+    r.second = lin_choose(n, k, m);
+    tensor += r.first.clocks + r.second.clocks + 10.0 * (m * n + m * k + n * k) / 3400;
   } else {
     small = lin_small_clocks(m, n, k);
-    tensor += lin_choose(m, n, k).clocks + 10.0 * (m * k + n * k) / 3400;
+    r.first = lin_choose(m, n, k);
+    tensor += r.first.clocks + 10.0 * (m * k + n * k) / 3400;
   }
-  return tensor < small;
+  r.tensor = tensor < small;
+  return r;
 }
 
 // Workspace pieces, 256-byte aligned.
@@ -367,7 +378,7 @@ static LinStored lin_store(LinCarve* ws, LinSplits* all, const float* src, int64
   return st;
 }
 
-static int lin_forward_tc(const LinMatrix& x, const LinMatrix& w, int64_t m, int64_t n, int64_t k,
+static int lin_forward_tc(const LinRoute& r, const LinMatrix& x, const LinMatrix& w, int64_t m, int64_t n, int64_t k,
                           const LinEpilogue& e, float* y, void* workspace, cudaStream_t s) {
   LinCarve ws = {(char*)workspace, 0};
   LinSplits all;
@@ -376,14 +387,13 @@ static int lin_forward_tc(const LinMatrix& x, const LinMatrix& w, int64_t m, int
   bool xt, wt;
   const LinStored xs = lin_store(&ws, &all, x.data, x.s0, x.s1, m, k, &xt);
   const LinStored wst = lin_store(&ws, &all, w.data, w.s0, w.s1, n, k, &wt);
-  const LinChoice c = lin_choose(m, n, k);
-  float* part = (float*)ws.take(lin_part_bytes(c));
+  float* part = (float*)ws.take(lin_part_bytes(r.first));
   int rc = lin_run_splits(all, s);
   if (rc != MM_OK) return rc;
-  return lin_run_gemm(xt ? xs.by_cols() : xs.by_rows(), wt ? wst.by_cols() : wst.by_rows(), y, e, c, part, s);
+  return lin_run_gemm(xt ? xs.by_cols() : xs.by_rows(), wt ? wst.by_cols() : wst.by_rows(), y, e, r.first, part, s);
 }
 
-static int lin_backward_tc(const LinMatrix& dy, const LinMatrix& x, const LinMatrix& w, const float* z, int act,
+static int lin_backward_tc(const LinRoute& r, const LinMatrix& dy, const LinMatrix& x, const LinMatrix& w, const float* z, int act,
                            int64_t m, int64_t n, int64_t k, float* dx, float* dw, float* db, float* dz,
                            void* workspace, cudaStream_t s) {
   LinCarve ws = {(char*)workspace, 0};
@@ -411,34 +421,32 @@ static int lin_backward_tc(const LinMatrix& dy, const LinMatrix& x, const LinMat
   }
   const LinEpilogue none = lin_epilogue(nullptr, nullptr, 0, nullptr, MM_LINEAR_NONE, false);
   if (dx) {
-    const LinChoice c = lin_choose(m, k, n);
-    float* part = (float*)ws.take(lin_part_bytes(c));
-    rc = lin_run_gemm(g.by_rows(), wt ? wst.by_rows() : wst.by_cols(), dx, none, c, part, s);
+    float* part = (float*)ws.take(lin_part_bytes(r.first));
+    rc = lin_run_gemm(g.by_rows(), wt ? wst.by_rows() : wst.by_cols(), dx, none, r.first, part, s);
     if (rc != MM_OK) return rc;
   }
   if (dw) {
-    const LinChoice c = lin_choose(n, k, m);
-    float* part = (float*)ws.take(lin_part_bytes(c));
-    rc = lin_run_gemm(g.by_cols(), xt ? xs.by_rows() : xs.by_cols(), dw, none, c, part, s);
+    float* part = (float*)ws.take(lin_part_bytes(r.second));
+    rc = lin_run_gemm(g.by_cols(), xt ? xs.by_rows() : xs.by_cols(), dw, none, r.second, part, s);
   }
   return rc;
 }
 
-static size_t lin_workspace(int64_t m, int64_t n, int64_t k, bool backward) {
+static size_t lin_workspace(const LinRoute& r, int64_t m, int64_t n, int64_t k, bool backward) {
   LinCarve ws = {nullptr, 0};
-  if (lin_on_tensor_cores(m, n, k, backward)) {
+  if (r.tensor) {
     ws.take(lin_plane_bytes(m, k));
     ws.take(4 * lin_flag_words(m, k));
     ws.take(lin_plane_bytes(n, k));
     ws.take(4 * lin_flag_words(n, k));
     if (!backward) {
-      ws.take(lin_part_bytes(lin_choose(m, n, k)));
+      ws.take(lin_part_bytes(r.first));
     } else {
       ws.take(lin_plane_bytes(m, n));
       ws.take(4 * lin_flag_words(m, n));
       ws.take(4 * lin_part_rows(m) * n);
-      ws.take(lin_part_bytes(lin_choose(m, k, n)));
-      ws.take(lin_part_bytes(lin_choose(n, k, m)));
+      ws.take(lin_part_bytes(r.first));
+      ws.take(lin_part_bytes(r.second));
     }
   } else if (backward) {
     ws.take(4 * m * n);
@@ -465,7 +473,7 @@ using namespace mm;
 
 extern "C" int mm_linear_workspace_size(int64_t m, int64_t n, int64_t k, int backward, size_t* bytes) {
   if (bytes == nullptr || m < 0 || n < 0 || k < 0) return fail(MM_ERR_INVALID, "mm_linear_workspace_size: invalid argument");
-  *bytes = lin_workspace(m, n, k, backward != 0);
+  *bytes = lin_workspace(lin_route(m, n, k, backward != 0), m, n, k, backward != 0);
   return MM_OK;
 }
 
@@ -473,7 +481,8 @@ extern "C" int mm_linear(const float* x, int64_t xs0, int64_t xs1, const float* 
                          const float* bias, const float* residual, int64_t residual_stride, int64_t m, int64_t n,
                          int64_t k, int act, int residual_before_act, float* y, float* z, void* workspace,
                          size_t workspace_bytes, void* stream) {
-  const size_t need = m < 0 || n < 0 || k < 0 ? 0 : lin_workspace(m, n, k, false);
+  const LinRoute route = lin_route(m, n, k, false);
+  const size_t need = lin_workspace(route, m, n, k, false);
   int rc = lin_check("mm_linear", m, n, k, act, workspace, workspace_bytes, need);
   if (rc != MM_OK) return rc;
   if (xs0 < 0 || xs1 < 0 || ws0 < 0 || ws1 < 0 || residual_stride < 0)
@@ -482,21 +491,22 @@ extern "C" int mm_linear(const float* x, int64_t xs0, int64_t xs1, const float* 
   if (!y || (k > 0 && (!x || !w))) return fail(MM_ERR_INVALID, "mm_linear: null data pointer");
   cudaStream_t s = resolve_stream(stream);
   const LinEpilogue e = lin_epilogue(bias, residual, residual_stride, z, act, residual_before_act != 0);
-  if (!lin_on_tensor_cores(m, n, k, false))
+  if (!route.tensor)
     return lin_product({x, w, y, xs0, xs1, ws0, ws1, (int)m, (int)n, (int)k}, e, s);
   Scratch scratch;
   if (workspace == nullptr) {
     if ((rc = scratch.get(need, s)) != MM_OK) return rc;
     workspace = scratch.data;
   }
-  return lin_forward_tc({x, xs0, xs1}, {w, ws0, ws1}, m, n, k, e, y, workspace, s);
+  return lin_forward_tc(route, {x, xs0, xs1}, {w, ws0, ws1}, m, n, k, e, y, workspace, s);
 }
 
 extern "C" int mm_linear_backward(const float* dy, int64_t dy_stride, const float* x, int64_t xs0, int64_t xs1,
                                   const float* w, int64_t ws0, int64_t ws1, const float* z, int64_t m, int64_t n,
                                   int64_t k, int act, float* dx, float* dw, float* db, float* dz, void* workspace,
                                   size_t workspace_bytes, void* stream) {
-  const size_t need = m < 0 || n < 0 || k < 0 ? 0 : lin_workspace(m, n, k, true);
+  const LinRoute route = lin_route(m, n, k, true);
+  const size_t need = lin_workspace(route, m, n, k, true);
   int rc = lin_check("mm_linear_backward", m, n, k, act, workspace, workspace_bytes, need);
   if (rc != MM_OK) return rc;
   if (dy_stride < 0 || xs0 < 0 || xs1 < 0 || ws0 < 0 || ws1 < 0)
@@ -516,8 +526,8 @@ extern "C" int mm_linear_backward(const float* dy, int64_t dy_stride, const floa
     if ((rc = scratch.get(need, s)) != MM_OK) return rc;
     workspace = scratch.data;
   }
-  if (lin_on_tensor_cores(m, n, k, true))
-    return lin_backward_tc({dy, dy_stride, 1}, {x, xs0, xs1}, {w, ws0, ws1}, z, act, m, n, k, dx, dw, db, dz,
+  if (route.tensor)
+    return lin_backward_tc(route, {dy, dy_stride, 1}, {x, xs0, xs1}, {w, ws0, ws1}, z, act, m, n, k, dx, dw, db, dz,
                            workspace, s);
   LinCarve ws = {(char*)workspace, 0};
   float* own = (float*)ws.take(4 * m * n);

@@ -458,7 +458,15 @@ static DeviceRuntime* runtime_owning(void* ptr) {
 
 extern "C" int mm_free(void* ptr, void* stream) {
   if (ptr == nullptr) return MM_OK;
-  DeviceRuntime* rt = runtime_owning(ptr);
+  // Usually the block is the current device's; only otherwise is its device
+  // looked up.
+  DeviceRuntime* rt = runtime_for(current_device());
+  if (rt != nullptr && rt->arena->owns(ptr)) {
+    std::string msg;
+    const int rc = rt->arena->free(ptr, stream ? (cudaStream_t)stream : rt->stream, &msg);
+    return rc == MM_OK ? MM_OK : fail(rc, msg);
+  }
+  rt = runtime_owning(ptr);
   if (rt == nullptr) return fail(MM_ERR_STATE, "mm_free: pointer's device has no runtime");
   int prev = current_device();
   if (prev != rt->device) cudaSetDevice(rt->device);

@@ -32,6 +32,15 @@ F resolve(const char* name) {
   return reinterpret_cast<F>(p);
 }
 
+// The symbol, looked up once per use in the source: a lookup walks every loaded
+// library (several microseconds), and autograd switches devices and asks for
+// streams several times per operator.
+#define MM_SYMBOL(F, name)                \
+  ([]() -> F {                            \
+    static const F f = resolve<F>(name);  \
+    return f;                             \
+  }())
+
 thread_local int t_current_device = 0;
 
 // Upper bound of every stream wait the guard makes (matrixman.config
@@ -40,14 +49,14 @@ std::atomic<int64_t> g_wait_timeout_ms{600000};
 
 int device_count() {
   int n = 0;
-  if (resolve<count_fn>("mm_device_count")(&n) != 0) return 0;
+  if (MM_SYMBOL(count_fn, "mm_device_count")(&n) != 0) return 0;
   return n;
 }
 
 void* runtime_stream(int device) {
   void* s = nullptr;
-  resolve<dev_fn>("mm_init")(device);
-  resolve<stream_fn>("mm_runtime_stream")(device, &s);
+  MM_SYMBOL(dev_fn, "mm_init")(device);
+  MM_SYMBOL(stream_fn, "mm_runtime_stream")(device, &s);
   return s;
 }
 
@@ -56,7 +65,7 @@ constexpr int MM_STATUS_TIMEOUT = 5;  // MM_ERR_TIMEOUT of the C ABI
 // Bounded synchronisation of a device's runtime stream: raises with the C
 // ABI's message when the wait gives up (MM_ERR_TIMEOUT) or fails.
 void sync_runtime_stream(int device, const char* what) {
-  const int rc = resolve<sync_fn>("mm_stream_sync")(runtime_stream(device), g_wait_timeout_ms.load());
+  const int rc = MM_SYMBOL(sync_fn, "mm_stream_sync")(runtime_stream(device), g_wait_timeout_ms.load());
   if (rc == 0) return;
   char msg[512] = {0};
   using err_fn = int (*)(char*, size_t);
@@ -71,7 +80,7 @@ using pin_free_fn = int (*)(void*);
 using is_pinned_fn = int (*)(const void*, int*);
 
 void free_pinned(void* p) {
-  if (p) resolve<pin_free_fn>("mm_host_free_pinned")(p);
+  if (p) MM_SYMBOL(pin_free_fn, "mm_host_free_pinned")(p);
 }
 
 // Page-locked host memory for Tensor.pin_memory() on this backend, so that
@@ -81,7 +90,7 @@ class PinnedAllocator final : public c10::Allocator {
   c10::DataPtr allocate(size_t n) override {
     void* p = nullptr;
     if (n > 0) {
-      TORCH_CHECK(resolve<pin_alloc_fn>("mm_host_alloc_pinned")(n, &p) == 0,
+      TORCH_CHECK(MM_SYMBOL(pin_alloc_fn, "mm_host_alloc_pinned")(n, &p) == 0,
                   "matrixman: pinned host allocation of ", n, " bytes failed");
     }
     return {p, p, &free_pinned, c10::Device(c10::DeviceType::CPU)};
@@ -104,7 +113,7 @@ class MatrixManHooks final : public at::PrivateUse1HooksInterface {
   }
   bool isPinnedPtr(const void* data) const override {
     int pinned = 0;
-    resolve<is_pinned_fn>("mm_host_is_pinned")(data, &pinned);
+    MM_SYMBOL(is_pinned_fn, "mm_host_is_pinned")(data, &pinned);
     return pinned != 0;
   }
   c10::Allocator* getPinnedMemoryAllocator() const override { return &g_pinned; }
@@ -127,13 +136,13 @@ class MatrixManGuardImpl final : public c10::impl::DeviceGuardImplInterface {
   void setDevice(c10::Device d) const override {
     TORCH_CHECK(d.type() == c10::DeviceType::PrivateUse1, "matrixman guard: wrong device type");
     int idx = d.index() < 0 ? 0 : d.index();
-    TORCH_CHECK(resolve<dev_fn>("mm_set_device")(idx) == 0, "matrixman guard: cannot select device ", idx);
+    TORCH_CHECK(MM_SYMBOL(dev_fn, "mm_set_device")(idx) == 0, "matrixman guard: cannot select device ", idx);
     t_current_device = idx;
   }
 
   void uncheckedSetDevice(c10::Device d) const noexcept override {
     int idx = d.index() < 0 ? 0 : d.index();
-    void* p = dlsym(RTLD_DEFAULT, "mm_set_device");
+    static void* const p = dlsym(RTLD_DEFAULT, "mm_set_device");
     if (p) reinterpret_cast<dev_fn>(p)(idx);
     t_current_device = idx;
   }
@@ -148,7 +157,7 @@ class MatrixManGuardImpl final : public c10::impl::DeviceGuardImplInterface {
   c10::Stream exchangeStream(c10::Stream s) const noexcept override { return s; }
 
   c10::DeviceIndex deviceCount() const noexcept override {
-    void* p = dlsym(RTLD_DEFAULT, "mm_device_count");
+    static void* const p = dlsym(RTLD_DEFAULT, "mm_device_count");
     if (!p) return 0;
     int n = 0;
     if (reinterpret_cast<count_fn>(p)(&n) != 0) return 0;
@@ -157,7 +166,7 @@ class MatrixManGuardImpl final : public c10::impl::DeviceGuardImplInterface {
 
   bool queryStream(const c10::Stream& s) const override {
     int done = 1;
-    resolve<query_fn>("mm_stream_query")(runtime_stream(s.device_index()), &done);
+    MM_SYMBOL(query_fn, "mm_stream_query")(runtime_stream(s.device_index()), &done);
     return done != 0;
   }
 

@@ -573,13 +573,9 @@ def pointer(t: MatrixManTensor) -> int:
 
 def new_dense(rt: DeviceRuntime, shape: tuple) -> MatrixManTensor:
     """A new contiguous float32 tensor; shape is a tuple of ints."""
-    n = 1
-    strides = []
-    for s in reversed(shape):
-        strides.append(n)
-        n *= s if s > 1 else 1
-    owner = rt.new_storage(numel(shape))
-    return MatrixManTensor._wrap(owner, shape, 0, tuple(reversed(strides)))
+    if len(shape) == 2:
+        return MatrixManTensor._wrap(rt.new_storage(shape[0] * shape[1]), shape, 0, (shape[1] or 1, 1))
+    return MatrixManTensor._wrap(rt.new_storage(numel(shape)), shape, 0, contiguous_strides(shape))
 
 
 def _norm_rows(x: MatrixManTensor, shape: tuple, width: int) -> tuple[MatrixManTensor, int]:
@@ -632,13 +628,16 @@ def layer_norm(x, normalized_shape, weight=None, bias=None, eps=1e-5):
     lead = full[:len(full) - len(shape)]
     rows = numel(lead)
     xr, stride = _norm_rows(x, shape, width)
-    y = new_dense(rt, full)
     stat = lead + (1,) * len(shape)
     strides = contiguous_strides(stat)
-    stats = rt.new_storage(2 * rows)  # mean, then rstd
-    mean, rstd = (MatrixManTensor._wrap(stats, stat, at, strides) for at in (0, rows))
+    at = (rows * width + 63) // 64 * 64  # one block: y, mean, rstd
+    owner = rt.new_storage(at + 2 * rows)
+    y = MatrixManTensor._wrap(owner, full, 0, contiguous_strides(full))
+    mean = MatrixManTensor._wrap(owner, stat, at, strides)
+    rstd = MatrixManTensor._wrap(owner, stat, at + rows, strides)
+    p = owner.pointer
     _launch("mm_layer_norm", pointer(xr), stride, rows, width, None if w is None else pointer(w),
-            None if b is None else pointer(b), eps, y._owner.pointer, stats.pointer, stats.pointer + 4 * rows, rt.stream)
+            None if b is None else pointer(b), eps, p, p + 4 * at, p + 4 * (at + rows), rt.stream)
     return y, mean, rstd
 
 

@@ -117,7 +117,7 @@ class DeviceStorage:
             self.numel = numel
             self.kind = "cuda_linear"
 
-    __slots__ = ("runtime", "pointer", "nbytes", "dtype", "kind", "layout", "_released",
+    __slots__ = ("runtime", "pointer", "nbytes", "dtype", "kind", "_released",
                  "__weakref__", "keepalive")
 
     def __init__(self, runtime: "DeviceRuntime", pointer: int, nbytes: int, dtype: torch.dtype,
@@ -127,9 +127,12 @@ class DeviceStorage:
         self.nbytes = int(nbytes)
         self.dtype = dtype
         self.kind = kind
-        self.layout = DeviceStorage._Layout(nbytes // ELEMENT_SIZE[dtype])
         self._released = False
         self.keepalive = None
+
+    @property
+    def layout(self) -> "_Layout":
+        return DeviceStorage._Layout(self.nbytes // ELEMENT_SIZE[self.dtype])
 
     @property
     def device_index(self) -> int:
@@ -195,13 +198,16 @@ class DeviceRuntime:
         under the safe sync policy a reused block makes that stream wait for
         the block's release event."""
         out = ctypes.c_void_p()
-        _lib.check(self.lib.mm_alloc(self.index, max(int(nbytes), 1), kind,
-                                     self.stream if stream is None else stream,
-                                     ctypes.byref(out)), "allocate")
-        return int(out.value)
+        status = self.lib.mm_alloc(self.index, max(int(nbytes), 1), kind,
+                                   self.stream if stream is None else stream, ctypes.byref(out))
+        if status:
+            _lib.check(status, "allocate")
+        return out.value
 
     def free(self, pointer: int) -> None:
-        _lib.check(self.lib.mm_free(ctypes.c_void_p(pointer), self.stream), "free")
+        status = self.lib.mm_free(pointer, self.stream)
+        if status:
+            _lib.check(status, "free")
 
     def new_storage(self, numel: int, dtype: torch.dtype = torch.float32,
                     kind: int = _lib.POOL_ACTIVATION, stream=None) -> DeviceStorage:

@@ -224,6 +224,9 @@ def broadcast_shapes(*shapes) -> tuple[int, ...]:
 # The wrapper subclass.
 # ---------------------------------------------------------------------------
 
+_dispatch = None  # dispatch.handle_torch_dispatch, once a tensor has been used
+
+
 class MatrixManTensor(torch.Tensor):
     """Wrapper around a device storage owner (reference tensor.py:307-367)."""
 
@@ -291,8 +294,11 @@ class MatrixManTensor(torch.Tensor):
 
     @classmethod
     def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
-        from . import dispatch
-        return dispatch.handle_torch_dispatch(cls, func, types, args, kwargs)
+        global _dispatch
+        if _dispatch is None:
+            from .dispatch import handle_torch_dispatch
+            _dispatch = handle_torch_dispatch
+        return _dispatch(cls, func, types, args, kwargs)
 
     def __repr__(self):
         return (f"MatrixManTensor(shape={tuple(self.shape)}, dtype={self.dtype}, device={self.device}, "

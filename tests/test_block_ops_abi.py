@@ -67,7 +67,7 @@ def test_linear_checks():
         assert call(**{name: None}) == _lib.MM_ERR_INVALID
     assert call(m=1 << 31) == _lib.MM_ERR_UNSUPPORTED
     assert call(work=FAKE + 4) == _lib.MM_ERR_INVALID
-    assert call(m=512, n=512, k=512, size=8) == _lib.MM_ERR_INVALID
+    assert call(m=4096, n=4096, k=4096, size=8) == _lib.MM_ERR_INVALID
     assert call(m=0) == _lib.MM_OK and call(n=0) == _lib.MM_OK
 
     ok = dict(dy=FAKE, dys=6, x=FAKE, xs0=8, xs1=1, w=FAKE, ws0=8, ws1=1, z=FAKE, m=4, n=6, k=8, act=4, dx=FAKE,
