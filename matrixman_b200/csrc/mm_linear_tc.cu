@@ -129,7 +129,8 @@ __device__ int g_lin_error = 0;
 enum { LG_ERR_FULL = 101, LG_ERR_EMPTY = 102, LG_ERR_ACC = 103, LG_ERR_FREE = 104, LG_ERR_DRAIN = 105 };
 
 constexpr int LG_BM = 128, LG_BK = 32;
-constexpr int LG_EPI_WARPS = 8, LG_WARP_TMA = 8, LG_WARP_MMA = 9, LG_THREADS = 320;
+constexpr int LG_ACCS = 4;  // accumulators in tensor memory (at most 512 columns)
+constexpr int LG_EPI_WARPS = 8, LG_WARP_TMA = 8, LG_WARP_MMA = 9, LG_ISSUERS = 2, LG_THREADS = 352;
 constexpr uint64_t LG_WAIT_NS = 200ull * 1000 * 1000;
 
 __device__ __forceinline__ uint32_t lg_smem(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -247,7 +248,7 @@ struct LgTile {
 
 template <int BN>
 constexpr int lg_stages() {
-  return BN == 256 ? 3 : BN == 128 ? 4 : 6;
+  return BN == 128 ? 4 : 6;
 }
 
 // One unit of work: an output tile and a range of its reduction's stages.
@@ -346,13 +347,95 @@ __device__ __forceinline__ void lin_fix(const LinGemm& a, int m0, int rows, int 
   if (lin_flagged(a.pb, n0, n1)) lin_fix_lines<true>(a, m0, m1, n0, n1);
 }
 
+// Columns [c0, c0 + N) of one row of a finished tile, held by one thread.
+template <int N>
+__device__ __forceinline__ void lg_finish(const LinGemm& a, const LgUnit& w, float (&acc)[N], int r, int c0, int bn,
+                                          const float* bias_s) {
+  if (w.part >= 0) {
+    float4* part = reinterpret_cast<float4*>(a.part + ((int64_t)w.part * LG_BM + r) * bn + c0);
+#pragma unroll
+    for (int j = 0; j < N / 4; ++j) part[j] = make_float4(acc[4 * j], acc[4 * j + 1], acc[4 * j + 2], acc[4 * j + 3]);
+    return;
+  }
+  const LinEpilogue& e = a.e;
+  const int64_t row = (int64_t)w.m0 + r;
+  if (row >= a.m) return;
+  int col = w.n0 + c0;
+  float* out = a.c + row * a.n + col;
+  const float* res = e.residual ? e.residual + row * e.rs + col : nullptr;
+  float* z = e.z ? e.z + row * a.n + col : nullptr;
+  const bool whole = a.vec && col + N <= a.n && (!res || e.residual_vec) && (!z || e.z_vec);
+#pragma unroll
+  for (int j = 0; j < N / 4; ++j) {
+    const float4 b = reinterpret_cast<const float4*>(bias_s + c0)[j];
+    acc[4 * j] += b.x; acc[4 * j + 1] += b.y; acc[4 * j + 2] += b.z; acc[4 * j + 3] += b.w;
+  }
+  if (whole) {
+    if (res && e.residual_first) {
+#pragma unroll
+      for (int j = 0; j < N / 4; ++j) {
+        const float4 t = reinterpret_cast<const float4*>(res)[j];
+        acc[4 * j] += t.x; acc[4 * j + 1] += t.y; acc[4 * j + 2] += t.z; acc[4 * j + 3] += t.w;
+      }
+    }
+    if (z) {
+#pragma unroll
+      for (int j = 0; j < N / 4; ++j)
+        reinterpret_cast<float4*>(z)[j] = make_float4(acc[4 * j], acc[4 * j + 1], acc[4 * j + 2], acc[4 * j + 3]);
+    }
+    if (e.act <= MM_LINEAR_RELU) {
+#pragma unroll
+      for (int j = 0; j < N / 4; ++j) {
+        float4 t = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (res && !e.residual_first) t = reinterpret_cast<const float4*>(res)[j];
+        float v[4] = {acc[4 * j], acc[4 * j + 1], acc[4 * j + 2], acc[4 * j + 3]};
+        if (e.act == MM_LINEAR_RELU) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) v[i] = lin_act_t<MM_LINEAR_RELU>(v[i]);
+        }
+        reinterpret_cast<float4*>(out)[j] = make_float4(v[0] + t.x, v[1] + t.y, v[2] + t.z, v[3] + t.w);
+      }
+      return;
+    }
+  }
+  // Eight columns at a time; the totals move down by eight registers per step,
+  // so that the activations' code is there once.
+#pragma unroll 1
+  for (int j = 0; j < N / 8; ++j, col += 8) {
+    const int left = a.n - col;
+    if (left <= 0) return;
+    float v[8], t[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = acc[i];
+    if (res) {
+      lin_load_row<8>(res + 8 * j, left, whole, t);
+      if (!whole && e.residual_first) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] += t[i];
+      }
+    }
+    if (!whole && z) lin_store_row<8>(z + 8 * j, left, false, v);
+    lin_act<8>(v, e.act);
+    if (res && !e.residual_first) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] += t[i];
+    }
+    lin_store_row<8>(out + 8 * j, left, whole, v);
+#pragma unroll
+    for (int i = 0; i + 8 < N; ++i) acc[i] = acc[i + 8];
+  }
+}
+
 // Persistent CTAs, one per SM.  Warps 0-7 add up and store, warp 8 loads (TMA),
-// warp 9 issues the MMAs.  The MMAs of one stage (32 of the reduction, twelve
-// products of 128 x BN x 16) go into one of two accumulators in tensor memory,
-// small products first; warps 0-7 add it to float32 totals in registers while
-// the next stage runs in the other.  The tensor core rounds its sums toward
-// zero, which over a long reduction drifts by about K 2^-24; with one stage per
-// accumulator only the two a1 b1 products of a stage are added at full size.
+// warps 9 and 10 issue the MMAs of alternate stages.  The MMAs of one stage (32
+// of the reduction, twelve products of 128 x BN x 16) go into one of four
+// accumulators in tensor memory, small products first; warps 0-7 add it to
+// float32 totals in registers while the next stages run in the others.  The
+// tensor core rounds its sums toward zero, which over a long reduction drifts
+// by about K 2^-24; with one stage per accumulator only the two a1 b1 products
+// of a stage are added at full size.  One issuer left the tensor core idle for
+// the 300 to 400 clocks of its waits and commits in each stage (2000 x 1280 x
+// 1000: 49 us, with two 44).
 template <int BN, bool AMN, bool BMN>
 __global__ void __launch_bounds__(LG_THREADS, 1) linear_gemm_kernel(const __grid_constant__ CUtensorMap ma,
                                                                     const __grid_constant__ CUtensorMap mb,
@@ -361,25 +444,27 @@ __global__ void __launch_bounds__(LG_THREADS, 1) linear_gemm_kernel(const __grid
   using TB = LgTile<BN, BMN>;
   constexpr int S = lg_stages<BN>();
   constexpr uint32_t stage_bytes = TA::bytes + TB::bytes;
-  constexpr uint32_t cols = 2 * BN;
+  constexpr int ACCS = LG_ACCS;
+  constexpr uint32_t cols = ACCS * BN;
   constexpr int HALF = BN / 2;  // columns per warp
   extern __shared__ uint8_t raw[];
   uint8_t* smem = raw + ((1024 - (lg_smem(raw) & 1023)) & 1023);
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + S * stage_bytes);
-  uint64_t *empty = full + S, *acc_full = empty + S, *acc_free = acc_full + 2, *drain = acc_free + 2;
-  uint32_t* slot = reinterpret_cast<uint32_t*>(drain + 1);
+  uint64_t *empty = full + S, *acc_full = empty + S, *acc_free = acc_full + ACCS, *drain = acc_free + ACCS;
+  uint32_t* slot = reinterpret_cast<uint32_t*>(drain + LG_ISSUERS);
   int* special = reinterpret_cast<int*>(slot + 1);
+  float* bias_s = reinterpret_cast<float*>(smem + S * stage_bytes + 256);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int i = 0; i < S; ++i) {
       lg_bar_init(&full[i], 1);
       lg_bar_init(&empty[i], 1);
     }
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < ACCS; ++i) {
       lg_bar_init(&acc_full[i], 1);
       lg_bar_init(&acc_free[i], LG_EPI_WARPS);
     }
-    lg_bar_init(drain, 1);
+    for (int i = 0; i < LG_ISSUERS; ++i) lg_bar_init(&drain[i], 1);
     *special = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -394,79 +479,84 @@ __global__ void __launch_bounds__(LG_THREADS, 1) linear_gemm_kernel(const __grid
   const uint32_t tmem = *slot;
   pdl_wait();
 
+  // The loading and the issuing warps work with one thread each.
   if (warp == LG_WARP_TMA) {
-    int st = 0, filled = 0;
-    uint32_t par = 1;
-    bool alive = true;
-    for (int u = blockIdx.x; u < a.units && alive; u += gridDim.x) {
-      const LgUnit w = lg_unit(a, u, BN);
-      for (int k = w.begin; k < w.end; ++k) {
-        if (!__all_sync(0xffffffffu, lg_wait(&empty[st], par, LG_ERR_EMPTY))) {
-          alive = false;
-          break;
-        }
-        if (lg_elect()) {
+    if (lane == 0) {
+      int st = 0, filled = 0;
+      uint32_t par = 1;
+      bool alive = true;
+      for (int u = blockIdx.x; u < a.units && alive; u += gridDim.x) {
+        const LgUnit w = lg_unit(a, u, BN);
+        for (int k = w.begin; k < w.end; ++k) {
+          if (!lg_wait(&empty[st], par, LG_ERR_EMPTY)) {
+            alive = false;
+            break;
+          }
           asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(lg_smem(&full[st])),
                        "r"(stage_bytes)
                        : "memory");
           uint8_t* dst = smem + (uint32_t)st * stage_bytes;
           TA::load(dst, &ma, &full[st], w.m0, k * LG_BK);
           TB::load(dst + TA::bytes, &mb, &full[st], w.n0, k * LG_BK);
-        }
-        ++filled;
-        if (++st == S) {
-          st = 0;
-          par ^= 1u;
-        }
-      }
-    }
-    // Nothing may land in shared memory after the CTA has gone: wait for the
-    // last fill of every stage (over already unless a wait gave up).
-    for (int i = max(0, filled - S); i < filled; ++i) lg_wait(&full[i % S], (uint32_t)(i / S) & 1u, LG_ERR_DRAIN);
-  } else if (warp == LG_WARP_MMA) {
-    constexpr uint32_t idesc = 1u << 4 | 1u << 7 | 1u << 10 | (AMN ? 1u << 15 : 0u) | (BMN ? 1u << 16 : 0u) |
-                               (uint32_t)(BN >> 3) << 17 | (uint32_t)(LG_BM >> 4) << 24;
-    int st = 0, buf = 0;
-    uint32_t par = 0, bpar = 1;
-    bool alive = true;
-    for (int u = blockIdx.x; u < a.units && alive; u += gridDim.x) {
-      const LgUnit w = lg_unit(a, u, BN);
-      for (int k = w.begin; k < w.end; ++k) {
-        const bool ok = lg_wait(&acc_free[buf], bpar, LG_ERR_FREE) && lg_wait(&full[st], par, LG_ERR_FULL);
-        if (!__all_sync(0xffffffffu, ok)) {
-          alive = false;
-          break;
-        }
-        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        if (lg_elect()) {
-          const uint32_t at = lg_smem(smem + (uint32_t)st * stage_bytes), bt = at + TA::bytes;
-          const uint32_t d = tmem + (uint32_t)(buf * BN);
-          constexpr int pa[6] = {2, 0, 1, 0, 1, 0}, pb[6] = {0, 2, 1, 1, 0, 0};
-#pragma unroll
-          for (int q = 0; q < 6; ++q)
-#pragma unroll
-            for (int kk = 0; kk < 2; ++kk)
-              lg_mma(d, TA::desc(at, pa[q], kk), TB::desc(bt, pb[q], kk), idesc, q + kk > 0 ? 1u : 0u);
-          lg_commit(&empty[st]);
-          lg_commit(&acc_full[buf]);
-        }
-        if (++st == S) {
-          st = 0;
-          par ^= 1u;
-        }
-        if (++buf == 2) {
-          buf = 0;
-          bpar ^= 1u;
+          ++filled;
+          if (++st == S) {
+            st = 0;
+            par ^= 1u;
+          }
         }
       }
+      // Nothing may land in shared memory after the CTA has gone: wait for the
+      // last fill of every stage (over already unless a wait gave up).
+      for (int i = max(0, filled - S); i < filled; ++i) lg_wait(&full[i % S], (uint32_t)(i / S) & 1u, LG_ERR_DRAIN);
     }
-    // No MMA may still write tensor memory when it is freed.
     __syncwarp();
-    if (lg_elect()) lg_commit(drain);
+  } else if (warp >= LG_WARP_MMA) {
+    const int issuer = warp - LG_WARP_MMA;
+    if (lane == 0) {
+      constexpr uint32_t idesc = 1u << 4 | 1u << 7 | 1u << 10 | (AMN ? 1u << 15 : 0u) | (BMN ? 1u << 16 : 0u) |
+                                 (uint32_t)(BN >> 3) << 17 | (uint32_t)(LG_BM >> 4) << 24;
+      const uint32_t base = lg_smem(smem);
+      int st = 0, buf = 0;
+      uint32_t par = 0, bpar = 1;
+      bool alive = true;
+      for (int u = blockIdx.x; u < a.units && alive; u += gridDim.x) {
+        const LgUnit w = lg_unit(a, u, BN);
+        for (int k = w.begin; k < w.end; ++k) {
+          if (buf % LG_ISSUERS == issuer) {
+            if (!lg_wait(&acc_free[buf], bpar, LG_ERR_FREE) || !lg_wait(&full[st], par, LG_ERR_FULL)) {
+              alive = false;
+              break;
+            }
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            const uint32_t at = base + (uint32_t)st * stage_bytes, bt = at + TA::bytes;
+            const uint32_t d = tmem + (uint32_t)(buf * BN);
+            constexpr int pa[6] = {2, 0, 1, 0, 1, 0}, pb[6] = {0, 2, 1, 1, 0, 0};
+#pragma unroll
+            for (int q = 0; q < 6; ++q)
+#pragma unroll
+              for (int kk = 0; kk < 2; ++kk)
+                lg_mma(d, TA::desc(at, pa[q], kk), TB::desc(bt, pb[q], kk), idesc, q + kk > 0 ? 1u : 0u);
+            lg_commit(&empty[st]);
+            lg_commit(&acc_full[buf]);
+          }
+          if (++st == S) {
+            st = 0;
+            par ^= 1u;
+          }
+          if (++buf == ACCS) {
+            buf = 0;
+            bpar ^= 1u;
+          }
+        }
+      }
+      // No MMA may still write tensor memory when it is freed.
+      lg_commit(&drain[issuer]);
+      lg_wait(&drain[issuer], 0u, LG_ERR_DRAIN);
+    }
     __syncwarp();
-    lg_wait(drain, 0u, LG_ERR_DRAIN);
   } else {
-    const int quarter = warp & 3, half = warp >> 2;
+    const int quarter = warp & 3, half = warp >> 2, row_in_tile = quarter * 32 + lane;
+    int tile = 0;
     const uint32_t base = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(half * HALF);
     int buf = 0;
     uint32_t par = 0;
@@ -477,6 +567,10 @@ __global__ void __launch_bounds__(LG_THREADS, 1) linear_gemm_kernel(const __grid
     if (inf) *special = 1;
     for (int u = blockIdx.x; u < a.units && alive; u += gridDim.x) {
       const LgUnit w = lg_unit(a, u, BN);
+      // The tile's bias, for use after its stages (two tiles' worth, so that no
+      // warp overwrites what a slower one still reads).
+      if (threadIdx.x < BN) bias_s[(tile & 1) * BN + threadIdx.x] = w.n0 + (int)threadIdx.x < a.n && a.e.bias ? a.e.bias[w.n0 + threadIdx.x] : 0.f;
+      asm volatile("bar.sync 1, %0;" ::"n"(LG_EPI_WARPS * 32) : "memory");
       float acc[HALF];
 #pragma unroll
       for (int i = 0; i < HALF; ++i) acc[i] = 0.f;
@@ -496,31 +590,14 @@ __global__ void __launch_bounds__(LG_THREADS, 1) linear_gemm_kernel(const __grid
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
         __syncwarp();
         if (lane == 0) lg_arrive(&acc_free[buf]);
-        if (++buf == 2) {
+        if (++buf == ACCS) {
           buf = 0;
           par ^= 1u;
         }
       }
       if (!alive) break;
-      const int64_t row = (int64_t)w.m0 + quarter * 32 + lane;
-      int col = w.n0 + half * HALF;
-      float* part = w.part >= 0 ? a.part + ((int64_t)w.part * LG_BM + quarter * 32 + lane) * BN + half * HALF : nullptr;
-      // Eight columns at a time; the totals move down by eight registers per
-      // step, so that the epilogue's code is there once.
-#pragma unroll 1
-      for (int j = 0; j < HALF / 8; ++j, col += 8) {
-        if (part) {
-          reinterpret_cast<float4*>(part)[2 * j] = make_float4(acc[0], acc[1], acc[2], acc[3]);
-          reinterpret_cast<float4*>(part)[2 * j + 1] = make_float4(acc[4], acc[5], acc[6], acc[7]);
-        } else if (row < a.m && col < a.n) {
-          float v[8];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) v[e] = acc[e];
-          lin_finish_row<8>(a.e, v, a.c, row, col, a.n, a.vec);
-        }
-#pragma unroll
-        for (int i = 0; i + 8 < HALF; ++i) acc[i] = acc[i + 8];
-      }
+      lg_finish<HALF>(a, w, acc, row_in_tile, half * HALF, BN, bias_s + (tile & 1) * BN);
+      ++tile;
     }
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -593,17 +670,19 @@ int lin_run_splits(const LinSplits& all, cudaStream_t s) {
 }
 
 // Tile width and division of the reduction, by an estimate in SM clocks: a
-// stage takes 6 BN clocks of MMAs (and no less than about 500 for its loads and
-// barriers), a tile about 4,000 more to fill the pipeline and store.  Whole
-// waves of tiles run undivided; the rest is divided where that ends sooner
-// although its partial tiles are written and read once more.
+// stage takes 850 (BN 128: 768 of MMAs) or 610 (BN 64: 384; loads and barriers
+// bound it), a tile about 4,000 more to fill the pipeline and store.  Tiles 256
+// wide, whose two accumulators leave the MMAs waiting for the additions, were
+// slower at every size (8192 x 2048 x 4096: 689 us, 128 wide 664, 64 wide 936).
+// Whole waves of tiles run undivided; the rest is divided where that ends
+// sooner although its partial tiles are written and read once more.
 LinChoice lin_choose(int64_t m, int64_t n, int64_t k) {
   const int sms = sm_count();
   LinChoice best = {};
-  for (int bn : {256, 128, 64}) {
+  for (int bn : {128, 64}) {
     const int64_t tm = (m + LG_BM - 1) / LG_BM, tn = (n + bn - 1) / bn, tiles = tm * tn;
     const int64_t stages = (k + LG_BK - 1) / LG_BK;
-    const double stage = 6.0 * bn < 500 ? 500 : 6.0 * bn, tile = 4000;
+    const double stage = bn == 128 ? 850 : 610, tile = 4000;
     const int64_t full = tiles / sms * sms, rest = tiles - full;
     const double base = (double)(full / sms) * (stages * stage + tile);
     for (int s = 1; s <= LIN_MAX_SPLITS; ++s) {
@@ -657,7 +736,8 @@ static int lin_map(const LinPlanes& p, int rows, CUtensorMap* out) {
 
 template <int BN, bool AMN, bool BMN>
 static int lin_launch(const CUtensorMap& ma, const CUtensorMap& mb, const LinGemm& g, cudaStream_t s) {
-  constexpr size_t smem = 1024 + (size_t)lg_stages<BN>() * (LG_BM + BN) * 192 + 256;
+  // alignment, stages, barriers, two tiles' bias
+  constexpr size_t smem = 1024 + (size_t)lg_stages<BN>() * (LG_BM + BN) * 192 + 256 + 8 * BN;
   auto kernel = linear_gemm_kernel<BN, AMN, BMN>;
   MM_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem),
           "mm_linear: shared memory attribute");
@@ -698,9 +778,7 @@ int lin_run_gemm(const LinPlanes& pa, const LinPlanes& pb, float* c, const LinEp
   int rc = lin_map(pa, LG_BM, &ma);
   if (rc == MM_OK) rc = lin_map(pb, ch.bn, &mb);
   if (rc != MM_OK) return rc;
-  rc = ch.bn == 256   ? lin_launch_bn<256>(pa.mn, pb.mn, ma, mb, g, s)
-       : ch.bn == 128 ? lin_launch_bn<128>(pa.mn, pb.mn, ma, mb, g, s)
-                      : lin_launch_bn<64>(pa.mn, pb.mn, ma, mb, g, s);
+  rc = ch.bn == 128 ? lin_launch_bn<128>(pa.mn, pb.mn, ma, mb, g, s) : lin_launch_bn<64>(pa.mn, pb.mn, ma, mb, g, s);
   if (rc != MM_OK) return rc;
   if (ch.splits > 1) {
     const unsigned grid = (unsigned)((ch.units - ch.full) / ch.splits * (LG_BM / 8));
