@@ -22,28 +22,38 @@ struct LinProduct {
 };
 
 // ---------------------------------------------------------------------------
-// Small products: 32 x 32 outputs per block, the reduction in chunks of 64
-// shared by eight warps (each takes eight of a chunk), whose sums are added in
-// order at the end.  A lane holds 4 x 8 outputs and reads its lines of A and B
-// in 16-byte pieces along the reduction: 12 such reads feed 128 multiply-adds.
-// Used where a product is so small that latency bounds it: many blocks with a
-// short walk each, one launch, no workspace.
+// Small products: 32 x 32 outputs per block, the reduction in chunks of eight
+// per warp (64 or 128), whose sums are added in order at the end.  A lane holds
+// 4 x 8 outputs and reads its lines of A and B in 16-byte pieces along the
+// reduction: 12 such reads feed 128 multiply-adds.  Used where a product is so
+// small that latency bounds it: many blocks with a short walk each, one launch,
+// no workspace.  Sixteen warps where a block has an SM to itself anyway.
 // ---------------------------------------------------------------------------
 
-constexpr int LS_T = 32, LS_K = 64, LS_ROW = LS_K + 4;  // + 4: 16-byte reads of neighbouring lines hit other banks
+constexpr int LS_T = 32;
+
+template <int NW>
+struct LsShape {
+  static constexpr int K = 8 * NW, ROW = K + 4;  // + 4: 16-byte reads of neighbouring lines hit other banks
+  static constexpr int TILE = LS_T * ROW;
+  // two buffers of A's and B's tile; at the end the warps' sums [NW][32][33]
+  static constexpr int FLOATS = 4 * TILE > NW * LS_T * 33 ? 4 * TILE : NW * LS_T * 33;
+};
 
 // How an operand's tile is read: 16 bytes along the reduction, along the lines,
 // or value by value.
 enum { LS_ALONG_K = 0, LS_ALONG_LINES = 1, LS_SINGLE = 2 };
 
-// The eight values of a 32 x 64 tile that a thread brings in.
+// The eight values of a 32 x K tile that a thread brings in.
+template <int NW>
 __device__ __forceinline__ void ls_fetch(const float* p, int64_t s0, int64_t s1, int lines, int k, int l0, int k0,
                                          int mode, float (&v)[8]) {
+  constexpr int KQ = 2 * NW;  // 16-byte pieces along the reduction
   const int t = threadIdx.x;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    const int line = mode == LS_ALONG_LINES ? (t & 7) * 4 : i * 16 + (t >> 4);
-    const int kk = mode == LS_ALONG_LINES ? i * 32 + (t >> 3) : (t & 15) * 4;
+    const int line = mode == LS_ALONG_LINES ? (t & 7) * 4 : i * 16 + t / KQ;
+    const int kk = mode == LS_ALONG_LINES ? i * 4 * NW + (t >> 3) : t % KQ * 4;
     const int l = l0 + line, kg = k0 + kk;
     if (mode == LS_ALONG_K && l < lines && kg + 4 <= k) {
       const float4 q = *reinterpret_cast<const float4*>(p + l * s0 + kg);
@@ -61,64 +71,73 @@ __device__ __forceinline__ void ls_fetch(const float* p, int64_t s0, int64_t s1,
   }
 }
 
+template <int NW>
 __device__ __forceinline__ void ls_put(float* tile, int mode, const float (&v)[8]) {
+  constexpr int KQ = 2 * NW, ROW = LsShape<NW>::ROW;
   const int t = threadIdx.x;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     if (mode == LS_ALONG_LINES) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) tile[((t & 7) * 4 + e) * LS_ROW + i * 32 + (t >> 3)] = v[4 * i + e];
+      for (int e = 0; e < 4; ++e) tile[((t & 7) * 4 + e) * ROW + i * 4 * NW + (t >> 3)] = v[4 * i + e];
     } else {
-      *reinterpret_cast<float4*>(tile + (i * 16 + (t >> 4)) * LS_ROW + (t & 15) * 4) =
+      *reinterpret_cast<float4*>(tile + (i * 16 + t / KQ) * ROW + t % KQ * 4) =
           make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
     }
   }
 }
 
-__global__ void __launch_bounds__(256) linear_small_kernel(LinProduct p, LinEpilogue e, int tiles_n, int amode,
-                                                           int bmode, int vec) {
-  __shared__ float4 mem[2 * 2 * LS_T * LS_ROW / 4];
-  float* tiles = reinterpret_cast<float*>(mem);
+template <int NW>
+__global__ void __launch_bounds__(NW * 32) linear_small_kernel(LinProduct p, LinEpilogue e, int tiles_n, int amode,
+                                                               int bmode, int vec) {
+  using S = LsShape<NW>;
+  extern __shared__ float4 ls_mem[];
+  float* tiles = reinterpret_cast<float*>(ls_mem);
   const int m0 = (int)(blockIdx.x / tiles_n) * LS_T, n0 = (int)(blockIdx.x % tiles_n) * LS_T;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int ga = lane >> 2, gb = lane & 3;  // A lines 4 ga + i, B lines gb + 4 j
   float acc[4][8] = {};
-  float av[8], bv[8];
+  float av[2][8], bv[2][8];  // the next two chunks, on their way
   pdl_wait();
-  ls_fetch(p.a, p.as0, p.as1, p.m, p.k, m0, 0, amode, av);
-  ls_fetch(p.b, p.bs0, p.bs1, p.n, p.k, n0, 0, bmode, bv);
-  int buf = 0;
-  for (int k0 = 0; k0 < p.k; k0 += LS_K, buf ^= 1) {
-    float* ta = tiles + buf * 2 * LS_T * LS_ROW;
-    float* tb = ta + LS_T * LS_ROW;
-    ls_put(ta, amode, av);
-    ls_put(tb, bmode, bv);
-    __syncthreads();  // also: every warp has finished with this buffer's last chunk
-    if (k0 + LS_K < p.k) {
-      ls_fetch(p.a, p.as0, p.as1, p.m, p.k, m0, k0 + LS_K, amode, av);
-      ls_fetch(p.b, p.bs0, p.bs1, p.n, p.k, n0, k0 + LS_K, bmode, bv);
-    }
 #pragma unroll
-    for (int q = 0; q < 2; ++q) {
-      const int kk = warp * 8 + q * 4;
-      float4 a[4], b[8];
+  for (int i = 0; i < 2; ++i) {
+    ls_fetch<NW>(p.a, p.as0, p.as1, p.m, p.k, m0, i * S::K, amode, av[i]);
+    ls_fetch<NW>(p.b, p.bs0, p.bs1, p.n, p.k, n0, i * S::K, bmode, bv[i]);
+  }
+  for (int k0 = 0; k0 < p.k; k0 += 2 * S::K) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) a[i] = *reinterpret_cast<const float4*>(ta + (ga * 4 + i) * LS_ROW + kk);
+    for (int i = 0; i < 2; ++i) {
+      if (k0 + i * S::K >= p.k) break;
+      float* ta = tiles + i * 2 * S::TILE;
+      float* tb = ta + S::TILE;
+      ls_put<NW>(ta, amode, av[i]);
+      ls_put<NW>(tb, bmode, bv[i]);
+      __syncthreads();  // also: every warp has finished with this buffer's last chunk
+      if (k0 + (i + 2) * S::K < p.k) {
+        ls_fetch<NW>(p.a, p.as0, p.as1, p.m, p.k, m0, k0 + (i + 2) * S::K, amode, av[i]);
+        ls_fetch<NW>(p.b, p.bs0, p.bs1, p.n, p.k, n0, k0 + (i + 2) * S::K, bmode, bv[i]);
+      }
 #pragma unroll
-      for (int j = 0; j < 8; ++j) b[j] = *reinterpret_cast<const float4*>(tb + (gb + 4 * j) * LS_ROW + kk);
+      for (int q = 0; q < 2; ++q) {
+        const int kk = warp * 8 + q * 4;
+        float4 a[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+        for (int x = 0; x < 4; ++x) a[x] = *reinterpret_cast<const float4*>(ta + (ga * 4 + x) * S::ROW + kk);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          acc[i][j] += a[i].x * b[j].x;
-          acc[i][j] += a[i].y * b[j].y;
-          acc[i][j] += a[i].z * b[j].z;
-          acc[i][j] += a[i].w * b[j].w;
+        for (int y = 0; y < 8; ++y) {
+          const float4 b = *reinterpret_cast<const float4*>(tb + (gb + 4 * y) * S::ROW + kk);
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            acc[x][y] += a[x].x * b.x;
+            acc[x][y] += a[x].y * b.y;
+            acc[x][y] += a[x].z * b.z;
+            acc[x][y] += a[x].w * b.w;
+          }
         }
+      }
     }
   }
   __syncthreads();
-  // The warps' sums, [8][32][33] floats, fit where the tiles were.
   float* red = tiles;
 #pragma unroll
   for (int i = 0; i < 4; ++i)
@@ -127,13 +146,26 @@ __global__ void __launch_bounds__(256) linear_small_kernel(LinProduct p, LinEpil
   __syncthreads();
   const int r = threadIdx.x >> 3, c = (threadIdx.x & 7) * 4;
   const int row = m0 + r, col = n0 + c;
-  if (row >= p.m || col >= p.n) return;
+  if (r >= LS_T || row >= p.m || col >= p.n) return;
   float v[4] = {};
 #pragma unroll
-  for (int w = 0; w < 8; ++w)
+  for (int w = 0; w < NW; ++w)
 #pragma unroll
     for (int j = 0; j < 4; ++j) v[j] += red[(w * LS_T + r) * 33 + c + j];
   lin_finish_row<4>(e, v, p.c, row, col, p.n, vec);
+}
+
+template <int NW>
+static cudaError_t lin_small(const LinProduct& p, const LinEpilogue& e, int64_t tiles, int tiles_n, int amode, int bmode,
+                             int vec, cudaStream_t s) {
+  constexpr size_t smem = LsShape<NW>::FLOATS * sizeof(float);
+  if (smem > 48 * 1024) {
+    const cudaError_t err =
+        cudaFuncSetAttribute(linear_small_kernel<NW>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (err != cudaSuccess) return err;
+  }
+  return launch_pdl(linear_small_kernel<NW>, dim3((unsigned)tiles), dim3(NW * 32), smem, s, p, e, tiles_n, amode, bmode,
+                    vec);
 }
 
 // ---------------------------------------------------------------------------
@@ -248,7 +280,7 @@ struct LinMatrix {
   int64_t s0, s1;
 };
 
-constexpr int LIN_TOKENS = 8;  // rows up to which a product is a walk over the weight
+constexpr int LIN_TOKENS = 16;  // rows up to which a product is a walk over the weight
 
 static bool lin_aligned(const float* p, int64_t stride) { return (uintptr_t)p % 16 == 0 && stride % 4 == 0; }
 
@@ -258,7 +290,7 @@ static void lin_tokens(const LinProduct& p, const LinEpilogue& e, cudaStream_t s
   // least one 16-byte piece per lane.
   const int64_t groups = (int64_t)((p.n + CN - 1) / CN) * ((p.m + MT - 1) / MT);
   int kw = 1;
-  while (kw < 8 && groups * kw * 2 <= (int64_t)sm_count() * 32 && p.k >= kw * 2 * 128) kw *= 2;
+  while (kw < 8 && groups * kw * 2 <= (int64_t)sm_count() * (MT == 1 ? 64 : 32) && p.k >= kw * 2 * 128) kw *= 2;
   const int per = 8 / kw * CN;
   const dim3 grid((unsigned)((p.n + per - 1) / per), (unsigned)((p.m + MT - 1) / MT));
   if (lin_aligned(p.a, p.m > 1 ? p.as0 : 0) && lin_aligned(p.b, p.n > 1 ? p.bs0 : 0) && p.k % 4 == 0)
@@ -278,7 +310,7 @@ static int lin_product(const LinProduct& p, const LinEpilogue& e, cudaStream_t s
   if (p.m == 0 || p.n == 0) return MM_OK;
   if (p.m <= LIN_TOKENS && p.as1 == 1 && p.bs1 == 1 && p.k > 0) {
     if (p.m == 1)
-      lin_tokens<1, 2>(p, e, s);
+      lin_tokens<1, 4>(p, e, s);
     else if (p.m == 2)
       lin_tokens<2, 2>(p, e, s);
     else if (p.m <= 4)
@@ -290,8 +322,10 @@ static int lin_product(const LinProduct& p, const LinEpilogue& e, cudaStream_t s
     const int64_t tiles = (int64_t)tiles_n * ((p.m + LS_T - 1) / LS_T);
     if (tiles > INT32_MAX) return fail(MM_ERR_UNSUPPORTED, "mm_linear: output too large");
     const int vec = p.n % 4 == 0 && (uintptr_t)p.c % 16 == 0;
-    launch_pdl(linear_small_kernel, dim3((unsigned)tiles), dim3(256), 0, s, p, e, tiles_n, ls_mode(p.a, p.as0, p.as1),
-               ls_mode(p.b, p.bs0, p.bs1), vec);
+    const int amode = ls_mode(p.a, p.as0, p.as1), bmode = ls_mode(p.b, p.bs0, p.bs1);
+    MM_CUDA(tiles <= sm_count() && p.k > 256 ? lin_small<16>(p, e, tiles, tiles_n, amode, bmode, vec, s)
+                                             : lin_small<8>(p, e, tiles, tiles_n, amode, bmode, vec, s),
+            "mm_linear launch");
   }
   MM_LAUNCH_CHECK("mm_linear launch");
   return MM_OK;
@@ -299,18 +333,23 @@ static int lin_product(const LinProduct& p, const LinEpilogue& e, cudaStream_t s
 
 constexpr int LIN_DZ_ROWS = 256;  // partial rows of the bias gradient
 
-// Clocks of a small product: 148 blocks at a time, a chunk of 64 of the
-// reduction in about 600 (latency with one block per SM, multiply-adds with
-// several), 1,500 to start and end each, and 3,000 once.
+// Clocks of a small product: a block per SM at a time, 64 of the reduction in
+// about 1,700 (with one block per SM latency, with several the multiply-adds
+// and their operands from shared memory), 3,500 to start and end, and 3,000
+// once.  Measured: 128 x 1024 x 1024 18 us, 512 x 512 x 512 19 us, 64 x 4096 x
+// 4096 112 us.
 static double lin_small_clocks(int64_t m, int64_t n, int64_t k) {
   const int64_t tiles = ((m + LS_T - 1) / LS_T) * ((n + LS_T - 1) / LS_T);
   const int64_t waves = (tiles + sm_count() - 1) / sm_count();
-  return 3000.0 + waves * (1500.0 + 600.0 * ((k + LS_K - 1) / LS_K));
+  return 3000.0 + waves * (3500.0 + 1700.0 * ((k + 63) / 64));
 }
 
 // How a call runs: on the tensor cores where the estimate of its products, with
 // 10 bytes per value to split the operands (about 3,400 bytes per clock) and
-// 5,000 clocks for the launches this takes, is below the small kernels'.
+// 24,000 clocks for the launches this takes (34,000 in the backward pass), is
+// below the small kernels'.  Measured on both sides: 128 x 1024 x 1024 25 us
+// against the small kernel's 18, 256 x 1024 x 1024 26 against 32, 8192 x 256 x
+// 256 24 against 68.
 // `first` is the forward product or dx, `second` dw.
 struct LinRoute {
   bool tensor;
@@ -320,7 +359,7 @@ struct LinRoute {
 static LinRoute lin_route(int64_t m, int64_t n, int64_t k, bool backward) {
   LinRoute r = {};
   if ((m <= LIN_TOKENS && !backward) || m <= 0 || n < 32 || k < 32) return r;
-  double small, tensor = 5000;
+  double small, tensor = backward ? 34000 : 24000;
   if (backward) {
     small = lin_small_clocks(m, k, n) + lin_small_clocks(n, k, m);
     r.first = lin_choose(m, k, n);

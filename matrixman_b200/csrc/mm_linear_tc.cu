@@ -248,7 +248,7 @@ struct LgTile {
 
 template <int BN>
 constexpr int lg_stages() {
-  return BN == 128 ? 4 : 6;
+  return BN == 128 ? 4 : 5;
 }
 
 // One unit of work: an output tile and a range of its reduction's stages.
@@ -347,82 +347,88 @@ __device__ __forceinline__ void lin_fix(const LinGemm& a, int m0, int rows, int 
   if (lin_flagged(a.pb, n0, n1)) lin_fix_lines<true>(a, m0, m1, n0, n1);
 }
 
-// Columns [c0, c0 + N) of one row of a finished tile, held by one thread.
+// The epilogue of N columns from col on of one row, held by one thread, where
+// all of them exist and rows are 16-byte aligned.
 template <int N>
-__device__ __forceinline__ void lg_finish(const LinGemm& a, const LgUnit& w, float (&acc)[N], int r, int c0, int bn,
-                                          const float* bias_s) {
-  if (w.part >= 0) {
-    float4* part = reinterpret_cast<float4*>(a.part + ((int64_t)w.part * LG_BM + r) * bn + c0);
-#pragma unroll
-    for (int j = 0; j < N / 4; ++j) part[j] = make_float4(acc[4 * j], acc[4 * j + 1], acc[4 * j + 2], acc[4 * j + 3]);
-    return;
-  }
+__device__ __forceinline__ void lg_finish_row(const LinGemm& a, float (&acc)[N], int64_t row, int col) {
   const LinEpilogue& e = a.e;
-  const int64_t row = (int64_t)w.m0 + r;
   if (row >= a.m) return;
-  int col = w.n0 + c0;
   float* out = a.c + row * a.n + col;
   const float* res = e.residual ? e.residual + row * e.rs + col : nullptr;
-  float* z = e.z ? e.z + row * a.n + col : nullptr;
-  const bool whole = a.vec && col + N <= a.n && (!res || e.residual_vec) && (!z || e.z_vec);
+  if (e.bias) {
 #pragma unroll
-  for (int j = 0; j < N / 4; ++j) {
-    const float4 b = reinterpret_cast<const float4*>(bias_s + c0)[j];
-    acc[4 * j] += b.x; acc[4 * j + 1] += b.y; acc[4 * j + 2] += b.z; acc[4 * j + 3] += b.w;
+    for (int j = 0; j < N / 4; ++j) {
+      const float4 b = reinterpret_cast<const float4*>(e.bias + col)[j];
+      acc[4 * j] += b.x; acc[4 * j + 1] += b.y; acc[4 * j + 2] += b.z; acc[4 * j + 3] += b.w;
+    }
   }
-  if (whole) {
-    if (res && e.residual_first) {
+  if (res && e.residual_first) {
 #pragma unroll
-      for (int j = 0; j < N / 4; ++j) {
-        const float4 t = reinterpret_cast<const float4*>(res)[j];
-        acc[4 * j] += t.x; acc[4 * j + 1] += t.y; acc[4 * j + 2] += t.z; acc[4 * j + 3] += t.w;
-      }
+    for (int j = 0; j < N / 4; ++j) {
+      const float4 t = reinterpret_cast<const float4*>(res)[j];
+      acc[4 * j] += t.x; acc[4 * j + 1] += t.y; acc[4 * j + 2] += t.z; acc[4 * j + 3] += t.w;
     }
-    if (z) {
+  }
+  if (e.z) {
+    float4* z = reinterpret_cast<float4*>(e.z + row * a.n + col);
 #pragma unroll
-      for (int j = 0; j < N / 4; ++j)
-        reinterpret_cast<float4*>(z)[j] = make_float4(acc[4 * j], acc[4 * j + 1], acc[4 * j + 2], acc[4 * j + 3]);
-    }
-    if (e.act <= MM_LINEAR_RELU) {
-#pragma unroll
-      for (int j = 0; j < N / 4; ++j) {
-        float4 t = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (res && !e.residual_first) t = reinterpret_cast<const float4*>(res)[j];
-        float v[4] = {acc[4 * j], acc[4 * j + 1], acc[4 * j + 2], acc[4 * j + 3]};
-        if (e.act == MM_LINEAR_RELU) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) v[i] = lin_act_t<MM_LINEAR_RELU>(v[i]);
-        }
-        reinterpret_cast<float4*>(out)[j] = make_float4(v[0] + t.x, v[1] + t.y, v[2] + t.z, v[3] + t.w);
-      }
-      return;
-    }
+    for (int j = 0; j < N / 4; ++j) z[j] = make_float4(acc[4 * j], acc[4 * j + 1], acc[4 * j + 2], acc[4 * j + 3]);
   }
   // Eight columns at a time; the totals move down by eight registers per step,
   // so that the activations' code is there once.
 #pragma unroll 1
-  for (int j = 0; j < N / 8; ++j, col += 8) {
-    const int left = a.n - col;
-    if (left <= 0) return;
+  for (int j = 0; j < N / 8; ++j) {
     float v[8], t[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = acc[i];
-    if (res) {
-      lin_load_row<8>(res + 8 * j, left, whole, t);
-      if (!whole && e.residual_first) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] += t[i];
-      }
-    }
-    if (!whole && z) lin_store_row<8>(z + 8 * j, left, false, v);
+    if (res && !e.residual_first) lin_load_row<8>(res + 8 * j, 8, true, t);
     lin_act<8>(v, e.act);
     if (res && !e.residual_first) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) v[i] += t[i];
     }
-    lin_store_row<8>(out + 8 * j, left, whole, v);
+    lin_store_row<8>(out + 8 * j, 8, true, v);
 #pragma unroll
     for (int i = 0; i + 8 < N; ++i) acc[i] = acc[i + 8];
+  }
+}
+
+// The epilogue elsewhere (a width that is no multiple of four, the last tile's
+// columns): of 32 x 32 outputs that a warp has put into shared memory (row r,
+// column c at 32 r + (c ^ r): no bank conflicts either way), a column per lane,
+// so that every row is read and written in one piece of 128 bytes whatever its
+// alignment.  1111 x 1502 x 2501: 72 us, a row per thread 83; where both apply
+// (2000 x 1280 x 1000) 47, a row per thread 41.
+template <int ACT>
+__device__ __forceinline__ void lg_finish_rows(const LinGemm& a, const float* tile, int row0, int col, int lane) {
+  const LinEpilogue& e = a.e;
+  const bool valid = col < a.n;
+  const int rows = min(32, a.m - row0);
+  const float bias = e.bias && valid ? e.bias[col] : 0.f;
+  const float* res = e.residual ? e.residual + (int64_t)row0 * e.rs + col : nullptr;
+  float* z = e.z ? e.z + (int64_t)row0 * a.n + col : nullptr;
+  float* out = a.c + (int64_t)row0 * a.n + col;
+  constexpr int U = 8;  // rows at a time: their residuals are on their way together
+  for (int r0 = 0; r0 < rows; r0 += U) {
+    float t[U] = {}, v[U];
+    if (res) {
+#pragma unroll
+      for (int i = 0; i < U; ++i)
+        if (valid && r0 + i < rows) t[i] = res[(r0 + i) * e.rs];
+    }
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const int r = r0 + i;
+      v[i] = tile[32 * r + (lane ^ r)] + bias;
+      if (e.residual_first) v[i] += t[i];
+      if (z && valid && r < rows) z[(int64_t)r * a.n] = v[i];
+    }
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      v[i] = lin_act_t<ACT>(v[i]);
+      if (!e.residual_first) v[i] += t[i];
+      if (valid && r0 + i < rows) out[(int64_t)(r0 + i) * a.n] = v[i];
+    }
   }
 }
 
@@ -453,7 +459,7 @@ __global__ void __launch_bounds__(LG_THREADS, 1) linear_gemm_kernel(const __grid
   uint64_t *empty = full + S, *acc_full = empty + S, *acc_free = acc_full + ACCS, *drain = acc_free + ACCS;
   uint32_t* slot = reinterpret_cast<uint32_t*>(drain + LG_ISSUERS);
   int* special = reinterpret_cast<int*>(slot + 1);
-  float* bias_s = reinterpret_cast<float*>(smem + S * stage_bytes + 256);
+  float* store = reinterpret_cast<float*>(smem + S * stage_bytes + 256);  // a 32 x 32 block per adding warp
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int i = 0; i < S; ++i) {
@@ -555,8 +561,8 @@ __global__ void __launch_bounds__(LG_THREADS, 1) linear_gemm_kernel(const __grid
     }
     __syncwarp();
   } else {
-    const int quarter = warp & 3, half = warp >> 2, row_in_tile = quarter * 32 + lane;
-    int tile = 0;
+    const int quarter = warp & 3, half = warp >> 2;
+    float* stage = store + warp * 1024;
     const uint32_t base = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(half * HALF);
     int buf = 0;
     uint32_t par = 0;
@@ -567,10 +573,6 @@ __global__ void __launch_bounds__(LG_THREADS, 1) linear_gemm_kernel(const __grid
     if (inf) *special = 1;
     for (int u = blockIdx.x; u < a.units && alive; u += gridDim.x) {
       const LgUnit w = lg_unit(a, u, BN);
-      // The tile's bias, for use after its stages (two tiles' worth, so that no
-      // warp overwrites what a slower one still reads).
-      if (threadIdx.x < BN) bias_s[(tile & 1) * BN + threadIdx.x] = w.n0 + (int)threadIdx.x < a.n && a.e.bias ? a.e.bias[w.n0 + threadIdx.x] : 0.f;
-      asm volatile("bar.sync 1, %0;" ::"n"(LG_EPI_WARPS * 32) : "memory");
       float acc[HALF];
 #pragma unroll
       for (int i = 0; i < HALF; ++i) acc[i] = 0.f;
@@ -596,8 +598,34 @@ __global__ void __launch_bounds__(LG_THREADS, 1) linear_gemm_kernel(const __grid
         }
       }
       if (!alive) break;
-      lg_finish<HALF>(a, w, acc, row_in_tile, half * HALF, BN, bias_s + (tile & 1) * BN);
-      ++tile;
+      const int64_t row = (int64_t)w.m0 + quarter * 32 + lane;
+      const int col = w.n0 + half * HALF;
+      if (w.part >= 0) {
+        float4* part = reinterpret_cast<float4*>(a.part + ((int64_t)w.part * LG_BM + quarter * 32 + lane) * BN + half * HALF);
+#pragma unroll
+        for (int j = 0; j < HALF / 4; ++j) part[j] = make_float4(acc[4 * j], acc[4 * j + 1], acc[4 * j + 2], acc[4 * j + 3]);
+        continue;
+      }
+      if (a.vec && col + HALF <= a.n) {
+        lg_finish_row<HALF>(a, acc, row, col);
+        continue;
+      }
+#pragma unroll
+      for (int j = 0; j < HALF / 32; ++j) {
+        __syncwarp();  // the last block has been read
+#pragma unroll
+        for (int i = 0; i < 32; ++i) stage[32 * lane + (i ^ lane)] = acc[32 * j + i];
+        __syncwarp();
+        const int c = col + 32 * j + lane, row0 = w.m0 + quarter * 32;
+        switch (a.e.act) {
+          case MM_LINEAR_RELU: lg_finish_rows<MM_LINEAR_RELU>(a, stage, row0, c, lane); break;
+          case MM_LINEAR_SILU: lg_finish_rows<MM_LINEAR_SILU>(a, stage, row0, c, lane); break;
+          case MM_LINEAR_SIGMOID: lg_finish_rows<MM_LINEAR_SIGMOID>(a, stage, row0, c, lane); break;
+          case MM_LINEAR_GELU: lg_finish_rows<MM_LINEAR_GELU>(a, stage, row0, c, lane); break;
+          case MM_LINEAR_GELU_TANH: lg_finish_rows<MM_LINEAR_GELU_TANH>(a, stage, row0, c, lane); break;
+          default: lg_finish_rows<MM_LINEAR_NONE>(a, stage, row0, c, lane); break;
+        }
+      }
     }
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -615,22 +643,24 @@ __global__ void __launch_bounds__(LG_THREADS, 1) linear_gemm_kernel(const __grid
 }
 
 // Tiles whose reduction was divided: the partial tiles are added in order and
-// go through the epilogue.  One block per 8 rows of a tile.
-__global__ void __launch_bounds__(256) linear_join_kernel(const LinGemm a, int bn) {
+// go through the epilogue, four columns per thread.  One block per 8 rows of a
+// tile.
+template <int BN>
+__global__ void __launch_bounds__(2 * BN) linear_join_kernel(const LinGemm a) {
   pdl_wait();
   const int tile = blockIdx.x / (LG_BM / 8), r0 = blockIdx.x % (LG_BM / 8) * 8;
-  const LgUnit w = lg_unit(a, a.full + tile * a.splits, bn);
-  const float* part = a.part + (int64_t)tile * a.splits * LG_BM * bn;
-  for (int i = threadIdx.x; i < 8 * bn; i += 256) {
-    const int r = r0 + i / bn, c = i % bn;
-    const int64_t row = w.m0 + r;
-    if (row >= a.m || w.n0 + c >= a.n) continue;
-    float v = 0.f;
-    for (int s = 0; s < a.splits; ++s) v += part[((int64_t)s * LG_BM + r) * bn + c];
-    a.c[row * a.n + w.n0 + c] = lin_finish(a.e, v, row, w.n0 + c, a.n);
+  const LgUnit w = lg_unit(a, a.full + tile * a.splits, BN);
+  const int r = r0 + threadIdx.x / (BN / 4), c = threadIdx.x % (BN / 4) * 4;
+  const float* part = a.part + ((int64_t)tile * a.splits * LG_BM + r) * BN + c;
+  float v[4] = {};
+#pragma unroll 4
+  for (int s = 0; s < a.splits; ++s) {
+    const float4 t = *reinterpret_cast<const float4*>(part + (int64_t)s * LG_BM * BN);
+    v[0] += t.x; v[1] += t.y; v[2] += t.z; v[3] += t.w;
   }
+  if (w.m0 + r < a.m && w.n0 + c < a.n) lin_finish_row<4>(a.e, v, a.c, w.m0 + r, w.n0 + c, a.n, a.vec);
   __syncthreads();
-  lin_fix(a, w.m0 + r0, 8, w.n0, bn);
+  lin_fix(a, w.m0 + r0, 8, w.n0, BN);
 }
 
 // ---------------------------------------------------------------------------
@@ -736,8 +766,9 @@ static int lin_map(const LinPlanes& p, int rows, CUtensorMap* out) {
 
 template <int BN, bool AMN, bool BMN>
 static int lin_launch(const CUtensorMap& ma, const CUtensorMap& mb, const LinGemm& g, cudaStream_t s) {
-  // alignment, stages, barriers, two tiles' bias
-  constexpr size_t smem = 1024 + (size_t)lg_stages<BN>() * (LG_BM + BN) * 192 + 256 + 8 * BN;
+  // alignment, stages, barriers, 32 x 32 blocks of the adding warps
+  constexpr size_t smem = 1024 + (size_t)lg_stages<BN>() * (LG_BM + BN) * 192 + 256 + LG_EPI_WARPS * 4096;
+  static_assert(smem <= 227 * 1024, "shared memory of a block");
   auto kernel = linear_gemm_kernel<BN, AMN, BMN>;
   MM_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem),
           "mm_linear: shared memory attribute");
@@ -765,8 +796,9 @@ int lin_run_gemm(const LinPlanes& pa, const LinPlanes& pb, float* c, const LinEp
   g.full = ch.full;
   g.splits = ch.splits;
   g.units = ch.units;
-  // The epilogue's eight columns are written as two 16-byte stores.
-  g.vec = g.n % 4 == 0 && (uintptr_t)c % 16 == 0;
+  // Whole rows of four columns may move in 16-byte pieces.
+  g.vec = g.n % 4 == 0 && (uintptr_t)c % 16 == 0 && (!e.bias || e.bias_vec) && (!e.residual || e.residual_vec) &&
+          (!e.z || e.z_vec);
   g.c = c;
   g.part = part;
   g.e = e;
@@ -782,7 +814,9 @@ int lin_run_gemm(const LinPlanes& pa, const LinPlanes& pb, float* c, const LinEp
   if (rc != MM_OK) return rc;
   if (ch.splits > 1) {
     const unsigned grid = (unsigned)((ch.units - ch.full) / ch.splits * (LG_BM / 8));
-    MM_CUDA(launch_pdl(linear_join_kernel, dim3(grid), dim3(256), 0, s, g, ch.bn), "mm_linear join launch");
+    MM_CUDA(ch.bn == 128 ? launch_pdl(linear_join_kernel<128>, dim3(grid), dim3(256), 0, s, g)
+                         : launch_pdl(linear_join_kernel<64>, dim3(grid), dim3(128), 0, s, g),
+            "mm_linear join launch");
   }
   return MM_OK;
 }
