@@ -31,7 +31,11 @@ namespace mm {
 
 constexpr int AW_BLOCK = 256;     // elements that share a scale
 constexpr int AW_THREADS = 256;
-constexpr int AW_CHUNK = 4096;    // elements per thread block, both state widths
+// Elements per thread block.  With 32-bit states twice as many left too few
+// blocks for small models (an MLP of 0.5 M parameters: 9.4 us, these 5.9).  With
+// 8-bit states each warp has one block of 256 and leaves (two per warp: 227 us
+// for 54 M elements, one 178).
+constexpr int AW_CHUNK = 2048, AW_CHUNK8 = AW_BLOCK * AW_THREADS / 32;
 constexpr int AW_ONE = 0x3F800000;  // 1.0f
 
 struct AwTensor {
@@ -73,13 +77,14 @@ __global__ void adamw_begin_kernel(const __grid_constant__ AwTable<MOST> tab, fl
   coef[i] = make_float2((float)(lr / (1.0 - pow(b1, (double)t))), (float)(1.0 / sqrt(1.0 - pow(b2, (double)t))));
 }
 
-// Magnitude code of q = size / scale: float32 bits above SHIFT, rounded to
-// even, counted down from TOP at 1.0.
-template <int SHIFT, int TOP, int LEAST>
-__device__ __forceinline__ uint32_t aw_code(float size, float inv) {
+// Magnitude code of q = size / scale <= 1: float32 bits above SHIFT, rounded to
+// even, counted down from TOP at 1.0.  Only the lowest byte counts (q is NaN in
+// a block whose scale is).
+template <int SHIFT, int TOP>
+__device__ __forceinline__ int aw_code(float size, float inv, int least) {
   const uint32_t bits = __float_as_uint(__fmul_rn(size, inv));
-  const int c = (int)((bits + ((1u << (SHIFT - 1)) - 1u) + ((bits >> SHIFT) & 1u)) >> SHIFT) - (AW_ONE >> SHIFT) + TOP;
-  return size > 0.f ? (uint32_t)min(max(c, LEAST), TOP) : 0u;
+  return max((int)((bits + ((1u << (SHIFT - 1)) - 1u) + ((bits >> SHIFT) & 1u)) >> SHIFT) - ((AW_ONE >> SHIFT) - TOP),
+             least);
 }
 
 template <int SHIFT, int TOP>
@@ -95,11 +100,11 @@ __device__ __forceinline__ float aw_decode_m(uint32_t byte, float scale) {
 
 __device__ __forceinline__ float aw_decode_r(uint32_t byte, float scale) { return aw_value<19, 255>(byte, scale); }
 
-// Largest magnitude of a warp's non-negative values, by their bits: a NaN's
-// bits are above an infinity's, so it reaches the scale and stays visible.
-__device__ __forceinline__ float aw_scale(float most_bits_as_float) {
-  const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(most_bits_as_float) & 0x7fffffffu);
-  return bits < 0x00800000u ? 0.f : __uint_as_float(bits);
+// Scale of a warp's largest magnitudes, by their bits: those of infinities and
+// NaNs are above all others, and make it NaN, so they stay visible.
+__device__ __forceinline__ float aw_scale(float most) {
+  const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(most) & 0x7fffffffu);
+  return __uint_as_float(bits < 0x00800000u ? 0u : bits >= 0x7f800000u ? 0x7fc00000u : bits);
 }
 
 __device__ __forceinline__ float aw_max(float a, float b) {
@@ -116,9 +121,17 @@ __device__ __forceinline__ float aw_update(float p, float m, float r, float2 coe
   return __fsub_rn(__fmul_rn(p, a.decay), __fmul_rn(__fdiv_rn(m, d), coef.x));
 }
 
-__device__ __forceinline__ float aw_grad(float g, float p, const AwScalars& a) {
-  if (a.maximize) g = -g;
-  return a.l2 != 0.f ? __fadd_rn(g, __fmul_rn(p, a.l2)) : g;
+// The gradients of N elements: negated to maximise, with coupled weight decay.
+template <int N>
+__device__ __forceinline__ void aw_grads(float* g, const float* p, const AwScalars& a) {
+  if (a.maximize) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) g[e] = -g[e];
+  }
+  if (a.l2 != 0.f) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) g[e] = __fadd_rn(g[e], __fmul_rn(p[e], a.l2));
+  }
 }
 
 // The tensor that chunk `chunk` belongs to.
@@ -152,9 +165,10 @@ __global__ void __launch_bounds__(AW_THREADS) adamw32_kernel(const __grid_consta
       float4 p4 = reinterpret_cast<const float4*>(p)[c], g4 = reinterpret_cast<const float4*>(g)[c];
       float4 m4 = reinterpret_cast<const float4*>(m)[c], v4 = reinterpret_cast<const float4*>(v)[c];
       float *pe = &p4.x, *ge = &g4.x, *me = &m4.x, *ve = &v4.x;
+      aw_grads<4>(ge, pe, a);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        ve[e] = aw_moments(me[e], ve[e], aw_grad(ge[e], pe[e], a), a);
+        ve[e] = aw_moments(me[e], ve[e], ge[e], a);
         pe[e] = aw_update(pe[e], me[e], __fsqrt_rn(ve[e]), coef, a);
       }
       reinterpret_cast<float4*>(p)[c] = p4;
@@ -164,9 +178,11 @@ __global__ void __launch_bounds__(AW_THREADS) adamw32_kernel(const __grid_consta
     return;
   }
   for (int c = threadIdx.x; c < left; c += AW_THREADS) {
-    float me = m[c];
-    const float ve = aw_moments(me, v[c], aw_grad(g[c], p[c], a), a);
-    p[c] = aw_update(p[c], me, __fsqrt_rn(ve), coef, a);
+    float me = m[c], ge = g[c];
+    const float pe = p[c];
+    aw_grads<1>(&ge, &pe, a);
+    const float ve = aw_moments(me, v[c], ge, a);
+    p[c] = aw_update(pe, me, __fsqrt_rn(ve), coef, a);
     m[c] = me;
     v[c] = ve;
   }
@@ -204,8 +220,14 @@ __device__ __forceinline__ void aw_unpack(uint2 c, uint32_t* out) {
   for (int e = 0; e < 8; ++e) out[e] = ((e < 4 ? c.x : c.y) >> (8 * (e & 3))) & 255u;
 }
 
+// The lowest bytes of eight words.
 __device__ __forceinline__ uint2 aw_pack(const uint32_t* c) {
-  return make_uint2(c[0] | c[1] << 8 | c[2] << 16 | c[3] << 24, c[4] | c[5] << 8 | c[6] << 16 | c[7] << 24);
+  uint32_t w[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    w[i] = __byte_perm(__byte_perm(c[4 * i], c[4 * i + 1], 0x0040), __byte_perm(c[4 * i + 2], c[4 * i + 3], 0x0040),
+                       0x5410);
+  return make_uint2(w[0], w[1]);
 }
 
 // Codes and scales of one block of 256 elements held by a warp, 8 per lane.
@@ -219,12 +241,12 @@ __device__ __forceinline__ void aw_encode_block(const float* m, const float* r, 
   }
   mm = aw_scale(mm);
   rr = aw_scale(rr);
-  const float im = __frcp_rn(mm), ir = __frcp_rn(rr);
+  const float im = mm == 0.f ? 0.f : __frcp_rn(mm), ir = rr == 0.f ? 0.f : __frcp_rn(rr);
   uint32_t cm[8], cr[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    cm[e] = mm == 0.f ? 0u : aw_code<20, 127, 0>(fabsf(m[e]), im) | (m[e] < 0.f ? 128u : 0u);
-    cr[e] = rr == 0.f ? 0u : aw_code<19, 255, 1>(r[e], ir);
+    cm[e] = (uint32_t)aw_code<20, 127>(fabsf(m[e]), im, 0) | ((__float_as_uint(m[e]) >> 24) & 128u);
+    cr[e] = (uint32_t)aw_code<19, 255>(r[e], ir, r[e] > 0.f ? 1 : 0);
   }
   reinterpret_cast<uint2*>(mc)[block * 32 + lane] = aw_pack(cm);
   reinterpret_cast<uint2*>(vc)[block * 32 + lane] = aw_pack(cr);
@@ -240,32 +262,34 @@ __global__ void __launch_bounds__(AW_THREADS) adamw8_kernel(const __grid_constan
   const int k = aw_find(tab, blockIdx.x);
   const AwTensor& t = tab.t[k];
   const float2 coef = coefs[k];
-  const int64_t chunk = (int64_t)(blockIdx.x - t.first) * AW_CHUNK;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const bool vec = t.aligned != 0;
-  for (int i = warp; i < AW_CHUNK / AW_BLOCK; i += AW_THREADS / 32) {
-    const int64_t base = chunk + (int64_t)i * AW_BLOCK;
-    if (base >= t.n) return;
-    const int64_t block = base / AW_BLOCK;
-    const int left = (int)min((int64_t)AW_BLOCK, t.n - base);
-    float p[8], g[8], m[8], r[8];
-    aw_load8(t.p + base, lane * 8, left, vec, p);
-    aw_load8(t.g + base, lane * 8, left, vec, g);
-    uint32_t cm[8], cr[8];
-    aw_unpack(reinterpret_cast<const uint2*>(t.m)[block * 32 + lane], cm);
-    aw_unpack(reinterpret_cast<const uint2*>(t.v)[block * 32 + lane], cr);
-    const float ms = t.ms[block], vs = t.vs[block];
+  const int64_t base = (int64_t)(blockIdx.x - t.first) * AW_CHUNK8 + warp * AW_BLOCK;
+  if (base >= t.n) return;
+  const int64_t block = base / AW_BLOCK;
+  const int left = (int)min((int64_t)AW_BLOCK, t.n - base);
+  float p[8], g[8], m[8], r[8];
+  aw_load8(t.p + base, lane * 8, left, vec, p);
+  aw_load8(t.g + base, lane * 8, left, vec, g);
+  uint32_t cm[8], cr[8];
+  aw_unpack(reinterpret_cast<const uint2*>(t.m)[block * 32 + lane], cm);
+  aw_unpack(reinterpret_cast<const uint2*>(t.v)[block * 32 + lane], cr);
+  const float ms = t.ms[block], vs = t.vs[block];
+  aw_grads<8>(g, p, a);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      m[e] = aw_decode_m(cm[e], ms);
-      const float rold = aw_decode_r(cr[e], vs);
-      r[e] = __fsqrt_rn(aw_moments(m[e], __fmul_rn(rold, rold), aw_grad(g[e], p[e], a), a));
-      p[e] = aw_update(p[e], m[e], r[e], coef, a);
-      if (lane * 8 + e >= left) m[e] = r[e] = 0.f;
-    }
-    aw_store8(t.p + base, lane * 8, left, vec, p);
-    aw_encode_block(m, r, (uint8_t*)t.m, (uint8_t*)t.v, t.ms, t.vs, block, lane);
+  for (int e = 0; e < 8; ++e) {
+    m[e] = aw_decode_m(cm[e], ms);
+    const float rold = aw_decode_r(cr[e], vs);
+    r[e] = __fsqrt_rn(aw_moments(m[e], __fmul_rn(rold, rold), g[e], a));
+    p[e] = aw_update(p[e], m[e], r[e], coef, a);
   }
+  if (left < AW_BLOCK) {  // nothing behind the tensor's end counts for the scale
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (lane * 8 + e >= left) m[e] = r[e] = 0.f;
+  }
+  aw_store8(t.p + base, lane * 8, left, vec, p);
+  aw_encode_block(m, r, (uint8_t*)t.m, (uint8_t*)t.v, t.ms, t.vs, block, lane);
 }
 
 // 8-bit states of given float32 moments: one warp per block of 256 elements.
@@ -320,7 +344,7 @@ static int aw_launch(const mm_adamw_tensor_t* in, int count, int bits, double lr
          in[i].step, (uint32_t)chunks, 0, in[i].numel};
     t.aligned = aw_aligned(t.p, 16) && aw_aligned(t.g, 16) &&
                 (bits == 8 || (aw_aligned(t.m, 16) && aw_aligned(t.v, 16)));
-    chunks += (t.n + AW_CHUNK - 1) / AW_CHUNK;
+    chunks += bits == 8 ? (t.n + AW_CHUNK8 - 1) / AW_CHUNK8 : (t.n + AW_CHUNK - 1) / AW_CHUNK;
   }
   if (chunks > INT32_MAX) return fail(MM_ERR_UNSUPPORTED, "mm_adamw: too many elements in one call");
   tab.count = count;

@@ -90,7 +90,8 @@ def _launch(name: str, *args) -> None:
     if token is not None:
         profiling.launch_times.end(token)
     profiling.count_launch(name)
-    if config.cudaDisableAsyncQueue or config.cudaDebug:
+    values = config._values
+    if values["cudaDisableAsyncQueue"] or values["cudaDebug"]:
         get_runtime().synchronize()
 
 

@@ -184,7 +184,9 @@ class AdamW(torch.optim.Optimizer):
         if self.state_bits == 32:
             return ops.clone(state["exp_avg"]), ops.clone(state["exp_avg_sq"])
         rt, n, shape = p.runtime, numel(p.shape), tuple(p.shape)
-        m, v = (MatrixManTensor._wrap(rt.new_storage(n), shape, 0, p._logical_strides) for _ in range(2))
+        at = (n + 63) // 64 * 64  # both in one block
+        owner = rt.new_storage(at + n)
+        m, v = (MatrixManTensor._wrap(owner, shape, o, p._logical_strides) for o in (0, at))
         ops._launch("mm_adamw_decode", *(_pointer(state[k]) for k in _CODES), n, _pointer(m), _pointer(v), rt.stream)
         return m, v
 
