@@ -324,7 +324,7 @@ def _norm_own(s):
             return _torch_view(torch.nn.functional.layer_norm(s["x"], s["weight"].shape, s["weight"], s["bias"], EPS))
     y = torch.nn.functional.layer_norm(s["x"], s["weight"].shape, s["weight"], s["bias"], EPS)
     grads = torch.autograd.grad(y, (s["x"], s["weight"], s["bias"]), s["grad"])
-    return [_torch_view(t.detach()) for t in (y, *grads)]
+    return [_torch_view(t) for t in (y, *grads)]
 
 
 def _linear_own(s):
@@ -336,7 +336,7 @@ def _linear_own(s):
                                                 residual=s.get("residual")))
     y = matrixman.linear(s["x"], s["weight"], s["bias"], activation=case["act"], residual=s.get("residual"))
     grads = torch.autograd.grad(y, (s["x"], s["weight"], s["bias"]), s["grad"])
-    return [_torch_view(t.detach()) for t in (y, *grads)]
+    return [_torch_view(t) for t in (y, *grads)]
 
 
 def _adamw_own(s):
