@@ -19,6 +19,10 @@ struct LinProduct {
   float* c;
   int64_t as0, as1, bs0, bs1;
   int m, n, k;
+  // A's values times act'(z), z strided like A (null: as they are)
+  const float* z;
+  int64_t zs0, zs1;
+  int act;
 };
 
 // ---------------------------------------------------------------------------
@@ -87,36 +91,41 @@ __device__ __forceinline__ void ls_put(float* tile, int mode, const float (&v)[8
   }
 }
 
-template <int NW>
-__global__ void __launch_bounds__(NW * 32) linear_small_kernel(LinProduct p, LinEpilogue e, int tiles_n, int amode,
-                                                               int bmode, int vec) {
+// How a small product reads and writes.
+struct LsModes {
+  int tiles_n, a, b, z, vec;
+};
+
+// One 32 x 32 tile of a product.
+template <int NW, bool SLOPE>
+__device__ __forceinline__ void ls_tile(const LinProduct& p, const LinEpilogue& e, const LsModes& md, int tile) {
   using S = LsShape<NW>;
   extern __shared__ float4 ls_mem[];
   float* tiles = reinterpret_cast<float*>(ls_mem);
-  const int m0 = (int)(blockIdx.x / tiles_n) * LS_T, n0 = (int)(blockIdx.x % tiles_n) * LS_T;
+  const int m0 = tile / md.tiles_n * LS_T, n0 = tile % md.tiles_n * LS_T;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int ga = lane >> 2, gb = lane & 3;  // A lines 4 ga + i, B lines gb + 4 j
   float acc[4][8] = {};
-  float av[2][8], bv[2][8];  // the next two chunks, on their way
-  pdl_wait();
+  float av[2][8], bv[2][8], zv[2][8];  // the next two chunks, on their way
+  auto fetch = [&](int i, int k0) {
+    ls_fetch<NW>(p.a, p.as0, p.as1, p.m, p.k, m0, k0, md.a, av[i]);
+    // (z in A's own order: the threads' values have to match)
+    if (SLOPE) ls_fetch<NW>(p.z, p.zs0, p.zs1, p.m, p.k, m0, k0, md.z, zv[i]);
+    ls_fetch<NW>(p.b, p.bs0, p.bs1, p.n, p.k, n0, k0, md.b, bv[i]);
+  };
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    ls_fetch<NW>(p.a, p.as0, p.as1, p.m, p.k, m0, i * S::K, amode, av[i]);
-    ls_fetch<NW>(p.b, p.bs0, p.bs1, p.n, p.k, n0, i * S::K, bmode, bv[i]);
-  }
+  for (int i = 0; i < 2; ++i) fetch(i, i * S::K);
   for (int k0 = 0; k0 < p.k; k0 += 2 * S::K) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       if (k0 + i * S::K >= p.k) break;
       float* ta = tiles + i * 2 * S::TILE;
       float* tb = ta + S::TILE;
-      ls_put<NW>(ta, amode, av[i]);
-      ls_put<NW>(tb, bmode, bv[i]);
+      if (SLOPE) lin_times_slope<8>(av[i], zv[i], p.act);
+      ls_put<NW>(ta, md.a, av[i]);
+      ls_put<NW>(tb, md.b, bv[i]);
       __syncthreads();  // also: every warp has finished with this buffer's last chunk
-      if (k0 + (i + 2) * S::K < p.k) {
-        ls_fetch<NW>(p.a, p.as0, p.as1, p.m, p.k, m0, k0 + (i + 2) * S::K, amode, av[i]);
-        ls_fetch<NW>(p.b, p.bs0, p.bs1, p.n, p.k, n0, k0 + (i + 2) * S::K, bmode, bv[i]);
-      }
+      if (k0 + (i + 2) * S::K < p.k) fetch(i, k0 + (i + 2) * S::K);
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
         const int kk = warp * 8 + q * 4;
@@ -152,20 +161,83 @@ __global__ void __launch_bounds__(NW * 32) linear_small_kernel(LinProduct p, Lin
   for (int w = 0; w < NW; ++w)
 #pragma unroll
     for (int j = 0; j < 4; ++j) v[j] += red[(w * LS_T + r) * 33 + c + j];
-  lin_finish_row<4>(e, v, p.c, row, col, p.n, vec);
+  lin_finish_row<4>(e, v, p.c, row, col, p.n, md.vec);
 }
 
 template <int NW>
-static cudaError_t lin_small(const LinProduct& p, const LinEpilogue& e, int64_t tiles, int tiles_n, int amode, int bmode,
-                             int vec, cudaStream_t s) {
+__global__ void __launch_bounds__(NW * 32) linear_small_kernel(LinProduct p, LinEpilogue e, LsModes md) {
+  pdl_wait();
+  ls_tile<NW, false>(p, e, md, blockIdx.x);
+}
+
+// All gradients of a small call in one launch: the tiles of dx, then those of
+// dw, then the columns of db (and dz itself where it is asked for), 32 to a
+// block.  Each block takes dz = dy act'(z) from dy and z as it reads them.
+struct LsBackward {
+  LinProduct dx, dw;
+  LsModes mx, mw;
+  LinEpilogue none;
+  int tiles_dx, tiles_dw;
+  float *db, *dz;
+};
+
+__global__ void __launch_bounds__(256) linear_small_backward_kernel(const __grid_constant__ LsBackward g) {
+  pdl_wait();
+  int block = blockIdx.x;
+  const bool slope = g.dw.z != nullptr;
+  if (block < g.tiles_dx) {
+    if (slope)
+      ls_tile<8, true>(g.dx, g.none, g.mx, block);
+    else
+      ls_tile<8, false>(g.dx, g.none, g.mx, block);
+    return;
+  }
+  block -= g.tiles_dx;
+  if (block < g.tiles_dw) {
+    if (slope)
+      ls_tile<8, true>(g.dw, g.none, g.mw, block);
+    else
+      ls_tile<8, false>(g.dw, g.none, g.mw, block);
+    return;
+  }
+  block -= g.tiles_dw;
+  // dw's A is dz transposed: its lines are dz's columns.
+  extern __shared__ float4 ls_mem[];
+  float* acc = reinterpret_cast<float*>(ls_mem);  // [8][33]
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int c = block * 32 + lane, n = g.dw.m, m = g.dw.k;
+  float s = 0.f;
+  if (c < n) {
+#pragma unroll 4
+    for (int r = warp; r < m; r += 8) {
+      float v[1] = {g.dw.a[c * g.dw.as0 + r * g.dw.as1]};
+      if (slope) {
+        const float z[1] = {g.dw.z[c * g.dw.zs0 + r * g.dw.zs1]};
+        lin_times_slope<1>(v, z, g.dw.act);
+      }
+      if (g.dz) g.dz[(int64_t)r * n + c] = v[0];
+      s += v[0];
+    }
+  }
+  acc[warp * 33 + lane] = s;
+  __syncthreads();
+  if (g.db && warp == 0 && c < n) {
+#pragma unroll
+    for (int j = 1; j < 8; ++j) s += acc[j * 33 + lane];
+    g.db[c] = s;
+  }
+}
+
+template <int NW>
+static cudaError_t lin_small(const LinProduct& p, const LinEpilogue& e, int64_t tiles, const LsModes& md,
+                             cudaStream_t s) {
   constexpr size_t smem = LsShape<NW>::FLOATS * sizeof(float);
   if (smem > 48 * 1024) {
     const cudaError_t err =
         cudaFuncSetAttribute(linear_small_kernel<NW>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (err != cudaSuccess) return err;
   }
-  return launch_pdl(linear_small_kernel<NW>, dim3((unsigned)tiles), dim3(NW * 32), smem, s, p, e, tiles_n, amode, bmode,
-                    vec);
+  return launch_pdl(linear_small_kernel<NW>, dim3((unsigned)tiles), dim3(NW * 32), smem, s, p, e, md);
 }
 
 // ---------------------------------------------------------------------------
@@ -238,25 +310,6 @@ __global__ void __launch_bounds__(256) linear_tokens_kernel(LinProduct p, LinEpi
   }
 }
 
-// dz = dy act'(z), dense [m, n], and the partial sums of its columns over the
-// rows blockIdx.y, + gridDim.y, ...
-__global__ void __launch_bounds__(256) linear_dz_kernel(const float* dy, int64_t dys, const float* z, int act, int m,
-                                                        int n, float* dz, float* part) {
-  const int c = blockIdx.x * 256 + threadIdx.x;
-  if (c >= n) return;
-  float s = 0.f;
-  for (int64_t row = blockIdx.y; row < m; row += gridDim.y) {
-    float g[1] = {dy[row * dys + c]};
-    if (z) {
-      const float zv[1] = {z[row * n + c]};
-      lin_times_slope<1>(g, zv, act);
-    }
-    dz[row * n + c] = g[0];
-    s += g[0];
-  }
-  part[(int64_t)blockIdx.y * n + c] = s;
-}
-
 // Adds the partial rows in a fixed order.
 __global__ void __launch_bounds__(256) linear_columns_kernel(const float* part, int rows, int n, float* db) {
   __shared__ float acc[8][33];
@@ -305,6 +358,20 @@ static int ls_mode(const float* p, int64_t s0, int64_t s1) {
   return LS_SINGLE;
 }
 
+// The modes of a small product, and its number of tiles.
+static int64_t ls_modes(const LinProduct& p, LsModes* md) {
+  md->tiles_n = (p.n + LS_T - 1) / LS_T;
+  md->a = ls_mode(p.a, p.as0, p.as1);
+  md->b = ls_mode(p.b, p.bs0, p.bs1);
+  md->z = LS_SINGLE;
+  if (p.z) {  // read in A's order, so in A's mode where z allows it
+    md->z = ls_mode(p.z, p.zs0, p.zs1);
+    if (md->z != md->a) md->a = md->z = LS_SINGLE;
+  }
+  md->vec = p.n % 4 == 0 && (uintptr_t)p.c % 16 == 0;
+  return (int64_t)md->tiles_n * ((p.m + LS_T - 1) / LS_T);
+}
+
 // A product on the multiply-add units.
 static int lin_product(const LinProduct& p, const LinEpilogue& e, cudaStream_t s) {
   if (p.m == 0 || p.n == 0) return MM_OK;
@@ -318,20 +385,15 @@ static int lin_product(const LinProduct& p, const LinEpilogue& e, cudaStream_t s
     else
       lin_tokens<8, 4>(p, e, s);
   } else {
-    const int tiles_n = (p.n + LS_T - 1) / LS_T;
-    const int64_t tiles = (int64_t)tiles_n * ((p.m + LS_T - 1) / LS_T);
+    LsModes md;
+    const int64_t tiles = ls_modes(p, &md);
     if (tiles > INT32_MAX) return fail(MM_ERR_UNSUPPORTED, "mm_linear: output too large");
-    const int vec = p.n % 4 == 0 && (uintptr_t)p.c % 16 == 0;
-    const int amode = ls_mode(p.a, p.as0, p.as1), bmode = ls_mode(p.b, p.bs0, p.bs1);
-    MM_CUDA(tiles <= sm_count() && p.k > 256 ? lin_small<16>(p, e, tiles, tiles_n, amode, bmode, vec, s)
-                                             : lin_small<8>(p, e, tiles, tiles_n, amode, bmode, vec, s),
+    MM_CUDA(tiles <= sm_count() && p.k > 256 ? lin_small<16>(p, e, tiles, md, s) : lin_small<8>(p, e, tiles, md, s),
             "mm_linear launch");
   }
   MM_LAUNCH_CHECK("mm_linear launch");
   return MM_OK;
 }
-
-constexpr int LIN_DZ_ROWS = 256;  // partial rows of the bias gradient
 
 // Clocks of a small product: a block per SM at a time, 64 of the reduction in
 // about 1,700 (with one block per SM latency, with several the multiply-adds
@@ -358,10 +420,11 @@ struct LinRoute {
 
 static LinRoute lin_route(int64_t m, int64_t n, int64_t k, bool backward) {
   LinRoute r = {};
-  if ((m <= LIN_TOKENS && !backward) || m <= 0 || n < 32 || k < 32) return r;
+  if ((m <= LIN_TOKENS && !backward) || m <= 0 || n <= 0 || k <= 0) return r;
   double small, tensor = backward ? 34000 : 24000;
   if (backward) {
-    small = lin_small_clocks(m, k, n) + lin_small_clocks(n, k, m);
+    // (each tile takes the slope of the dz it reads: some 60 operations per value)
+    small = lin_small_clocks(m, k, n) + lin_small_clocks(n, k, m) + 60.0 * m * n * (k / 16 + 2) / (sm_count() * 128);
     r.first = lin_choose(m, k, n);
     r.second = lin_choose(n, k, m);
     tensor += r.first.clocks + r.second.clocks + 10.0 * (m * n + m * k + n * k) / 3400;
@@ -487,9 +550,6 @@ static size_t lin_workspace(const LinRoute& r, int64_t m, int64_t n, int64_t k, 
       ws.take(lin_part_bytes(r.first));
       ws.take(lin_part_bytes(r.second));
     }
-  } else if (backward) {
-    ws.take(4 * m * n);
-    ws.take(4 * LIN_DZ_ROWS * n);
   }
   return ws.used;
 }
@@ -531,7 +591,7 @@ extern "C" int mm_linear(const float* x, int64_t xs0, int64_t xs1, const float* 
   cudaStream_t s = resolve_stream(stream);
   const LinEpilogue e = lin_epilogue(bias, residual, residual_stride, z, act, residual_before_act != 0);
   if (!route.tensor)
-    return lin_product({x, w, y, xs0, xs1, ws0, ws1, (int)m, (int)n, (int)k}, e, s);
+    return lin_product({x, w, y, xs0, xs1, ws0, ws1, (int)m, (int)n, (int)k, nullptr, 0, 0, MM_LINEAR_NONE}, e, s);
   Scratch scratch;
   if (workspace == nullptr) {
     if ((rc = scratch.get(need, s)) != MM_OK) return rc;
@@ -568,22 +628,21 @@ extern "C" int mm_linear_backward(const float* dy, int64_t dy_stride, const floa
   if (route.tensor)
     return lin_backward_tc(route, {dy, dy_stride, 1}, {x, xs0, xs1}, {w, ws0, ws1}, z, act, m, n, k, dx, dw, db, dz,
                            workspace, s);
-  LinCarve ws = {(char*)workspace, 0};
-  float* own = (float*)ws.take(4 * m * n);
-  float* part = (float*)ws.take(4 * LIN_DZ_ROWS * n);
-  float* g = dz ? dz : own;
-  const int rows = m < LIN_DZ_ROWS ? (int)m : LIN_DZ_ROWS;
-  linear_dz_kernel<<<dim3((unsigned)((n + 255) / 256), rows), 256, 0, s>>>(
-      dy, dy_stride, act == MM_LINEAR_NONE ? nullptr : z, act, (int)m, (int)n, g, part);
-  MM_LAUNCH_CHECK("mm_linear_backward launch");
-  if (db) {
-    linear_columns_kernel<<<(unsigned)((n + 31) / 32), 256, 0, s>>>(part, rows, (int)n, db);
-    MM_LAUNCH_CHECK("mm_linear_backward launch");
-  }
-  const LinEpilogue none = lin_epilogue(nullptr, nullptr, 0, nullptr, MM_LINEAR_NONE, false);
-  if (dx) {
-    rc = lin_product({g, w, dx, n, 1, ws1, ws0, (int)m, (int)k, (int)n}, none, s);
-    if (rc != MM_OK) return rc;
-  }
-  return dw ? lin_product({g, x, dw, 1, n, xs1, xs0, (int)n, (int)k, (int)m}, none, s) : MM_OK;
+  LsBackward g = {};
+  const float* zp = act == MM_LINEAR_NONE ? nullptr : z;
+  g.none = lin_epilogue(nullptr, nullptr, 0, nullptr, MM_LINEAR_NONE, false);
+  g.dx = {dy, w, dx, dy_stride, 1, ws1, ws0, (int)m, (int)k, (int)n, zp, n, 1, act};
+  g.dw = {dy, x, dw, 1, dy_stride, xs1, xs0, (int)n, (int)k, (int)m, zp, 1, n, act};
+  const int64_t tx = ls_modes(g.dx, &g.mx), tw = ls_modes(g.dw, &g.mw);
+  g.tiles_dx = dx ? (int)tx : 0;
+  g.tiles_dw = dw ? (int)tw : 0;
+  g.db = db;
+  g.dz = dz;
+  const int64_t blocks = (dx ? tx : 0) + (dw ? tw : 0) + (db || dz ? (n + 31) / 32 : 0);
+  if (blocks > INT32_MAX) return fail(MM_ERR_UNSUPPORTED, "mm_linear_backward: output too large");
+  if (blocks == 0) return MM_OK;
+  MM_CUDA(launch_pdl(linear_small_backward_kernel, dim3((unsigned)blocks), dim3(256),
+                     LsShape<8>::FLOATS * sizeof(float), s, g),
+          "mm_linear_backward launch");
+  return MM_OK;
 }

@@ -699,11 +699,13 @@ int lin_run_splits(const LinSplits& all, cudaStream_t s) {
   return e == cudaSuccess ? MM_OK : cuda_fail(e, "mm_linear split launch");
 }
 
-// Tile width and division of the reduction, by an estimate in SM clocks: a
-// stage takes 850 (BN 128: 768 of MMAs) or 610 (BN 64: 384; loads and barriers
-// bound it), a tile about 4,000 more to fill the pipeline and store.  Tiles 256
-// wide, whose two accumulators leave the MMAs waiting for the additions, were
-// slower at every size (8192 x 2048 x 4096: 689 us, 128 wide 664, 64 wide 936).
+// Tile width and division of the reduction, by an estimate in SM clocks.  What
+// bounds a stage is its way from L2, about 42 bytes per clock and SM: 48 KB take
+// 1,150 clocks (BN 128; its MMAs 768), 36 KB 880 (BN 64; 384).  A tile takes
+// about 4,000 more to fill the pipeline and store.  Tiles 256 wide need 72 KB
+// per 1,536 clocks of MMAs, but have only two accumulators, and the MMAs wait
+// for the additions: slower at every size (8192 x 2048 x 4096: 689 us, 128 wide
+// 664, 64 wide 936; asking L2 for the stages ahead of their loads made it 835).
 // Whole waves of tiles run undivided; the rest is divided where that ends
 // sooner although its partial tiles are written and read once more.
 LinChoice lin_choose(int64_t m, int64_t n, int64_t k) {
@@ -712,7 +714,7 @@ LinChoice lin_choose(int64_t m, int64_t n, int64_t k) {
   for (int bn : {128, 64}) {
     const int64_t tm = (m + LG_BM - 1) / LG_BM, tn = (n + bn - 1) / bn, tiles = tm * tn;
     const int64_t stages = (k + LG_BK - 1) / LG_BK;
-    const double stage = bn == 128 ? 850 : 610, tile = 4000;
+    const double stage = bn == 128 ? 1150 : 880, tile = 4000;
     const int64_t full = tiles / sms * sms, rest = tiles - full;
     const double base = (double)(full / sms) * (stages * stage + tile);
     for (int s = 1; s <= LIN_MAX_SPLITS; ++s) {
@@ -721,7 +723,7 @@ LinChoice lin_choose(int64_t m, int64_t n, int64_t k) {
       if (rest) {
         const int64_t waves = (rest * s + sms - 1) / sms;
         t += waves * (((stages + s - 1) / s) * stage + tile);
-        if (s > 1) t += 4000 + (double)rest * s * LG_BM * bn * 8 / 3500;  // about 3,500 bytes per clock
+        if (s > 1) t += 10000 + (double)rest * s * LG_BM * bn * 8 / 3500;  // one more launch, 3,500 bytes per clock
       }
       if (best.bn == 0 || t < best.clocks)
         best = {bn, (int)full, s, (int)tm, (int)tn, (int)stages, (int)(full + rest * s), t};

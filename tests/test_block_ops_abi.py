@@ -83,7 +83,7 @@ def test_linear_checks():
         assert back(**{name: None}) == _lib.MM_ERR_INVALID
     for name in ("m", "n", "k", "dys", "xs0", "xs1", "ws0", "ws1"):
         assert back(**{name: -1}) == _lib.MM_ERR_INVALID
-    assert back(size=8) == _lib.MM_ERR_INVALID
+    assert back(m=4096, n=4096, k=4096, dys=4096, size=8) == _lib.MM_ERR_INVALID
     assert back(work=FAKE + 8) == _lib.MM_ERR_INVALID
     assert back(act=9) == _lib.MM_ERR_INVALID
     assert back(dx=None, dw=None, db=None) == _lib.MM_OK

@@ -114,7 +114,8 @@ def check(mm, x, w, b, r, act, first=False, grad=True):
 @pytest.mark.parametrize("m,n,k", [
     (1, 1, 1), (1, 5, 3), (1, 512, 784), (1, 257, 1030), (2, 64, 64), (3, 10, 256), (7, 100, 33), (16, 130, 129),
     (17, 33, 700), (31, 65, 4096), (33, 127, 128), (64, 64, 65), (100, 300, 200), (128, 256, 512), (129, 257, 31),
-    (256, 512, 784), (255, 1000, 1281), (700, 129, 40), (513, 384, 96), (2000, 40, 8)])
+    (256, 512, 784), (255, 1000, 1281), (700, 129, 40), (513, 384, 96), (2000, 40, 8),
+    (5000, 7, 300), (4000, 300, 7), (9001, 10, 16), (300, 1, 600), (600, 300, 1)])
 def test_sizes(mm, m, n, k):
     check(mm, randn(m, k, seed=1), randn(n, k, seed=2), randn(n, seed=3), None, "none")
 
