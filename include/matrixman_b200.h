@@ -154,6 +154,9 @@ int mm_shutdown(int device);
 /* Make `device` current for the calling thread. */
 int mm_set_device(int device);
 
+/* The calling thread's current device. */
+int mm_get_device(int* out);
+
 /* The device's runtime stream (created by mm_init). */
 int mm_runtime_stream(int device, void** stream_out);
 

@@ -121,6 +121,7 @@ SIGNATURES = {
     "mm_init": [_i],
     "mm_shutdown": [_i],
     "mm_set_device": [_i],
+    "mm_get_device": [ctypes.POINTER(_i)],
     "mm_runtime_stream": [_i, ctypes.POINTER(_vp)],
     "mm_stream_create": [_i, ctypes.POINTER(_vp)],
     "mm_stream_destroy": [_vp],

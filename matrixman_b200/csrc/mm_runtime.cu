@@ -319,6 +319,12 @@ extern "C" int mm_set_device(int device) {
   return MM_OK;
 }
 
+extern "C" int mm_get_device(int* out) {
+  if (out == nullptr) return fail(MM_ERR_INVALID, "mm_get_device: null output");
+  MM_CUDA(cudaGetDevice(out), "cudaGetDevice");
+  return MM_OK;
+}
+
 extern "C" int mm_runtime_stream(int device, void** stream_out) {
   DeviceRuntime* rt = runtime_for(device);
   if (rt == nullptr) return fail(MM_ERR_STATE, "mm_runtime_stream: device not initialised");

@@ -13,6 +13,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib, ops
+from .privateuse import native_calls
 from .tensor import MatrixManTensor, is_contiguous, numel, view_strides
 
 ACTIVATIONS = _lib.LINEAR_ACTS
@@ -49,6 +50,9 @@ def _dense_rows(t: MatrixManTensor) -> tuple[MatrixManTensor, int]:
 def _forward(x, weight, bias, residual, act: int, first: bool, keep: bool):
     """(y, z) of the output's shape: z is what the activation was applied to
     (None unless kept)."""
+    done = ops.native_call("linear", "mm_linear", x, weight, bias, residual, act, first, keep)
+    if done is not None:
+        return done
     rt = x.runtime
     x2, m, xs = _matrix(x)
     n, k = weight.shape
@@ -78,13 +82,20 @@ class _Linear(torch.autograd.Function):
     def backward(ctx, dy):
         x, weight, z = ctx.saved_tensors
         need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
+        want_z = need_r and ctx.first
+        if need_x or need_w or need_b or want_z:
+            done = ops.native_call("linear_backward", "mm_linear_backward", dy, x, weight, z, ctx.act, need_x, need_w,
+                                   need_b, want_z)
+            if done is not None:
+                dx, dw, db, dz = done
+                return dx, dw, db, dz if ctx.first else (dy if need_r else None), None, None
         dy = ops.require_mm(dy, "linear gradient")
         rt = dy.runtime
         n, k = weight.shape
         dx = ops.new_dense(rt, tuple(x.shape)) if need_x else None
         dw = ops.new_dense(rt, (n, k)) if need_w else None
         db = ops.new_dense(rt, (n,)) if need_b else None
-        dz = ops.new_dense(rt, tuple(dy.shape)) if need_r and ctx.first else None
+        dz = ops.new_dense(rt, tuple(dy.shape)) if want_z else None
         if need_x or need_w or need_b or dz is not None:
             g, gs = _dense_rows(dy)
             x2, m, xs = _matrix(x)
@@ -121,13 +132,26 @@ def linear(x, weight, bias=None, *, activation: str | None = None, residual=None
     Differentiable once in x, weight, bias and residual.  float32 throughout;
     weight and bias may be CPU tensors (uploaded once, as for the other
     operators) when they need no gradient."""
-    x = ops.require_mm(x, "linear")
-    ops.require_f32(x, "linear")
     act = ACTIVATIONS.get(activation) if activation is not None else 0
     if act is None:
         raise ValueError(f"MatrixMan/CUDA: linear activation must be one of {sorted(ACTIVATIONS)}, "
                          f"got {activation!r}")
     grad = torch.is_grad_enabled()
+    first = bool(residual_before_act)
+    if grad:
+        native = native_calls()
+        if native is not None and native.linear_ready(x, weight, bias, residual):
+            if x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad) or (
+                    residual is not None and residual.requires_grad):
+                return _Linear.apply(x, weight, bias, residual, act, first)
+            return _forward(x, weight, bias, residual, act, first, False)[0]
+    else:
+        done = ops.native_call("linear", "mm_linear", x, weight, bias, residual, act, first, False)
+        if done is not None:
+            return done[0]
+    # Everything but the ordinary case: CPU parameters, strides that take a copy, and what is refused.
+    x = ops.require_mm(x, "linear")
+    ops.require_f32(x, "linear")
     weight = _operand(x, weight, "weight", grad)
     if bias is not None:
         bias = _operand(x, bias, "bias", grad)
@@ -154,7 +178,6 @@ def linear(x, weight, bias=None, *, activation: str | None = None, residual=None
                      residual=None if residual is None else residual.unsqueeze(0),
                      residual_before_act=residual_before_act)
         return out.squeeze(0)
-    first = bool(residual_before_act)
     if grad and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad) or
                  (residual is not None and residual.requires_grad)):
         return _Linear.apply(x, weight, bias, residual, act, first)

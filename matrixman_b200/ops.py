@@ -14,7 +14,7 @@ import math
 
 import torch
 
-from . import _lib
+from . import _lib, privateuse
 from . import telemetry as profiling
 from .config import config
 from .runtime import DeviceRuntime, activate_stream, get_runtime
@@ -93,6 +93,24 @@ def _launch(name: str, *args) -> None:
     values = config._values
     if values["cudaDisableAsyncQueue"] or values["cudaDebug"]:
         get_runtime().synchronize()
+
+
+def native_call(function: str, name: str, *args):
+    """The result of one of the C++ extension's operator calls, which makes its
+    own output tensors; None where it leaves the call to the Python code (or
+    launches are being timed or synchronised one by one)."""
+    native = privateuse._native
+    values = config._values
+    if (native is None or values["cudaDisableAsyncQueue"] or values["cudaDebug"]
+            or profiling.gpu_timing_enabled()):
+        return None
+    result = getattr(native, function)(*args)
+    if result is None:
+        return None
+    if type(result) is int:
+        _lib.check(result, name)
+    profiling.count_launch(name)
+    return result
 
 
 def _p(desc: _lib.MMTensor):
@@ -618,6 +636,10 @@ def _norm_shape(x: MatrixManTensor, normalized_shape) -> tuple[int, ...]:
 def layer_norm(x, normalized_shape, weight=None, bias=None, eps=1e-5):
     """(y, mean, rstd) of native_layer_norm; mean and rstd keep the leading
     dimensions and have size 1 in the normalized ones."""
+    if len(normalized_shape) == 1:
+        done = native_call("layer_norm", "mm_layer_norm", x, normalized_shape[0], weight, bias, eps)
+        if done is not None:
+            return done
     x = require_mm(x, "LayerNorm")
     require_f32(x, "LayerNorm")
     shape = _norm_shape(x, normalized_shape)
@@ -644,6 +666,11 @@ def layer_norm(x, normalized_shape, weight=None, bias=None, eps=1e-5):
 
 def layer_norm_backward(dy, x, normalized_shape, mean, rstd, weight, bias, mask):
     """(dx, dweight, dbias) of native_layer_norm_backward; None where the mask is false."""
+    if len(normalized_shape) == 1:
+        done = native_call("layer_norm_backward", "mm_layer_norm_backward", dy, x, normalized_shape[0], mean, rstd,
+                           weight, bias, *mask)
+        if done is not None:
+            return done
     for t in (dy, x, mean, rstd):
         require_f32(require_mm(t, "LayerNorm backward"), "LayerNorm backward")
     shape = _norm_shape(x, normalized_shape)

@@ -112,5 +112,13 @@ def register_native_hooks() -> bool:
     # The guard's stream waits are bounded like every other host wait.
     from .config import config
     module.set_wait_timeout_ms(int(config.waitTimeoutMs))
+    from .runtime import DeviceStorage
+    from .tensor import MatrixManTensor
+    module.bind_tensors(MatrixManTensor, DeviceStorage, device_for)
     _native = module
     return True
+
+
+def native_calls():
+    """The C++ extension's operator calls, or None before it is loaded."""
+    return _native
