@@ -498,6 +498,75 @@ py::object linear_backward(py::handle dy_, py::handle x_, py::handle w_, py::han
   return py::make_tuple(dx, dw, db, dz);
 }
 
+using adamw_fn = int (*)(const void*, int, int, double, double, double, double, double, int, int, int, void*, size_t,
+                         void*);
+using decode_fn = int (*)(const void*, const void*, const void*, const void*, int64_t, void*, void*, void*);
+
+// An optimiser step over parameters with gradients and the states of
+// optim.AdamW (dicts): the table of addresses and the native call.  True, an
+// int (its status), or None where a tensor is not as usual.
+py::object adamw_step(const py::list& params, const py::list& states, int bits, double lr, double beta1, double beta2,
+                      double eps, double decay, bool maximize) {
+  static const py::object& grad_name = *new py::object(py::str("grad"));
+  static const py::object& step_name = *new py::object(py::str("step"));
+  static const py::object* const wide = new py::object[2]{py::str("exp_avg"), py::str("exp_avg_sq")};
+  static const py::object* const narrow = new py::object[4]{py::str("exp_avg_code"), py::str("exp_avg_sq_code"),
+                                                            py::str("exp_avg_scale"), py::str("exp_avg_sq_scale")};
+  const size_t count = params.size();
+  if (!names().ready || count == 0 || states.size() != count) return py::none();
+  std::vector<int64_t> table(8 * count);
+  std::vector<py::object> held;
+  Target t;
+  auto state_of = [&](const py::handle& state, const py::object& name, Operand* out) {
+    PyObject* v = PyDict_GetItemWithError(state.ptr(), name.ptr());
+    return v != nullptr && operand(v, out) && out->given && t.owns(*out);
+  };
+  for (size_t i = 0; i < count; ++i) {
+    Operand p, g, m, v, ms, vs, step;
+    if (!operand(params[i], &p) || !p.given || !p.t->is_non_overlapping_and_dense()) return py::none();
+    if (i == 0 ? !t.of(p) : !t.owns(p)) return py::none();
+    held.push_back(attribute(params[i].ptr(), grad_name));
+    if (!operand(held.back(), &g) || !g.given || !t.owns(g) || g.t->sizes() != p.t->sizes() ||
+        g.t->strides() != p.t->strides())
+      return py::none();
+    const py::handle state = states[i];
+    if (!PyDict_Check(state.ptr()) || !state_of(state, step_name, &step)) return py::none();
+    if (bits == 8) {
+      if (!state_of(state, narrow[0], &m) || !state_of(state, narrow[1], &v) || !state_of(state, narrow[2], &ms) ||
+          !state_of(state, narrow[3], &vs))
+        return py::none();
+    } else if (!state_of(state, wide[0], &m) || !state_of(state, wide[1], &v) || m.t->sizes() != p.t->sizes() ||
+               v.t->sizes() != p.t->sizes() || m.t->strides() != p.t->strides() || v.t->strides() != p.t->strides()) {
+      return py::none();
+    }
+    const Operand* order[] = {&p, &g, &m, &v, &ms, &vs, &step};
+    for (int j = 0; j < 7; ++j) table[8 * i + j] = (int64_t)(intptr_t)order[j]->ptr;
+    table[8 * i + 7] = p.t->numel();
+  }
+  const int status = MM_SYMBOL(adamw_fn, "mm_adamw")(table.data(), (int)count, bits, lr, beta1, beta2, eps, decay, 1,
+                                                     maximize, 1, nullptr, 0, t.stream);
+  return status == 0 ? py::object(py::bool_(true)) : py::object(py::int_(status));
+}
+
+// The float32 values of 8-bit states, of a parameter's shape and strides.
+py::object adamw_values(py::handle p_, py::handle mc_, py::handle ms_, py::handle vc_, py::handle vs_) {
+  Operand p, mc, ms, vc, vs;
+  Target t;
+  if (!names().ready || !operand(p_, &p) || !operand(mc_, &mc) || !operand(ms_, &ms) || !operand(vc_, &vc) ||
+      !operand(vs_, &vs) || !p.given || !mc.given || !ms.given || !vc.given || !vs.given ||
+      !p.t->is_non_overlapping_and_dense() || !t.of(p))
+    return py::none();
+  const int64_t n = p.t->numel(), at = (n + 63) / 64 * 64;  // both in one block
+  char* ptr = nullptr;
+  py::object owner = new_storage(t, at + n, &ptr);
+  if (!owner) return py::none();
+  const int status = MM_SYMBOL(decode_fn, "mm_adamw_decode")(mc.ptr, ms.ptr, vc.ptr, vs.ptr, n, ptr, ptr + 4 * at,
+                                                             t.stream);
+  if (status != 0) return py::int_(status);
+  const py::tuple shape = int_tuple(p.t->sizes()), strides = int_tuple(p.t->strides());
+  return py::make_tuple(new_tensor(t, owner, shape, strides, 0), new_tensor(t, owner, shape, strides, at));
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -510,5 +579,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("layer_norm_backward", &layer_norm_backward, "mm_layer_norm_backward with its outputs, or None");
   m.def("linear", &linear, "mm_linear with its outputs, or None");
   m.def("linear_ready", &linear_ready, "Whether linear would take these operands");
+  m.def("adamw_step", &adamw_step, "mm_adamw over parameters and their states, or None");
+  m.def("adamw_values", &adamw_values, "mm_adamw_decode with its outputs, or None");
   m.def("linear_backward", &linear_backward, "mm_linear_backward with its outputs, or None");
 }

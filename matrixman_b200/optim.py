@@ -146,6 +146,23 @@ class AdamW(torch.optim.Optimizer):
         return (_pointer(p), _pointer(grad), _pointer(m), _pointer(v), ms, vs, _pointer(state["step"]),
                 numel(p.shape))
 
+    def _step(self, params: list, states: list, factors: tuple, maximize: bool) -> None:
+        """A step whose tensors need checks or copies first."""
+        rt = params[0].runtime
+        rows, held = [], []
+        for p, state in zip(params, states):
+            grad = ops.require_mm(p.grad, "AdamW gradient")
+            ops.require_f32(grad, "AdamW gradient")
+            _check_storage(p, "AdamW parameter")
+            if grad.runtime is not rt or p.runtime is not rt:
+                raise RuntimeError("MatrixMan/CUDA: AdamW parameter and gradient are on different devices")
+            grad = _in_order(grad, p)
+            held.append(grad)
+            rows.append(self._row(p, grad, state))
+        lr, beta1, beta2, eps, weight_decay = factors
+        run_adamw(rt, rows, self.state_bits, lr=lr, beta1=beta1, beta2=beta2, eps=eps, weight_decay=weight_decay,
+                  decoupled=True, maximize=maximize, advance=True)
+
     @torch.no_grad()
     def step(self, closure=None):
         """One step over every parameter that has a gradient."""
@@ -157,22 +174,12 @@ class AdamW(torch.optim.Optimizer):
             params = [p for p in group["params"] if p.grad is not None]
             if not params:
                 continue
-            rt = params[0].runtime
-            rows, held = [], []
-            for p in params:
-                grad = p.grad
-                if type(grad) is not MatrixManTensor:
-                    grad = ops.require_mm(grad, "AdamW gradient")
-                if grad.dtype != torch.float32 or grad._owner.runtime is not rt or p._owner.runtime is not rt:
-                    ops.require_f32(grad, "AdamW gradient")
-                    raise RuntimeError("MatrixMan/CUDA: AdamW parameter and gradient are on different devices")
-                if not _same_order(grad, p):
-                    grad = _in_order(grad, p)
-                    held.append(grad)
-                rows.append(self._row(p, grad, self._state_of(p)))
             beta1, beta2 = group["betas"]
-            run_adamw(rt, rows, self.state_bits, lr=float(group["lr"]), beta1=beta1, beta2=beta2, eps=group["eps"],
-                      weight_decay=group["weight_decay"], decoupled=True, maximize=group["maximize"], advance=True)
+            factors = (float(group["lr"]), beta1, beta2, group["eps"], group["weight_decay"])
+            states = [self._state_of(p) for p in params]
+            if ops.native_call("adamw_step", "mm_adamw", params, states, self.state_bits, *factors,
+                               group["maximize"]) is None:
+                self._step(params, states, factors, group["maximize"])
             torch.autograd.graph.increment_version(params)
         return loss
 
@@ -183,6 +190,9 @@ class AdamW(torch.optim.Optimizer):
         state = self._state_of(p)
         if self.state_bits == 32:
             return ops.clone(state["exp_avg"]), ops.clone(state["exp_avg_sq"])
+        done = ops.native_call("adamw_values", "mm_adamw_decode", p, *(state[k] for k in _CODES))
+        if done is not None:
+            return done
         rt, n, shape = p.runtime, numel(p.shape), tuple(p.shape)
         at = (n + 63) // 64 * 64  # both in one block
         owner = rt.new_storage(at + n)

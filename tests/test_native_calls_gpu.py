@@ -135,3 +135,37 @@ def test_out_of_memory_is_an_error_of_the_call(mm):
     finally:
         assert lib.mm_debug_fail_alloc_after(rt.index, ctypes.c_int64(-1)) == 0
     assert mm.linear(x[:1], w).shape == (1, 1 << 20)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adamw(mm, monkeypatch, bits):
+    from matrixman_b200 import ops
+    native = ops.native_call
+    shapes = [(300,), (17, 40), (0, 3), (1,)]
+    runs = []
+    for call in (native, lambda *a: None):
+        answered = []
+
+        def counted(*args, call=call, answered=answered):
+            r = call(*args)
+            answered.append(r is not None)
+            return r
+
+        monkeypatch.setattr(ops, "native_call", counted)
+        params = [torch.nn.Parameter(mm.to_device(randn(*s, seed=i))) for i, s in enumerate(shapes)]
+        opt = mm.optim.AdamW(params, lr=1e-2, state_bits=bits, maximize=True)
+        for step in range(3):
+            for i, p in enumerate(params):
+                p.grad = mm.to_device(randn(*shapes[i], seed=10 * step + i))
+            opt.step()
+        out = [p.detach().cpu() for p in params] + [v.cpu() for p in params for v in opt.state_values(p)]
+        runs.append((out, answered))
+    assert all(torch.equal(a, b) for a, b in zip(runs[0][0], runs[1][0]))
+    assert all(runs[0][1]) and not any(runs[1][1])
+    # a gradient in another order, and one of another kind, go through the Python code
+    monkeypatch.setattr(ops, "native_call", native)
+    p = torch.nn.Parameter(mm.to_device(torch.zeros(6, 4)))
+    opt = mm.optim.AdamW([p], lr=1.0, weight_decay=0.0, state_bits=bits)
+    p.grad = mm.to_device(torch.ones(4, 6)).t()
+    opt.step()
+    assert ((p.detach().cpu() + 1).abs() <= 2.0 ** -19).all()
