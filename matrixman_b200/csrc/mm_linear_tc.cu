@@ -708,6 +708,10 @@ int lin_run_splits(const LinSplits& all, cudaStream_t s) {
 // 664, 64 wide 936; asking L2 for the stages ahead of their loads made it 835).
 // Whole waves of tiles run undivided; the rest is divided where that ends
 // sooner although its partial tiles are written and read once more.
+// Sharing the rest's stages out evenly, across the tiles' borders, is slower:
+// CTAs that share operand tiles are then at different stages and find them in
+// L2 less often (forward 1111 x 1502 x 2501: 72 -> 79 us, gradients 156 -> 170;
+// gradients of 2000 x 1280 x 1000: 118 -> 121).
 LinChoice lin_choose(int64_t m, int64_t n, int64_t k) {
   const int sms = sm_count();
   LinChoice best = {};
