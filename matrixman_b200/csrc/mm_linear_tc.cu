@@ -174,19 +174,73 @@ __device__ __forceinline__ void lg_arrive(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(lg_smem(bar)) : "memory");
 }
 
+// The cluster's address of CTA 0's barrier (or another one's of this CTA).
+__device__ __forceinline__ uint32_t lg_lead(uint64_t* bar) {
+  uint32_t addr;
+  asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(addr) : "r"(lg_smem(bar)));
+  return addr;
+}
+
+// (Tensor memory's reads are over by then, and no other memory has to be seen:
+// a release to the cluster would take 1,000 to 2,000 clocks.)
+__device__ __forceinline__ void lg_arrive_at(uint32_t bar) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+
+// All threads of the CTA, of both in a pair.
+template <bool PAIR>
+__device__ __forceinline__ void lg_sync() {
+  if (PAIR) {
+    asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+  } else {
+    __syncthreads();
+  }
+}
+
+// When the MMAs issued so far are done, arrive on the barrier; in a pair on
+// both CTAs'.
+template <bool PAIR>
 __device__ __forceinline__ void lg_commit(uint64_t* bar) {
+  if (PAIR) {
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+            lg_smem(bar)),
+        "h"((uint16_t)3)
+        : "memory");
+    return;
+  }
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(lg_smem(bar))
                : "memory");
 }
 
-__device__ __forceinline__ void lg_load(void* dst, const CUtensorMap* map, uint64_t* bar, int x, int y) {
+template <bool PAIR>
+__device__ __forceinline__ void lg_load(void* dst, const CUtensorMap* map, uint32_t bar, int x, int y) {
+  if (PAIR) {  // the barrier may be the other CTA's
+    asm volatile(
+        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, "
+        "%3, %4}], [%5];" ::"r"(lg_smem(dst)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(0), "r"(bar)
+        : "memory");
+    return;
+  }
   asm volatile(
       "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
-      ::"r"(lg_smem(dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(0), "r"(lg_smem(bar))
+      ::"r"(lg_smem(dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(0), "r"(bar)
       : "memory");
 }
 
+template <bool PAIR>
 __device__ __forceinline__ void lg_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  if (PAIR) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+    return;
+  }
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
@@ -236,19 +290,21 @@ struct LgTile {
     const uint32_t lo = ((at >> 4) & 0x3fffu) | ((MN ? 12288u >> 4 : 1u) << 16);
     return (uint64_t)hi << 32 | lo;
   }
-  static __device__ __forceinline__ void load(uint8_t* dst, const CUtensorMap* map, uint64_t* bar, int row, int k) {
+  template <bool PAIR>
+  static __device__ __forceinline__ void load(uint8_t* dst, const CUtensorMap* map, uint32_t bar, int row, int k) {
     if (MN) {
 #pragma unroll
-      for (int g = 0; g < ROWS / 64; ++g) lg_load(dst + g * 12288, map, bar, row + 64 * g, k);
+      for (int g = 0; g < ROWS / 64; ++g) lg_load<PAIR>(dst + g * 12288, map, bar, row + 64 * g, k);
     } else {
-      lg_load(dst, map, bar, k, row);
+      lg_load<PAIR>(dst, map, bar, k, row);
     }
   }
 };
 
-template <int BN>
+// Stages that shared memory holds: 48 KB each, or 36.
+template <int BN, bool PAIR>
 constexpr int lg_stages() {
-  return BN == 128 ? 4 : 5;
+  return BN == 128 && !PAIR ? 4 : 5;
 }
 
 // One unit of work: an output tile and a range of its reduction's stages.
@@ -272,7 +328,7 @@ __device__ __forceinline__ LgUnit lg_unit(const LinGemm& a, int u, int bn) {
   const int per = LIN_GROUP * a.tiles_n;
   const int group = tile / per, in = tile - group * per;
   const int rows = min(LIN_GROUP, a.tiles_m - group * LIN_GROUP);
-  w.m0 = (group * LIN_GROUP + in % rows) * LG_BM;
+  w.m0 = (group * LIN_GROUP + in % rows) * a.bm;
   w.n0 = (in / rows) * bn;
   w.begin = (int)((int64_t)a.stages * split / splits);
   w.end = (int)((int64_t)a.stages * (split + 1) / splits);
@@ -442,13 +498,17 @@ __device__ __forceinline__ void lg_finish_rows(const LinGemm& a, const float* ti
 // of a stage are added at full size.  One issuer left the tensor core idle for
 // the 300 to 400 clocks of its waits and commits in each stage (2000 x 1280 x
 // 1000: 49 us, with two 44).
-template <int BN, bool AMN, bool BMN>
+//
+// PAIR: two CTAs on neighbouring SMs share a tile of 256 rows.  Each loads its
+// 128 rows of A and half of B's, which is what bounds a stage (36 KB in place
+// of 48); CTA 0 issues the MMAs of both, each CTA keeps and stores its rows.
+template <int BN, bool AMN, bool BMN, bool PAIR>
 __global__ void __launch_bounds__(LG_THREADS, 1) linear_gemm_kernel(const __grid_constant__ CUtensorMap ma,
                                                                     const __grid_constant__ CUtensorMap mb,
                                                                     const LinGemm a) {
   using TA = LgTile<LG_BM, AMN>;
-  using TB = LgTile<BN, BMN>;
-  constexpr int S = lg_stages<BN>();
+  using TB = LgTile<PAIR ? BN / 2 : BN, BMN>;
+  constexpr int S = lg_stages<BN, PAIR>();
   constexpr uint32_t stage_bytes = TA::bytes + TB::bytes;
   constexpr int ACCS = LG_ACCS;
   constexpr uint32_t cols = ACCS * BN;
@@ -461,6 +521,9 @@ __global__ void __launch_bounds__(LG_THREADS, 1) linear_gemm_kernel(const __grid
   int* special = reinterpret_cast<int*>(slot + 1);
   float* store = reinterpret_cast<float*>(smem + S * stage_bytes + 256);  // a 32 x 32 block per adding warp
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // (a cluster is a pair, and neighbours in the grid)
+  const int rank = PAIR ? blockIdx.x & 1 : 0, worker = blockIdx.x >> (PAIR ? 1 : 0);
+  const int workers = gridDim.x >> (PAIR ? 1 : 0), row_in_tile = rank * LG_BM;
   if (threadIdx.x == 0) {
     for (int i = 0; i < S; ++i) {
       lg_bar_init(&full[i], 1);
@@ -468,19 +531,25 @@ __global__ void __launch_bounds__(LG_THREADS, 1) linear_gemm_kernel(const __grid
     }
     for (int i = 0; i < ACCS; ++i) {
       lg_bar_init(&acc_full[i], 1);
-      lg_bar_init(&acc_free[i], LG_EPI_WARPS);
+      lg_bar_init(&acc_free[i], PAIR ? 2 * LG_EPI_WARPS : LG_EPI_WARPS);
     }
     for (int i = 0; i < LG_ISSUERS; ++i) lg_bar_init(&drain[i], 1);
     *special = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == LG_WARP_MMA) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(lg_smem(slot)), "r"(cols)
-                 : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    if (PAIR) {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(lg_smem(slot)), "r"(cols)
+                   : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    } else {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(lg_smem(slot)), "r"(cols)
+                   : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-  __syncthreads();
+  lg_sync<PAIR>();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = *slot;
   pdl_wait();
@@ -491,19 +560,22 @@ __global__ void __launch_bounds__(LG_THREADS, 1) linear_gemm_kernel(const __grid
       int st = 0, filled = 0;
       uint32_t par = 1;
       bool alive = true;
-      for (int u = blockIdx.x; u < a.units && alive; u += gridDim.x) {
+      for (int u = worker; u < a.units && alive; u += workers) {
         const LgUnit w = lg_unit(a, u, BN);
         for (int k = w.begin; k < w.end; ++k) {
           if (!lg_wait(&empty[st], par, LG_ERR_EMPTY)) {
             alive = false;
             break;
           }
-          asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(lg_smem(&full[st])),
-                       "r"(stage_bytes)
-                       : "memory");
+          // (in a pair CTA 0's barrier counts the bytes of both)
+          if (rank == 0)
+            asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(lg_smem(&full[st])),
+                         "r"(PAIR ? 2 * stage_bytes : stage_bytes)
+                         : "memory");
           uint8_t* dst = smem + (uint32_t)st * stage_bytes;
-          TA::load(dst, &ma, &full[st], w.m0, k * LG_BK);
-          TB::load(dst + TA::bytes, &mb, &full[st], w.n0, k * LG_BK);
+          const uint32_t bar = PAIR ? lg_lead(&full[st]) : lg_smem(&full[st]);
+          TA::template load<PAIR>(dst, &ma, bar, w.m0 + row_in_tile, k * LG_BK);
+          TB::template load<PAIR>(dst + TA::bytes, &mb, bar, w.n0 + rank * (BN / 2), k * LG_BK);
           ++filled;
           if (++st == S) {
             st = 0;
@@ -512,20 +584,22 @@ __global__ void __launch_bounds__(LG_THREADS, 1) linear_gemm_kernel(const __grid
         }
       }
       // Nothing may land in shared memory after the CTA has gone: wait for the
-      // last fill of every stage (over already unless a wait gave up).
-      for (int i = max(0, filled - S); i < filled; ++i) lg_wait(&full[i % S], (uint32_t)(i / S) & 1u, LG_ERR_DRAIN);
+      // last fill of every stage (over already unless a wait gave up), in a
+      // pair's CTA 1 for the MMAs that have read it.
+      for (int i = max(0, filled - S); i < filled; ++i)
+        lg_wait(rank == 0 ? &full[i % S] : &empty[i % S], (uint32_t)(i / S) & 1u, LG_ERR_DRAIN);
     }
     __syncwarp();
   } else if (warp >= LG_WARP_MMA) {
     const int issuer = warp - LG_WARP_MMA;
-    if (lane == 0) {
+    if (lane == 0 && rank == 0) {
       constexpr uint32_t idesc = 1u << 4 | 1u << 7 | 1u << 10 | (AMN ? 1u << 15 : 0u) | (BMN ? 1u << 16 : 0u) |
-                                 (uint32_t)(BN >> 3) << 17 | (uint32_t)(LG_BM >> 4) << 24;
+                                 (uint32_t)(BN >> 3) << 17 | (uint32_t)((PAIR ? 2 * LG_BM : LG_BM) >> 4) << 24;
       const uint32_t base = lg_smem(smem);
       int st = 0, buf = 0;
       uint32_t par = 0, bpar = 1;
       bool alive = true;
-      for (int u = blockIdx.x; u < a.units && alive; u += gridDim.x) {
+      for (int u = worker; u < a.units && alive; u += workers) {
         const LgUnit w = lg_unit(a, u, BN);
         for (int k = w.begin; k < w.end; ++k) {
           if (buf % LG_ISSUERS == issuer) {
@@ -541,9 +615,9 @@ __global__ void __launch_bounds__(LG_THREADS, 1) linear_gemm_kernel(const __grid
             for (int q = 0; q < 6; ++q)
 #pragma unroll
               for (int kk = 0; kk < 2; ++kk)
-                lg_mma(d, TA::desc(at, pa[q], kk), TB::desc(bt, pb[q], kk), idesc, q + kk > 0 ? 1u : 0u);
-            lg_commit(&empty[st]);
-            lg_commit(&acc_full[buf]);
+                lg_mma<PAIR>(d, TA::desc(at, pa[q], kk), TB::desc(bt, pb[q], kk), idesc, q + kk > 0 ? 1u : 0u);
+            lg_commit<PAIR>(&empty[st]);
+            lg_commit<PAIR>(&acc_full[buf]);
           }
           if (++st == S) {
             st = 0;
@@ -556,7 +630,7 @@ __global__ void __launch_bounds__(LG_THREADS, 1) linear_gemm_kernel(const __grid
         }
       }
       // No MMA may still write tensor memory when it is freed.
-      lg_commit(&drain[issuer]);
+      lg_commit<PAIR>(&drain[issuer]);
       lg_wait(&drain[issuer], 0u, LG_ERR_DRAIN);
     }
     __syncwarp();
@@ -571,7 +645,7 @@ __global__ void __launch_bounds__(LG_THREADS, 1) linear_gemm_kernel(const __grid
     for (int i = threadIdx.x; i < a.flags_a; i += LG_EPI_WARPS * 32) inf |= a.pa.flags[i];
     for (int i = threadIdx.x; i < a.flags_b; i += LG_EPI_WARPS * 32) inf |= a.pb.flags[i];
     if (inf) *special = 1;
-    for (int u = blockIdx.x; u < a.units && alive; u += gridDim.x) {
+    for (int u = worker; u < a.units && alive; u += workers) {
       const LgUnit w = lg_unit(a, u, BN);
       float acc[HALF];
 #pragma unroll
@@ -591,17 +665,23 @@ __global__ void __launch_bounds__(LG_THREADS, 1) linear_gemm_kernel(const __grid
         }
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
         __syncwarp();
-        if (lane == 0) lg_arrive(&acc_free[buf]);
+        if (lane == 0) {
+          if (PAIR)
+            lg_arrive_at(lg_lead(&acc_free[buf]));
+          else
+            lg_arrive(&acc_free[buf]);
+        }
         if (++buf == ACCS) {
           buf = 0;
           par ^= 1u;
         }
       }
       if (!alive) break;
-      const int64_t row = (int64_t)w.m0 + quarter * 32 + lane;
+      const int in_tile = row_in_tile + quarter * 32;
+      const int64_t row = (int64_t)w.m0 + in_tile + lane;
       const int col = w.n0 + half * HALF;
       if (w.part >= 0) {
-        float4* part = reinterpret_cast<float4*>(a.part + ((int64_t)w.part * LG_BM + quarter * 32 + lane) * BN + half * HALF);
+        float4* part = reinterpret_cast<float4*>(a.part + ((int64_t)w.part * a.bm + in_tile + lane) * BN + half * HALF);
 #pragma unroll
         for (int j = 0; j < HALF / 4; ++j) part[j] = make_float4(acc[4 * j], acc[4 * j + 1], acc[4 * j + 2], acc[4 * j + 3]);
         continue;
@@ -616,7 +696,7 @@ __global__ void __launch_bounds__(LG_THREADS, 1) linear_gemm_kernel(const __grid
 #pragma unroll
         for (int i = 0; i < 32; ++i) stage[32 * lane + (i ^ lane)] = acc[32 * j + i];
         __syncwarp();
-        const int c = col + 32 * j + lane, row0 = w.m0 + quarter * 32;
+        const int c = col + 32 * j + lane, row0 = w.m0 + in_tile;
         switch (a.e.act) {
           case MM_LINEAR_RELU: lg_finish_rows<MM_LINEAR_RELU>(a, stage, row0, c, lane); break;
           case MM_LINEAR_SILU: lg_finish_rows<MM_LINEAR_SILU>(a, stage, row0, c, lane); break;
@@ -629,15 +709,18 @@ __global__ void __launch_bounds__(LG_THREADS, 1) linear_gemm_kernel(const __grid
     }
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-  __syncthreads();
+  lg_sync<PAIR>();  // in a pair: nothing of the other CTA is on its way to this one
   if (warp == LG_WARP_MMA) {
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(cols) : "memory");
+    if (PAIR)
+      asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(cols) : "memory");
+    else
+      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(cols) : "memory");
   }
   if (*special) {
-    for (int u = blockIdx.x; u < a.units; u += gridDim.x) {
+    for (int u = worker; u < a.units; u += workers) {
       const LgUnit w = lg_unit(a, u, BN);
-      if (w.part < 0) lin_fix(a, w.m0, LG_BM, w.n0, BN);
+      if (w.part < 0) lin_fix(a, w.m0 + row_in_tile, LG_BM, w.n0, BN);
     }
   }
 }
@@ -648,14 +731,14 @@ __global__ void __launch_bounds__(LG_THREADS, 1) linear_gemm_kernel(const __grid
 template <int BN>
 __global__ void __launch_bounds__(2 * BN) linear_join_kernel(const LinGemm a) {
   pdl_wait();
-  const int tile = blockIdx.x / (LG_BM / 8), r0 = blockIdx.x % (LG_BM / 8) * 8;
+  const int tile = blockIdx.x / (a.bm / 8), r0 = blockIdx.x % (a.bm / 8) * 8;
   const LgUnit w = lg_unit(a, a.full + tile * a.splits, BN);
   const int r = r0 + threadIdx.x / (BN / 4), c = threadIdx.x % (BN / 4) * 4;
-  const float* part = a.part + ((int64_t)tile * a.splits * LG_BM + r) * BN + c;
+  const float* part = a.part + ((int64_t)tile * a.splits * a.bm + r) * BN + c;
   float v[4] = {};
 #pragma unroll 4
   for (int s = 0; s < a.splits; ++s) {
-    const float4 t = *reinterpret_cast<const float4*>(part + (int64_t)s * LG_BM * BN);
+    const float4 t = *reinterpret_cast<const float4*>(part + (int64_t)s * a.bm * BN);
     v[0] += t.x; v[1] += t.y; v[2] += t.z; v[3] += t.w;
   }
   if (w.m0 + r < a.m && w.n0 + c < a.n) lin_finish_row<4>(a.e, v, a.c, w.m0 + r, w.n0 + c, a.n, a.vec);
@@ -699,45 +782,52 @@ int lin_run_splits(const LinSplits& all, cudaStream_t s) {
   return e == cudaSuccess ? MM_OK : cuda_fail(e, "mm_linear split launch");
 }
 
-// Tile width and division of the reduction, by an estimate in SM clocks.  What
-// bounds a stage is its way from L2, about 42 bytes per clock and SM: 48 KB take
-// 1,150 clocks (BN 128; its MMAs 768), 36 KB 880 (BN 64; 384).  A tile takes
-// about 4,000 more to fill the pipeline and store.  Tiles 256 wide need 72 KB
-// per 1,536 clocks of MMAs, but have only two accumulators, and the MMAs wait
-// for the additions: slower at every size (8192 x 2048 x 4096: 689 us, 128 wide
-// 664, 64 wide 936; asking L2 for the stages ahead of their loads made it 835).
+// Tiles and division of the reduction, by an estimate in SM clocks.  What bounds
+// a stage is shared memory at 128 bytes per clock: each of its twelve MMAs reads
+// its operands there and TMA writes them once.  128 x 128: 12 x 8 KB + 48 KB,
+// 1,125 clocks (1,150 to 1,250 measured; the MMAs alone 768); 128 x 64: 12 x 6 +
+// 36, 844 (880; 384); 256 x 128 of a CTA pair, per CTA: 12 x 6 + 36, 844 (980;
+// 768).  Pairs are the best where there is work for all of them (us, without and
+// with): 8192 x 2048 x 4096 686 -> 607, 2048 x 2048 x 2048 110 -> 95, gradients of
+// 2000 x 1280 x 1000 118 -> 104.  A tile takes about 4,000 more to fill the
+// pipeline and store.  Tiles 256 wide of one CTA were slower at every size, as
+// they leave only two accumulators and the MMAs wait for the additions; so was
+// asking L2 for the stages ahead of their loads.
 // Whole waves of tiles run undivided; the rest is divided where that ends
-// sooner although its partial tiles are written and read once more.
-// Sharing the rest's stages out evenly, across the tiles' borders, is slower:
-// CTAs that share operand tiles are then at different stages and find them in
-// L2 less often (forward 1111 x 1502 x 2501: 72 -> 79 us, gradients 156 -> 170;
-// gradients of 2000 x 1280 x 1000: 118 -> 121).
+// sooner although its partial tiles are written and read once more.  Sharing
+// the rest's stages out evenly, across the tiles' borders, is slower: CTAs that
+// share operand tiles are then at different stages and find them in L2 less
+// often (forward 1111 x 1502 x 2501: 72 -> 79 us, gradients 156 -> 170).
 LinChoice lin_choose(int64_t m, int64_t n, int64_t k) {
-  const int sms = sm_count();
+  static const struct {
+    int bm, bn;
+    double stage;
+  } kinds[] = {{256, 128, 980}, {128, 128, 1150}, {128, 64, 880}};
   LinChoice best = {};
-  for (int bn : {128, 64}) {
-    const int64_t tm = (m + LG_BM - 1) / LG_BM, tn = (n + bn - 1) / bn, tiles = tm * tn;
+  for (const auto& kind : kinds) {
+    const int workers = kind.bm == 256 ? sm_count() / 2 : sm_count();
+    const int64_t tm = (m + kind.bm - 1) / kind.bm, tn = (n + kind.bn - 1) / kind.bn, tiles = tm * tn;
     const int64_t stages = (k + LG_BK - 1) / LG_BK;
-    const double stage = bn == 128 ? 1150 : 880, tile = 4000;
-    const int64_t full = tiles / sms * sms, rest = tiles - full;
-    const double base = (double)(full / sms) * (stages * stage + tile);
+    const double tile = 4000;
+    const int64_t full = tiles / workers * workers, rest = tiles - full;
+    const double base = (double)(full / workers) * (stages * kind.stage + tile);
     for (int s = 1; s <= LIN_MAX_SPLITS; ++s) {
-      if (s > 1 && (rest == 0 || s > stages || rest * s > LIN_MAX_PARTS)) break;
+      if (s > 1 && (rest == 0 || s > stages || rest * s > 2 * workers)) break;
       double t = base;
       if (rest) {
-        const int64_t waves = (rest * s + sms - 1) / sms;
-        t += waves * (((stages + s - 1) / s) * stage + tile);
-        if (s > 1) t += 10000 + (double)rest * s * LG_BM * bn * 8 / 3500;  // one more launch, 3,500 bytes per clock
+        const int64_t waves = (rest * s + workers - 1) / workers;
+        t += waves * (((stages + s - 1) / s) * kind.stage + tile);
+        if (s > 1) t += 10000 + (double)rest * s * kind.bm * kind.bn * 8 / 3500;  // one more launch, 3,500 bytes per clock
       }
       if (best.bn == 0 || t < best.clocks)
-        best = {bn, (int)full, s, (int)tm, (int)tn, (int)stages, (int)(full + rest * s), t};
+        best = {kind.bm, kind.bn, (int)full, s, (int)tm, (int)tn, (int)stages, (int)(full + rest * s), t};
     }
   }
   return best;
 }
 
 int64_t lin_part_bytes(const LinChoice& c) {
-  return c.splits > 1 ? (int64_t)(c.units - c.full) * LG_BM * c.bn * 4 : 0;
+  return c.splits > 1 ? (int64_t)(c.units - c.full) * c.bm * c.bn * 4 : 0;
 }
 
 // Blocks that linear_split_kernel made of an operand.
@@ -770,25 +860,28 @@ static int lin_map(const LinPlanes& p, int rows, CUtensorMap* out) {
   return MM_OK;
 }
 
-template <int BN, bool AMN, bool BMN>
+template <int BN, bool AMN, bool BMN, bool PAIR>
 static int lin_launch(const CUtensorMap& ma, const CUtensorMap& mb, const LinGemm& g, cudaStream_t s) {
   // alignment, stages, barriers, 32 x 32 blocks of the adding warps
-  constexpr size_t smem = 1024 + (size_t)lg_stages<BN>() * (LG_BM + BN) * 192 + 256 + LG_EPI_WARPS * 4096;
+  constexpr size_t smem =
+      1024 + (size_t)lg_stages<BN, PAIR>() * (LG_BM + (PAIR ? BN / 2 : BN)) * 192 + 256 + LG_EPI_WARPS * 4096;
   static_assert(smem <= 227 * 1024, "shared memory of a block");
-  auto kernel = linear_gemm_kernel<BN, AMN, BMN>;
+  auto kernel = linear_gemm_kernel<BN, AMN, BMN, PAIR>;
   MM_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem),
           "mm_linear: shared memory attribute");
-  const int sms = sm_count();
-  MM_CUDA(launch_pdl(kernel, dim3((unsigned)(g.units < sms ? g.units : sms)), dim3(LG_THREADS), smem, s, ma, mb, g),
+  const int size = PAIR ? 2 : 1, workers = sm_count() / size;
+  MM_CUDA(launch_pdl_cluster(kernel, dim3((unsigned)(size * (g.units < workers ? g.units : workers))),
+                             dim3(LG_THREADS), size, smem, s, ma, mb, g),
           "mm_linear launch");
   return MM_OK;
 }
 
-template <int BN>
-static int lin_launch_bn(bool amn, bool bmn, const CUtensorMap& ma, const CUtensorMap& mb, const LinGemm& g,
-                         cudaStream_t s) {
-  if (amn) return bmn ? lin_launch<BN, true, true>(ma, mb, g, s) : lin_launch<BN, true, false>(ma, mb, g, s);
-  return bmn ? lin_launch<BN, false, true>(ma, mb, g, s) : lin_launch<BN, false, false>(ma, mb, g, s);
+template <int BN, bool PAIR>
+static int lin_launch_kind(bool amn, bool bmn, const CUtensorMap& ma, const CUtensorMap& mb, const LinGemm& g,
+                           cudaStream_t s) {
+  if (amn)
+    return bmn ? lin_launch<BN, true, true, PAIR>(ma, mb, g, s) : lin_launch<BN, true, false, PAIR>(ma, mb, g, s);
+  return bmn ? lin_launch<BN, false, true, PAIR>(ma, mb, g, s) : lin_launch<BN, false, false, PAIR>(ma, mb, g, s);
 }
 
 int lin_run_gemm(const LinPlanes& pa, const LinPlanes& pb, float* c, const LinEpilogue& e, const LinChoice& ch,
@@ -796,6 +889,7 @@ int lin_run_gemm(const LinPlanes& pa, const LinPlanes& pb, float* c, const LinEp
   LinGemm g;
   g.m = (int)pa.lines;
   g.n = (int)pb.lines;
+  g.bm = ch.bm;
   g.stages = ch.stages;
   g.tiles_m = ch.tiles_m;
   g.tiles_n = ch.tiles_n;
@@ -814,12 +908,14 @@ int lin_run_gemm(const LinPlanes& pa, const LinPlanes& pb, float* c, const LinEp
   g.flags_b = lin_flag_count(pb);
   CUtensorMap ma, mb;
   int rc = lin_map(pa, LG_BM, &ma);
-  if (rc == MM_OK) rc = lin_map(pb, ch.bn, &mb);
+  if (rc == MM_OK) rc = lin_map(pb, ch.bm == 256 ? ch.bn / 2 : ch.bn, &mb);
   if (rc != MM_OK) return rc;
-  rc = ch.bn == 128 ? lin_launch_bn<128>(pa.mn, pb.mn, ma, mb, g, s) : lin_launch_bn<64>(pa.mn, pb.mn, ma, mb, g, s);
+  rc = ch.bm == 256   ? lin_launch_kind<128, true>(pa.mn, pb.mn, ma, mb, g, s)
+       : ch.bn == 128 ? lin_launch_kind<128, false>(pa.mn, pb.mn, ma, mb, g, s)
+                      : lin_launch_kind<64, false>(pa.mn, pb.mn, ma, mb, g, s);
   if (rc != MM_OK) return rc;
   if (ch.splits > 1) {
-    const unsigned grid = (unsigned)((ch.units - ch.full) / ch.splits * (LG_BM / 8));
+    const unsigned grid = (unsigned)((ch.units - ch.full) / ch.splits * (ch.bm / 8));
     MM_CUDA(ch.bn == 128 ? launch_pdl(linear_join_kernel<128>, dim3(grid), dim3(256), 0, s, g)
                          : launch_pdl(linear_join_kernel<64>, dim3(grid), dim3(128), 0, s, g),
             "mm_linear join launch");

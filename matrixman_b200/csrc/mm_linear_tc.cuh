@@ -40,10 +40,9 @@ struct LinPlanes {
 
 constexpr int LIN_GROUP = 8;        // rows of tiles that run together
 constexpr int LIN_MAX_SPLITS = 32;
-constexpr int LIN_MAX_PARTS = 296;  // partial tiles
 
 struct LinChoice {
-  int bn;               // columns of a tile (128 rows)
+  int bm, bn;           // rows of a tile (256: of a CTA pair's) and columns
   int full;             // tiles that run undivided
   int splits;           // parts of the reduction of each tile behind them
   int tiles_m, tiles_n, stages, units;
@@ -51,7 +50,7 @@ struct LinChoice {
 };
 
 struct LinGemm {
-  int m, n, stages, tiles_m, tiles_n, full, splits, units, vec;
+  int m, n, bm, stages, tiles_m, tiles_n, full, splits, units, vec;
   float* c;      // dense [m][n]
   float* part;   // partial tiles
   LinEpilogue e;

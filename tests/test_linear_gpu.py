@@ -120,6 +120,14 @@ def test_sizes(mm, m, n, k):
     check(mm, randn(m, k, seed=1), randn(n, k, seed=2), randn(n, seed=3), None, "none")
 
 
+# Tiles shared by two CTAs: in whole rounds with a rest, with divided reductions,
+# with operands along and across the reduction, rows that end in either half.
+@pytest.mark.parametrize("m,n,k", [(511, 1300, 2049), (2570, 1001, 33), (2500, 1100, 70), (500, 380, 6000)])
+def test_tiles_of_cta_pairs(mm, m, n, k):
+    check(mm, randn(m, k, seed=1), randn(n, k, seed=2), randn(n, seed=3), None, "none")
+    check(mm, randn(m, k, seed=4), randn(n, k, seed=5) / math.sqrt(k), randn(n, seed=6), randn(m, n, seed=7), "gelu")
+
+
 @pytest.mark.parametrize("act", ACTS)
 @pytest.mark.parametrize("mode", ["plain", "bias", "residual", "residual first", "both"])
 def test_epilogues(mm, act, mode):
@@ -167,6 +175,24 @@ def test_non_finite_inputs_reach_their_rows_only(mm):
         assert torch.equal(got[3], want[3])  # infinities of the weights' signs
         rest = [i for i in range(m) if i not in (1, 3)]
         assert torch.isfinite(got[rest]).all()
+
+
+@pytest.mark.parametrize("m,n,k", [(1500, 1500, 100), (511, 1300, 2049)])
+def test_infinities_in_both_halves_of_a_pairs_tile(mm, m, n, k):
+    x, w = randn(m, k, seed=1), randn(n, k, seed=2)
+    rows, cols = (5, 200, 300, m - 1), (3, 70, 127, n - 1)
+    for i, r in enumerate(rows):
+        x[r, 7 * i + 3] = float("-inf") if i % 2 else float("inf")
+    for i, c in enumerate(cols):
+        w[c, 5 * i + 40] = float("inf")
+    got, want = mm.linear(mm.to_device(x), mm.to_device(w)).cpu(), x @ w.t()
+    hit = torch.zeros(m, n, dtype=torch.bool)
+    hit[list(rows)] = True
+    hit[:, list(cols)] = True
+    assert torch.equal(torch.isnan(got), torch.isnan(want)) and not torch.isfinite(got[hit]).any()
+    same = hit & ~torch.isnan(want)
+    assert torch.equal(got[same], want[same])
+    assert torch.isfinite(got[~hit]).all()
 
 
 def test_strides_and_leading_dimensions(mm):
