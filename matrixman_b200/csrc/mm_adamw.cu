@@ -43,7 +43,6 @@ struct AwTensor {
   const float* g;
   void *m, *v;
   float *ms, *vs;
-  float* step;
   uint32_t first;   // first chunk; the end of the table's last tensor is AwTable::chunks
   uint32_t aligned; // p, g (and 32-bit m, v) are 16-byte aligned
   int64_t n;
@@ -56,7 +55,15 @@ struct AwTable {
   int count;
 };
 
+// The driver copies a launch's parameters, so few tensors have a small table and
+// the first kernel one of the steps alone.
 constexpr int AW_FEW = 16, AW_MANY = 400;
+
+template <int MOST>
+struct AwSteps {
+  float* step[MOST];
+  int count;
+};
 
 struct AwScalars {
   float b1, omb1, b2, omb2, eps, decay, l2;  // decay = 1 - lr wd (decoupled); l2 = wd (coupled) or 0
@@ -65,14 +72,14 @@ struct AwScalars {
 
 // A step's own factors of each tensor: lr / (1 - b1^t) and 1 / sqrt(1 - b2^t).
 template <int MOST>
-__global__ void adamw_begin_kernel(const __grid_constant__ AwTable<MOST> tab, float2* coef, double lr, double b1,
+__global__ void adamw_begin_kernel(const __grid_constant__ AwSteps<MOST> tab, float2* coef, double lr, double b1,
                                    double b2, int advance) {
   const int i = blockIdx.x * blockDim.x + threadIdx.x;
   if (i >= tab.count) return;
-  float t = *tab.t[i].step;
+  float t = *tab.step[i];
   if (advance) {
     t += 1.f;
-    *tab.t[i].step = t;
+    *tab.step[i] = t;
   }
   coef[i] = make_float2((float)(lr / (1.0 - pow(b1, (double)t))), (float)(1.0 / sqrt(1.0 - pow(b2, (double)t))));
 }
@@ -337,18 +344,20 @@ template <int MOST>
 static int aw_launch(const mm_adamw_tensor_t* in, int count, int bits, double lr, double b1, double b2, int advance,
                      const AwScalars& a, float2* coef, cudaStream_t s) {
   AwTable<MOST> tab;
+  AwSteps<MOST> steps;
   int64_t chunks = 0;
   for (int i = 0; i < count; ++i) {
     AwTensor& t = tab.t[i];
     t = {in[i].param, in[i].grad, in[i].exp_avg, in[i].exp_avg_sq, in[i].exp_avg_scale, in[i].exp_avg_sq_scale,
-         in[i].step, (uint32_t)chunks, 0, in[i].numel};
+         (uint32_t)chunks, 0, in[i].numel};
+    steps.step[i] = in[i].step;
     t.aligned = aw_aligned(t.p, 16) && aw_aligned(t.g, 16) &&
                 (bits == 8 || (aw_aligned(t.m, 16) && aw_aligned(t.v, 16)));
     chunks += bits == 8 ? (t.n + AW_CHUNK8 - 1) / AW_CHUNK8 : (t.n + AW_CHUNK - 1) / AW_CHUNK;
   }
   if (chunks > INT32_MAX) return fail(MM_ERR_UNSUPPORTED, "mm_adamw: too many elements in one call");
-  tab.count = count;
-  adamw_begin_kernel<MOST><<<(count + 127) / 128, 128, 0, s>>>(tab, coef, lr, b1, b2, advance);
+  tab.count = steps.count = count;
+  adamw_begin_kernel<MOST><<<(count + 127) / 128, 128, 0, s>>>(steps, coef, lr, b1, b2, advance);
   MM_LAUNCH_CHECK("mm_adamw launch");
   if (chunks == 0) return MM_OK;  // every tensor is empty: only the steps move
   if (bits == 32)
@@ -414,8 +423,8 @@ extern "C" int mm_adamw(const mm_adamw_tensor_t* tensors, int count, int state_b
   float2* coef = (float2*)workspace;
   for (int at = 0; at < count; at += AW_MANY) {
     const int n = count - at < AW_MANY ? count - at : AW_MANY;
-    const int rc = n <= AW_FEW ? aw_launch<AW_FEW>(tensors + at, n, state_bits, lr, beta1, beta2, advance, a, coef + at, s)
-                               : aw_launch<AW_MANY>(tensors + at, n, state_bits, lr, beta1, beta2, advance, a, coef + at, s);
+    const auto launch = n <= AW_FEW ? aw_launch<AW_FEW> : aw_launch<AW_MANY>;
+    const int rc = launch(tensors + at, n, state_bits, lr, beta1, beta2, advance, a, coef + at, s);
     if (rc != MM_OK) return rc;
   }
   return MM_OK;

@@ -176,14 +176,13 @@ class AdamW(torch.optim.Optimizer):
                 continue
             beta1, beta2 = group["betas"]
             factors = (float(group["lr"]), beta1, beta2, group["eps"], group["weight_decay"])
-            states = [self._state_of(p) for p in params]
+            states = [self.state.get(p) or self._state_of(p) for p in params]
             if ops.native_call("adamw_step", "mm_adamw", params, states, self.state_bits, *factors,
                                group["maximize"]) is None:
                 self._step(params, states, factors, group["maximize"])
             torch.autograd.graph.increment_version(params)
         return loss
 
-    @torch.no_grad()
     def state_values(self, p) -> tuple[MatrixManTensor, MatrixManTensor]:
         """(exp_avg, exp_avg_sq) of a parameter as new float32 tensors (8-bit
         states: the values that the codes stand for)."""
