@@ -42,6 +42,12 @@ cudaStream_t resolve_stream(void* stream);
 // ---------------------------------------------------------------------------
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
+// From here on (in every block) the next kernel's blocks may take the room that
+// this one's leave.
+__device__ __forceinline__ void pdl_trigger() {
+  if (threadIdx.x == 0) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
 inline bool pdl_enabled() {
   static const bool on = [] {
     const char* env = std::getenv("MATRIXMAN_PDL");

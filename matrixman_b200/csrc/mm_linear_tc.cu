@@ -63,6 +63,7 @@ __global__ void __launch_bounds__(256) linear_split_kernel(const __grid_constant
   float sum[8] = {}, next[8], znext[8] = {};
   int inf = 0;
   pdl_wait();
+  pdl_trigger();
   const bool any = left > 0;
   auto fetch = [&](int64_t r) {
     const float* src = s.src + r * s.s0;
@@ -348,7 +349,7 @@ __device__ __forceinline__ float lin_value(const LinPlanes& p, int64_t line, int
   const int64_t plane = p.mn ? p.k * p.ld : p.lines * p.ld;
   float v = 0.f;
 #pragma unroll
-  for (int q = 2; q >= 0; --q) v += __uint_as_float((uint32_t)p.planes[q * plane + at] << 16);
+  for (int q = 2; q >= 0; --q) v += __uint_as_float((uint32_t)__ldcg(&p.planes[q * plane + at]) << 16);
   return v;
 }
 
@@ -362,7 +363,7 @@ __device__ __forceinline__ bool lin_flagged(const LinPlanes& p, int l0, int l1) 
   int any = 0;
   for (int i = threadIdx.x; i < (b1 - b0) * across; i += blockDim.x) {
     const int block = b0 + i / across, at = i % across;
-    any |= p.flags[p.mn ? at * blocks_c + block : block * blocks_c + at];
+    any |= __ldcg(&p.flags[p.mn ? at * blocks_c + block : block * blocks_c + at]);
   }
   return __syncthreads_or(any) != 0;
 }
@@ -552,7 +553,8 @@ __global__ void __launch_bounds__(LG_THREADS, 1) linear_gemm_kernel(const __grid
   lg_sync<PAIR>();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = *slot;
-  pdl_wait();
+  if (!a.early) pdl_wait();
+  pdl_trigger();
 
   // The loading and the issuing warps work with one thread each.
   if (warp == LG_WARP_TMA) {
@@ -642,8 +644,8 @@ __global__ void __launch_bounds__(LG_THREADS, 1) linear_gemm_kernel(const __grid
     uint32_t par = 0;
     bool alive = true;
     int inf = 0;  // read while the first stages are on their way
-    for (int i = threadIdx.x; i < a.flags_a; i += LG_EPI_WARPS * 32) inf |= a.pa.flags[i];
-    for (int i = threadIdx.x; i < a.flags_b; i += LG_EPI_WARPS * 32) inf |= a.pb.flags[i];
+    for (int i = threadIdx.x; i < a.flags_a; i += LG_EPI_WARPS * 32) inf |= __ldcg(&a.pa.flags[i]);
+    for (int i = threadIdx.x; i < a.flags_b; i += LG_EPI_WARPS * 32) inf |= __ldcg(&a.pb.flags[i]);
     if (inf) *special = 1;
     for (int u = worker; u < a.units && alive; u += workers) {
       const LgUnit w = lg_unit(a, u, BN);
@@ -723,6 +725,7 @@ __global__ void __launch_bounds__(LG_THREADS, 1) linear_gemm_kernel(const __grid
       if (w.part < 0) lin_fix(a, w.m0 + row_in_tile, LG_BM, w.n0, BN);
     }
   }
+  if (a.early) pdl_wait();
 }
 
 // Tiles whose reduction was divided: the partial tiles are added in order and
@@ -730,7 +733,8 @@ __global__ void __launch_bounds__(LG_THREADS, 1) linear_gemm_kernel(const __grid
 // tile.
 template <int BN>
 __global__ void __launch_bounds__(2 * BN) linear_join_kernel(const LinGemm a) {
-  pdl_wait();
+  if (!a.early) pdl_wait();
+  pdl_trigger();
   const int tile = blockIdx.x / (a.bm / 8), r0 = blockIdx.x % (a.bm / 8) * 8;
   const LgUnit w = lg_unit(a, a.full + tile * a.splits, BN);
   const int r = r0 + threadIdx.x / (BN / 4), c = threadIdx.x % (BN / 4) * 4;
@@ -738,12 +742,13 @@ __global__ void __launch_bounds__(2 * BN) linear_join_kernel(const LinGemm a) {
   float v[4] = {};
 #pragma unroll 4
   for (int s = 0; s < a.splits; ++s) {
-    const float4 t = *reinterpret_cast<const float4*>(part + (int64_t)s * a.bm * BN);
+    const float4 t = __ldcg(reinterpret_cast<const float4*>(part + (int64_t)s * a.bm * BN));
     v[0] += t.x; v[1] += t.y; v[2] += t.z; v[3] += t.w;
   }
   if (w.m0 + r < a.m && w.n0 + c < a.n) lin_finish_row<4>(a.e, v, a.c, w.m0 + r, w.n0 + c, a.n, a.vec);
   __syncthreads();
   lin_fix(a, w.m0 + r0, 8, w.n0, BN);
+  if (a.early) pdl_wait();
 }
 
 // ---------------------------------------------------------------------------
@@ -885,8 +890,8 @@ static int lin_launch_kind(bool amn, bool bmn, const CUtensorMap& ma, const CUte
 }
 
 int lin_run_gemm(const LinPlanes& pa, const LinPlanes& pb, float* c, const LinEpilogue& e, const LinChoice& ch,
-                 float* part, cudaStream_t s) {
-  LinGemm g;
+                 float* part, bool early, LinGemm* out, cudaStream_t s) {
+  LinGemm& g = *out;
   g.m = (int)pa.lines;
   g.n = (int)pb.lines;
   g.bm = ch.bm;
@@ -906,20 +911,24 @@ int lin_run_gemm(const LinPlanes& pa, const LinPlanes& pb, float* c, const LinEp
   g.pb = pb;
   g.flags_a = lin_flag_count(pa);
   g.flags_b = lin_flag_count(pb);
+  g.early = early;
   CUtensorMap ma, mb;
   int rc = lin_map(pa, LG_BM, &ma);
   if (rc == MM_OK) rc = lin_map(pb, ch.bm == 256 ? ch.bn / 2 : ch.bn, &mb);
   if (rc != MM_OK) return rc;
-  rc = ch.bm == 256   ? lin_launch_kind<128, true>(pa.mn, pb.mn, ma, mb, g, s)
-       : ch.bn == 128 ? lin_launch_kind<128, false>(pa.mn, pb.mn, ma, mb, g, s)
-                      : lin_launch_kind<64, false>(pa.mn, pb.mn, ma, mb, g, s);
-  if (rc != MM_OK) return rc;
-  if (ch.splits > 1) {
-    const unsigned grid = (unsigned)((ch.units - ch.full) / ch.splits * (ch.bm / 8));
-    MM_CUDA(ch.bn == 128 ? launch_pdl(linear_join_kernel<128>, dim3(grid), dim3(256), 0, s, g)
-                         : launch_pdl(linear_join_kernel<64>, dim3(grid), dim3(128), 0, s, g),
-            "mm_linear join launch");
-  }
+  return ch.bm == 256   ? lin_launch_kind<128, true>(pa.mn, pb.mn, ma, mb, g, s)
+         : ch.bn == 128 ? lin_launch_kind<128, false>(pa.mn, pb.mn, ma, mb, g, s)
+                        : lin_launch_kind<64, false>(pa.mn, pb.mn, ma, mb, g, s);
+}
+
+int lin_run_join(const LinGemm& gemm, const LinChoice& ch, bool early, cudaStream_t s) {
+  if (ch.splits == 1) return MM_OK;
+  LinGemm g = gemm;
+  g.early = early;
+  const unsigned grid = (unsigned)((ch.units - ch.full) / ch.splits * (ch.bm / 8));
+  MM_CUDA(ch.bn == 128 ? launch_pdl(linear_join_kernel<128>, dim3(grid), dim3(256), 0, s, g)
+                       : launch_pdl(linear_join_kernel<64>, dim3(grid), dim3(128), 0, s, g),
+          "mm_linear join launch");
   return MM_OK;
 }
 

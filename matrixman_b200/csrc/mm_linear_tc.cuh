@@ -56,6 +56,7 @@ struct LinGemm {
   LinEpilogue e;
   LinPlanes pa, pb;
   int flags_a, flags_b;  // their numbers of flags
+  int early;             // see lin_backward_tc
 };
 
 int64_t lin_flag_words(int64_t rows, int64_t cols);
@@ -65,9 +66,11 @@ void lin_add_split(LinSplits* all, const LinSplit& s);
 int lin_run_splits(const LinSplits& all, cudaStream_t s);
 LinChoice lin_choose(int64_t m, int64_t n, int64_t k);
 int64_t lin_part_bytes(const LinChoice& c);
-// C[m, n] = A B^T through the epilogue.
+// C[m, n] = A B^T through the epilogue, up to the divided tiles' sums; the latter
+// (if any; g from lin_run_gemm).
 int lin_run_gemm(const LinPlanes& a, const LinPlanes& b, float* c, const LinEpilogue& e, const LinChoice& ch,
-                 float* part, cudaStream_t s);
+                 float* part, bool early, LinGemm* g, cudaStream_t s);
+int lin_run_join(const LinGemm& g, const LinChoice& ch, bool early, cudaStream_t s);
 int lin_kernel_error(int* code, int clear);
 
 }  // namespace mm
