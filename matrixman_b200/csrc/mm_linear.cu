@@ -242,36 +242,44 @@ static cudaError_t lin_small(const LinProduct& p, const LinEpilogue& e, int64_t 
 
 // ---------------------------------------------------------------------------
 // A few rows (tokens) times a weight with dense rows: bound by reading the
-// weight once.  A group of KW warps computes CN columns for MT rows, each warp
-// every KW-th piece of the reduction, 32 lanes x VEC values at a time.
+// weight once.  A group of KW warps computes up to CN columns for MT rows, each
+// warp every KW-th piece of the reduction, 32 lanes x VEC values at a time.  BLOCKS
+// per SM and UNROLL keep some 64 to 128 KB of the weight on their way per SM; more
+// registers for more loads per warp cost blocks, and one more wave costs more (us,
+// weight from HBM, 4096 x 4096: 1 row 13.9, floor 10.3; 2 rows 14.2; 4 rows 15.4; 8
+// rows 19.9; 16 rows, the weight once more from L2, 31.3.  Four columns always and
+// no rule for even waves: 14.9, 16.6, 20.2, 31.8, 47.8).
 // ---------------------------------------------------------------------------
 
-template <int MT, int CN, int VEC>
-__global__ void __launch_bounds__(256) linear_tokens_kernel(LinProduct p, LinEpilogue e, int kw) {
+template <int MT, int CN, int BLOCKS, int UNROLL, int VEC>
+__global__ void __launch_bounds__(256, BLOCKS) linear_tokens_kernel(LinProduct p, LinEpilogue e, int kw, int cols) {
   __shared__ float red[8][MT * CN];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int part = warp % kw;
-  const int n0 = (int)(blockIdx.x * (8 / kw) + warp / kw) * CN;
+  const int n0 = (int)(blockIdx.x * (8 / kw) + warp / kw) * cols, count = min(cols, p.n - n0);
   const int m0 = blockIdx.y * MT;
   float acc[MT][CN] = {};
   pdl_wait();
-  const float* wp[CN];
-#pragma unroll
-  for (int j = 0; j < CN; ++j) wp[j] = p.b + (int64_t)min(n0 + j, p.n - 1) * p.bs0;
+  const float* wp = p.b + (int64_t)n0 * p.bs0;
   const float* xp[MT];
 #pragma unroll
   for (int i = 0; i < MT; ++i) xp[i] = p.a + (int64_t)min(m0 + i, p.m - 1) * p.as0;
   const int step = 32 * VEC * kw;
-#pragma unroll 4
+#pragma unroll UNROLL
   for (int k = (part * 32 + lane) * VEC; k < p.k; k += step) {
-    float w[CN][VEC], x[MT][VEC];
+    float w[CN][VEC] = {}, x[MT][VEC];
+    const float* at = wp + k;
 #pragma unroll
-    for (int j = 0; j < CN; ++j) {
+    for (int j = 0; j < CN; ++j, at += p.bs0) {
+      if (j >= count) {
+        if (MT == 1) break;
+        continue;
+      }
       if (VEC == 4) {
-        const float4 t = __ldcs(reinterpret_cast<const float4*>(wp[j] + k));
+        const float4 t = __ldcs(reinterpret_cast<const float4*>(at));
         w[j][0] = t.x; w[j][VEC > 1 ? 1 : 0] = t.y; w[j][VEC > 2 ? 2 : 0] = t.z; w[j][VEC > 3 ? 3 : 0] = t.w;
       } else {
-        w[j][0] = __ldcs(wp[j] + k);
+        w[j][0] = __ldcs(at);
       }
     }
 #pragma unroll
@@ -302,8 +310,8 @@ __global__ void __launch_bounds__(256) linear_tokens_kernel(LinProduct p, LinEpi
   // One thread per output of the block: (8 / kw) groups x MT x CN.
   for (int t = threadIdx.x; t < 8 / kw * MT * CN; t += 256) {
     const int g = t / (MT * CN), o = t % (MT * CN);
-    const int row = m0 + o / CN, col = (int)(blockIdx.x * (8 / kw) + g) * CN + o % CN;
-    if (row >= p.m || col >= p.n) continue;
+    const int row = m0 + o / CN, col = (int)(blockIdx.x * (8 / kw) + g) * cols + o % CN;
+    if (row >= p.m || col >= p.n || o % CN >= cols) continue;
     float v = 0.f;
     for (int q = 0; q < kw; ++q) v += red[g * kw + q][o];
     p.c[(int64_t)row * p.n + col] = lin_finish(e, v, row, col, p.n);
@@ -340,19 +348,32 @@ constexpr int LIN_TOKENS = 16;  // rows up to which a product is a walk over the
 
 static bool lin_aligned(const float* p, int64_t stride) { return (uintptr_t)p % 16 == 0 && stride % 4 == 0; }
 
-template <int MT, int CN>
+template <int MT, int CN, int BLOCKS, int UNROLL>
 static void lin_tokens(const LinProduct& p, const LinEpilogue& e, cudaStream_t s) {
-  // Warps per column group: as many as keep the GPU's warp slots busy, with at
-  // least one 16-byte piece per lane.
-  const int64_t groups = (int64_t)((p.n + CN - 1) / CN) * ((p.m + MT - 1) / MT);
-  int kw = 1;
-  while (kw < 8 && groups * kw * 2 <= (int64_t)sm_count() * (MT == 1 ? 64 : 32) && p.k >= kw * 2 * 128) kw *= 2;
-  const int per = 8 / kw * CN;
+  // Warps per column group and columns per group: waves of blocks times a
+  // block's steps (a piece of each column and, from L1, of each row of A) and its
+  // start and end (about four steps).
+  const bool wide = lin_aligned(p.a, p.m > 1 ? p.as0 : 0) && lin_aligned(p.b, p.n > 1 ? p.bs0 : 0) && p.k % 4 == 0;
+  const int64_t rows = (p.m + MT - 1) / MT, slots = (int64_t)sm_count() * BLOCKS, piece = wide ? 128 : 32;
+  int kw = 1, cols = 1;
+  double best = 0;
+  for (int w = 1; w <= 8 && (w == 1 || p.k > (w / 2) * piece); w *= 2)
+    for (int c = 1; c <= CN; ++c) {
+      const int64_t blocks = (p.n + 8 / w * c - 1) / (8 / w * c) * rows;
+      const double t = (double)((blocks + slots - 1) / slots) *
+                       ((double)((p.k + w * piece - 1) / (w * piece)) * (c + 0.25 * MT) + 4);
+      if (best == 0 || t < best) {
+        best = t;
+        kw = w;
+        cols = c;
+      }
+    }
+  const int per = 8 / kw * cols;
   const dim3 grid((unsigned)((p.n + per - 1) / per), (unsigned)((p.m + MT - 1) / MT));
-  if (lin_aligned(p.a, p.m > 1 ? p.as0 : 0) && lin_aligned(p.b, p.n > 1 ? p.bs0 : 0) && p.k % 4 == 0)
-    launch_pdl(linear_tokens_kernel<MT, CN, 4>, grid, dim3(256), 0, s, p, e, kw);
+  if (wide)
+    launch_pdl(linear_tokens_kernel<MT, CN, BLOCKS, UNROLL, 4>, grid, dim3(256), 0, s, p, e, kw, cols);
   else
-    launch_pdl(linear_tokens_kernel<MT, CN, 1>, grid, dim3(256), 0, s, p, e, kw);
+    launch_pdl(linear_tokens_kernel<MT, CN, BLOCKS, UNROLL, 1>, grid, dim3(256), 0, s, p, e, kw, cols);
 }
 
 static int ls_mode(const float* p, int64_t s0, int64_t s1) {
@@ -380,13 +401,13 @@ static int lin_product(const LinProduct& p, const LinEpilogue& e, cudaStream_t s
   if (p.m == 0 || p.n == 0) return MM_OK;
   if (p.m <= LIN_TOKENS && p.as1 == 1 && p.bs1 == 1 && p.k > 0) {
     if (p.m == 1)
-      lin_tokens<1, 4>(p, e, s);
+      lin_tokens<1, 8, 4, 1>(p, e, s);
     else if (p.m == 2)
-      lin_tokens<2, 2>(p, e, s);
+      lin_tokens<2, 4, 4, 1>(p, e, s);
     else if (p.m <= 4)
-      lin_tokens<4, 4>(p, e, s);
+      lin_tokens<4, 8, 2, 1>(p, e, s);
     else
-      lin_tokens<8, 4>(p, e, s);
+      lin_tokens<8, 4, 2, 2>(p, e, s);
   } else {
     LsModes md;
     const int64_t tiles = ls_modes(p, &md);

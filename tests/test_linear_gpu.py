@@ -115,7 +115,8 @@ def check(mm, x, w, b, r, act, first=False, grad=True):
     (1, 1, 1), (1, 5, 3), (1, 512, 784), (1, 257, 1030), (2, 64, 64), (3, 10, 256), (7, 100, 33), (16, 130, 129),
     (17, 33, 700), (31, 65, 4096), (33, 127, 128), (64, 64, 65), (100, 300, 200), (128, 256, 512), (129, 257, 31),
     (256, 512, 784), (255, 1000, 1281), (700, 129, 40), (513, 384, 96), (2000, 40, 8),
-    (5000, 7, 300), (4000, 300, 7), (9001, 10, 16), (300, 1, 600), (600, 300, 1)])
+    (5000, 7, 300), (4000, 300, 7), (9001, 10, 16), (300, 1, 600), (600, 300, 1),
+    (1, 4097, 1030), (1, 40001, 64), (2, 3001, 400), (3, 2501, 260), (4, 9000, 132), (12, 1301, 700), (16, 4099, 36)])
 def test_sizes(mm, m, n, k):
     check(mm, randn(m, k, seed=1), randn(n, k, seed=2), randn(n, seed=3), None, "none")
 
@@ -269,7 +270,7 @@ def test_empty_sizes(mm):
         assert torch.equal(grads[2].cpu(), torch.full((n,), float(m)))
 
 
-@pytest.mark.parametrize("m,n,k", [(3, 200, 300), (300, 500, 260)])
+@pytest.mark.parametrize("m,n,k", [(3, 200, 300), (300, 500, 260), (511, 1300, 2049)])
 def test_same_bits_twice_and_in_replayed_graphs(mm, m, n, k):
     x, w, b, dy = randn(m, k, seed=1), randn(n, k, seed=2), randn(n, seed=3), randn(m, n, seed=4)
     args = [mm.to_device(t) for t in (x, w, b)]
