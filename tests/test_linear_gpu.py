@@ -12,10 +12,13 @@ argument's rounding).  That worst case grows with k; the norm of the whole
 error grows with sqrt(k), as k roundings of either sign add up, and is held to
 (sqrt(k) + 32) u of the norm of the products' magnitudes."""
 
+import ctypes
 import math
 
 import pytest
 import torch
+
+from matrixman_b200 import _lib, ops
 
 pytestmark = pytest.mark.gpu
 
@@ -302,6 +305,42 @@ def test_same_bits_twice_and_in_replayed_graphs(mm, m, n, k):
     ga.replay()  # the two graphs' workspaces are their own
     assert all(torch.equal(p.cpu(), q) for p, q in zip(outa, one))
     assert all(torch.equal(p.cpu(), q) for p, q in zip(outb, two))
+
+
+def test_two_streams_at_once(mm):
+    """Calls on two streams, each of several kernels that overlap, give the bits of calls one at a time."""
+    lib = _lib.load()
+    sizes = [(511, 1300, 2049), (700, 640, 900)]
+    calls = []
+    for i, (m, n, k) in enumerate(sizes):
+        x, w, dy = (mm.to_device(randn(*s, seed=10 * i + j)) for j, s in enumerate(((m, k), (n, k), (m, n))))
+        rt = x.runtime
+        calls.append(((m, n, k), x, w, dy, [ops.empty(rt, s) for s in ((m, n), (m, k), (n, k), (n,))]))
+
+    def queue(call, stream):
+        (m, n, k), x, w, dy, (y, dx, dw, db) = call
+        at = [t.element_ptr for t in (x, w, dy, y, dx, dw, db)]
+        assert lib.mm_linear(at[0], k, 1, at[1], k, 1, None, None, 0, m, n, k, 0, 0, at[3], None, None, 0, stream) == 0
+        assert lib.mm_linear_backward(at[2], n, at[0], k, 1, at[1], k, 1, None, m, n, k, 0, at[4], at[5], at[6], None,
+                                      None, 0, stream) == 0
+
+    alone = []
+    for call in calls:
+        queue(call, rt.stream)
+        alone.append([t.cpu() for t in call[4]])
+    streams = [ctypes.c_void_p(), ctypes.c_void_p()]
+    for s in streams:
+        _lib.check(lib.mm_stream_create(rt.index, ctypes.byref(s)), "stream")
+    rt.synchronize()
+    for _ in range(5):
+        for call, s in zip(calls, streams):
+            queue(call, s)
+    for s in streams:
+        _lib.check(lib.mm_stream_sync(s, 20000), "stream wait")
+    for call, want in zip(calls, alone):
+        assert all(torch.equal(t.cpu(), v) for t, v in zip(call[4], want))
+    for s in streams:
+        _lib.check(lib.mm_stream_destroy(s), "stream")
 
 
 def test_refusals(mm):
