@@ -182,10 +182,11 @@ __device__ __forceinline__ uint32_t lg_lead(uint64_t* bar) {
   return addr;
 }
 
-// (Tensor memory's reads are over by then, and no other memory has to be seen:
-// a release to the cluster would take 1,000 to 2,000 clocks.)
+// (It says that tensor memory has been read; no other memory has to be seen by
+// the other CTA.  A release to the cluster waits for the stores under way, 1,000
+// to 2,000 clocks.)
 __device__ __forceinline__ void lg_arrive_at(uint32_t bar) {
-  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+  asm volatile("mbarrier.arrive.release.cta.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
 // All threads of the CTA, of both in a pair.
