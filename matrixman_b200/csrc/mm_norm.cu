@@ -318,11 +318,14 @@ __global__ void __launch_bounds__(256) ln_columns_kernel(LnArgs a) {
   a.part[((int64_t)gridDim.y + blockIdx.y) * a.width + c] = db;
 }
 
-// dw (blockIdx.y 0) or db (1) of 32 columns: eight threads per column add the
-// partial rows k, k + 8, ..., then their sums are added in order.
-__global__ void __launch_bounds__(256) ln_finish_kernel(const float* __restrict__ part, int blocks, int width,
-                                                        float* dw, float* db) {
-  __shared__ float acc[8][33];
+// dw (blockIdx.y 0) or db (1) of 32 columns: 32 threads per column add the
+// partial rows k, k + 32, ..., then their sums are added in order (latency: with
+// eight threads per column and a plain launch the backward pass took 4 to 6 us
+// more, 143 in place of 138 at 16384 x 4096, 29 in place of 23 at 5003 x 1250).
+__global__ void __launch_bounds__(1024) ln_finish_kernel(const float* part, int blocks, int width, float* dw,
+                                                         float* db) {
+  __shared__ float acc[32][33];
+  pdl_wait();
   float* out = blockIdx.y ? db : dw;
   if (!out) return;
   const int lane = threadIdx.x & 31, k = threadIdx.x >> 5;
@@ -330,12 +333,13 @@ __global__ void __launch_bounds__(256) ln_finish_kernel(const float* __restrict_
   part += (int64_t)blockIdx.y * blocks * width;
   float s = 0.f;
   if (c < width)
-    for (int r = k; r < blocks; r += 8) s += part[(int64_t)r * width + c];
+#pragma unroll 4
+    for (int r = k; r < blocks; r += 32) s += part[(int64_t)r * width + c];
   acc[k][lane] = s;
   __syncthreads();
   if (k == 0 && c < width) {
 #pragma unroll
-    for (int j = 1; j < 8; ++j) s += acc[j][lane];
+    for (int j = 1; j < 32; ++j) s += acc[j][lane];
     out[c] = s;
   }
 }
@@ -529,8 +533,9 @@ extern "C" int mm_layer_norm_backward(const float* dy, int64_t dy_stride, const 
   }
   MM_LAUNCH_CHECK("mm_layer_norm_backward launch");
   if (cols) {
-    ln_finish_kernel<<<dim3((a.width + 31) / 32, 2), 256, 0, s>>>(a.part, blocks, a.width, dweight, dbias);
-    MM_LAUNCH_CHECK("mm_layer_norm_backward columns launch");
+    MM_CUDA(launch_pdl(ln_finish_kernel, dim3((a.width + 31) / 32, 2), dim3(1024), 0, s, (const float*)a.part,
+                       (int)blocks, (int)a.width, dweight, dbias),
+            "mm_layer_norm_backward columns launch");
   }
   return MM_OK;
 }
