@@ -588,9 +588,12 @@ __global__ void __launch_bounds__(LG_THREADS, 1) linear_gemm_kernel(const __grid
       }
       // Nothing may land in shared memory after the CTA has gone: wait for the
       // last fill of every stage (over already unless a wait gave up), in a
-      // pair's CTA 1 for the MMAs that have read it.
+      // pair's CTA 1 for the MMAs that have read it, and there for the last
+      // arrivals of CTA 0's issuers (CTA 0 waits for its own below).
       for (int i = max(0, filled - S); i < filled; ++i)
         lg_wait(rank == 0 ? &full[i % S] : &empty[i % S], (uint32_t)(i / S) & 1u, LG_ERR_DRAIN);
+      if (rank == 1)
+        for (int i = 0; i < LG_ISSUERS; ++i) lg_wait(&drain[i], 0u, LG_ERR_DRAIN);
     }
     __syncwarp();
   } else if (warp >= LG_WARP_MMA) {
@@ -712,7 +715,7 @@ __global__ void __launch_bounds__(LG_THREADS, 1) linear_gemm_kernel(const __grid
     }
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-  lg_sync<PAIR>();  // in a pair: nothing of the other CTA is on its way to this one
+  lg_sync<PAIR>();  // in a pair: both CTAs have waited for all that arrives in their shared memory
   if (warp == LG_WARP_MMA) {
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     if (PAIR)

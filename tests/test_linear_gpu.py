@@ -370,3 +370,29 @@ def test_cpu_weights(mm):
     x, w, b = randn(5, 40, seed=1), randn(30, 40, seed=2), randn(30, seed=3)
     got = mm.linear(mm.to_device(x), w, b).cpu()
     assert torch.equal(got, mm.linear(mm.to_device(x), mm.to_device(w), mm.to_device(b)).cpu())
+
+
+def test_short_pair_products_one_behind_the_other(mm):
+    """Hundreds of short products of CTA pairs, each starting on the SMs that the one before leaves: a CTA that
+    left while an arrival was on its way to it would disturb the barriers of the next one there."""
+    lib = _lib.load()
+    m, n, k = 2500, 1100, 70
+    x, w, dy = mm.to_device(randn(m, k, seed=1)), mm.to_device(randn(n, k, seed=2)), mm.to_device(randn(m, n, seed=3))
+    rt = x.runtime
+    dx, dw = ops.empty(rt, (m, k)), ops.empty(rt, (n, k))
+    y = ops.empty(rt, (m, n))
+
+    def queue():
+        assert lib.mm_linear(x.element_ptr, k, 1, w.element_ptr, k, 1, None, None, 0, m, n, k, 0, 0, y.element_ptr, None,
+                             None, 0, rt.stream) == 0
+        assert lib.mm_linear_backward(dy.element_ptr, n, x.element_ptr, k, 1, w.element_ptr, k, 1, None, m, n, k, 0,
+                                      dx.element_ptr, dw.element_ptr, None, None, None, 0, rt.stream) == 0
+
+    queue()
+    want = [t.cpu() for t in (y, dx, dw)]
+    for _ in range(300):
+        queue()
+    assert all(torch.equal(t.cpu(), v) for t, v in zip((y, dx, dw), want))
+    code = ctypes.c_int(-1)
+    _lib.check(lib.mm_kernel_error(rt.index, ctypes.byref(code), 0))
+    assert code.value == 0
