@@ -140,27 +140,39 @@ __device__ __forceinline__ void lg_bar_init(uint64_t* bar, uint32_t count) {
   asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(lg_smem(bar)), "r"(count));
 }
 
+// CLUSTER: threads of both CTAs arrive.
+template <bool CLUSTER>
 __device__ __forceinline__ bool lg_try(uint64_t* bar, uint32_t parity) {
   uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok)
-      : "r"(lg_smem(bar)), "r"(parity), "r"(1000u)
-      : "memory");
+  if (CLUSTER)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(lg_smem(bar)), "r"(parity), "r"(1000u)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(lg_smem(bar)), "r"(parity), "r"(1000u)
+        : "memory");
   return ok != 0;
 }
 
 // Bounded wait.  It gives up after 200 ms, or soon after another wait did, and
 // records which one; a drain (wait for this CTA's own copies and MMAs) ignores
 // the others' errors.
+template <bool CLUSTER = false>
 __device__ __forceinline__ bool lg_wait(uint64_t* bar, uint32_t parity, int code) {
-  if (lg_try(bar, parity)) return true;
+  if (lg_try<CLUSTER>(bar, parity)) return true;
   uint64_t t0, t;
   asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t0));
   for (uint32_t i = 1; i < (1u << 26); ++i) {
-    if (lg_try(bar, parity)) return true;
+    if (lg_try<CLUSTER>(bar, parity)) return true;
     if ((i & 63) == 0) {
       if (code != LG_ERR_DRAIN && *reinterpret_cast<volatile int*>(&g_lin_error) != 0) return false;
       asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
@@ -182,11 +194,15 @@ __device__ __forceinline__ uint32_t lg_lead(uint64_t* bar) {
   return addr;
 }
 
-// (It says that tensor memory has been read; no other memory has to be seen by
-// the other CTA.  A release to the cluster waits for the stores under way, 1,000
-// to 2,000 clocks.)
+// To a barrier of the pair's CTA 0 from either CTA, so with the cluster's scope.  It
+// says that tensor memory has been read: tcgen05.wait::ld has ended and
+// tcgen05.fence::before_thread_sync stands before it, which order the reads
+// before it, and the fence behind the wait of CTA 0's issuer orders its MMAs
+// after it, whatever the arrival's semantics; no other memory has to be seen by
+// the other CTA, so it is relaxed (a release to the cluster waits for the stores
+// under way, 1,000 to 2,000 clocks).
 __device__ __forceinline__ void lg_arrive_at(uint32_t bar) {
-  asm volatile("mbarrier.arrive.release.cta.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
 // All threads of the CTA, of both in a pair.
@@ -566,7 +582,7 @@ __global__ void __launch_bounds__(LG_THREADS, 1) linear_gemm_kernel(const __grid
       for (int u = worker; u < a.units && alive; u += workers) {
         const LgUnit w = lg_unit(a, u, BN);
         for (int k = w.begin; k < w.end; ++k) {
-          if (!lg_wait(&empty[st], par, LG_ERR_EMPTY)) {
+          if (!lg_wait<PAIR>(&empty[st], par, LG_ERR_EMPTY)) {
             alive = false;
             break;
           }
@@ -591,9 +607,9 @@ __global__ void __launch_bounds__(LG_THREADS, 1) linear_gemm_kernel(const __grid
       // pair's CTA 1 for the MMAs that have read it, and there for the last
       // arrivals of CTA 0's issuers (CTA 0 waits for its own below).
       for (int i = max(0, filled - S); i < filled; ++i)
-        lg_wait(rank == 0 ? &full[i % S] : &empty[i % S], (uint32_t)(i / S) & 1u, LG_ERR_DRAIN);
+        lg_wait<PAIR>(rank == 0 ? &full[i % S] : &empty[i % S], (uint32_t)(i / S) & 1u, LG_ERR_DRAIN);
       if (rank == 1)
-        for (int i = 0; i < LG_ISSUERS; ++i) lg_wait(&drain[i], 0u, LG_ERR_DRAIN);
+        for (int i = 0; i < LG_ISSUERS; ++i) lg_wait<PAIR>(&drain[i], 0u, LG_ERR_DRAIN);
     }
     __syncwarp();
   } else if (warp >= LG_WARP_MMA) {
@@ -609,7 +625,7 @@ __global__ void __launch_bounds__(LG_THREADS, 1) linear_gemm_kernel(const __grid
         const LgUnit w = lg_unit(a, u, BN);
         for (int k = w.begin; k < w.end; ++k) {
           if (buf % LG_ISSUERS == issuer) {
-            if (!lg_wait(&acc_free[buf], bpar, LG_ERR_FREE) || !lg_wait(&full[st], par, LG_ERR_FULL)) {
+            if (!lg_wait<PAIR>(&acc_free[buf], bpar, LG_ERR_FREE) || !lg_wait<PAIR>(&full[st], par, LG_ERR_FULL)) {
               alive = false;
               break;
             }
@@ -657,7 +673,7 @@ __global__ void __launch_bounds__(LG_THREADS, 1) linear_gemm_kernel(const __grid
 #pragma unroll
       for (int i = 0; i < HALF; ++i) acc[i] = 0.f;
       for (int k = w.begin; k < w.end; ++k) {
-        if (!__all_sync(0xffffffffu, lg_wait(&acc_full[buf], par, LG_ERR_ACC))) {
+        if (!__all_sync(0xffffffffu, lg_wait<PAIR>(&acc_full[buf], par, LG_ERR_ACC))) {
           alive = false;
           break;
         }
