@@ -521,7 +521,14 @@ int mm_conv2d_tc_region(const mm_tensor_t* x, const float* w_hi, const float* w_
  * frees its tensor memory and returns, and the host reads the code here. */
 int mm_kernel_error(int device, int* code_out, int clear);
 
-/* Test hook for the bounded-wait error path of mm_conv2d_tc (no counterpart in
+/* A word of host memory that a kernel of mm_linear or mm_linear_backward sets to
+ * its code (101 to 105) when it gives up a bounded wait, after which outputs of
+ * that call are incomplete.  Readable without a call once the stream has been
+ * waited for; mm_kernel_error reports it too, and clears it. */
+int mm_fault_word(int device, int** word_out);
+
+/* Test hook for the bounded-wait error path of mm_conv2d_tc, and of mm_linear and
+ * mm_linear_backward where they run on the tensor cores (no counterpart in
  * the reference): for later launches on `device`, the budget of every
  * device-side wait (wait_ns <= 0 restores the default 200 ms) and, when
  * drop_first_load != 0, CTA 0 leaves its first k-block's loads unissued so that

@@ -33,6 +33,10 @@ int cuda_fail(cudaError_t err, const char* action);
 
 cudaStream_t resolve_stream(void* stream);
 
+// The device's fault word (mm_fault_word): page-locked host memory that kernels
+// may write, made by mm_init and never freed; null before that.
+int* fault_word(int device);
+
 // ---------------------------------------------------------------------------
 // Programmatic dependent launch (PDL).  A kernel launched with launch_pdl may
 // be scheduled while the previous kernel in the stream drains; it must call

@@ -64,7 +64,7 @@
 namespace mm {
 
 __device__ int g_tc_error = 0;
-int lin_kernel_error(int* code, int clear);  // the same of the linear operator's kernel
+void lin_debug_fault(int device, int64_t wait_ns, int drop);  // mm_debug_tc_fault of the linear operator's kernel
 
 constexpr int TC_BM = 128;        // pixels per tile (MMA M)
 constexpr int TC_BK = 32;         // channels per k-block (128 bytes of fp32)
@@ -1761,9 +1761,9 @@ extern "C" int mm_conv2d_tc_region(const mm_tensor_t* x, const float* w_hi, cons
 }
 
 // Test hook for the bounded-wait error path (no counterpart in the
-// reference): sets the budget of the kernel's waits on `device` (wait_ns <= 0:
-// the default 200 ms) and whether CTA 0 leaves its first k-block unissued, for
-// every later launch on that device.
+// reference): sets the budget of the waits of this kernel and of the linear
+// operator's on `device` (wait_ns <= 0: the default 200 ms) and whether CTA 0
+// leaves its first k-block unissued, for every later launch on that device.
 extern "C" int mm_debug_tc_fault(int device, int64_t wait_ns, int drop_first_load) {
   int prev = 0;
   cudaGetDevice(&prev);
@@ -1774,6 +1774,7 @@ extern "C" int mm_debug_tc_fault(int device, int64_t wait_ns, int drop_first_loa
   if (e == cudaSuccess) e = cudaMemcpyToSymbol(g_tc_drop_first_load, &drop, sizeof(drop));
   if (prev != device) cudaSetDevice(prev);
   if (e != cudaSuccess) return cuda_fail(e, "mm_debug_tc_fault");
+  lin_debug_fault(device, wait_ns, drop);
   return MM_OK;
 }
 
@@ -1788,12 +1789,12 @@ extern "C" int mm_kernel_error(int device, int* code_out, int clear) {
     int zero = 0;
     e = cudaMemcpyToSymbol(g_tc_error, &zero, sizeof(int));
   }
-  int linear = 0;
-  const int rc = e == cudaSuccess ? lin_kernel_error(&linear, clear) : MM_OK;
   if (prev != device) cudaSetDevice(prev);
   if (e != cudaSuccess) return cuda_fail(e, "mm_kernel_error");
-  if (rc != MM_OK) return rc;
-  if (code == 0) code = linear;
+  if (volatile int* word = fault_word(device)) {  // the linear operator's kernel
+    if (code == 0) code = *word;
+    if (clear) *word = 0;
+  }
   *code_out = code;
   return MM_OK;
 }

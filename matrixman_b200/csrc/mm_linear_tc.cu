@@ -18,6 +18,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
 #include <string>
 
 #include "mm_linear_tc.cuh"
@@ -125,14 +126,15 @@ __global__ void __launch_bounds__(256) linear_split_kernel(const __grid_constant
 // Tensor-core product
 // ---------------------------------------------------------------------------
 
-__device__ int g_lin_error = 0;
-
 enum { LG_ERR_FULL = 101, LG_ERR_EMPTY = 102, LG_ERR_ACC = 103, LG_ERR_FREE = 104, LG_ERR_DRAIN = 105 };
 
 constexpr int LG_BM = 128, LG_BK = 32;
 constexpr int LG_ACCS = 4;  // accumulators in tensor memory (at most 512 columns)
 constexpr int LG_EPI_WARPS = 8, LG_WARP_TMA = 8, LG_WARP_MMA = 9, LG_ISSUERS = 2, LG_THREADS = 352;
-constexpr uint64_t LG_WAIT_NS = 200ull * 1000 * 1000;
+constexpr int64_t LG_WAIT_NS = 200ll * 1000 * 1000;
+// Set by mm_debug_tc_fault for a device's later launches (0: the limit above).
+static std::atomic<int64_t> g_lin_wait_ns[64];
+static std::atomic<int> g_lin_drop[64];
 
 __device__ __forceinline__ uint32_t lg_smem(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 
@@ -163,23 +165,24 @@ __device__ __forceinline__ bool lg_try(uint64_t* bar, uint32_t parity) {
   return ok != 0;
 }
 
-// Bounded wait.  It gives up after 200 ms, or soon after another wait did, and
-// records which one; a drain (wait for this CTA's own copies and MMAs) ignores
-// the others' errors.
+// Bounded wait.  It gives up after 200 ms and records which one did in the
+// device's fault word, which is host memory: the host sees it at its next wait
+// for the stream.  Nothing else reads it, so one launch's error shortens no
+// wait of another's.
 template <bool CLUSTER = false>
-__device__ __forceinline__ bool lg_wait(uint64_t* bar, uint32_t parity, int code) {
+__device__ __forceinline__ bool lg_wait(const LinGemm& a, uint64_t* bar, uint32_t parity, int code) {
   if (lg_try<CLUSTER>(bar, parity)) return true;
   uint64_t t0, t;
   asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t0));
   for (uint32_t i = 1; i < (1u << 26); ++i) {
     if (lg_try<CLUSTER>(bar, parity)) return true;
     if ((i & 63) == 0) {
-      if (code != LG_ERR_DRAIN && *reinterpret_cast<volatile int*>(&g_lin_error) != 0) return false;
       asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-      if (t - t0 > LG_WAIT_NS) break;
+      if ((int64_t)(t - t0) > a.wait_ns) break;
     }
   }
-  atomicCAS(&g_lin_error, 0, code);
+  volatile int* fault = a.fault;
+  if (fault != nullptr && *fault == 0) *fault = code;  // (of several, one of them)
   return false;
 }
 
@@ -576,15 +579,20 @@ __global__ void __launch_bounds__(LG_THREADS, 1) linear_gemm_kernel(const __grid
   // The loading and the issuing warps work with one thread each.
   if (warp == LG_WARP_TMA) {
     if (lane == 0) {
-      int st = 0, filled = 0;
+      int st = 0, filled = 0, dropped = -1;
       uint32_t par = 1;
       bool alive = true;
       for (int u = worker; u < a.units && alive; u += workers) {
         const LgUnit w = lg_unit(a, u, BN);
         for (int k = w.begin; k < w.end; ++k) {
-          if (!lg_wait<PAIR>(&empty[st], par, LG_ERR_EMPTY)) {
+          if (!lg_wait<PAIR>(a, &empty[st], par, LG_ERR_EMPTY)) {
             alive = false;
             break;
+          }
+          if (filled == 0 && a.drop && blockIdx.x == 0) {  // see mm_debug_tc_fault
+            dropped = filled++;
+            ++st;
+            continue;
           }
           // (in a pair CTA 0's barrier counts the bytes of both)
           if (rank == 0)
@@ -607,9 +615,10 @@ __global__ void __launch_bounds__(LG_THREADS, 1) linear_gemm_kernel(const __grid
       // pair's CTA 1 for the MMAs that have read it, and there for the last
       // arrivals of CTA 0's issuers (CTA 0 waits for its own below).
       for (int i = max(0, filled - S); i < filled; ++i)
-        lg_wait<PAIR>(rank == 0 ? &full[i % S] : &empty[i % S], (uint32_t)(i / S) & 1u, LG_ERR_DRAIN);
+        if (i != dropped)
+          lg_wait<PAIR>(a, rank == 0 ? &full[i % S] : &empty[i % S], (uint32_t)(i / S) & 1u, LG_ERR_DRAIN);
       if (rank == 1)
-        for (int i = 0; i < LG_ISSUERS; ++i) lg_wait<PAIR>(&drain[i], 0u, LG_ERR_DRAIN);
+        for (int i = 0; i < LG_ISSUERS; ++i) lg_wait<PAIR>(a, &drain[i], 0u, LG_ERR_DRAIN);
     }
     __syncwarp();
   } else if (warp >= LG_WARP_MMA) {
@@ -625,7 +634,7 @@ __global__ void __launch_bounds__(LG_THREADS, 1) linear_gemm_kernel(const __grid
         const LgUnit w = lg_unit(a, u, BN);
         for (int k = w.begin; k < w.end; ++k) {
           if (buf % LG_ISSUERS == issuer) {
-            if (!lg_wait<PAIR>(&acc_free[buf], bpar, LG_ERR_FREE) || !lg_wait<PAIR>(&full[st], par, LG_ERR_FULL)) {
+            if (!lg_wait<PAIR>(a, &acc_free[buf], bpar, LG_ERR_FREE) || !lg_wait<PAIR>(a, &full[st], par, LG_ERR_FULL)) {
               alive = false;
               break;
             }
@@ -653,7 +662,7 @@ __global__ void __launch_bounds__(LG_THREADS, 1) linear_gemm_kernel(const __grid
       }
       // No MMA may still write tensor memory when it is freed.
       lg_commit<PAIR>(&drain[issuer]);
-      lg_wait(&drain[issuer], 0u, LG_ERR_DRAIN);
+      lg_wait(a, &drain[issuer], 0u, LG_ERR_DRAIN);
     }
     __syncwarp();
   } else {
@@ -673,7 +682,7 @@ __global__ void __launch_bounds__(LG_THREADS, 1) linear_gemm_kernel(const __grid
 #pragma unroll
       for (int i = 0; i < HALF; ++i) acc[i] = 0.f;
       for (int k = w.begin; k < w.end; ++k) {
-        if (!__all_sync(0xffffffffu, lg_wait<PAIR>(&acc_full[buf], par, LG_ERR_ACC))) {
+        if (!__all_sync(0xffffffffu, lg_wait<PAIR>(a, &acc_full[buf], par, LG_ERR_ACC))) {
           alive = false;
           break;
         }
@@ -775,13 +784,10 @@ __global__ void __launch_bounds__(2 * BN) linear_join_kernel(const LinGemm a) {
 // Host side
 // ---------------------------------------------------------------------------
 
-int lin_kernel_error(int* code, int clear) {
-  cudaError_t e = cudaMemcpyFromSymbol(code, g_lin_error, sizeof(int));
-  if (e == cudaSuccess && clear && *code != 0) {
-    const int zero = 0;
-    e = cudaMemcpyToSymbol(g_lin_error, &zero, sizeof(int));
-  }
-  return e == cudaSuccess ? MM_OK : cuda_fail(e, "mm_kernel_error");
+void lin_debug_fault(int device, int64_t wait_ns, int drop) {
+  if (device < 0 || device >= 64) return;
+  g_lin_wait_ns[device] = wait_ns > 0 ? wait_ns : 0;
+  g_lin_drop[device] = drop;
 }
 
 int64_t lin_flag_words(int64_t rows, int64_t cols) {
@@ -932,6 +938,12 @@ int lin_run_gemm(const LinPlanes& pa, const LinPlanes& pb, float* c, const LinEp
   g.flags_a = lin_flag_count(pa);
   g.flags_b = lin_flag_count(pb);
   g.early = early;
+  int device = 0;
+  cudaGetDevice(&device);
+  g.fault = fault_word(device);
+  const int64_t limit = device >= 0 && device < 64 ? g_lin_wait_ns[device].load() : 0;
+  g.wait_ns = limit > 0 ? limit : LG_WAIT_NS;
+  g.drop = device >= 0 && device < 64 ? g_lin_drop[device].load() : 0;
   CUtensorMap ma, mb;
   int rc = lin_map(pa, LG_BM, &ma);
   if (rc == MM_OK) rc = lin_map(pb, ch.bm == 256 ? ch.bn / 2 : ch.bn, &mb);

@@ -57,6 +57,9 @@ struct LinGemm {
   LinPlanes pa, pb;
   int flags_a, flags_b;  // their numbers of flags
   int early;             // see lin_backward_tc
+  int* fault;            // the device's fault word (host memory), or null
+  int64_t wait_ns;       // limit of the kernel's waits
+  int drop;              // test hook: CTA 0 leaves its first loads out
 };
 
 int64_t lin_flag_words(int64_t rows, int64_t cols);
@@ -71,6 +74,6 @@ int64_t lin_part_bytes(const LinChoice& c);
 int lin_run_gemm(const LinPlanes& a, const LinPlanes& b, float* c, const LinEpilogue& e, const LinChoice& ch,
                  float* part, bool early, LinGemm* g, cudaStream_t s);
 int lin_run_join(const LinGemm& g, const LinChoice& ch, bool early, cudaStream_t s);
-int lin_kernel_error(int* code, int clear);
+void lin_debug_fault(int device, int64_t wait_ns, int drop);
 
 }  // namespace mm

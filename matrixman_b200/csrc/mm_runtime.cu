@@ -131,6 +131,10 @@ static DeviceRuntime* runtime_for(int device) {
   return g_rt[device];
 }
 
+static int* g_fault[64] = {nullptr};  // written under g_rt_mu, once per device
+
+int* fault_word(int device) { return device >= 0 && device < 64 ? g_fault[device] : nullptr; }
+
 static int current_device() {
   int d = 0;
   cudaGetDevice(&d);
@@ -283,6 +287,12 @@ extern "C" int mm_init(int device) {
   if (prop.major != 10)
     return fail(MM_ERR_UNSUPPORTED, std::string("mm_init: ") + prop.name +
                                         " is not an sm_100 (B200) device; this build targets sm_100a only");
+  if (g_fault[device] == nullptr) {
+    void* word = nullptr;
+    MM_CUDA(cudaHostAlloc(&word, sizeof(int), cudaHostAllocPortable | cudaHostAllocMapped), "fault word");
+    *(int*)word = 0;
+    g_fault[device] = (int*)word;
+  }
   auto* rt = new DeviceRuntime();
   rt->device = device;
   rt->sm_count = prop.multiProcessorCount;
@@ -323,6 +333,12 @@ extern "C" int mm_get_device(int* out) {
   if (out == nullptr) return fail(MM_ERR_INVALID, "mm_get_device: null output");
   MM_CUDA(cudaGetDevice(out), "cudaGetDevice");
   return MM_OK;
+}
+
+extern "C" int mm_fault_word(int device, int** word_out) {
+  if (word_out == nullptr) return fail(MM_ERR_INVALID, "mm_fault_word: null output");
+  *word_out = fault_word(device);
+  return *word_out ? MM_OK : fail(MM_ERR_STATE, "mm_fault_word: device not initialised");
 }
 
 extern "C" int mm_runtime_stream(int device, void** stream_out) {

@@ -24,6 +24,8 @@ using dev_fn = int (*)(int);
 using stream_fn = int (*)(int, void**);
 using sync_fn = int (*)(void*, int64_t);
 using query_fn = int (*)(void*, int*);
+using fault_fn = int (*)(int, int**);
+using kernel_error_fn = int (*)(int, int*, int);
 
 template <class F>
 F resolve(const char* name) {
@@ -67,7 +69,15 @@ constexpr int MM_STATUS_TIMEOUT = 5;  // MM_ERR_TIMEOUT of the C ABI
 // ABI's message when the wait gives up (MM_ERR_TIMEOUT) or fails.
 void sync_runtime_stream(int device, const char* what) {
   const int rc = MM_SYMBOL(sync_fn, "mm_stream_sync")(runtime_stream(device), g_wait_timeout_ms.load());
-  if (rc == 0) return;
+  if (rc == 0) {
+    int* fault = nullptr;
+    if (MM_SYMBOL(fault_fn, "mm_fault_word")(device, &fault) != 0 || *(volatile int*)fault == 0) return;
+    int code = 0;
+    MM_SYMBOL(kernel_error_fn, "mm_kernel_error")(device, &code, 1);
+    TORCH_CHECK(code == 0, "matrixman guard: ", what, " of device ", device,
+                ": a tensor-core kernel stopped after a bounded wait (code ", code, ")");
+    return;
+  }
   char msg[512] = {0};
   using err_fn = int (*)(char*, size_t);
   if (void* p = dlsym(RTLD_DEFAULT, "mm_last_error")) reinterpret_cast<err_fn>(p)(msg, sizeof(msg));

@@ -518,11 +518,7 @@ def conv_tc(x: MatrixManTensor, w_hi: MatrixManTensor, w_lo: MatrixManTensor, k_
 
 def check_kernel_error(device: int) -> None:
     """Raise if a device-side bounded wait gave up (the kernel returned early)."""
-    code = ctypes.c_int(0)
-    _lib.check(_lib_handle().mm_kernel_error(int(device), ctypes.byref(code), 1), "kernel status")
-    if code.value:
-        raise _lib.MatrixManNativeError(
-            f"MatrixMan/CUDA: a tensor-core kernel stopped after a bounded wait (code {code.value})")
+    get_runtime(device).check_kernel_error()
 
 
 def gemm(x, w_kn, bias=None, alpha=1.0, beta=1.0, act=_lib.ACT_NONE, out=None) -> MatrixManTensor:

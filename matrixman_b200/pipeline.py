@@ -171,6 +171,7 @@ def infer(model, x: torch.Tensor, chunks: int = 4, device=None, sizes=None) -> t
                 # done with them (below).
                 keep.append((xd, y))
         _lib.check(lib.mm_stream_sync(ctypes.c_void_p(down), runtime.config.waitTimeoutMs), "synchronize")
+        rt.raise_fault()
     finally:
         try:
             lib.mm_stream_sync(ctypes.c_void_p(down), runtime.config.waitTimeoutMs)
@@ -228,6 +229,7 @@ def infer_stream(model, batches, device=None, depth: int = 2):
     def _finish(item):
         done, out, _keep, evs = item
         _lib.check(lib.mm_event_sync(done, runtime.config.waitTimeoutMs), "readback wait")
+        rt.raise_fault()
         for h in evs:  # this batch's events are no longer waited on
             lib.mm_event_destroy(h)
         return out

@@ -187,6 +187,9 @@ class DeviceRuntime:
             1 if config.scratchPool == "deferred" else 0,
             1 if config.cudaDisableAllocPool else 0,
         ), "configure pool")
+        word = ctypes.c_void_p()
+        _lib.check(lib.mm_fault_word(self.index, ctypes.byref(word)), "fault word")
+        self._fault = ctypes.c_int.from_address(word.value)
         self.closed = False
         self._param_cache: dict[tuple, tuple] = {}
         self.capturing = False
@@ -263,6 +266,21 @@ class DeviceRuntime:
     def synchronize(self, timeout_ms: int | None = None) -> None:
         timeout = config.waitTimeoutMs if timeout_ms is None else int(timeout_ms)
         _lib.check(self.lib.mm_stream_sync(self.stream, timeout), "synchronize")
+        self.raise_fault()
+
+    def raise_fault(self) -> None:
+        """After a wait for the device: raise if a linear kernel left its call
+        incomplete (reads host memory only)."""
+        if self._fault.value:
+            self.check_kernel_error()
+
+    def check_kernel_error(self) -> None:
+        """Raise if a device-side bounded wait gave up (the kernel returned early)."""
+        code = ctypes.c_int(0)
+        _lib.check(self.lib.mm_kernel_error(self.index, ctypes.byref(code), 1), "kernel status")
+        if code.value:
+            raise _lib.MatrixManNativeError(
+                f"MatrixMan/CUDA: a tensor-core kernel stopped after a bounded wait (code {code.value})")
 
     # -- parameters ----------------------------------------------------------
     @staticmethod

@@ -396,3 +396,56 @@ def test_short_pair_products_one_behind_the_other(mm):
     code = ctypes.c_int(-1)
     _lib.check(lib.mm_kernel_error(rt.index, ctypes.byref(code), 0))
     assert code.value == 0
+
+
+@pytest.mark.parametrize("m,n,k", [(2500, 1100, 70), (511, 1300, 2049), (128, 1000, 4096)])
+def test_bounded_waits_run_out_and_recover(mm, m, n, k):
+    """With the test hook CTA 0 leaves its first loads out and the limit of a wait is 1 ms, so the waits for that
+    stage run out: the kernel records a code, waits for its own copies and MMAs, frees tensor memory and
+    returns, and the next wait of the host raises.  Calls after that are whole, and are not hurried by a code
+    that nobody has read."""
+    lib = _lib.load()
+    x, w, dy = mm.to_device(randn(m, k, seed=1)), mm.to_device(randn(n, k, seed=2)), mm.to_device(randn(m, n, seed=3))
+    rt = x.runtime
+    xg, wg = x.detach().requires_grad_(True), w.detach().requires_grad_(True)
+
+    def forward():
+        with torch.no_grad():
+            return mm.linear(x, w)
+
+    def grads():
+        return torch.autograd.grad(mm.linear(xg, wg), (xg, wg), dy)
+
+    want = [t.cpu() for t in (forward(), *grads())]
+    rt.synchronize()
+    code = ctypes.c_int(-1)
+    for call in (forward, grads):
+        _lib.check(lib.mm_debug_tc_fault(rt.index, 1_000_000, 1))
+        try:
+            call()
+        finally:
+            _lib.check(lib.mm_debug_tc_fault(rt.index, 0, 0))
+        with pytest.raises(_lib.MatrixManNativeError, match=r"code 10[1-5]"):
+            rt.synchronize(timeout_ms=30_000)
+        _lib.check(lib.mm_kernel_error(rt.index, ctypes.byref(code), 0))
+        assert code.value == 0  # reported once
+        assert all(torch.equal(t.cpu(), v) for t, v in zip((forward(), *grads()), want))
+    # a readback and torch's own synchronisation report it too, mm_kernel_error to C callers
+    for wait in (lambda y: y.cpu(), lambda y: torch.Stream(device=y.device).synchronize()):
+        _lib.check(lib.mm_debug_tc_fault(rt.index, 1_000_000, 1))
+        try:
+            y = forward()
+        finally:
+            _lib.check(lib.mm_debug_tc_fault(rt.index, 0, 0))
+        with pytest.raises(RuntimeError, match=r"code 10[1-5]"):
+            wait(y)
+    _lib.check(lib.mm_debug_tc_fault(rt.index, 1_000_000, 1))
+    try:
+        forward()
+    finally:
+        _lib.check(lib.mm_debug_tc_fault(rt.index, 0, 0))
+    y = forward()  # the code stands, this call is whole
+    _lib.check(lib.mm_stream_sync(rt.stream, 30_000))
+    _lib.check(lib.mm_kernel_error(rt.index, ctypes.byref(code), 1))
+    assert 101 <= code.value <= 105
+    assert torch.equal(y.cpu(), want[0])
