@@ -220,6 +220,11 @@ int mm_host_arena_create(int64_t capacity_bytes, int deferred, void** arena_out)
 int mm_host_arena_destroy(void* arena);
 int mm_host_arena_alloc(void* arena, size_t bytes, int kind, void** out);
 int mm_host_arena_free(void* arena, void* ptr);
+/* The same on another stream than the arena's own (0), and the number of stream
+ * waits that allocations have made so far. */
+int mm_host_arena_alloc_on(void* arena, size_t bytes, int kind, int stream, void** out);
+int mm_host_arena_free_on(void* arena, void* ptr, int stream);
+int mm_host_arena_waits(void* arena, int64_t* out);
 int mm_host_arena_complete(void* arena, int64_t generation);
 int mm_host_arena_generation(void* arena, int64_t* out);
 int mm_host_arena_fail_after(void* arena, int64_t n);

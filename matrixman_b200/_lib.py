@@ -143,6 +143,9 @@ SIGNATURES = {
     "mm_host_arena_destroy": [_vp],
     "mm_host_arena_alloc": [_vp, _sz, _i, ctypes.POINTER(_vp)],
     "mm_host_arena_free": [_vp, _vp],
+    "mm_host_arena_alloc_on": [_vp, _sz, _i, _i, ctypes.POINTER(_vp)],
+    "mm_host_arena_free_on": [_vp, _vp, _i],
+    "mm_host_arena_waits": [_vp, ctypes.POINTER(_i64)],
     "mm_host_arena_complete": [_vp, _i64],
     "mm_host_arena_generation": [_vp, ctypes.POINTER(_i64)],
     "mm_host_arena_fail_after": [_vp, _i64],

@@ -59,7 +59,8 @@ class Arena {
     std::vector<Block*> owned;  // every block the graph may touch
   };
 
-  explicit Arena(Backend backend) : be_(backend) {}
+  // `home`: a stream that outlives the arena's use (the device's runtime stream).
+  Arena(Backend backend, Stream home) : be_(backend), home_(home) {}
   ~Arena() { release_all(); }
 
   void configure(bool sync_safe, bool deferred_act, bool deferred_scratch, bool disable_pool) {
@@ -114,8 +115,10 @@ class Arena {
         Block* b = it->second.back();
         it->second.pop_back();
         stats_.cached_bytes[kind] -= (int64_t)b->size;
-        // (reuse on the stream of the release is ordered already)
-        if (sync_safe_ && b->has_event && b->release_stream != stream) be_.stream_wait(stream, b->ev);
+        // Reuse on the stream of the release is ordered already; but equal handles
+        // are one stream only where it cannot have been destroyed in between.
+        const bool same = stream == home_ && b->release_stream == home_;
+        if (sync_safe_ && b->has_event && !same) be_.stream_wait(stream, b->ev);
         live_[b->ptr] = b;
         account_live(b, +1);
         ++stats_.pool_hits[kind];
@@ -322,6 +325,7 @@ class Arena {
   }
 
   Backend be_;
+  Stream home_;
   std::mutex mu_;
   bool sync_safe_ = true;
   bool deferred_[2] = {false, false};

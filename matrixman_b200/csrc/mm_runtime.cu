@@ -76,6 +76,7 @@ struct HostArenaState {
   int64_t used = 0;
   int64_t generation = 1;
   int64_t completed = 0;
+  int64_t waits = 0;  // stream waits made
   std::unordered_map<void*, size_t> sizes;
 };
 
@@ -106,7 +107,7 @@ struct HostArenaBackend {
   void event_destroy(Event) {}
   void event_record(Event& e, Stream) { e = st->generation++; }
   bool event_done(Event e) { return e <= st->completed; }
-  void stream_wait(Stream, Event) {}
+  void stream_wait(Stream, Event) { ++st->waits; }
   void stream_sync(Stream) {}
   void device_sync() { st->completed = st->generation; }
 };
@@ -303,7 +304,7 @@ extern "C" int mm_init(int device) {
   }
   CudaArenaBackend be;
   be.device = device;
-  rt->arena.reset(new Arena<CudaArenaBackend>(be));
+  rt->arena.reset(new Arena<CudaArenaBackend>(be, rt->stream));
   if (const char* env = std::getenv("MATRIXMAN_TEST_FAIL_ALLOC_AFTER")) {
     rt->arena->set_fail_after(std::atoll(env));
   }
@@ -535,7 +536,7 @@ extern "C" int mm_host_arena_create(int64_t capacity_bytes, int deferred, void**
   h->state.capacity = capacity_bytes;
   HostArenaBackend be;
   be.st = &h->state;
-  h->arena.reset(new Arena<HostArenaBackend>(be));
+  h->arena.reset(new Arena<HostArenaBackend>(be, 0));
   h->arena->configure(true, deferred != 0, deferred != 0, false);
   *arena_out = h;
   return MM_OK;
@@ -547,14 +548,20 @@ extern "C" int mm_host_arena_destroy(void* arena) {
 }
 
 extern "C" int mm_host_arena_alloc(void* arena, size_t bytes, int kind, void** out) {
+  return mm_host_arena_alloc_on(arena, bytes, kind, 0, out);
+}
+
+extern "C" int mm_host_arena_free(void* arena, void* ptr) { return mm_host_arena_free_on(arena, ptr, 0); }
+
+extern "C" int mm_host_arena_alloc_on(void* arena, size_t bytes, int kind, int stream, void** out) {
   std::string msg;
-  int rc = ((HostArena*)arena)->arena->alloc(bytes, kind, 0, out, &msg);
+  int rc = ((HostArena*)arena)->arena->alloc(bytes, kind, stream, out, &msg);
   return rc == MM_OK ? MM_OK : fail(rc, msg);
 }
 
-extern "C" int mm_host_arena_free(void* arena, void* ptr) {
+extern "C" int mm_host_arena_free_on(void* arena, void* ptr, int stream) {
   std::string msg;
-  int rc = ((HostArena*)arena)->arena->free(ptr, 0, &msg);
+  int rc = ((HostArena*)arena)->arena->free(ptr, stream, &msg);
   return rc == MM_OK ? MM_OK : fail(rc, msg);
 }
 
@@ -566,6 +573,11 @@ extern "C" int mm_host_arena_complete(void* arena, int64_t generation) {
 
 extern "C" int mm_host_arena_generation(void* arena, int64_t* out) {
   *out = ((HostArena*)arena)->state.generation;
+  return MM_OK;
+}
+
+extern "C" int mm_host_arena_waits(void* arena, int64_t* out) {
+  *out = ((HostArena*)arena)->state.waits;
   return MM_OK;
 }
 

@@ -127,3 +127,17 @@ def test_size_classes_bound_waste():
     st = a.stats()
     assert st["cached_bytes"]["activation"] <= sum(max(512, int(s * 1.125) + 512) for s in sizes)
     a.close()
+
+
+@pytest.mark.parametrize("freed,taken,waits", [(0, 0, 0), (0, 1, 1), (1, 0, 1), (1, 2, 1), (1, 1, 1)])
+def test_reuse_is_ordered_behind_the_release(freed, taken, waits):
+    """Only the arena's own stream needs no wait: another one's handle may belong
+    to a new stream by now, the one of the release being destroyed."""
+    a = HostArena()
+    p = ctypes.c_void_p(a.alloc(4096, _lib.POOL_SCRATCH))
+    _lib.check(a.lib.mm_host_arena_free_on(a.h, p, freed))
+    q, n = ctypes.c_void_p(), ctypes.c_int64()
+    _lib.check(a.lib.mm_host_arena_alloc_on(a.h, 4096, _lib.POOL_SCRATCH, taken, ctypes.byref(q)))
+    _lib.check(a.lib.mm_host_arena_waits(a.h, ctypes.byref(n)))
+    assert q.value == p.value and n.value == waits
+    a.close()
