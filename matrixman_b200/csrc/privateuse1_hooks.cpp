@@ -516,6 +516,13 @@ using adamw_fn = int (*)(const void*, int, int, double, double, double, double, 
                          void*);
 using decode_fn = int (*)(const void*, const void*, const void*, const void*, int64_t, void*, void*, void*);
 
+// Whether 8-bit codes (four to a float) and their scales are those of p's elements.
+bool holds_codes(const Operand& codes, const Operand& scales, const Operand& p) {
+  const int64_t blocks = (p.t->numel() + 255) / 256;
+  return codes.t->numel() == 64 * blocks && scales.t->numel() == blocks && codes.t->is_contiguous() &&
+         scales.t->is_contiguous();
+}
+
 // An optimiser step over parameters with gradients and the states of
 // optim.AdamW (dicts): the table of addresses and the native call.  True, an
 // int (its status), or None where a tensor is not as usual.
@@ -545,10 +552,10 @@ py::object adamw_step(const py::list& params, const py::list& states, int bits, 
         g.t->strides() != p.t->strides())
       return py::none();
     const py::handle state = states[i];
-    if (!PyDict_Check(state.ptr()) || !state_of(state, step_name, &step)) return py::none();
+    if (!PyDict_Check(state.ptr()) || !state_of(state, step_name, &step) || step.t->numel() != 1) return py::none();
     if (bits == 8) {
       if (!state_of(state, narrow[0], &m) || !state_of(state, narrow[1], &v) || !state_of(state, narrow[2], &ms) ||
-          !state_of(state, narrow[3], &vs))
+          !state_of(state, narrow[3], &vs) || !holds_codes(m, ms, p) || !holds_codes(v, vs, p))
         return py::none();
     } else if (!state_of(state, wide[0], &m) || !state_of(state, wide[1], &v) || m.t->sizes() != p.t->sizes() ||
                v.t->sizes() != p.t->sizes() || m.t->strides() != p.t->strides() || v.t->strides() != p.t->strides()) {
@@ -569,7 +576,8 @@ py::object adamw_values(py::handle p_, py::handle mc_, py::handle ms_, py::handl
   Target t;
   if (!names().ready || !operand(p_, &p) || !operand(mc_, &mc) || !operand(ms_, &ms) || !operand(vc_, &vc) ||
       !operand(vs_, &vs) || !p.given || !mc.given || !ms.given || !vc.given || !vs.given ||
-      !p.t->is_non_overlapping_and_dense() || !t.of(p))
+      !p.t->is_non_overlapping_and_dense() || !holds_codes(mc, ms, p) || !holds_codes(vc, vs, p) || !t.of(p) ||
+      !t.owns(mc) || !t.owns(ms) || !t.owns(vc) || !t.owns(vs))
     return py::none();
   const int64_t n = p.t->numel(), at = (n + 63) / 64 * 64;  // both in one block
   char* ptr = nullptr;

@@ -13,7 +13,7 @@ import array
 import torch
 
 from . import _lib, ops
-from .tensor import MatrixManTensor, contiguous_strides, is_dense, numel
+from .tensor import MatrixManTensor, contiguous_strides, is_contiguous, is_dense, numel
 
 BLOCK = 256  # elements that share a scale of the 8-bit states
 _CODES = ("exp_avg_code", "exp_avg_scale", "exp_avg_sq_code", "exp_avg_sq_scale")
@@ -134,14 +134,40 @@ class AdamW(torch.optim.Optimizer):
             state.update(self._new_state(p))
         return state
 
+    def _check_state(self, p: MatrixManTensor, state: dict) -> dict:
+        """A state (the program may have set it) of the kinds and sizes that the
+        kernels reach by its addresses."""
+        n = numel(p.shape)
+        blocks = (n + BLOCK - 1) // BLOCK
+        sizes = {"step": 1}
+        if self.state_bits == 8:
+            sizes.update(zip(_CODES, (blocks * BLOCK // 4, blocks) * 2))
+        else:
+            sizes.update(exp_avg=n, exp_avg_sq=n)
+        for name, size in sizes.items():
+            if name not in state:
+                raise RuntimeError(f"MatrixMan/CUDA: AdamW state has no {name}")
+            t = ops.require_mm(state[name], f"AdamW state {name}")
+            ops.require_f32(t, f"AdamW state {name}")
+            if t.runtime is not p.runtime:
+                raise RuntimeError(f"MatrixMan/CUDA: AdamW state {name} is on another device than its parameter")
+            if name in ("exp_avg", "exp_avg_sq"):
+                if tuple(t.shape) != tuple(p.shape) or not _same_order(t, p):
+                    raise RuntimeError(f"MatrixMan/CUDA: AdamW state {name} must have its parameter's shape and "
+                                       f"strides, {tuple(p.shape)} and {p._logical_strides}, got {tuple(t.shape)} "
+                                       f"and {t._logical_strides}")
+            elif numel(t.shape) != size or not is_contiguous(t.shape, t._logical_strides):
+                raise RuntimeError(f"MatrixMan/CUDA: AdamW state {name} must hold {size} dense values, "
+                                   f"got {tuple(t.shape)}")
+        return state
+
     def _row(self, p: MatrixManTensor, grad: MatrixManTensor, state: dict) -> tuple:
+        self._check_state(p, state)
         if self.state_bits == 8:
             m, v = state["exp_avg_code"], state["exp_avg_sq_code"]
             ms, vs = _pointer(state["exp_avg_scale"]), _pointer(state["exp_avg_sq_scale"])
         else:
             m, v = state["exp_avg"], state["exp_avg_sq"]
-            if not (_same_order(m, p) and _same_order(v, p)):
-                raise RuntimeError("MatrixMan/CUDA: AdamW state does not have its parameter's strides")
             ms = vs = 0
         return (_pointer(p), _pointer(grad), _pointer(m), _pointer(v), ms, vs, _pointer(state["step"]),
                 numel(p.shape))
@@ -186,7 +212,7 @@ class AdamW(torch.optim.Optimizer):
     def state_values(self, p) -> tuple[MatrixManTensor, MatrixManTensor]:
         """(exp_avg, exp_avg_sq) of a parameter as new float32 tensors (8-bit
         states: the values that the codes stand for)."""
-        state = self._state_of(p)
+        state = self._check_state(p, self._state_of(p))
         if self.state_bits == 32:
             return ops.clone(state["exp_avg"]), ops.clone(state["exp_avg_sq"])
         done = ops.native_call("adamw_values", "mm_adamw_decode", p, *(state[k] for k in _CODES))
@@ -203,7 +229,7 @@ class AdamW(torch.optim.Optimizer):
     def set_state_values(self, p, exp_avg, exp_avg_sq, step=None) -> None:
         """Set a parameter's moments (float32, its shape; CPU or MatrixMan
         tensors) and, if given, its step count."""
-        state = self._state_of(p)
+        state = self._check_state(p, self._state_of(p))
         rt = p.runtime
         given = []
         for name, t in (("exp_avg", exp_avg), ("exp_avg_sq", exp_avg_sq)):

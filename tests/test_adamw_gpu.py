@@ -318,3 +318,31 @@ def test_refusals(mm):
         o = torch.optim.AdamW([p], fused=True, amsgrad=True)
         p.grad = mm.to_device(torch.zeros(8))
         o.step()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_states_that_do_not_fit_their_parameter(mm, bits):
+    """The C++ calls leave them to the Python code, which refuses them; nothing is launched and nothing moves."""
+    from matrixman_b200 import telemetry
+    from matrixman_b200.privateuse import native_calls
+    names = ("exp_avg", "exp_avg_sq") if bits == 32 else ("exp_avg_code", "exp_avg_scale", "exp_avg_sq_code",
+                                                          "exp_avg_sq_scale")
+    for name in (*names, "step"):
+        p = torch.nn.Parameter(mm.to_device(torch.ones(1000)))
+        p.grad = mm.to_device(torch.ones(1000))
+        opt = mm.optim.AdamW([p], state_bits=bits)
+        opt.step()
+        want = p.detach().cpu()
+        right = opt.state[p][name]
+        for wrong in (mm.to_device(torch.zeros(max(right.numel() - 1, 0))), mm.to_device(torch.zeros(2000))[::2]):
+            if name in ("exp_avg", "exp_avg_sq") or wrong.numel() != right.numel():
+                opt.state[p][name] = wrong
+                assert native_calls().adamw_step([p], [opt.state[p]], bits, 1e-3, 0.9, 0.999, 1e-8, 0.0, False) is None
+                before = dict(telemetry.launches)
+                for call in (opt.step, lambda: opt.state_values(p)):
+                    with pytest.raises(RuntimeError, match="AdamW state"):
+                        call()
+                assert dict(telemetry.launches) == before
+        opt.state[p][name] = right
+        assert torch.equal(p.detach().cpu(), want)
+        opt.step()
