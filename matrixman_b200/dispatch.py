@@ -625,6 +625,8 @@ def _fused_adam(decoupled, params, grads, exp_avgs, exp_avg_sqs, max_exp_avg_sqs
         ops._runtime_of(p, g, m, v, step)
         if any(tuple(t.shape) != tuple(p.shape) for t in (g, m, v)):
             raise RuntimeError("MatrixMan/CUDA: fused Adam needs equal shapes of parameter, gradient and states")
+        if step.numel() != 1:
+            raise RuntimeError(f"MatrixMan/CUDA: fused Adam needs one value per step, got {tuple(step.shape)}")
         if not (optim._same_order(m, p) and optim._same_order(v, p)):
             raise NotImplementedError("MatrixMan/CUDA: fused Adam states must have their parameter's strides")
         g = optim._in_order(g, p)

@@ -116,3 +116,14 @@ def test_state_of_another_shape_with_as_many_values(rt, launches):
     with pytest.raises(RuntimeError, match="strides"):
         opt.step()
     assert launches == []
+
+
+@pytest.mark.parametrize("shape", [(0,), (2,)])
+def test_fused_step_of_another_size(rt, launches, shape):
+    p, g, m, v = (tensor(rt, 40) for _ in range(4))
+    kw = dict(lr=1e-3, beta1=0.9, beta2=0.999, weight_decay=0.0, eps=1e-8, amsgrad=False, maximize=False)
+    for op in (torch.ops.aten._fused_adamw_, torch.ops.aten._fused_adam_):
+        op([p], [g], [m], [v], [], [tensor(rt)], **kw)
+        with pytest.raises(RuntimeError, match="one value per step"):
+            op([p], [g], [m], [v], [], [tensor(rt, *shape)], **kw)
+    assert launches == ["mm_adamw"] * 2
