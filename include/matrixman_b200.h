@@ -425,7 +425,8 @@ typedef struct mm_adamw_tensor {
  * step over `count` tensors: m = b1 m + (1 - b1) g, v = b2 v + (1 - b2) g^2,
  * p = p (1 - lr wd) - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps).
  * t is *step, after adding 1 to it when `advance` (each tensor then needs a step
- * of its own).  state_bits 32 or 8.  8-bit states: a block of 256 elements has
+ * of its own).  Parameters and states may not overlap; any of them, or a step
+ * that advances, given twice is refused.  state_bits 32 or 8.  8-bit states: a block of 256 elements has
  * one scale, the largest magnitude; m is held as sign and 7-bit code (8 steps
  * per power of two over 16 powers of two, code 0 is zero), v as an 8-bit code of
  * its square root (16 steps; at least code 1 unless v is 0).  A non-finite

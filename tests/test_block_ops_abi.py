@@ -120,3 +120,32 @@ def test_adamw_checks():
     assert lib.mm_adamw_encode(FAKE, FAKE, 5, FAKE + 1, FAKE, FAKE, FAKE, None) == _lib.MM_ERR_INVALID
     assert lib.mm_adamw_decode(FAKE, FAKE, None, FAKE, 5, FAKE, FAKE, None) == _lib.MM_ERR_INVALID
     assert lib.mm_adamw_decode(None, None, None, None, 0, None, None, None) == _lib.MM_OK
+
+
+def test_adamw_refuses_the_same_memory_twice():
+    """The workspace is too small, which is said only of calls whose tensors are their own."""
+    lib = _lib.load()
+
+    def call(rows, bits=32, advance=1):
+        table = (ctypes.c_int64 * (8 * len(rows)))(*(v for r in rows for v in r))
+        status = lib.mm_adamw(table, len(rows), bits, 1e-3, 0.9, 0.99, 1e-8, 0.0, 1, 0, advance, FAKE, 1, None)
+        assert status == _lib.MM_ERR_INVALID
+        return "workspace" if "workspace" in _lib.last_error() else "shares" if "shares" in _lib.last_error() else "?"
+
+    def row(i, **kw):
+        names = ("p", "g", "m", "v", "ms", "vs", "step")
+        got = {k: FAKE + 4096 * (16 * i + j) for j, k in enumerate(names)} | {"n": 10} | kw
+        return [got[k] for k in (*names, "n")]
+
+    for bits in (32, 8):
+        assert call([row(0), row(1), row(2)], bits) == "workspace"
+        first = dict(zip(("p", "g", "m", "v", "ms", "vs", "step"), row(0)))
+        for name in ("p", "m", "v", "step") + (("ms", "vs") if bits == 8 else ()):
+            assert call([row(0), row(1), row(2, **{name: first[name]})], bits) == "shares"
+            assert call([row(0), row(1, p=first[name])], bits) == "shares"
+        assert call([row(0, v=first["m"])], bits) == "shares"
+        assert call([row(0), row(1, g=first["g"])], bits) == "workspace"  # gradients are only read
+        assert call([row(0), row(1, step=first["step"])], bits, advance=0) == "workspace"
+        assert call([row(0), row(1, n=0, p=first["p"], m=first["m"], v=0)], bits) == "workspace"  # nothing to write
+    assert call([row(i) for i in range(1000)]) == "workspace"
+    assert call([row(i) for i in range(1000)] + [row(1000, m=row(3)[2])]) == "shares"
