@@ -67,7 +67,9 @@ class AdamW(torch.optim.Optimizer):
     Parameters and gradients are float32 MatrixMan tensors of one device per
     group; a parameter fills its storage span (any order of dimensions) and
     shares it with no other.  The step count lives on the device, so a captured
-    step can be replayed."""
+    step can be replayed; every parameter with a gradient must have its state by
+    then (from a step, or set), and lr, betas, eps and weight_decay stay what
+    they were at capture."""
 
     def __init__(self, params, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2, *,
                  maximize: bool = False, state_bits: int = 32):
@@ -115,6 +117,9 @@ class AdamW(torch.optim.Optimizer):
     # -- state ---------------------------------------------------------------
     def _new_state(self, p: MatrixManTensor) -> dict:
         rt = p.runtime
+        if rt.capturing:  # the zeros would be part of the graph, and every replay a first step
+            raise RuntimeError("MatrixMan/CUDA: AdamW cannot make a parameter's state during graph capture; take a "
+                               "step or set the state (set_state_values, load_state_dict) before capturing")
         state = {"step": ops.full(rt, (), 0.0)}
         if self.state_bits == 32:
             for name in ("exp_avg", "exp_avg_sq"):

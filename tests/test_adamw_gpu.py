@@ -346,3 +346,30 @@ def test_states_that_do_not_fit_their_parameter(mm, bits):
         opt.state[p][name] = right
         assert torch.equal(p.detach().cpu(), want)
         opt.step()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_first_step_may_not_be_the_captured_one(mm, bits):
+    host, params = params_of(mm, [(700,), (33, 9)])
+    opt = mm.optim.AdamW(params, lr=1e-2, state_bits=bits)
+    for p, g in zip(params, grads_of([(700,), (33, 9)], 1)):
+        p.grad = mm.to_device(g)
+    rt = params[0].runtime
+    rt.synchronize()
+    rt.capture_begin()
+    try:
+        with pytest.raises(RuntimeError, match="capture"):
+            opt.step()
+    finally:
+        rt.capture_end().destroy()
+    assert all(torch.equal(p.detach().cpu(), h) for p, h in zip(params, host))
+    # states that were set take the place of a step
+    for p in params:
+        opt.set_state_values(p, torch.zeros(p.shape), torch.zeros(p.shape), step=0)
+    rt.synchronize()
+    rt.capture_begin()
+    opt.step()
+    graph = rt.capture_end()
+    graph.replay()
+    graph.replay()
+    assert [float(opt.state[p]["step"].cpu()) for p in params] == [2.0, 2.0]

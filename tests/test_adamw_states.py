@@ -127,3 +127,26 @@ def test_fused_step_of_another_size(rt, launches, shape):
         with pytest.raises(RuntimeError, match="one value per step"):
             op([p], [g], [m], [v], [], [tensor(rt, *shape)], **kw)
     assert launches == ["mm_adamw"] * 2
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_no_state_is_made_during_capture(rt, launches, monkeypatch, bits):
+    monkeypatch.setattr(ops, "full", lambda rt, shape, value: tensor(rt, *shape))
+    monkeypatch.setattr(ops, "fill_", lambda t, value: t)
+    params = [torch.nn.Parameter(tensor(rt, 300)) for _ in range(2)]
+    opt = matrixman.optim.AdamW(params, state_bits=bits)
+    params[0].grad = tensor(rt, 300)
+    opt.step()
+    params[1].grad = tensor(rt, 300)
+    rt.capturing = True
+    for call in (opt.step, lambda: opt.state_values(params[1]),
+                 lambda: opt.set_state_values(params[1], tensor(rt, 300), tensor(rt, 300))):
+        with pytest.raises(RuntimeError, match="capture"):
+            call()
+    assert launches == ["mm_adamw"] and not opt.state.get(params[1])
+    params[1].grad = None
+    opt.step()
+    rt.capturing = False
+    params[1].grad = tensor(rt, 300)
+    opt.step()
+    assert launches == ["mm_adamw"] * 3
