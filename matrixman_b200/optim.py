@@ -9,6 +9,7 @@ The reference steps Adam through element-wise operators, tensor by tensor
 from __future__ import annotations
 
 import array
+import copy
 
 import torch
 
@@ -280,12 +281,11 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError("MatrixMan/CUDA: AdamW state_dict has other parameter groups")
         index = [i for g in groups for i in g["params"]]
         params = [p for g in self.param_groups for p in g["params"]]
+        if any(g.get("amsgrad") for g in groups):
+            raise NotImplementedError("MatrixMan/CUDA: AdamW does not implement amsgrad")
+        # Everything that a group holds, a scheduler's "initial_lr" among it.
         for group, saved in zip(self.param_groups, groups):
-            if saved.get("amsgrad"):
-                raise NotImplementedError("MatrixMan/CUDA: AdamW does not implement amsgrad")
-            for key in ("lr", "betas", "eps", "weight_decay", "maximize"):
-                if key in saved:
-                    group[key] = saved[key]
+            group.update(copy.deepcopy({k: v for k, v in saved.items() if k != "params"}))
         self.state.clear()
         for i, p in zip(index, params):
             saved = state_dict["state"].get(i)

@@ -150,3 +150,18 @@ def test_no_state_is_made_during_capture(rt, launches, monkeypatch, bits):
     params[1].grad = tensor(rt, 300)
     opt.step()
     assert launches == ["mm_adamw"] * 3
+
+
+def test_loading_keeps_what_a_scheduler_left_in_the_groups(rt, launches):
+    p = torch.nn.Parameter(tensor(rt, 300))
+    opt = matrixman.optim.AdamW([p], lr=0.5)
+    scheduler = torch.optim.lr_scheduler.StepLR(opt, step_size=2, gamma=0.1)
+    saved, at = opt.state_dict(), scheduler.state_dict()
+    new = matrixman.optim.AdamW([torch.nn.Parameter(tensor(rt, 300))], lr=1.0)
+    new.load_state_dict(saved)
+    assert new.param_groups[0]["initial_lr"] == 0.5 and len(new.param_groups[0]["params"]) == 1
+    assert new.param_groups[0]["params"][0] is not p
+    resumed = torch.optim.lr_scheduler.StepLR(new, step_size=2, gamma=0.1, last_epoch=at["last_epoch"])
+    assert resumed.base_lrs == [0.5]
+    saved["param_groups"][0]["lr"] = 7.0
+    assert new.param_groups[0]["lr"] == 0.5
