@@ -275,7 +275,7 @@ class AdamW(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict: dict) -> None:
         """Load ``state_dict()`` of this class (either ``state_bits``) or of
-        torch.optim.AdamW."""
+        torch.optim.AdamW; what cannot be loaded leaves the optimiser as it was."""
         groups = state_dict["param_groups"]
         if [len(g["params"]) for g in groups] != [len(g["params"]) for g in self.param_groups]:
             raise ValueError("MatrixMan/CUDA: AdamW state_dict has other parameter groups")
@@ -283,13 +283,22 @@ class AdamW(torch.optim.Optimizer):
         params = [p for g in self.param_groups for p in g["params"]]
         if any(g.get("amsgrad") for g in groups):
             raise NotImplementedError("MatrixMan/CUDA: AdamW does not implement amsgrad")
-        # Everything that a group holds, a scheduler's "initial_lr" among it.
-        for group, saved in zip(self.param_groups, groups):
-            group.update(copy.deepcopy({k: v for k, v in saved.items() if k != "params"}))
-        self.state.clear()
-        for i, p in zip(index, params):
-            saved = state_dict["state"].get(i)
-            if saved:
-                step = saved["step"]
-                step = step.cpu() if isinstance(step, MatrixManTensor) else step
-                self.set_state_values(p, saved["exp_avg"], saved["exp_avg_sq"], step=float(step))
+        states, settings = dict(self.state), [dict(g) for g in self.param_groups]
+        try:
+            # Everything that a group holds, a scheduler's "initial_lr" among it.
+            for group, saved in zip(self.param_groups, groups):
+                group.update(copy.deepcopy({k: v for k, v in saved.items() if k != "params"}))
+            self.state.clear()
+            for i, p in zip(index, params):
+                saved = state_dict["state"].get(i)
+                if saved:
+                    step = saved["step"]
+                    step = step.cpu() if isinstance(step, MatrixManTensor) else step
+                    self.set_state_values(p, saved["exp_avg"], saved["exp_avg_sq"], step=float(step))
+        except Exception:
+            self.state.clear()
+            self.state.update(states)
+            for group, before in zip(self.param_groups, settings):
+                group.clear()
+                group.update(before)
+            raise

@@ -165,3 +165,22 @@ def test_loading_keeps_what_a_scheduler_left_in_the_groups(rt, launches):
     assert resumed.base_lrs == [0.5]
     saved["param_groups"][0]["lr"] = 7.0
     assert new.param_groups[0]["lr"] == 0.5
+
+
+def test_what_cannot_be_loaded_changes_nothing(rt, launches, monkeypatch):
+    monkeypatch.setattr(ops, "full", lambda rt, shape, value: tensor(rt, *shape))
+    monkeypatch.setattr(ops, "fill_", lambda t, value: t)
+    params = [torch.nn.Parameter(tensor(rt, 300)) for _ in range(2)]
+    opt = matrixman.optim.AdamW(params, lr=0.5)
+    for p in params:
+        opt.state[p] = state_of(rt, (300,), 32)
+    before = {p: dict(opt.state[p]) for p in params}
+    right = {"step": 1.0, "exp_avg": tensor(rt, 300), "exp_avg_sq": tensor(rt, 300)}
+    for wrong in ({"step": 1.0, "exp_avg": tensor(rt, 299), "exp_avg_sq": tensor(rt, 300)},
+                  {"step": 1.0, "exp_avg": tensor(rt, 300)}):
+        saved = {"state": {0: right, 1: wrong}, "param_groups": [{"params": [0, 1], "lr": 0.25, "other": 1}]}
+        with pytest.raises((ValueError, KeyError)):
+            opt.load_state_dict(saved)
+        assert opt.param_groups[0]["lr"] == 0.5 and "other" not in opt.param_groups[0]
+        assert opt.param_groups[0]["params"] == params
+        assert all(opt.state[p][k] is v for p in params for k, v in before[p].items())
