@@ -26,10 +26,9 @@ __device__ __forceinline__ float lin_act_t(float z) {
   return z;
 }
 
-// act'(z); ReLU's slope at 0 is 0.
+// act'(z) but ReLU's, which selects (below).
 template <int ACT>
 __device__ __forceinline__ float lin_slope_t(float z) {
-  if (ACT == MM_LINEAR_RELU) return z > 0.f ? 1.f : 0.f;
   if (ACT == MM_LINEAR_SILU) {
     const float s = lin_sigmoid(z);
     return s * (1.f + z * (1.f - s));
@@ -65,10 +64,18 @@ __device__ __forceinline__ void lin_act(float (&v)[N], int act) {
 #undef LIN_CALL
 }
 
-// v *= act'(z).
+// dy act'(z).  ReLU drops dy where z <= 0 whatever it is (an infinity or NaN times
+// 0 would be NaN), and passes it where z is NaN, as threshold_backward does.
+template <int ACT>
+__device__ __forceinline__ float lin_grad_t(float dy, float z) {
+  if (ACT == MM_LINEAR_RELU) return z <= 0.f ? 0.f : dy;
+  return dy * lin_slope_t<ACT>(z);
+}
+
+// v = v act'(z).
 template <int N>
 __device__ __forceinline__ void lin_times_slope(float (&v)[N], const float (&z)[N], int act) {
-#define LIN_CALL(A) _Pragma("unroll") for (int e = 0; e < N; ++e) v[e] *= lin_slope_t<A>(z[e]);
+#define LIN_CALL(A) _Pragma("unroll") for (int e = 0; e < N; ++e) v[e] = lin_grad_t<A>(v[e], z[e]);
   LIN_BY_ACT(LIN_CALL)
 #undef LIN_CALL
 }

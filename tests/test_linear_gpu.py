@@ -449,3 +449,38 @@ def test_bounded_waits_run_out_and_recover(mm, m, n, k):
     _lib.check(lib.mm_kernel_error(rt.index, ctypes.byref(code), 1))
     assert 101 <= code.value <= 105
     assert torch.equal(y.cpu(), want[0])
+
+
+@pytest.mark.parametrize("m,n,k", [(5, 40, 24), (60, 96, 50), (700, 640, 300), (2500, 1100, 70)])
+@pytest.mark.parametrize("mode", ["plain", "residual", "residual first"])
+def test_relu_drops_non_finite_gradients_where_it_was_off(mm, m, n, k, mode):
+    """As threshold_backward: the gradient is selected, not multiplied by 0, and passes where z is NaN."""
+    x, w, r, dy = randn(m, k, seed=1), randn(n, k, seed=2), randn(m, n, seed=3), randn(m, n, seed=4)
+    x[1, 3] = float("nan")  # z's row 1
+    first = mode == "residual first"
+    res = None if mode == "plain" else mm.to_device(r).requires_grad_(True)
+    lx, lw, lb = (mm.to_device(t).requires_grad_(True) for t in (x, w, torch.zeros(n)))
+    y = mm.linear(lx, lw, lb, activation="relu", residual=res, residual_before_act=first)
+    z, ez, _ = products(x, w)
+    if first:
+        z, ez = z + r.double(), ez + 4 * U * r.double().abs()
+    dy[z.abs() <= ez + 4 * U * z.abs()] = 0.0  # either sign of the computed z is right there
+    off = (z < -1e-3).nonzero()
+    hit = off[:: max(len(off) // 50, 1)]
+    for i, (a, b) in enumerate(hit.tolist()):
+        dy[a, b] = (float("inf"), float("-inf"), float("nan"))[i % 3]
+    leaves = (lx, lw, lb) + ((res,) if res is not None else ())
+    grads = [g.cpu() for g in torch.autograd.grad(y, leaves, mm.to_device(dy))]
+    # What the framework's own ReLU makes of the same z and gradient, and its sums in float64.
+    zt = mm.to_device(z.float()).requires_grad_(True)
+    dz = torch.autograd.grad(torch.relu(zt), zt, mm.to_device(dy))[0].cpu()
+    assert torch.isfinite(dz).all() and torch.equal(dz[1], dy[1]) and (dz[hit[:, 0], hit[:, 1]] == 0).all()
+    want, bound, _ = products(dz, w.t())
+    close("dx", grads[0], want, bound)
+    got, ok = grads[1], [c for c in range(k) if c != 3]
+    want, bound, _ = products(dz.t(), x[:, ok].t().nan_to_num(0.0))
+    close("dw", got[:, ok], want, bound)
+    close("db", grads[2], dz.double().sum(0), (m + 8) * U * dz.double().abs().sum(0))
+    if res is not None:
+        expect = dz if first else dy
+        assert torch.equal(grads[3].nan_to_num(7.0, 8.0, 9.0), expect.nan_to_num(7.0, 8.0, 9.0))
