@@ -58,10 +58,6 @@ def get_backend() -> Backend:
         install_privateuse1_factory_kernels()
         from .privateuse import register_native_hooks
         register_native_hooks()  # C++ DeviceGuard + hooks (indexing, pin_memory)
-        # Backward passes run on the calling thread: every device has one stream
-        # and every operator is queued from Python, so autograd's worker thread
-        # would only add two thread switches (about 70 us) to each call.
-        torch.autograd.set_multithreading_enabled(False)
         rt = runtime.get_runtime(runtime.current_device())
         _banner(rt)
         _backend = Backend()

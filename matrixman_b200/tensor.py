@@ -292,6 +292,13 @@ class MatrixManTensor(torch.Tensor):
             register_native_hooks()
         return torch.Tensor.requires_grad_(self, requires_grad)
 
+    def backward(self, *args, **kwargs):
+        # On the calling thread: every device has one stream and every operator is
+        # queued from Python, so autograd's worker thread would only add two thread
+        # switches (about 40 us) to the call.
+        with torch.autograd.set_multithreading_enabled(False):
+            return torch.Tensor.backward(self, *args, **kwargs)
+
     @classmethod
     def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
         global _dispatch
