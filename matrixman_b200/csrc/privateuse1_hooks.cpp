@@ -232,6 +232,16 @@ using linear_back_fn = int (*)(const void*, int64_t, const void*, int64_t, int64
                                const void*, int64_t, int64_t, int64_t, int, void*, void*, void*, void*, void*, size_t,
                                void*);
 
+// A call into the native library without the interpreter's lock (as ctypes makes
+// it): a full launch queue or an allocation may block, and the program's other
+// threads go on meanwhile.  Every tensor whose address it takes is held by the
+// caller.
+template <class F, class... Args>
+int unlocked(F f, Args... args) {
+  py::gil_scoped_release released;
+  return f(args...);
+}
+
 // A matrixman tensor's metadata and address.
 struct Operand {
   bool given = false;
@@ -325,7 +335,7 @@ py::tuple int_tuple(at::IntArrayRef v) {
 py::object new_storage(const Target& t, int64_t numel, char** ptr) {
   const size_t bytes = (size_t)(numel > 0 ? numel : 1) * 4;
   void* p = nullptr;
-  if (MM_SYMBOL(alloc_fn, "mm_alloc")(t.index, bytes, 0, t.stream, &p) != 0) return py::object();
+  if (unlocked(MM_SYMBOL(alloc_fn, "mm_alloc"), t.index, bytes, 0, t.stream, &p) != 0) return py::object();
   *ptr = (char*)p;
   return names().storage(t.runtime, (int64_t)(intptr_t)p, bytes, names().f32, 0);
 }
@@ -387,8 +397,8 @@ py::object layer_norm(py::handle x_, int64_t width, py::handle w_, py::handle b_
   char* p = nullptr;
   py::object owner = new_storage(t, at + 2 * rows, &p);
   if (!owner) return py::none();
-  const int status = MM_SYMBOL(norm_fn, "mm_layer_norm")(x.ptr, stride, rows, width, w.ptr, b.ptr, eps, p, p + 4 * at,
-                                                         p + 4 * (at + rows), t.stream);
+  const int status = unlocked(MM_SYMBOL(norm_fn, "mm_layer_norm"), x.ptr, stride, rows, width, w.ptr, b.ptr, eps, p,
+                              p + 4 * at, p + 4 * (at + rows), t.stream);
   if (status != 0) return py::int_(status);
   std::vector<int64_t> shape = x.t->sizes().vec();
   py::object y = new_tensor(t, owner, int_tuple(shape), dense_strides(shape), 0);
@@ -423,9 +433,9 @@ py::object layer_norm_backward(py::handle dy_, py::handle x_, int64_t width, py:
     if (need_w) dw = new_tensor(t, owner, shape, one, 0);
     if (need_b) db = new_tensor(t, owner, shape, one, each);
   }
-  const int status = MM_SYMBOL(norm_back_fn, "mm_layer_norm_backward")(
-      dy.ptr, gs, x.ptr, xs, rows, width, mean.ptr, rstd.ptr, w.ptr, px, need_w ? pw : nullptr,
-      need_b ? pw + 4 * each : nullptr, nullptr, 0, t.stream);
+  const int status = unlocked(MM_SYMBOL(norm_back_fn, "mm_layer_norm_backward"), dy.ptr, gs, x.ptr, xs, rows, width,
+                              mean.ptr, rstd.ptr, w.ptr, px, need_w ? pw : nullptr, need_b ? pw + 4 * each : nullptr,
+                              nullptr, 0, t.stream);
   if (status != 0) return py::int_(status);
   return py::make_tuple(dx, dw, db);
 }
@@ -478,9 +488,9 @@ py::object linear(py::handle x_, py::handle w_, py::handle b_, py::handle r_, in
   char *py_ = nullptr, *pz = nullptr;
   py::object y = new_dense(c.t, c.shape, &py_), z = py::none();
   if (!y || (keep && !(z = new_dense(c.t, c.shape, &pz)))) return py::none();
-  const int status = MM_SYMBOL(linear_fn, "mm_linear")(c.x.ptr, c.xs0, c.xs1, c.w.ptr, c.w.t->stride(0),
-                                                       c.w.t->stride(1), c.b.ptr, c.r.ptr, c.rs, c.m, c.n, c.k, act,
-                                                       first, py_, pz, nullptr, 0, c.t.stream);
+  const int status = unlocked(MM_SYMBOL(linear_fn, "mm_linear"), c.x.ptr, c.xs0, c.xs1, c.w.ptr, c.w.t->stride(0),
+                              c.w.t->stride(1), c.b.ptr, c.r.ptr, c.rs, c.m, c.n, c.k, act, first, py_, pz, nullptr, 0,
+                              c.t.stream);
   if (status != 0) return py::int_(status);
   return py::make_tuple(y, z);
 }
@@ -505,9 +515,9 @@ py::object linear_backward(py::handle dy_, py::handle x_, py::handle w_, py::han
   if (need_w && !(dw = new_dense(t, wn, &pw))) return py::none();
   if (need_b && !(db = new_dense(t, at::IntArrayRef(wn, 1), &pb))) return py::none();
   if (need_z && !(dz = new_dense(t, dy.t->sizes(), &pz))) return py::none();
-  const int status = MM_SYMBOL(linear_back_fn, "mm_linear_backward")(
-      dy.ptr, gs, x.ptr, xs0, xs1, w.ptr, w.t->stride(0), w.t->stride(1), z.ptr, m, n, k, act, px, pw, pb, pz, nullptr,
-      0, t.stream);
+  const int status = unlocked(MM_SYMBOL(linear_back_fn, "mm_linear_backward"), dy.ptr, gs, x.ptr, xs0, xs1, w.ptr,
+                              w.t->stride(0), w.t->stride(1), z.ptr, m, n, k, act, px, pw, pb, pz, nullptr, 0,
+                              t.stream);
   if (status != 0) return py::int_(status);
   return py::make_tuple(dx, dw, db, dz);
 }
@@ -536,17 +546,20 @@ py::object adamw_step(const py::list& params, const py::list& states, int bits, 
   const size_t count = params.size();
   if (!names().ready || count == 0 || states.size() != count) return py::none();
   std::vector<int64_t> table(8 * count);
-  std::vector<py::object> held;
-  held.reserve(count);
+  std::vector<py::object> held;  // the lists and dicts are the program's: it may change them during the call
+  held.reserve(8 * count);
   Target t;
   auto state_of = [&](const py::handle& state, const py::object& name, Operand* out) {
     PyObject* v = PyDict_GetItemWithError(state.ptr(), name.ptr());
-    return v != nullptr && operand(v, out) && out->given && t.owns(*out);
+    if (v == nullptr) return false;
+    held.push_back(py::reinterpret_borrow<py::object>(v));
+    return operand(v, out) && out->given && t.owns(*out);
   };
   for (size_t i = 0; i < count; ++i) {
     Operand p, g, m, v, ms, vs, step;
     if (!operand(params[i], &p) || !p.given || !p.t->is_non_overlapping_and_dense()) return py::none();
     if (i == 0 ? !t.of(p) : !t.owns(p)) return py::none();
+    held.push_back(params[i]);
     held.push_back(attribute(params[i].ptr(), grad_name));
     if (!operand(held.back(), &g) || !g.given || !t.owns(g) || g.t->sizes() != p.t->sizes() ||
         g.t->strides() != p.t->strides())
@@ -565,8 +578,8 @@ py::object adamw_step(const py::list& params, const py::list& states, int bits, 
     for (int j = 0; j < 7; ++j) table[8 * i + j] = (int64_t)(intptr_t)order[j]->ptr;
     table[8 * i + 7] = p.t->numel();
   }
-  const int status = MM_SYMBOL(adamw_fn, "mm_adamw")(table.data(), (int)count, bits, lr, beta1, beta2, eps, decay, 1,
-                                                     maximize, 1, nullptr, 0, t.stream);
+  const int status = unlocked(MM_SYMBOL(adamw_fn, "mm_adamw"), table.data(), (int)count, bits, lr, beta1, beta2, eps,
+                              decay, 1, maximize, 1, nullptr, 0, t.stream);
   return status == 0 ? py::object(py::bool_(true)) : py::object(py::int_(status));
 }
 
@@ -583,8 +596,8 @@ py::object adamw_values(py::handle p_, py::handle mc_, py::handle ms_, py::handl
   char* ptr = nullptr;
   py::object owner = new_storage(t, at + n, &ptr);
   if (!owner) return py::none();
-  const int status = MM_SYMBOL(decode_fn, "mm_adamw_decode")(mc.ptr, ms.ptr, vc.ptr, vs.ptr, n, ptr, ptr + 4 * at,
-                                                             t.stream);
+  const int status = unlocked(MM_SYMBOL(decode_fn, "mm_adamw_decode"), mc.ptr, ms.ptr, vc.ptr, vs.ptr, n, ptr,
+                              ptr + 4 * at, t.stream);
   if (status != 0) return py::int_(status);
   const py::tuple shape = int_tuple(p.t->sizes()), strides = int_tuple(p.t->strides());
   return py::make_tuple(new_tensor(t, owner, shape, strides, 0), new_tensor(t, owner, shape, strides, at));

@@ -169,3 +169,42 @@ def test_adamw(mm, monkeypatch, bits):
     p.grad = mm.to_device(torch.ones(4, 6)).t()
     opt.step()
     assert ((p.detach().cpu() + 1).abs() <= 2.0 ** -19).all()
+
+
+def test_other_threads_run_while_a_call_waits_for_the_queue(mm):
+    """More launches than the queue holds: the C++ call blocks, and without the interpreter's lock. (Threads are
+    not switched by time here, so another one runs only where this one lets go.)"""
+    import sys
+    import threading
+    from matrixman_b200.privateuse import native_calls
+    native = native_calls()
+    p = torch.nn.Parameter(mm.to_device(torch.zeros(1 << 24)))
+    p.grad = mm.to_device(torch.ones(1 << 24))
+    opt = mm.optim.AdamW([p], weight_decay=0.0)
+    opt.step()
+    params, states = [p], [opt.state[p]]
+    p.runtime.synchronize()
+    ticks, stop = [0], threading.Event()
+
+    def tick():
+        while not stop.is_set():
+            ticks[0] += 1
+            stop.wait(1e-4)
+
+    interval = sys.getswitchinterval()
+    t = threading.Thread(target=tick)
+    t.start()
+    while not ticks[0]:
+        stop.wait(1e-3)
+    sys.setswitchinterval(60)
+    try:
+        before = ticks[0]
+        for _ in range(1500):
+            native.adamw_step(params, states, 32, 1e-3, 0.9, 0.999, 1e-8, 0.0, False)
+        after = ticks[0]
+    finally:
+        sys.setswitchinterval(interval)
+        stop.set()
+        t.join()
+    assert after - before >= 10
+    assert float(opt.state[p]["step"].cpu()) == 1501.0
