@@ -393,18 +393,20 @@ py::object layer_norm(py::handle x_, int64_t width, py::handle w_, py::handle b_
   if (d < 1 || width < 1 || x.size(d - 1) != width || !is_vector(w, width) || !is_vector(b, width)) return py::none();
   const int64_t stride = row_stride(x, width);
   if (stride < 0 || !t.of(x) || !t.owns(w) || !t.owns(b)) return py::none();
-  const int64_t rows = x.t->numel() / width, at = (rows * width + 63) / 64 * 64;  // one block: y, mean, rstd
-  char* p = nullptr;
-  py::object owner = new_storage(t, at + 2 * rows, &p);
+  const int64_t rows = x.t->numel() / width;
+  // mean and rstd share a block, apart from y's: they are kept for the backward pass, y may go.
+  char *py_ = nullptr, *ps = nullptr;
+  py::object y = new_dense(t, x.t->sizes(), &py_);
+  if (!y) return py::none();
+  py::object owner = new_storage(t, 2 * rows, &ps);
   if (!owner) return py::none();
-  const int status = unlocked(MM_SYMBOL(norm_fn, "mm_layer_norm"), x.ptr, stride, rows, width, w.ptr, b.ptr, eps, p,
-                              p + 4 * at, p + 4 * (at + rows), t.stream);
+  const int status = unlocked(MM_SYMBOL(norm_fn, "mm_layer_norm"), x.ptr, stride, rows, width, w.ptr, b.ptr, eps, py_,
+                              ps, ps + 4 * rows, t.stream);
   if (status != 0) return py::int_(status);
   std::vector<int64_t> shape = x.t->sizes().vec();
-  py::object y = new_tensor(t, owner, int_tuple(shape), dense_strides(shape), 0);
   shape.back() = 1;
   py::tuple stat = int_tuple(shape), strides = dense_strides(shape);
-  return py::make_tuple(y, new_tensor(t, owner, stat, strides, at), new_tensor(t, owner, stat, strides, at + rows));
+  return py::make_tuple(y, new_tensor(t, owner, stat, strides, 0), new_tensor(t, owner, stat, strides, rows));
 }
 
 py::object layer_norm_backward(py::handle dy_, py::handle x_, int64_t width, py::handle mean_, py::handle rstd_,

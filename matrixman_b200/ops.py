@@ -649,14 +649,13 @@ def layer_norm(x, normalized_shape, weight=None, bias=None, eps=1e-5):
     xr, stride = _norm_rows(x, shape, width)
     stat = lead + (1,) * len(shape)
     strides = contiguous_strides(stat)
-    at = (rows * width + 63) // 64 * 64  # one block: y, mean, rstd
-    owner = rt.new_storage(at + 2 * rows)
-    y = MatrixManTensor._wrap(owner, full, 0, contiguous_strides(full))
-    mean = MatrixManTensor._wrap(owner, stat, at, strides)
-    rstd = MatrixManTensor._wrap(owner, stat, at + rows, strides)
-    p = owner.pointer
+    y = new_dense(rt, full)
+    # mean and rstd share a block, apart from y's: they are kept for the backward pass, y may go.
+    owner = rt.new_storage(2 * rows)
+    mean = MatrixManTensor._wrap(owner, stat, 0, strides)
+    rstd = MatrixManTensor._wrap(owner, stat, rows, strides)
     _launch("mm_layer_norm", pointer(xr), stride, rows, width, None if w is None else pointer(w),
-            None if b is None else pointer(b), eps, p, p + 4 * at, p + 4 * (at + rows), rt.stream)
+            None if b is None else pointer(b), eps, pointer(y), pointer(mean), pointer(rstd), rt.stream)
     return y, mean, rstd
 
 

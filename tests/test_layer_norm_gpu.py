@@ -223,3 +223,21 @@ def test_refusals(mm):
     with pytest.raises(RuntimeError):
         y = F.layer_norm(x.requires_grad_(True), (8,), w, None, EPS)
         torch.autograd.grad(y, w, x.detach())
+
+
+@pytest.mark.parametrize("native", [True, False])
+def test_the_backward_pass_keeps_the_statistics_but_not_the_output(mm, monkeypatch, native):
+    from matrixman_b200 import ops
+    if not native:
+        monkeypatch.setattr(ops, "native_call", lambda *a: None)
+    x = mm.to_device(torch.ones(4096, 512)).requires_grad_(True)
+    rt = x.runtime
+    live = lambda: rt.pool_stats()["live_bytes"]["activation"]
+    start = live()
+    y = F.layer_norm(x, (512,))
+    assert live() - start >= 4 * 4096 * 512
+    s = y.sum(dim=1)
+    del y
+    assert live() - start <= 3 * 4 * 4096 + 3 * 512  # mean, rstd, s
+    s.sum(dim=0).backward()
+    assert x.grad.shape == x.shape
