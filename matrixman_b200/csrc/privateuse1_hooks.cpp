@@ -585,14 +585,17 @@ py::object adamw_step(const py::list& params, const py::list& states, int bits, 
   return status == 0 ? py::object(py::bool_(true)) : py::object(py::int_(status));
 }
 
-// The float32 values of 8-bit states, of a parameter's shape and strides.
-py::object adamw_values(py::handle p_, py::handle mc_, py::handle ms_, py::handle vc_, py::handle vs_) {
-  Operand p, mc, ms, vc, vs;
+// The float32 values of 8-bit states, of a parameter's shape and strides (the step
+// is only looked at: the whole state has to fit).
+py::object adamw_values(py::handle p_, py::handle mc_, py::handle ms_, py::handle vc_, py::handle vs_,
+                        py::handle step_) {
+  Operand p, mc, ms, vc, vs, step;
   Target t;
   if (!names().ready || !operand(p_, &p) || !operand(mc_, &mc) || !operand(ms_, &ms) || !operand(vc_, &vc) ||
-      !operand(vs_, &vs) || !p.given || !mc.given || !ms.given || !vc.given || !vs.given ||
+      !operand(vs_, &vs) || !operand(step_, &step) || !p.given || !mc.given || !ms.given || !vc.given || !vs.given ||
+      !step.given || step.t->numel() != 1 ||
       !p.t->is_non_overlapping_and_dense() || !holds_codes(mc, ms, p) || !holds_codes(vc, vs, p) || !t.of(p) ||
-      !t.owns(mc) || !t.owns(ms) || !t.owns(vc) || !t.owns(vs))
+      !t.owns(mc) || !t.owns(ms) || !t.owns(vc) || !t.owns(vs) || !t.owns(step))
     return py::none();
   const int64_t n = p.t->numel(), at = (n + 63) / 64 * 64;  // both in one block
   char* ptr = nullptr;

@@ -218,12 +218,14 @@ class AdamW(torch.optim.Optimizer):
     def state_values(self, p) -> tuple[MatrixManTensor, MatrixManTensor]:
         """(exp_avg, exp_avg_sq) of a parameter as new float32 tensors (8-bit
         states: the values that the codes stand for)."""
-        state = self._check_state(p, self._state_of(p))
+        state = self._state_of(p)
+        if self.state_bits == 8:
+            done = ops.native_call("adamw_values", "mm_adamw_decode", p, *(state.get(k) for k in (*_CODES, "step")))
+            if done is not None:
+                return done
+        self._check_state(p, state)
         if self.state_bits == 32:
             return ops.clone(state["exp_avg"]), ops.clone(state["exp_avg_sq"])
-        done = ops.native_call("adamw_values", "mm_adamw_decode", p, *(state[k] for k in _CODES))
-        if done is not None:
-            return done
         rt, n, shape = p.runtime, numel(p.shape), tuple(p.shape)
         at = (n + 63) // 64 * 64  # both in one block
         owner = rt.new_storage(at + n)

@@ -1,4 +1,5 @@
-"""Autograd's worker threads are the program's own setting."""
+"""Autograd's worker threads: off around backward(), and by init only where the
+process sees a single GPU."""
 
 import threading
 
@@ -25,7 +26,6 @@ class Where(torch.autograd.Function):
 @pytest.mark.parametrize("on", [True, False])
 def test_the_setting_is_left_as_it_was(mm, on):
     with torch.autograd.set_multithreading_enabled(on):
-        mm.init()
         assert torch._C._is_multithreading_enabled() == on
         x = mm.to_device(torch.ones(4, 8)).requires_grad_(True)
         w = mm.to_device(torch.ones(6, 8)).requires_grad_(True)
@@ -41,7 +41,17 @@ def test_the_setting_is_left_as_it_was(mm, on):
         with pytest.raises(RuntimeError):
             y.backward(mm.to_device(torch.ones(4, 7)))
         assert torch._C._is_multithreading_enabled() == on
-    assert torch._C._is_multithreading_enabled()
+
+
+@pytest.mark.parametrize("devices", [1, 2, 8])
+def test_init_leaves_it_where_workers_could_run_side_by_side(mm, monkeypatch, devices):
+    from matrixman_b200 import api, runtime
+    monkeypatch.setattr(runtime, "device_count", lambda: devices)
+    for on in (True, False):
+        with torch.autograd.set_multithreading_enabled(on):
+            monkeypatch.setattr(api, "_backend", None)
+            mm.init()
+            assert torch._C._is_multithreading_enabled() == (on and devices > 1)
 
 
 def test_a_scalar_loss_and_another_thread(mm):
@@ -63,5 +73,5 @@ def test_a_scalar_loss_and_another_thread(mm):
     t = threading.Thread(target=work)
     t.start()
     t.join(60)
-    assert got == [(True, True)]
+    assert got == [(True, True)]  # (the setting is each thread's own)
     assert torch.equal(w.grad.cpu(), torch.full((6, 8), 8.0))
