@@ -588,12 +588,16 @@ static size_t lin_workspace(const LinRoute& r, int64_t m, int64_t n, int64_t k, 
   return ws.used;
 }
 
-static int lin_check(const char* who, int64_t m, int64_t n, int64_t k, int act, const void* workspace,
-                     size_t workspace_bytes, size_t need) {
-  const std::string name(who);
-  if (m < 0 || n < 0 || k < 0) return fail(MM_ERR_INVALID, name + ": negative size");
+// Before anything is computed from them.
+static int lin_check_sizes(const char* who, int64_t m, int64_t n, int64_t k) {
+  if (m < 0 || n < 0 || k < 0) return fail(MM_ERR_INVALID, std::string(who) + ": negative size");
   if (m > INT32_MAX / 2 || n > INT32_MAX / 2 || k > INT32_MAX / 2)
-    return fail(MM_ERR_UNSUPPORTED, name + ": dimension too large");
+    return fail(MM_ERR_UNSUPPORTED, std::string(who) + ": dimension too large");
+  return MM_OK;
+}
+
+static int lin_check(const char* who, int act, const void* workspace, size_t workspace_bytes, size_t need) {
+  const std::string name(who);
   if (act < MM_LINEAR_NONE || act > MM_LINEAR_GELU_TANH) return fail(MM_ERR_INVALID, name + ": unknown activation");
   if (workspace != nullptr && (workspace_bytes < need || (uintptr_t)workspace % 256 != 0))
     return fail(MM_ERR_INVALID, name + ": the workspace is misaligned or too small");
@@ -605,7 +609,8 @@ static int lin_check(const char* who, int64_t m, int64_t n, int64_t k, int act, 
 using namespace mm;
 
 extern "C" int mm_linear_workspace_size(int64_t m, int64_t n, int64_t k, int backward, size_t* bytes) {
-  if (bytes == nullptr || m < 0 || n < 0 || k < 0) return fail(MM_ERR_INVALID, "mm_linear_workspace_size: invalid argument");
+  if (bytes == nullptr) return fail(MM_ERR_INVALID, "mm_linear_workspace_size: null output");
+  if (const int rc = lin_check_sizes("mm_linear_workspace_size", m, n, k)) return rc;
   *bytes = lin_workspace(lin_route(m, n, k, backward != 0), m, n, k, backward != 0);
   return MM_OK;
 }
@@ -614,10 +619,11 @@ extern "C" int mm_linear(const float* x, int64_t xs0, int64_t xs1, const float* 
                          const float* bias, const float* residual, int64_t residual_stride, int64_t m, int64_t n,
                          int64_t k, int act, int residual_before_act, float* y, float* z, void* workspace,
                          size_t workspace_bytes, void* stream) {
+  int rc = lin_check_sizes("mm_linear", m, n, k);
+  if (rc != MM_OK) return rc;
   const LinRoute route = lin_route(m, n, k, false);
   const size_t need = lin_workspace(route, m, n, k, false);
-  int rc = lin_check("mm_linear", m, n, k, act, workspace, workspace_bytes, need);
-  if (rc != MM_OK) return rc;
+  if ((rc = lin_check("mm_linear", act, workspace, workspace_bytes, need)) != MM_OK) return rc;
   if (xs0 < 0 || xs1 < 0 || ws0 < 0 || ws1 < 0 || residual_stride < 0)
     return fail(MM_ERR_INVALID, "mm_linear: negative stride");
   if (m == 0 || n == 0) return MM_OK;
@@ -638,10 +644,11 @@ extern "C" int mm_linear_backward(const float* dy, int64_t dy_stride, const floa
                                   const float* w, int64_t ws0, int64_t ws1, const float* z, int64_t m, int64_t n,
                                   int64_t k, int act, float* dx, float* dw, float* db, float* dz, void* workspace,
                                   size_t workspace_bytes, void* stream) {
+  int rc = lin_check_sizes("mm_linear_backward", m, n, k);
+  if (rc != MM_OK) return rc;
   const LinRoute route = lin_route(m, n, k, true);
   const size_t need = lin_workspace(route, m, n, k, true);
-  int rc = lin_check("mm_linear_backward", m, n, k, act, workspace, workspace_bytes, need);
-  if (rc != MM_OK) return rc;
+  if ((rc = lin_check("mm_linear_backward", act, workspace, workspace_bytes, need)) != MM_OK) return rc;
   if (dy_stride < 0 || xs0 < 0 || xs1 < 0 || ws0 < 0 || ws1 < 0)
     return fail(MM_ERR_INVALID, "mm_linear_backward: negative stride");
   if (!dx && !dw && !db && !dz) return MM_OK;

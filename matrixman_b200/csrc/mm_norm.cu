@@ -484,6 +484,8 @@ extern "C" int mm_layer_norm(const float* x, int64_t x_stride, int64_t rows, int
 extern "C" int mm_layer_norm_backward_workspace_size(int64_t rows, int64_t width, size_t* bytes) {
   if (bytes == nullptr || rows < 0 || width < 0)
     return fail(MM_ERR_INVALID, "mm_layer_norm_backward_workspace_size: invalid argument");
+  if (width > INT32_MAX / 2 || rows > INT32_MAX)
+    return fail(MM_ERR_UNSUPPORTED, "mm_layer_norm_backward_workspace_size: too many rows or columns");
   *bytes = (size_t)(2 * ln_partial_rows(rows) * width) * sizeof(float);
   return MM_OK;
 }

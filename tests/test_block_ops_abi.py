@@ -149,3 +149,25 @@ def test_adamw_refuses_the_same_memory_twice():
         assert call([row(0), row(1, n=0, p=first["p"], m=first["m"], v=0)], bits) == "workspace"  # nothing to write
     assert call([row(i) for i in range(1000)]) == "workspace"
     assert call([row(i) for i in range(1000)] + [row(1000, m=row(3)[2])]) == "shares"
+
+
+def test_workspace_sizes_of_refused_dimensions():
+    """What the calls refuse has no size (products of such dimensions overflow)."""
+    lib = _lib.load()
+    for big in (1 << 31, 1 << 40, 1 << 62):
+        for sizes in ((big, 8, 8), (8, big, 8), (8, 8, big), (big, big, big)):
+            for back in (0, 1):
+                size = ctypes.c_size_t(77)
+                assert lib.mm_linear_workspace_size(*sizes, back, ctypes.byref(size)) == _lib.MM_ERR_UNSUPPORTED
+                assert size.value == 77
+            assert lib.mm_linear(FAKE, 8, 1, FAKE, 8, 1, None, None, 0, *sizes, 0, 0, FAKE, None, None, 0,
+                                 None) == _lib.MM_ERR_UNSUPPORTED
+            assert lib.mm_linear_backward(FAKE, 8, FAKE, 8, 1, FAKE, 8, 1, None, *sizes, 0, FAKE, FAKE, FAKE, None, None,
+                                          0, None) == _lib.MM_ERR_UNSUPPORTED
+        for sizes in ((big, 8), (8, big)):
+            size = ctypes.c_size_t(77)
+            assert lib.mm_layer_norm_backward_workspace_size(*sizes, ctypes.byref(size)) == _lib.MM_ERR_UNSUPPORTED
+            assert size.value == 77
+    size = ctypes.c_size_t(0)
+    assert lib.mm_linear_workspace_size(-1, 8, 8, 0, ctypes.byref(size)) == _lib.MM_ERR_INVALID
+    assert lib.mm_linear_workspace_size(4096, 4096, 4096, 1, ctypes.byref(size)) == _lib.MM_OK and size.value > 0
