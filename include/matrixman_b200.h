@@ -385,7 +385,9 @@ typedef enum mm_linear_act {
  * s1 between columns), bias [n] or NULL, residual [m, n] (dense rows
  * residual_stride apart) or NULL, y dense [m, n].  z (dense [m, n] or NULL)
  * receives the values that the activation is applied to, which the backward
- * pass needs.  float32 accuracy throughout.  workspace: device memory, 256-byte
+ * pass needs.  float32 accuracy for operands of at least 2^-110 (8e-34); where the
+ * call runs on the tensor cores smaller ones are held to within 2^-133.
+ * workspace: device memory, 256-byte
  * aligned, of mm_linear_workspace_size(m, n, k, 0) bytes, or NULL to take it from
  * the scratch pool.  Extends mm_gemm (which has no residual, GELU or gradient). */
 int mm_linear(const float* x, int64_t xs0, int64_t xs1, const float* w, int64_t ws0, int64_t ws1,

@@ -3,8 +3,9 @@
 //
 // A float32 value is the exact sum of three bf16 values: a1 = a rounded to
 // bf16, a2 = (a - a1) rounded to bf16, a3 = a - a1 - a2 (24 significant bits =
-// 3 x 8, and bf16 has float32's exponents, so nothing is scaled and no value of
-// the range is lost).  Of the nine products of pieces the six largest are
+// 3 x 8, and bf16 has float32's exponents, so nothing is scaled).  That holds from
+// 2^-110 (8e-34) on; bf16's smallest step is 2^-133, so a smaller value is kept to
+// within 2^-133 (products with values around 1e-36: 3e-5 relative).  Of the nine products of pieces the six largest are
 // formed, a1 b1, a1 b2, a2 b1, a2 b2, a1 b3, a3 b1; the other three are below
 // 2^-24 of the whole.  Six bf16 products instead of one bound the rate at a
 // sixth of the bf16 rate.

@@ -484,3 +484,15 @@ def test_relu_drops_non_finite_gradients_where_it_was_off(mm, m, n, k, mode):
     if res is not None:
         expect = dz if first else dy
         assert torch.equal(grads[3].nan_to_num(7.0, 8.0, 9.0), expect.nan_to_num(7.0, 8.0, 9.0))
+
+
+@pytest.mark.parametrize("m,n,k", [(10, 300, 260), (100, 64, 256), (2500, 1100, 70)])
+@pytest.mark.parametrize("exponent", [-100, -109, -116, -124, -140])
+def test_operands_near_the_smallest_numbers(mm, m, n, k, exponent):
+    """Three bf16 pieces hold a value exactly from 2^-110 on, a smaller one to within bf16's smallest step,
+    2^-133 (the last piece is cut off there)."""
+    x, w = torch.ldexp(randn(m, k, seed=1), torch.tensor(exponent)), torch.ldexp(randn(n, k, seed=2), torch.tensor(60))
+    z, ez, _ = products(x, w)
+    bound = ez + 2.0 ** -133 * w.double().abs().sum(1)
+    close("x", mm.linear(mm.to_device(x), mm.to_device(w)).cpu(), z, bound)
+    close("w", mm.linear(mm.to_device(w), mm.to_device(x)).cpu(), z.t(), bound.t())
