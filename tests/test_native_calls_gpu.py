@@ -208,3 +208,36 @@ def test_other_threads_run_while_a_call_waits_for_the_queue(mm):
         t.join()
     assert after - before >= 10
     assert float(opt.state[p]["step"].cpu()) == 1501.0
+
+
+def test_two_threads_at_once(mm):
+    """Calls of several overlapping kernels, queued on one stream by two threads in turns of their own making."""
+    import threading
+    work = []
+    for i, (m, n, k) in enumerate([(511, 1300, 2049), (2500, 1100, 70)]):
+        x, w = (mm.to_device(randn(*s, seed=10 * i + j)).requires_grad_(True) for j, s in enumerate(((m, k), (n, k))))
+        g, ln = mm.to_device(randn(m, n, seed=10 * i + 5)), mm.to_device(randn(n, seed=10 * i + 6)).requires_grad_(True)
+
+        def step(x=x, w=w, g=g, ln=ln, n=n):
+            y = F.layer_norm(mm.linear(x, w, activation="gelu"), (n,), ln)
+            return [y.detach(), *torch.autograd.grad(y, (x, w, ln), g)]
+
+        work.append((step, [t.cpu() for t in step()]))
+    bad = []
+
+    def run(step, want):
+        try:
+            with torch.autograd.set_multithreading_enabled(False):
+                for _ in range(40):
+                    got = step()
+                if not all(torch.equal(t.cpu(), v) for t, v in zip(got, want)):
+                    bad.append("other bits")
+        except Exception as e:  # for the assertion below
+            bad.append(e)
+
+    threads = [threading.Thread(target=run, args=w) for w in work]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(120)
+    assert not bad and not any(t.is_alive() for t in threads)
