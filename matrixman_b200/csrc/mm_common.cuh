@@ -34,8 +34,9 @@ int cuda_fail(cudaError_t err, const char* action);
 cudaStream_t resolve_stream(void* stream);
 
 // The device's fault word (mm_fault_word): page-locked host memory that kernels
-// may write, made by mm_init and never freed; null before that.
-int* fault_word(int device);
+// may write, made by mm_init or the first launch that needs it (`make`) and never
+// freed; null before that.
+int* fault_word(int device, bool make);
 
 // ---------------------------------------------------------------------------
 // Programmatic dependent launch (PDL).  A kernel launched with launch_pdl may

@@ -1791,7 +1791,7 @@ extern "C" int mm_kernel_error(int device, int* code_out, int clear) {
   }
   if (prev != device) cudaSetDevice(prev);
   if (e != cudaSuccess) return cuda_fail(e, "mm_kernel_error");
-  if (volatile int* word = fault_word(device)) {  // the linear operator's kernel
+  if (volatile int* word = fault_word(device, false)) {  // the linear operator's kernel
     if (code == 0) code = *word;
     if (clear) *word = 0;
   }

@@ -941,7 +941,8 @@ int lin_run_gemm(const LinPlanes& pa, const LinPlanes& pb, float* c, const LinEp
   g.early = early;
   int device = 0;
   cudaGetDevice(&device);
-  g.fault = fault_word(device);
+  g.fault = fault_word(device, true);
+  if (g.fault == nullptr) return fail(MM_ERR_OOM, "mm_linear: no page-locked memory for the fault word");
   const int64_t limit = device >= 0 && device < 64 ? g_lin_wait_ns[device].load() : 0;
   g.wait_ns = limit > 0 ? limit : LG_WAIT_NS;
   g.drop = device >= 0 && device < 64 ? g_lin_drop[device].load() : 0;

@@ -132,9 +132,25 @@ static DeviceRuntime* runtime_for(int device) {
   return g_rt[device];
 }
 
-static int* g_fault[64] = {nullptr};  // written under g_rt_mu, once per device
+static std::mutex g_fault_mu;
+static std::atomic<int*> g_fault[64];
 
-int* fault_word(int device) { return device >= 0 && device < 64 ? g_fault[device] : nullptr; }
+int* fault_word(int device, bool make) {
+  if (device < 0 || device >= 64) return nullptr;
+  int* word = g_fault[device].load();
+  if (word != nullptr || !make) return word;
+  std::lock_guard<std::mutex> g(g_fault_mu);
+  if (g_fault[device].load() == nullptr) {
+    void* p = nullptr;
+    if (cudaHostAlloc(&p, sizeof(int), cudaHostAllocPortable | cudaHostAllocMapped) != cudaSuccess) {
+      cudaGetLastError();
+      return nullptr;
+    }
+    *(int*)p = 0;
+    g_fault[device].store((int*)p);
+  }
+  return g_fault[device].load();
+}
 
 static int current_device() {
   int d = 0;
@@ -288,12 +304,7 @@ extern "C" int mm_init(int device) {
   if (prop.major != 10)
     return fail(MM_ERR_UNSUPPORTED, std::string("mm_init: ") + prop.name +
                                         " is not an sm_100 (B200) device; this build targets sm_100a only");
-  if (g_fault[device] == nullptr) {
-    void* word = nullptr;
-    MM_CUDA(cudaHostAlloc(&word, sizeof(int), cudaHostAllocPortable | cudaHostAllocMapped), "fault word");
-    *(int*)word = 0;
-    g_fault[device] = (int*)word;
-  }
+  if (fault_word(device, true) == nullptr) return fail(MM_ERR_OOM, "mm_init: no page-locked memory for the fault word");
   auto* rt = new DeviceRuntime();
   rt->device = device;
   rt->sm_count = prop.multiProcessorCount;
@@ -338,7 +349,7 @@ extern "C" int mm_get_device(int* out) {
 
 extern "C" int mm_fault_word(int device, int** word_out) {
   if (word_out == nullptr) return fail(MM_ERR_INVALID, "mm_fault_word: null output");
-  *word_out = fault_word(device);
+  *word_out = fault_word(device, false);
   return *word_out ? MM_OK : fail(MM_ERR_STATE, "mm_fault_word: device not initialised");
 }
 

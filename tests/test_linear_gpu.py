@@ -496,3 +496,40 @@ def test_operands_near_the_smallest_numbers(mm, m, n, k, exponent):
     bound = ez + 2.0 ** -133 * w.double().abs().sum(1)
     close("x", mm.linear(mm.to_device(x), mm.to_device(w)).cpu(), z, bound)
     close("w", mm.linear(mm.to_device(w), mm.to_device(x)).cpu(), z.t(), bound.t())
+
+
+def test_fault_is_recorded_without_a_runtime():
+    """A C caller with streams and workspaces of its own need not call mm_init: a wait that gives up is recorded for
+    it all the same (in a process of its own, on torch's memory)."""
+    import subprocess
+    import sys
+    from .conftest import ROOT
+    code = """
+import ctypes, torch
+from matrixman_b200 import _lib
+lib = _lib.load()
+m, n, k = 2500, 1100, 70
+x, w, y = (torch.ones(s, device="cuda") for s in ((m, k), (n, k), (m, n)))
+size, code, word = ctypes.c_size_t(), ctypes.c_int(-1), ctypes.c_void_p()
+assert lib.mm_fault_word(0, ctypes.byref(word)) == _lib.MM_ERR_STATE
+assert lib.mm_linear_workspace_size(m, n, k, 0, ctypes.byref(size)) == 0
+work = torch.empty(size.value, dtype=torch.uint8, device="cuda")
+def call():
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    assert lib.mm_linear(x.data_ptr(), k, 1, w.data_ptr(), k, 1, None, None, 0, m, n, k, 0, 0, y.data_ptr(), None,
+                         work.data_ptr(), size.value, s.cuda_stream) == 0, _lib.last_error()
+    torch.cuda.synchronize()
+    assert lib.mm_kernel_error(0, ctypes.byref(code), 1) == 0
+    return code.value
+assert call() == 0 and torch.equal(y, torch.full_like(y, 70.0))
+assert lib.mm_debug_tc_fault(0, 1_000_000, 1) == 0
+got = call()
+assert lib.mm_debug_tc_fault(0, 0, 0) == 0
+assert 101 <= got <= 105, got
+y.zero_()
+assert call() == 0 and torch.equal(y, torch.full_like(y, 70.0))
+print("recorded", got)
+"""
+    run = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True, timeout=120)
+    assert run.returncode == 0 and "recorded" in run.stdout, run.stderr[-2000:]
