@@ -408,6 +408,33 @@ int mm_linear_backward(const float* dy, int64_t dy_stride, const float* x, int64
                        size_t workspace_bytes, void* stream);
 int mm_linear_workspace_size(int64_t m, int64_t n, int64_t k, int backward, size_t* bytes);
 
+/* Group norm and activation (mm_linear_act) of feature maps [n, channels, pixels],
+ * pixels of any spatial rank: y = act((x - mean) * rstd * weight + bias), mean and
+ * var over each image's pixels and channels of one group, rstd = 1 / sqrt(var + eps).
+ * channels_last: pixel s of image i holds its channels densely at
+ * x + i * x_image + s * x_row, and y is dense [n, pixels, channels]; otherwise
+ * channel c holds its pixels densely at x + i * x_image + c * x_row, and y is dense
+ * [n, channels, pixels].  weight and bias [channels] may be NULL.  mean and rstd
+ * [n, groups] are kept for the backward pass.  workspace: device memory, 16-byte
+ * aligned, of mm_group_norm_workspace_size bytes, or NULL to take it from the scratch
+ * pool.  No counterpart in the reference, whose only normalisation is eval BatchNorm. */
+int mm_group_norm(const float* x, int64_t x_image, int64_t x_row, int64_t n, int64_t channels, int64_t pixels,
+                  int64_t groups, int channels_last, const float* weight, const float* bias, double eps, int act,
+                  float* y, float* mean, float* rstd, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Gradients of mm_group_norm from dy (laid out as x, at its own distances): with
+ * xh = (x - mean) * rstd, dz = dy * act'(xh * weight + bias) and g = dz * weight,
+ * dx = rstd * (g - mean(g) - xh * mean(g * xh)), dweight = sum of dz * xh and
+ * dbias = sum of dz over images and pixels.  dx (dense, in y's order), dweight and
+ * dbias may be NULL.  Workspace as for the forward pass.  The sums are added in a
+ * fixed order: equal inputs give equal bits. */
+int mm_group_norm_backward(const float* dy, int64_t dy_image, int64_t dy_row, const float* x, int64_t x_image,
+                           int64_t x_row, int64_t n, int64_t channels, int64_t pixels, int64_t groups,
+                           int channels_last, const float* mean, const float* rstd, const float* weight,
+                           const float* bias, int act, float* dx, float* dweight, float* dbias, void* workspace,
+                           size_t workspace_bytes, void* stream);
+int mm_group_norm_workspace_size(int64_t n, int64_t channels, int64_t pixels, int64_t groups, size_t* bytes);
+
 /* One tensor of an optimiser step, numel consecutive float32 elements.  With
  * 32-bit states exp_avg and exp_avg_sq point to float32 and the scales are
  * NULL; with 8-bit states they point to one code byte per element (8-byte

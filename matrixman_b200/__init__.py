@@ -37,6 +37,7 @@ from .detect import postprocess_detections
 from .frames import preprocess_frames
 from . import optim
 from .fused_linear import linear
+from .fused_norm import group_norm
 from .preparation import auto_prepare, prepare, prepare_cuda, prepare_opengl
 from .tensor import Gm45Tensor, MatrixManTensor, install_tensor_method, is_matrixman_tensor
 
@@ -101,6 +102,7 @@ class _MatrixManModule(types.ModuleType):
 sys.modules[__name__].__class__ = _MatrixManModule
 
 __all__ = [
+    "group_norm",
     "infer",
     "infer_stream",
     "linear",

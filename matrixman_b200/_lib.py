@@ -211,6 +211,10 @@ SIGNATURES = {
     "mm_linear_backward": [_fp, _i64, _fp, _i64, _i64, _fp, _i64, _i64, _fp, _i64, _i64, _i64, _i, _fp, _fp, _fp,
                            _fp, _vp, _sz, _vp],
     "mm_linear_workspace_size": [_i64, _i64, _i64, _i, ctypes.POINTER(_sz)],
+    "mm_group_norm": [_fp, _i64, _i64, _i64, _i64, _i64, _i64, _i, _fp, _fp, _d, _i, _fp, _fp, _fp, _vp, _sz, _vp],
+    "mm_group_norm_backward": [_fp, _i64, _i64, _fp, _i64, _i64, _i64, _i64, _i64, _i64, _i, _fp, _fp, _fp, _fp, _i,
+                               _fp, _fp, _fp, _vp, _sz, _vp],
+    "mm_group_norm_workspace_size": [_i64, _i64, _i64, _i64, ctypes.POINTER(_sz)],
     "mm_adamw": [_vp, _i, _i, _d, _d, _d, _d, _d, _i, _i, _i, _vp, _sz, _vp],
     "mm_adamw_workspace_size": [_i, ctypes.POINTER(_sz)],
     "mm_adamw_encode": [_fp, _fp, _i64, _vp, _fp, _vp, _fp, _vp],

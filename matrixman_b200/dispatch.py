@@ -595,6 +595,16 @@ def _native_layer_norm_backward(grad_out, x, normalized_shape, mean, rstd, weigh
     return ops.layer_norm_backward(grad_out, x, normalized_shape, mean, rstd, weight, bias, output_mask)
 
 
+@_register(aten.native_group_norm.default)
+def _native_group_norm(x, weight, bias, N, C, HxW, group, eps):
+    return ops.group_norm(x, group, weight, bias, eps)
+
+
+@_register(aten.native_group_norm_backward.default)
+def _native_group_norm_backward(grad_out, x, mean, rstd, weight, N, C, HxW, group, output_mask):
+    return ops.group_norm_backward(grad_out, x, mean, rstd, weight, None, group, output_mask)
+
+
 # -- torch.optim.AdamW / Adam with fused=True ---------------------------------
 
 @_register(aten._foreach_add_.Scalar)

@@ -1,0 +1,57 @@
+"""``matrixman.group_norm``: group norm with the activation that follows it, in one
+call, with gradients.
+
+The reference normalises with eval BatchNorm only (backends/cuda/batch_norm.py)
+and runs the activation as an operator of its own.  Here one native call reads
+the feature maps and writes ``act(group_norm(x))`` in their memory order, and its
+backward pass computes the gradients of the maps and both parameters.
+"""
+
+from __future__ import annotations
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib, ops
+from .tensor import MatrixManTensor
+
+
+class _GroupNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, groups, eps, act):
+        y, mean, rstd = ops.group_norm(x, groups, weight, bias, eps, act)
+        ctx.groups, ctx.act = groups, act
+        ctx.save_for_backward(x, weight, bias, mean, rstd)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, weight, bias, mean, rstd = ctx.saved_tensors
+        mask = ctx.needs_input_grad[:3]
+        return (*ops.group_norm_backward(dy, x, mean, rstd, weight, bias, ctx.groups, mask, ctx.act), None, None, None)
+
+
+def group_norm(x, num_groups: int, weight=None, bias=None, eps: float = 1e-5, *,
+               activation: str | None = None) -> MatrixManTensor:
+    """``act(torch.nn.functional.group_norm(x, num_groups, weight, bias, eps))`` in one
+    native call.
+
+    x ``[N, C, *]`` with any number of spatial dimensions, channels last in memory
+    (the order of prepared models; read and written once) or first; other strides
+    are copied to channels last.  The result has x's order.  activation: None /
+    "none", "relu", "silu", "sigmoid", "gelu" or "gelu_tanh".  Differentiable once
+    in x, weight and bias.  float32 throughout; weight and bias may be CPU tensors
+    (uploaded once, as for the other operators) when they need no gradient."""
+    act = _lib.LINEAR_ACTS.get(activation) if activation is not None else 0
+    if act is None:
+        raise ValueError(f"MatrixMan/CUDA: group_norm activation must be one of {sorted(_lib.LINEAR_ACTS)}, "
+                         f"got {activation!r}")
+    ops.require_mm(x, "group_norm")
+    if torch.is_grad_enabled():
+        for name, t in (("weight", weight), ("bias", bias)):
+            if isinstance(t, torch.Tensor) and t.requires_grad and not isinstance(t, MatrixManTensor):
+                raise RuntimeError(f"MatrixMan/CUDA: group_norm {name} needs a gradient and must be a MatrixMan tensor")
+        if x.requires_grad or any(t is not None and t.requires_grad for t in (weight, bias)):
+            return _GroupNorm.apply(x, weight, bias, int(num_groups), float(eps), act)
+    return ops.group_norm(x, num_groups, weight, bias, float(eps), act)[0]

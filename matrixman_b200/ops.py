@@ -698,6 +698,117 @@ def layer_norm_backward(dy, x, normalized_shape, mean, rstd, weight, bias, mask)
     return dx, dw, db
 
 
+def _map_rows(x: MatrixManTensor) -> tuple[MatrixManTensor, bool, int, int]:
+    """Feature maps [N, C, *spatial] as the group-norm kernels read them: a tensor,
+    whether its channels are the dense dimension (else its pixels are), and the
+    distances of images and of pixels (or channels).  Copied, to channels last, only
+    where the strides force it."""
+    shape, st = tuple(x.shape), x._logical_strides
+    channels, pixels = shape[1], numel(shape[2:])
+    flat = view_strides(shape[2:], st[2:], (pixels,)) if len(shape) > 2 else (channels,)
+    if numel(shape) == 0:
+        return x, True, 0, 0
+    if flat is not None:
+        if pixels > 1 and flat[0] == 1 and (channels == 1 or st[1] != 1):
+            return x, False, st[0], st[1]
+        if channels == 1 or st[1] == 1:
+            return x, True, st[0], flat[0]
+    return materialize(x, _map_strides(shape, True)), True, channels * pixels, channels
+
+
+def _map_strides(shape: tuple, last: bool) -> tuple[int, ...]:
+    """Strides of dense feature maps, channels last or first."""
+    if not last:
+        return contiguous_strides(shape)
+    c = max(shape[1], 1)
+    spatial = contiguous_strides(shape[2:])
+    return (c * max(numel(shape[2:]), 1), 1, *(s * c for s in spatial))
+
+
+def _map_like(rt, shape: tuple, last: bool, like: tuple) -> MatrixManTensor:
+    """New dense feature maps in one of the two orders, with the strides `like`
+    where these say the same (dimensions of size one may have any)."""
+    strides = _map_strides(shape, last)
+    if all(n == 1 or a == b for n, a, b in zip(shape, strides, like)):
+        strides = like
+    return MatrixManTensor._wrap(rt.new_storage(numel(shape)), shape, 0, strides)
+
+
+def _group_vector(rt, value, channels: int, name: str) -> MatrixManTensor | None:
+    if value is None:
+        return None
+    t = device_operand(rt, value, f"GroupNorm {name}")
+    require_f32(t, f"GroupNorm {name}")
+    if tuple(t.shape) != (channels,):
+        raise RuntimeError(f"MatrixMan/CUDA: GroupNorm {name} must be [{channels}], got {tuple(t.shape)}")
+    return t if channels <= 1 or t._logical_strides[0] == 1 else materialize(t)
+
+
+def _group_check(x, groups: int) -> tuple[int, ...]:
+    require_f32(require_mm(x, "GroupNorm"), "GroupNorm")
+    shape = tuple(x.shape)
+    if len(shape) < 2:
+        raise RuntimeError("MatrixMan/CUDA: GroupNorm input must be [N, C, *]")
+    if groups < 1 or shape[1] % groups:
+        raise RuntimeError(f"MatrixMan/CUDA: GroupNorm cannot divide {shape[1]} channels into {groups} groups")
+    if numel(shape[1:]) == 0:
+        raise NotImplementedError("MatrixMan/CUDA: GroupNorm of images without channels or pixels is not implemented")
+    return shape
+
+
+def group_norm(x, groups: int, weight=None, bias=None, eps=1e-5, act: int = 0):
+    """(y, mean, rstd): act(group norm), in x's memory order, and the statistics
+    [N, groups]."""
+    groups = int(groups)
+    shape = _group_check(x, groups)
+    rt = x.runtime
+    w = _group_vector(rt, weight, shape[1], "weight")
+    b = _group_vector(rt, bias, shape[1], "bias")
+    xr, last, image, row = _map_rows(x)
+    n, c, pixels = shape[0], shape[1], numel(shape[2:])
+    y = _map_like(rt, shape, last, x._logical_strides)
+    owner = rt.new_storage(2 * n * groups)  # mean and rstd are kept for the backward pass, y may go
+    mean, rstd = (MatrixManTensor._wrap(owner, (n, groups), i * n * groups, (groups, 1)) for i in (0, 1))
+    _launch("mm_group_norm", pointer(xr), image, row, n, c, pixels, groups, last, None if w is None else pointer(w),
+            None if b is None else pointer(b), eps, act, pointer(y), pointer(mean), pointer(rstd), None, 0, rt.stream)
+    return y, mean, rstd
+
+
+def group_norm_backward(dy, x, mean, rstd, weight, bias, groups: int, mask, act: int = 0):
+    """(dx, dweight, dbias) of group_norm; None where the mask is false.  bias is
+    only read with an activation."""
+    groups = int(groups)
+    shape = _group_check(x, groups)
+    for t in (dy, mean, rstd):
+        require_f32(require_mm(t, "GroupNorm backward"), "GroupNorm backward")
+    if tuple(dy.shape) != shape:
+        raise RuntimeError("MatrixMan/CUDA: GroupNorm backward needs equal shapes of gradient and input")
+    rt = _runtime_of(dy, x, mean, rstd)
+    n, c, pixels = shape[0], shape[1], numel(shape[2:])
+    if numel(mean.shape) != n * groups or numel(rstd.shape) != n * groups:
+        raise RuntimeError("MatrixMan/CUDA: GroupNorm backward statistics do not match the input's groups")
+    mean, rstd = (t if is_contiguous(t.shape, t._logical_strides) else materialize(t) for t in (mean, rstd))
+    need_x, need_w, need_b = mask
+    w = _group_vector(rt, weight, c, "weight")
+    b = _group_vector(rt, bias, c, "bias") if act else None
+    xr, last, xi, xs = _map_rows(x)
+    gr, glast, gi, gs = _map_rows(dy)
+    if glast != last:
+        gr = materialize(dy, _map_strides(shape, last))
+        gi, gs = c * pixels, c if last else pixels
+    dx = _map_like(rt, shape, last, x._logical_strides) if need_x else None
+    dw = db = None
+    if need_w or need_b:
+        each = (c + 63) // 64 * 64  # both start at a 256-byte boundary of one block
+        owner = rt.new_storage(2 * each)
+        dw = MatrixManTensor._wrap(owner, (c,), 0, (1,)) if need_w else None
+        db = MatrixManTensor._wrap(owner, (c,), each, (1,)) if need_b else None
+    _launch("mm_group_norm_backward", pointer(gr), gi, gs, pointer(xr), xi, xs, n, c, pixels, groups, last,
+            pointer(mean), pointer(rstd), None if w is None else pointer(w), None if b is None else pointer(b), act,
+            *(None if t is None else pointer(t) for t in (dx, dw, db)), None, 0, rt.stream)
+    return dx, dw, db
+
+
 def softmax(x, dim, log=False) -> MatrixManTensor:
     x = require_mm(x, "softmax")
     require_f32(x, "softmax")
