@@ -435,6 +435,32 @@ int mm_group_norm_backward(const float* dy, int64_t dy_image, int64_t dy_row, co
                            size_t workspace_bytes, void* stream);
 int mm_group_norm_workspace_size(int64_t n, int64_t channels, int64_t pixels, int64_t groups, size_t* bytes);
 
+/* One tensor whose norm is taken: numel consecutive float32 elements. */
+typedef struct mm_grad {
+  float* data;
+  int64_t numel;
+} mm_grad_t;
+
+typedef enum mm_norm_order {
+  MM_NORM_INF = 0, /* largest magnitude */
+  MM_NORM_1 = 1,
+  MM_NORM_2 = 2
+} mm_norm_order_t;
+
+/* The norm of all elements of `count` tensors together into *norm (device memory;
+ * 0 for no elements), summed in 64 bits in a fixed order, and, unless coef is NULL,
+ * min(1, max_norm / (norm + 1e-6)) into *coef (NaN for a NaN norm).  workspace: device
+ * memory, 8-byte aligned, of mm_grad_norm_workspace_size(count) bytes, or NULL to take
+ * it from the scratch pool.  No counterpart in the reference. */
+int mm_grad_norm(const mm_grad_t* grads, int count, int order, double max_norm, float* norm, float* coef,
+                 void* workspace, size_t workspace_bytes, void* stream);
+
+/* The same, and every element multiplied by that coefficient in place.  Tensors that
+ * overlap are refused.  Workspace as for mm_grad_norm. */
+int mm_grad_clip(const mm_grad_t* grads, int count, int order, double max_norm, float* norm, void* workspace,
+                 size_t workspace_bytes, void* stream);
+int mm_grad_norm_workspace_size(int count, size_t* bytes);
+
 /* One tensor of an optimiser step, numel consecutive float32 elements.  With
  * 32-bit states exp_avg and exp_avg_sq point to float32 and the scales are
  * NULL; with 8-bit states they point to one code byte per element (8-byte
@@ -468,6 +494,12 @@ int mm_adamw(const mm_adamw_tensor_t* tensors, int count, int state_bits, double
              double eps, double weight_decay, int decoupled, int maximize, int advance, void* workspace,
              size_t workspace_bytes, void* stream);
 int mm_adamw_workspace_size(int count, size_t* bytes);
+
+/* The same with every gradient multiplied by *grad_scale (device memory, or NULL for
+ * mm_adamw itself) as it is read, before anything else; the gradients stay as they are. */
+int mm_adamw_scaled(const mm_adamw_tensor_t* tensors, int count, int state_bits, double lr, double beta1, double beta2,
+                    double eps, double weight_decay, int decoupled, int maximize, int advance,
+                    const float* grad_scale, void* workspace, size_t workspace_bytes, void* stream);
 
 /* 8-bit states of numel dense float32 moments, and the values that 8-bit states
  * stand for (decoding what was encoded and encoding it again gives the same

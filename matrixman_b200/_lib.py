@@ -35,6 +35,7 @@ ACT_NONE, ACT_RELU, ACT_SILU, ACT_SIGMOID = 0, 1, 2, 3
 (UNARY_COPY, UNARY_SILU, UNARY_RELU, UNARY_SIGMOID, UNARY_ADD_SCALAR, UNARY_MUL_SCALAR,
  UNARY_DIV_SCALAR, UNARY_NEG, UNARY_CLAMP) = range(9)
 BINARY_ADD, BINARY_SUB, BINARY_MUL, BINARY_DIV = range(4)
+NORM_ORDERS = {float("inf"): 0, 1.0: 1, 2.0: 2}
 LINEAR_ACTS = {"none": 0, "relu": 1, "silu": 2, "sigmoid": 3, "gelu": 4, "gelu_tanh": 5}
 PW3_THRESHOLD_BACKWARD, PW3_ADDCMUL, PW3_ADDCDIV, PW3_LERP, PW3_SQRT = range(5)
 
@@ -215,7 +216,11 @@ SIGNATURES = {
     "mm_group_norm_backward": [_fp, _i64, _i64, _fp, _i64, _i64, _i64, _i64, _i64, _i64, _i, _fp, _fp, _fp, _fp, _i,
                                _fp, _fp, _fp, _vp, _sz, _vp],
     "mm_group_norm_workspace_size": [_i64, _i64, _i64, _i64, ctypes.POINTER(_sz)],
+    "mm_grad_norm": [_vp, _i, _i, _d, _fp, _fp, _vp, _sz, _vp],
+    "mm_grad_clip": [_vp, _i, _i, _d, _fp, _vp, _sz, _vp],
+    "mm_grad_norm_workspace_size": [_i, ctypes.POINTER(_sz)],
     "mm_adamw": [_vp, _i, _i, _d, _d, _d, _d, _d, _i, _i, _i, _vp, _sz, _vp],
+    "mm_adamw_scaled": [_vp, _i, _i, _d, _d, _d, _d, _d, _i, _i, _i, _fp, _vp, _sz, _vp],
     "mm_adamw_workspace_size": [_i, ctypes.POINTER(_sz)],
     "mm_adamw_encode": [_fp, _fp, _i64, _vp, _fp, _vp, _fp, _vp],
     "mm_adamw_decode": [_vp, _fp, _vp, _fp, _i64, _fp, _fp, _vp],

@@ -70,6 +70,7 @@ struct AwSteps {
 struct AwScalars {
   float b1, omb1, b2, omb2, eps, decay, l2;  // decay = 1 - lr wd (decoupled); l2 = wd (coupled) or 0
   int maximize;
+  const float* scale;  // what gradients are multiplied by first, or null
 };
 
 // A step's own factors of each tensor: lr / (1 - b1^t) and 1 / sqrt(1 - b2^t).
@@ -130,9 +131,15 @@ __device__ __forceinline__ float aw_update(float p, float m, float r, float2 coe
   return __fsub_rn(__fmul_rn(p, a.decay), __fmul_rn(__fdiv_rn(m, d), coef.x));
 }
 
-// The gradients of N elements: negated to maximise, with coupled weight decay.
+// The gradients of N elements: scaled (rounded, as scaling them in place would),
+// negated to maximise, with coupled weight decay.
 template <int N>
 __device__ __forceinline__ void aw_grads(float* g, const float* p, const AwScalars& a) {
+  if (a.scale) {
+    const float c = *a.scale;
+#pragma unroll
+    for (int e = 0; e < N; ++e) g[e] = __fmul_rn(g[e], c);
+  }
   if (a.maximize) {
 #pragma unroll
     for (int e = 0; e < N; ++e) g[e] = -g[e];
@@ -420,6 +427,14 @@ extern "C" int mm_adamw_workspace_size(int count, size_t* bytes) {
 extern "C" int mm_adamw(const mm_adamw_tensor_t* tensors, int count, int state_bits, double lr, double beta1,
                         double beta2, double eps, double weight_decay, int decoupled, int maximize, int advance,
                         void* workspace, size_t workspace_bytes, void* stream) {
+  return mm_adamw_scaled(tensors, count, state_bits, lr, beta1, beta2, eps, weight_decay, decoupled, maximize, advance,
+                         nullptr, workspace, workspace_bytes, stream);
+}
+
+extern "C" int mm_adamw_scaled(const mm_adamw_tensor_t* tensors, int count, int state_bits, double lr, double beta1,
+                               double beta2, double eps, double weight_decay, int decoupled, int maximize,
+                               int advance, const float* grad_scale, void* workspace, size_t workspace_bytes,
+                               void* stream) {
   if (count < 0 || (count > 0 && tensors == nullptr)) return fail(MM_ERR_INVALID, "mm_adamw: invalid tensor list");
   if (state_bits != 32 && state_bits != 8) return fail(MM_ERR_UNSUPPORTED, "mm_adamw: states are held in 32 or 8 bits");
   if (!(beta1 >= 0 && beta1 < 1 && beta2 >= 0 && beta2 < 1))
@@ -446,6 +461,7 @@ extern "C" int mm_adamw(const mm_adamw_tensor_t* tensors, int count, int state_b
   a.decay = decoupled ? (float)(1.0 - lr * weight_decay) : 1.f;
   a.l2 = decoupled ? 0.f : (float)weight_decay;
   a.maximize = maximize != 0;
+  a.scale = grad_scale;
   cudaStream_t s = resolve_stream(stream);
   Scratch scratch;
   if (workspace == nullptr) {

@@ -247,7 +247,7 @@ struct Operand {
   bool given = false;
   const at::Tensor* t = nullptr;
   PyObject* owner = nullptr;  // borrowed: the tensor holds it
-  char* ptr = nullptr;
+  char* ptr = nullptr;  // stays null where nothing is given
   int64_t size(int i) const { return t->size(i); }
   int64_t dim() const { return t->dim(); }
 };
@@ -524,8 +524,8 @@ py::object linear_backward(py::handle dy_, py::handle x_, py::handle w_, py::han
   return py::make_tuple(dx, dw, db, dz);
 }
 
-using adamw_fn = int (*)(const void*, int, int, double, double, double, double, double, int, int, int, void*, size_t,
-                         void*);
+using adamw_fn = int (*)(const void*, int, int, double, double, double, double, double, int, int, int, const void*,
+                         void*, size_t, void*);
 using decode_fn = int (*)(const void*, const void*, const void*, const void*, int64_t, void*, void*, void*);
 
 // Whether 8-bit codes (four to a float) and their scales are those of p's elements.
@@ -536,10 +536,11 @@ bool holds_codes(const Operand& codes, const Operand& scales, const Operand& p) 
 }
 
 // An optimiser step over parameters with gradients and the states of
-// optim.AdamW (dicts): the table of addresses and the native call.  True, an
-// int (its status), or None where a tensor is not as usual.
+// optim.AdamW (dicts): the table of addresses and the native call.  scale: what
+// gradients are multiplied by, or None.  True, an int (its status), or None where
+// a tensor is not as usual.
 py::object adamw_step(const py::list& params, const py::list& states, int bits, double lr, double beta1, double beta2,
-                      double eps, double decay, bool maximize) {
+                      double eps, double decay, bool maximize, const py::handle& scale_) {
   static const py::object& grad_name = *new py::object(name("grad"));
   static const py::object& step_name = *new py::object(name("step"));
   static const py::object* const wide = new py::object[2]{name("exp_avg"), name("exp_avg_sq")};
@@ -551,6 +552,8 @@ py::object adamw_step(const py::list& params, const py::list& states, int bits, 
   std::vector<py::object> held;  // the lists and dicts are the program's: it may change them during the call
   held.reserve(8 * count);
   Target t;
+  Operand scale;
+  if (!operand(scale_, &scale)) return py::none();
   auto state_of = [&](const py::handle& state, const py::object& name, Operand* out) {
     PyObject* v = PyDict_GetItemWithError(state.ptr(), name.ptr());
     if (v == nullptr) return false;
@@ -580,8 +583,9 @@ py::object adamw_step(const py::list& params, const py::list& states, int bits, 
     for (int j = 0; j < 7; ++j) table[8 * i + j] = (int64_t)(intptr_t)order[j]->ptr;
     table[8 * i + 7] = p.t->numel();
   }
-  const int status = unlocked(MM_SYMBOL(adamw_fn, "mm_adamw"), table.data(), (int)count, bits, lr, beta1, beta2, eps,
-                              decay, 1, maximize, 1, nullptr, 0, t.stream);
+  if (!t.owns(scale) || (scale.given && scale.t->numel() != 1)) return py::none();
+  const int status = unlocked(MM_SYMBOL(adamw_fn, "mm_adamw_scaled"), table.data(), (int)count, bits, lr, beta1,
+                              beta2, eps, decay, 1, maximize, 1, scale.ptr, nullptr, 0, t.stream);
   return status == 0 ? py::object(py::bool_(true)) : py::object(py::int_(status));
 }
 
@@ -620,7 +624,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("layer_norm_backward", &layer_norm_backward, "mm_layer_norm_backward with its outputs, or None");
   m.def("linear", &linear, "mm_linear with its outputs, or None");
   m.def("linear_ready", &linear_ready, "Whether linear would take these operands");
-  m.def("adamw_step", &adamw_step, "mm_adamw over parameters and their states, or None");
+  m.def("adamw_step", &adamw_step, "mm_adamw over parameters and their states, or None", py::arg("params"),
+        py::arg("states"), py::arg("bits"), py::arg("lr"), py::arg("beta1"), py::arg("beta2"), py::arg("eps"),
+        py::arg("decay"), py::arg("maximize"), py::arg("scale") = py::none());
   m.def("adamw_values", &adamw_values, "mm_adamw_decode with its outputs, or None");
   m.def("linear_backward", &linear_backward, "mm_linear_backward with its outputs, or None");
 }

@@ -1,9 +1,11 @@
 """AdamW whose step runs over all tensors in one native call, with the moments
-held in 32 or in 8 bits.
+held in 32 or in 8 bits, and the norm of all gradients together, clipping by it in
+place or inside the step.
 
 The reference steps Adam through element-wise operators, tensor by tensor
-(backends/opengl/dispatch.py:171-179 lerp_, :264-290 addcmul_ / addcdiv_); here
-``mm_adamw`` walks every parameter of a group in one pass.
+(backends/opengl/dispatch.py:171-179 lerp_, :264-290 addcmul_ / addcdiv_) and has
+no norm of several tensors; here ``mm_adamw`` walks every parameter of a group in
+one pass, and ``mm_grad_norm`` / ``mm_grad_clip`` every gradient.
 """
 
 from __future__ import annotations
@@ -41,16 +43,121 @@ def _in_order(t: MatrixManTensor, like: MatrixManTensor) -> MatrixManTensor:
     return t if _same_order(t, like) else ops.materialize(t, like._logical_strides)
 
 
+# ---------------------------------------------------------------------------
+# The norm of all gradients together
+# ---------------------------------------------------------------------------
+
+def _norm_order(norm_type) -> int:
+    order = _lib.NORM_ORDERS.get(float(norm_type))
+    if order is None:
+        raise NotImplementedError(f"MatrixMan/CUDA: the gradient norm's order must be 1, 2 or inf, got {norm_type}")
+    return order
+
+
+def _grads_of(parameters) -> list:
+    """The gradients of an iterable of parameters, or of one; those without are left out."""
+    if isinstance(parameters, torch.Tensor):
+        parameters = [parameters]
+    return [p.grad for p in parameters if p.grad is not None]
+
+
+def _grad_runtime(grads: list):
+    rt = None
+    for g in grads:
+        ops.require_f32(ops.require_mm(g, "gradient norm"), "gradient norm")
+        if rt is None:
+            rt = g.runtime
+        elif g.runtime is not rt:
+            raise RuntimeError("MatrixMan/CUDA: the gradient norm needs gradients of one matrixman device")
+    return ops.get_runtime() if rt is None else rt
+
+
+def _is_apart(t: MatrixManTensor) -> bool:
+    """Whether no two elements share memory (by strides in order; a few that do not
+    overlap all the same are not recognised)."""
+    reach = 0
+    for stride, n in sorted((st, n) for n, st in zip(t.shape, t._logical_strides) if n > 1):
+        if stride <= reach:
+            return False
+        reach += (n - 1) * stride
+    return True
+
+
+def _grad_table(grads: list) -> tuple[array.array, list]:
+    """mm_grad_t rows, and the tensors that they point into: the gradients, or dense
+    copies of those that do not fill their storage span."""
+    held = [g if is_dense(g.shape, g._logical_strides) else ops.materialize(g) for g in grads]
+    return array.array("q", [v for g in held for v in (_pointer(g), numel(g.shape))]), held
+
+
+def _norm_and_coef(grads: list, order: int, max_norm: float) -> tuple[MatrixManTensor, MatrixManTensor]:
+    """The norm and the coefficient that clips to max_norm, on the device."""
+    rt = _grad_runtime(grads)
+    table, held = _grad_table(grads)
+    owner = rt.new_storage(2)
+    norm, coef = (MatrixManTensor._wrap(owner, (), i, ()) for i in (0, 1))
+    ops._launch("mm_grad_norm", table.buffer_info()[0], len(held), order, max_norm, _pointer(norm), _pointer(coef),
+                None, 0, rt.stream)
+    return norm, coef
+
+
+def grad_norm(parameters, norm_type: float = 2.0) -> MatrixManTensor:
+    """The norm of the gradients of `parameters` (an iterable, or one) as if they were
+    one vector, on their device: order 1, 2 or inf, summed in 64 bits.  Parameters
+    without a gradient are left out; of no gradients it is 0."""
+    order = _norm_order(norm_type)
+    return _norm_and_coef(_grads_of(parameters), order, 0.0)[0]
+
+
+@torch.no_grad()
+def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0,
+                    error_if_nonfinite: bool = False) -> MatrixManTensor:
+    """Scale the gradients of `parameters` in place by min(1, max_norm / (norm + 1e-6)),
+    and return the norm that they had, on their device, as
+    torch.nn.utils.clip_grad_norm_ does.  A NaN norm makes every gradient NaN, an
+    infinite one makes them 0 (NaN where they were infinite); with
+    ``error_if_nonfinite`` the norm is read back first, and either raises.  The
+    gradients are of one device and share no memory with each other."""
+    order = _norm_order(norm_type)
+    max_norm = float(max_norm)
+    if not max_norm >= 0.0:
+        raise ValueError(f"MatrixMan/CUDA: clip_grad_norm_ max_norm must be non-negative, got {max_norm}")
+    grads = _grads_of(parameters)
+    rt = _grad_runtime(grads)
+    if error_if_nonfinite:
+        if rt.capturing:
+            raise RuntimeError("MatrixMan/CUDA: clip_grad_norm_ cannot read the norm back during graph capture")
+        norm = _norm_and_coef(grads, order, 0.0)[0].cpu()
+        if not torch.isfinite(norm):
+            raise RuntimeError(f"MatrixMan/CUDA: the gradients' norm of order {norm_type} is {norm.item()}, so they are "
+                               "not clipped (error_if_nonfinite)")
+    for g in grads:
+        if not _is_apart(g):
+            raise NotImplementedError("MatrixMan/CUDA: clip_grad_norm_ needs gradients whose elements share no memory, "
+                                      f"got strides {g._logical_strides}")
+    table, held = _grad_table(grads)
+    norm = ops.new_dense(rt, ())
+    ops._launch("mm_grad_clip", table.buffer_info()[0], len(held), order, max_norm, _pointer(norm), None, 0, rt.stream)
+    for g, copy_ in zip(grads, held):
+        if g is not copy_:
+            ops.copy_into(copy_, g)
+    torch.autograd.graph.increment_version(grads)
+    return norm
+
+
 def run_adamw(rt, rows: list, state_bits: int, *, lr: float, beta1: float, beta2: float, eps: float,
-              weight_decay: float, decoupled: bool, maximize: bool, advance: bool) -> None:
+              weight_decay: float, decoupled: bool, maximize: bool, advance: bool, scale=None) -> None:
     """One native step over ``rows`` of (param, grad, exp_avg, exp_avg_sq,
     exp_avg_scale, exp_avg_sq_scale, step, numel): addresses and a count, laid
-    out as mm_adamw_tensor_t."""
+    out as mm_adamw_tensor_t; scale: address of what gradients are multiplied by."""
     if not rows:
         return
     table = array.array("q", [v for row in rows for v in row])
-    ops._launch("mm_adamw", table.buffer_info()[0], len(rows), state_bits, lr, beta1, beta2, eps, weight_decay,
-                decoupled, maximize, advance, None, 0, rt.stream)
+    factors = (state_bits, lr, beta1, beta2, eps, weight_decay, decoupled, maximize, advance)
+    if scale is None:
+        ops._launch("mm_adamw", table.buffer_info()[0], len(rows), *factors, None, 0, rt.stream)
+    else:
+        ops._launch("mm_adamw_scaled", table.buffer_info()[0], len(rows), *factors, scale, None, 0, rt.stream)
 
 
 class AdamW(torch.optim.Optimizer):
@@ -65,6 +172,11 @@ class AdamW(torch.optim.Optimizer):
     float32 in either form, and ``state_dict`` holds them so, so a checkpoint
     of one form loads into the other.
 
+    ``max_grad_norm`` clips each step: the gradients of all groups together (then of
+    one device) are scaled to that 2-norm as ``clip_grad_norm_`` would, but while the
+    step reads them: ``grad`` itself is not changed.  ``grad_norm`` is the norm that
+    the last such step saw, on the device.
+
     Parameters and gradients are float32 MatrixMan tensors of one device per
     group; a parameter fills its storage span (any order of dimensions) and
     shares it with no other.  The step count lives on the device, so a captured
@@ -73,7 +185,7 @@ class AdamW(torch.optim.Optimizer):
     they were at capture."""
 
     def __init__(self, params, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2, *,
-                 maximize: bool = False, state_bits: int = 32):
+                 maximize: bool = False, state_bits: int = 32, max_grad_norm: float | None = None):
         if isinstance(lr, torch.Tensor):
             raise NotImplementedError("MatrixMan/CUDA: AdamW takes lr as a number")
         if not lr >= 0.0:
@@ -86,7 +198,11 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError(f"MatrixMan/CUDA: AdamW weight_decay must be non-negative, got {weight_decay}")
         if state_bits not in (32, 8):
             raise ValueError(f"MatrixMan/CUDA: AdamW state_bits must be 32 or 8, got {state_bits}")
+        if max_grad_norm is not None and not max_grad_norm >= 0.0:
+            raise ValueError(f"MatrixMan/CUDA: AdamW max_grad_norm must be non-negative, got {max_grad_norm}")
         self.state_bits = int(state_bits)
+        self.max_grad_norm = max_grad_norm
+        self.grad_norm: MatrixManTensor | None = None
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay,
                                       maximize=bool(maximize)))
 
@@ -178,7 +294,7 @@ class AdamW(torch.optim.Optimizer):
         return (_pointer(p), _pointer(grad), _pointer(m), _pointer(v), ms, vs, _pointer(state["step"]),
                 numel(p.shape))
 
-    def _step(self, params: list, states: list, factors: tuple, maximize: bool) -> None:
+    def _step(self, params: list, states: list, factors: tuple, maximize: bool, scale) -> None:
         """A step whose tensors need checks or copies first."""
         rt = params[0].runtime
         rows, held = [], []
@@ -193,7 +309,7 @@ class AdamW(torch.optim.Optimizer):
             rows.append(self._row(p, grad, state))
         lr, beta1, beta2, eps, weight_decay = factors
         run_adamw(rt, rows, self.state_bits, lr=lr, beta1=beta1, beta2=beta2, eps=eps, weight_decay=weight_decay,
-                  decoupled=True, maximize=maximize, advance=True)
+                  decoupled=True, maximize=maximize, advance=True, scale=None if scale is None else _pointer(scale))
 
     @torch.no_grad()
     def step(self, closure=None):
@@ -202,6 +318,10 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
+        scale = None
+        if self.max_grad_norm is not None:
+            grads = [p.grad for group in self.param_groups for p in group["params"] if p.grad is not None]
+            self.grad_norm, scale = _norm_and_coef(grads, _lib.NORM_ORDERS[2.0], float(self.max_grad_norm))
         for group in self.param_groups:
             params = [p for p in group["params"] if p.grad is not None]
             if not params:
@@ -210,8 +330,8 @@ class AdamW(torch.optim.Optimizer):
             factors = (float(group["lr"]), beta1, beta2, group["eps"], group["weight_decay"])
             states = [self.state.get(p) or self._state_of(p) for p in params]
             if ops.native_call("adamw_step", "mm_adamw", params, states, self.state_bits, *factors,
-                               group["maximize"]) is None:
-                self._step(params, states, factors, group["maximize"])
+                               group["maximize"], scale) is None:
+                self._step(params, states, factors, group["maximize"], scale)
             torch.autograd.graph.increment_version(params)
         return loss
 
