@@ -9,65 +9,31 @@
 //
 // Both passes are bound by memory: forward 8 bytes per element, backward 12.
 //
-// The walking kernels take any size.  A block walks a segment of an image's
-// pixels and leaves each channel's moments (or sums) in the workspace, a second
-// kernel joins them by group, a third reads the map again and writes y (or dx):
-// 12 (20) bytes per element.
+// Maps whose groups fit a cluster's shared memory are read once
+// (mm_group_norm_resident.cu).  The walking kernels here take any size.  A block
+// walks a segment of an image's pixels and leaves each channel's moments (or sums) in
+// the workspace, a second kernel joins them by group, a third reads the map again and
+// writes y (or dx): 12 (20) bytes per element.
 //
 // Moments are held as a mean and a sum of squared distances from it and joined
 // by d^2 n1 n2 / (n1 + n2) (Chan, Golub, LeVeque 1979), so large offsets do not
-// cancel.  All sums are float32 in a fixed order, without atomics: the same
+// cancel; those of 16 rows are taken around the first row's values (see
+// mm_group_norm_resident.cu).  All sums are float32 in a fixed order, without atomics: the same
 // inputs give the same bits.
 #include <cuda_runtime.h>
 #include <math.h>
 #include <stdint.h>
 
 #include <string>
+#include <type_traits>
 
-#include "mm_linear.cuh"
+#include "mm_group_norm.cuh"
 
 namespace mm {
 
-constexpr int GN_THREADS = 256;
-constexpr int GN_WARPS = GN_THREADS / 32;
-constexpr int GN_ROWS = 4;  // rows (channels last) or vectors (first) loaded at a time by the walking kernels
-
-struct GnArgs {
-  const float *x, *dy, *w, *b;
-  float *y, *mean, *rstd;   // y is dx in the backward pass
-  float* part;              // [2][n segs][channels]: mean and squared distances; sums of dz and dz xh
-  float* sums;              // backward: [2][n][groups], means of g and g xh
-  int64_t xi, xr, gi, gr;   // distances of images, and of pixels (channels last) or channels, in x and dy
-  int64_t segs_n;           // segs * n
-  int n, channels, groups, each, pixels;
-  int segs, seg;            // segments of an image, pixels of each but the last
-  int cols;                 // channels of a block's columns (channels last)
-  int act;
-  float eps;
-};
-
-template <int VEC>
-__device__ __forceinline__ void gn_load(const float* p, float* v) {
-  if (VEC == 4) {
-    const float4 t = *reinterpret_cast<const float4*>(p);
-    v[0] = t.x; v[1] = t.y; v[2] = t.z; v[3] = t.w;
-  } else if (VEC == 2) {
-    const float2 t = *reinterpret_cast<const float2*>(p);
-    v[0] = t.x; v[1] = t.y;
-  } else {
-    v[0] = *p;
-  }
-}
-
-template <int VEC>
-__device__ __forceinline__ void gn_store(float* p, const float* v) {
-  if (VEC == 4)
-    *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
-  else if (VEC == 2)
-    *reinterpret_cast<float2*>(p) = make_float2(v[0], v[1]);
-  else
-    *p = v[0];
-}
+// Rows (channels last) or vectors (first) that a thread of the walking kernels has under
+// way: x for the moments, x for the result, x and dy.
+constexpr int GN_ROWS = 8, GN_APPLY_ROWS = 4, GN_BACK_ROWS = 4;
 
 // Joins (n2, mean2, m2) into (n, mean, m).
 __device__ __forceinline__ void gn_join(float& n, float& mean, float& m, float n2, float mean2, float m2) {
@@ -88,8 +54,10 @@ __device__ __forceinline__ void gn_join(float& n, float& mean, float& m, float n
 template <int VEC, bool LAST>
 struct GnWalk {
   int image, seg, c, at, step, end;  // c < 0: nothing; pixels at, at + step, ... < end
-  __device__ __forceinline__ GnWalk(const GnArgs& a) {
-    int64_t id = blockIdx.x;
+  // back: from the last segment to the first, since the end of what the kernel before
+  // read is still in L2.
+  __device__ __forceinline__ GnWalk(const GnArgs& a, bool back = false) {
+    int64_t id = back ? gridDim.x - 1 - blockIdx.x : blockIdx.x;
     if (LAST) {
       const int q_n = a.cols / VEC, p_n = GN_THREADS / q_n;
       const int q = threadIdx.x % q_n, p = threadIdx.x / q_n;
@@ -192,39 +160,48 @@ __device__ __forceinline__ void gn_leave(const GnArgs& a, const GnWalk<VEC, LAST
 }
 
 template <int VEC, bool LAST>
-__global__ void __launch_bounds__(GN_THREADS) gn_moments_kernel(GnArgs a) {
+__global__ void __launch_bounds__(GN_THREADS, 4) gn_moments_kernel(GnArgs a) {
   const GnWalk<VEC, LAST> k(a);
   const float* x = a.x + k.offset(a.xi, a.xr);
   float n = 0.f, mean[VEC], m2[VEC];
 #pragma unroll
   for (int e = 0; e < VEC; ++e) mean[e] = m2[e] = 0.f;
   if (k.c >= 0) {
-    for (int px = k.at; px < k.end; px += GN_ROWS * k.step) {
-      float v[GN_ROWS][VEC];
-      int rows = 0;
+    // GN_ROWS rows around the first one's values, joined to the rows before
+    auto batch = [&](auto rows_, int px) {
+      constexpr int ROWS = decltype(rows_)::value;
+      float v[ROWS][VEC], sum[VEC], squares[VEC], less[VEC];
 #pragma unroll
-      for (int r = 0; r < GN_ROWS; ++r)
-        if (px + r * (int64_t)k.step < k.end) {
-          gn_load<VEC>(x + k.pixel(px + r * k.step, a.xr), v[r]);
-          rows = r + 1;
-        }
-      const float nb = (float)rows, share = nb / (n + nb);
+      for (int r = 0; r < ROWS; ++r) gn_load<VEC>(x + k.pixel(px + r * k.step, a.xr), v[r]);
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
-        float s = 0.f, q = 0.f;
+        less[e] = -v[0][e];
+        sum[e] = squares[e] = 0.f;
+      }
 #pragma unroll
-        for (int r = 0; r < GN_ROWS; ++r)
-          if (r < rows) s += v[r][e];
-        s = rows == GN_ROWS ? s * (1.f / GN_ROWS) : s / nb;
+      for (int r = 1; r < ROWS; ++r) {
+        gn_add<VEC, VEC>(v[r], v[r], less);
+        gn_add<VEC, VEC>(sum, sum, v[r]);
+        gn_fma<VEC, VEC, VEC>(squares, v[r], v[r], squares);
+      }
+      constexpr float nb = (float)ROWS, inv = 1.f / nb;
+      const float share = nb / (n + nb);
 #pragma unroll
-        for (int r = 0; r < GN_ROWS; ++r)
-          if (r < rows) q += (v[r][e] - s) * (v[r][e] - s);
-        const float d = s - mean[e];
+      for (int e = 0; e < VEC; ++e) {
+        const float d = -less[e] + sum[e] * inv - mean[e];
         mean[e] += d * share;
-        m2[e] += q + d * d * n * share;
+        m2[e] += squares[e] - sum[e] * sum[e] * inv + d * d * n * share;
       }
       n += nb;
+    };
+    int px = k.at;
+    for (; px + (GN_ROWS - 1) * (int64_t)k.step < k.end; px += GN_ROWS * k.step)
+      batch(std::integral_constant<int, GN_ROWS>{}, px);
+    if (px + (GN_ROWS / 2 - 1) * (int64_t)k.step < k.end) {
+      batch(std::integral_constant<int, GN_ROWS / 2>{}, px);
+      px += GN_ROWS / 2 * k.step;
     }
+    for (; px < k.end; px += k.step) batch(std::integral_constant<int, 1>{}, px);
   }
   gn_leave<VEC, LAST>(a, k, n, mean, m2, [](float& an, float& au, float& av, float bn, float bu, float bv) {
     gn_join(an, au, av, bn, bu, bv);
@@ -285,55 +262,49 @@ __global__ void __launch_bounds__(T) gn_join_moments_kernel(GnArgs a) {
 }
 
 template <int VEC, bool LAST>
-__global__ void __launch_bounds__(GN_THREADS) gn_apply_kernel(GnArgs a) {
-  const GnWalk<VEC, LAST> k(a);
+__global__ void __launch_bounds__(GN_THREADS, 4) gn_apply_kernel(GnArgs a) {
+  const GnWalk<VEC, LAST> k(a, true);
   pdl_wait();
   if (k.c < 0) return;
-  float mean[VEC], rstd[VEC], w[VEC], b[VEC];
+  float mean[VEC], rstd[VEC], w[VEC], b[VEC];  // mean is negated
   gn_of_groups<VEC, LAST>(a, k, a.mean, mean);
   gn_of_groups<VEC, LAST>(a, k, a.rstd, rstd);
   gn_of_channels<VEC, LAST>(a.w, k.c, 1.f, w);
   gn_of_channels<VEC, LAST>(a.b, k.c, 0.f, b);
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) {
+    mean[e] = -mean[e];
+    w[e] *= rstd[e];
+  }
   const float* x = a.x + k.offset(a.xi, a.xr);
   float* y = a.y + k.out(a);
-  for (int px = k.at; px < k.end; px += GN_ROWS * k.step) {
-    float v[GN_ROWS * VEC];
+  auto apply = [&](auto rows_, int px) {
+    constexpr int N = decltype(rows_)::value * VEC;
+    float v[N];
 #pragma unroll
-    for (int r = 0; r < GN_ROWS; ++r)
-      if (px + r * (int64_t)k.step < k.end) gn_load<VEC>(x + k.pixel(px + r * k.step, a.xr), v + r * VEC);
+    for (int r = 0; r < N / VEC; ++r) gn_load<VEC>(x + k.pixel(px + r * k.step, a.xr), v + r * VEC);
+    gn_add<N, VEC>(v, v, mean);
+    gn_fma<N, VEC, VEC>(v, v, w, b);
+    gn_act<N>(v, a.act);
 #pragma unroll
-    for (int i = 0; i < GN_ROWS * VEC; ++i) v[i] = (v[i] - mean[i % VEC]) * rstd[i % VEC] * w[i % VEC] + b[i % VEC];
-    lin_act<GN_ROWS * VEC>(v, a.act);
-#pragma unroll
-    for (int r = 0; r < GN_ROWS; ++r)
-      if (px + r * (int64_t)k.step < k.end) gn_store<VEC>(y + k.pixel(px + r * k.step, a.channels), v + r * VEC);
-  }
-}
-
-// xh and dz of N / VEC vectors of x (in `xh` on entry) and dy (in `dz`).
-template <int VEC, int N>
-__device__ __forceinline__ void gn_slopes(float (&xh)[N], float (&dz)[N], const float* mean, const float* rstd,
-                                          const float* w, const float* b, int act) {
-  float z[N];
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    xh[i] = (xh[i] - mean[i % VEC]) * rstd[i % VEC];
-    z[i] = xh[i] * w[i % VEC] + b[i % VEC];
-  }
-  lin_times_slope<N>(dz, z, act);
+    for (int r = 0; r < N / VEC; ++r) gn_store<VEC>(y + k.pixel(px + r * k.step, a.channels), v + r * VEC);
+  };
+  int px = k.at;
+  for (; px + (GN_APPLY_ROWS - 1) * (int64_t)k.step < k.end; px += GN_APPLY_ROWS * k.step)
+    apply(std::integral_constant<int, GN_APPLY_ROWS>{}, px);
+  for (; px < k.end; px += k.step) apply(std::integral_constant<int, 1>{}, px);
 }
 
 // PASS 0: each channel's sums of dz and dz xh; 1: dx.
 template <int VEC, bool LAST, int PASS>
-__global__ void __launch_bounds__(GN_THREADS) gn_backward_kernel(GnArgs a) {
-  constexpr int ROWS = 2;  // (both maps are loaded)
-  const GnWalk<VEC, LAST> k(a);
-  float u[VEC], v[VEC], mean[VEC], rstd[VEC], w[VEC], b[VEC];
+__global__ void __launch_bounds__(GN_THREADS, 3) gn_backward_kernel(GnArgs a) {
+  const GnWalk<VEC, LAST> k(a, PASS == 1);
+  float u[VEC], v[VEC], less[VEC], rstd[VEC], w[VEC], b[VEC];  // less: -mean
 #pragma unroll
   for (int e = 0; e < VEC; ++e) u[e] = v[e] = 0.f;
   if (PASS == 1) pdl_wait();
   if (k.c >= 0) {
-    gn_of_groups<VEC, LAST>(a, k, a.mean, mean);
+    gn_of_groups<VEC, LAST>(a, k, a.mean, less);
     gn_of_groups<VEC, LAST>(a, k, a.rstd, rstd);
     gn_of_channels<VEC, LAST>(a.w, k.c, 1.f, w);
     gn_of_channels<VEC, LAST>(a.b, k.c, 0.f, b);
@@ -341,37 +312,45 @@ __global__ void __launch_bounds__(GN_THREADS) gn_backward_kernel(GnArgs a) {
       gn_of_groups<VEC, LAST>(a, k, a.sums, u);
       gn_of_groups<VEC, LAST>(a, k, a.sums + (int64_t)a.n * a.groups, v);
     }
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      less[e] = -less[e];
+      if (PASS == 1) {
+        u[e] *= -rstd[e];
+        v[e] *= -rstd[e];
+      }
+    }
     const float* x = a.x + k.offset(a.xi, a.xr);
     const float* dy = a.dy + k.offset(a.gi, a.gr);
     float* dx = PASS == 1 ? a.y + k.out(a) : nullptr;
-    for (int px = k.at; px < k.end; px += ROWS * k.step) {
-      float xh[ROWS * VEC], dz[ROWS * VEC];
+    auto step = [&](auto rows_, int px) {
+      constexpr int N = decltype(rows_)::value * VEC;
+      float xh[N], dz[N];
 #pragma unroll
-      for (int r = 0; r < ROWS; ++r) {
-        if (px + r * (int64_t)k.step < k.end) {
-          gn_load<VEC>(x + k.pixel(px + r * k.step, a.xr), xh + r * VEC);
-          gn_load<VEC>(dy + k.pixel(px + r * k.step, a.gr), dz + r * VEC);
-        } else {
+      for (int r = 0; r < N / VEC; ++r) {
+        gn_load<VEC>(x + k.pixel(px + r * k.step, a.xr), xh + r * VEC);
+        gn_load<VEC>(dy + k.pixel(px + r * k.step, a.gr), dz + r * VEC);
+      }
 #pragma unroll
-          for (int e = 0; e < VEC; ++e) xh[r * VEC + e] = mean[e], dz[r * VEC + e] = 0.f;
+      for (int r = 0; r < N; r += VEC) {  // (a vector at a time, for the registers)
+        float(&h)[VEC] = *reinterpret_cast<float(*)[VEC]>(xh + r);
+        float(&z)[VEC] = *reinterpret_cast<float(*)[VEC]>(dz + r);
+        gn_slopes<VEC>(h, z, less, rstd, w, b, a.act);
+        if (PASS == 0) {
+          gn_add<VEC, VEC>(u, u, z);
+          gn_fma<VEC, VEC, VEC>(v, z, h, v);
+        } else {  // dx = rstd w dz - (rstd s2 xh + rstd s1)
+          gn_fma<VEC, VEC, VEC>(h, h, v, u);
+          gn_mul<VEC, VEC>(z, z, w);
+          gn_fma<VEC, VEC, VEC>(z, z, rstd, h);
+          gn_store<VEC>(dx + k.pixel(px + r / VEC * k.step, a.channels), z);
         }
       }
-      gn_slopes<VEC>(xh, dz, mean, rstd, w, b, a.act);
-      if (PASS == 0) {
-#pragma unroll
-        for (int i = 0; i < ROWS * VEC; ++i) {
-          u[i % VEC] += dz[i];
-          v[i % VEC] += dz[i] * xh[i];
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < ROWS * VEC; ++i)
-          dz[i] = rstd[i % VEC] * (dz[i] * w[i % VEC] - u[i % VEC] - xh[i] * v[i % VEC]);
-#pragma unroll
-        for (int r = 0; r < ROWS; ++r)
-          if (px + r * (int64_t)k.step < k.end) gn_store<VEC>(dx + k.pixel(px + r * k.step, a.channels), dz + r * VEC);
-      }
-    }
+    };
+    int px = k.at;
+    for (; px + (GN_BACK_ROWS - 1) * (int64_t)k.step < k.end; px += GN_BACK_ROWS * k.step)
+      step(std::integral_constant<int, GN_BACK_ROWS>{}, px);
+    for (; px < k.end; px += k.step) step(std::integral_constant<int, 1>{}, px);
   }
   if (PASS == 0)
     gn_leave<VEC, LAST>(a, k, 0.f, u, v, [](float&, float& au, float& av, float, float bu, float bv) {
@@ -380,51 +359,61 @@ __global__ void __launch_bounds__(GN_THREADS) gn_backward_kernel(GnArgs a) {
     });
 }
 
-// Means of g and g xh of one image and group per block.
-template <int T>
-__global__ void __launch_bounds__(T) gn_join_sums_kernel(GnArgs a) {
-  __shared__ float2 sm[T / 32];
+constexpr int GN_COLUMNS = 4;  // channels of a block that adds partial rows
+constexpr int GN_COLUMN_THREADS = GN_THREADS / GN_COLUMNS;
+
+// db and dw of a block's channels: 64 threads per channel add the partial rows k, k +
+// 64, ..., then their sums are added in order.
+__device__ __forceinline__ void gn_add_rows(const GnArgs& a, int block, float2 (*acc)[GN_COLUMNS + 1]) {
+  const int lane = threadIdx.x % GN_COLUMNS, k = threadIdx.x / GN_COLUMNS;
+  const int c = block * GN_COLUMNS + lane;
+  const float* pu = a.part + c;
+  const float* pv = pu + a.segs_n * a.channels;
+  float2 s = make_float2(0.f, 0.f);
+  if (c < a.channels)
+#pragma unroll 8
+    for (int64_t r = k; r < a.segs_n; r += GN_COLUMN_THREADS) {
+      s.x += pu[r * a.channels];
+      s.y += pv[r * a.channels];
+    }
+  acc[k][lane] = s;
+  __syncthreads();
+  if (k == 0 && c < a.channels) {
+    for (int j = 1; j < GN_COLUMN_THREADS; ++j) {
+      s.x += acc[j][lane].x;
+      s.y += acc[j][lane].y;
+    }
+    if (a.db) a.db[c] = s.x;
+    if (a.dw) a.dw[c] = s.y;
+  }
+}
+
+// Means of g and g xh of one image and group per block; the first `columns` blocks add
+// the partial rows.
+__global__ void __launch_bounds__(GN_THREADS) gn_join_sums_kernel(GnArgs a, int columns) {
+  __shared__ float2 acc[GN_COLUMN_THREADS][GN_COLUMNS + 1];
   pdl_wait();
-  const int image = blockIdx.x / a.groups, group = blockIdx.x % a.groups;
+  if ((int)blockIdx.x < columns) {
+    gn_add_rows(a, blockIdx.x, acc);
+    return;
+  }
+  const int id = blockIdx.x - columns, image = id / a.groups, group = id % a.groups;
   const float* pu = a.part + (int64_t)image * a.segs * a.channels + group * a.each;
   const float* pv = pu + a.segs_n * a.channels;
   const int64_t count = (int64_t)a.segs * a.each;
   const float inv = 1.f / ((float)a.pixels * (float)a.each);
   float s1 = 0.f, s2 = 0.f;
-  for (int64_t i = threadIdx.x; i < count; i += T) {
+#pragma unroll 4
+  for (int64_t i = threadIdx.x; i < count; i += GN_THREADS) {
     const int64_t at = i / a.each * a.channels + i % a.each;
     const float w = a.w ? a.w[group * a.each + i % a.each] : 1.f;
     s1 += w * pu[at];
     s2 += w * pv[at];
   }
-  gn_sum2<T>(s1, s2, sm);
+  gn_sum2<GN_THREADS>(s1, s2, &acc[0][0]);
   if (threadIdx.x == 0) {
-    a.sums[blockIdx.x] = s1 * inv;
-    a.sums[(int64_t)a.n * a.groups + blockIdx.x] = s2 * inv;
-  }
-}
-
-// db (blockIdx.y 0) or dw (1) of 32 channels: 32 threads per channel add the
-// partial rows k, k + 32, ..., then their sums are added in order.
-__global__ void __launch_bounds__(1024) gn_columns_kernel(const float* part, int64_t rows, int channels, float* db,
-                                                          float* dw) {
-  __shared__ float acc[32][33];
-  pdl_wait();
-  float* out = blockIdx.y ? dw : db;
-  if (!out) return;
-  const int lane = threadIdx.x & 31, k = threadIdx.x >> 5;
-  const int c = blockIdx.x * 32 + lane;
-  part += (int64_t)blockIdx.y * rows * channels;
-  float s = 0.f;
-  if (c < channels)
-#pragma unroll 4
-    for (int64_t r = k; r < rows; r += 32) s += part[r * channels + c];
-  acc[k][lane] = s;
-  __syncthreads();
-  if (k == 0 && c < channels) {
-#pragma unroll
-    for (int j = 1; j < 32; ++j) s += acc[j][lane];
-    out[c] = s;
+    a.sums[id] = s1 * inv;
+    a.sums[(int64_t)a.n * a.groups + id] = s2 * inv;
   }
 }
 
@@ -440,22 +429,31 @@ static int gn_vec(const GnArgs& a, bool last) {
   return bits % 4 == 0 ? 4 : bits % 2 == 0 ? 2 : 1;
 }
 
-constexpr int64_t GN_BLOCKS = 148 * 8;  // walking blocks that a call of large maps has at least
-constexpr int GN_LEAST = 64;            // pixels of a segment, at least (a multiple of what a load takes)
+constexpr int64_t GN_BLOCKS = 148 * 16;  // walking blocks of a call of large maps: four on each SM, four times
+constexpr int GN_LEAST = 64;             // pixels of a segment, at least (a multiple of what a load takes);
+                                         // of few channels as many more as a block has rows under way
 
-// Segments of an image for the walking kernels: enough blocks to fill the GPU,
-// whatever the vector width is, so that the workspace's size follows from the sizes alone.
-static int gn_segments(int64_t n, int64_t channels, int64_t pixels) {
-  const int64_t columns = n * ((channels + 127) / 128);
-  int64_t segs = (GN_BLOCKS + columns - 1) / columns;
-  const int64_t most = (pixels + GN_LEAST - 1) / GN_LEAST;
-  if (segs > most) segs = most;
-  return (int)(segs < 1 ? 1 : segs);
+// Segments of an image for the walking kernels: enough blocks (channels first: warps of
+// one channel) to fill the GPU, whatever the vector width is, so that the workspace's
+// size follows from the sizes alone.
+static int64_t gn_segments(int64_t n, int64_t channels, int64_t pixels, bool last) {
+  const int64_t walkers = last ? n * ((channels + 127) / 128) : (n * channels + GN_WARPS - 1) / GN_WARPS;
+  const int64_t least = last && channels < 128 ? GN_LEAST * 128 / channels : GN_LEAST;
+  const int64_t segs = (GN_BLOCKS + walkers - 1) / walkers, most = (pixels + least - 1) / least;
+  return segs < most ? segs : most;
+}
+
+static void gn_cut(GnArgs* a, bool last) {
+  if (a->n == 0 || a->channels == 0 || a->pixels == 0) return;
+  const int64_t segs = gn_segments(a->n, a->channels, a->pixels, last);
+  a->seg = (int)((((int64_t)a->pixels + segs - 1) / segs + GN_LEAST - 1) / GN_LEAST * GN_LEAST);
+  a->segs = (a->pixels - 1) / a->seg + 1;
+  a->segs_n = (int64_t)a->n * a->segs;
 }
 
 static int gn_setup(const char* who, const float* x, int64_t xi, int64_t xr, int64_t n, int64_t channels,
-                    int64_t pixels, int64_t groups, const float* w, const float* b, float* mean, float* rstd, int act,
-                    GnArgs* a) {
+                    int64_t pixels, int64_t groups, bool last, const float* w, const float* b, float* mean, float* rstd,
+                    int act, GnArgs* a) {
   const std::string name(who);
   if (n < 0 || channels < 0 || pixels < 0 || xi < 0 || xr < 0)
     return fail(MM_ERR_INVALID, name + ": negative size or stride");
@@ -481,10 +479,7 @@ static int gn_setup(const char* who, const float* x, int64_t xi, int64_t xr, int
   a->act = act;
   if (n == 0 || channels == 0 || pixels == 0) return MM_OK;
   if (!x) return fail(MM_ERR_INVALID, name + ": null data pointer");
-  const int segs = gn_segments(n, channels, pixels);
-  a->seg = (int)(((pixels + segs - 1) / segs + GN_LEAST - 1) / GN_LEAST * GN_LEAST);
-  a->segs = (int)((pixels + a->seg - 1) / a->seg);
-  a->segs_n = n * a->segs;
+  gn_cut(a, last);
   return MM_OK;
 }
 
@@ -496,40 +491,46 @@ static dim3 gn_grid(GnArgs& a) {
   return dim3((unsigned)a.segs_n, (unsigned)((a.channels + a.cols - 1) / a.cols));
 }
 
-// A block of 32 threads per image and group where its partial values are few.
-template <class K, class... Args>
-static cudaError_t gn_launch_join(K small, K large, const GnArgs& a, cudaStream_t s) {
-  const bool few = (int64_t)a.segs * a.each <= 128;
-  return launch_pdl(few ? small : large, dim3((unsigned)((int64_t)a.n * a.groups)), dim3(few ? 32 : 256), 0, s, a);
-}
-
 template <int VEC, bool LAST>
 static cudaError_t gn_walk_forward(GnArgs a, cudaStream_t s) {
   const dim3 grid = gn_grid<VEC, LAST>(a);
   gn_moments_kernel<VEC, LAST><<<grid, GN_THREADS, 0, s>>>(a);
   cudaError_t e = cudaGetLastError();
-  if (e == cudaSuccess) e = gn_launch_join(gn_join_moments_kernel<32>, gn_join_moments_kernel<256>, a, s);
+  // (few partial values per image and group: a warp each)
+  const bool few = (int64_t)a.segs * a.each <= 128;
+  if (e == cudaSuccess)
+    e = launch_pdl(few ? gn_join_moments_kernel<32> : gn_join_moments_kernel<256>,
+                   dim3((unsigned)((int64_t)a.n * a.groups)), dim3(few ? 32 : 256), 0, s, a);
   return e == cudaSuccess ? launch_pdl(gn_apply_kernel<VEC, LAST>, grid, dim3(GN_THREADS), 0, s, a) : e;
 }
 
+static int gn_column_blocks(const GnArgs& a) {
+  return a.dw || a.db ? (a.channels + GN_COLUMNS - 1) / GN_COLUMNS : 0;
+}
+
 template <int VEC, bool LAST>
-static cudaError_t gn_walk_backward(GnArgs a, float* dw, float* db, cudaStream_t s) {
+static cudaError_t gn_walk_backward(GnArgs a, cudaStream_t s) {
   const dim3 grid = gn_grid<VEC, LAST>(a);
   gn_backward_kernel<VEC, LAST, 0><<<grid, GN_THREADS, 0, s>>>(a);
   cudaError_t e = cudaGetLastError();
-  if (e == cudaSuccess && (dw || db))
-    e = launch_pdl(gn_columns_kernel, dim3((a.channels + 31) / 32, 2), dim3(1024), 0, s, (const float*)a.part,
-                   (int64_t)a.segs_n, (int)a.channels, db, dw);
-  if (e == cudaSuccess && a.y) {
-    e = gn_launch_join(gn_join_sums_kernel<32>, gn_join_sums_kernel<256>, a, s);
-    if (e == cudaSuccess) e = launch_pdl(gn_backward_kernel<VEC, LAST, 1>, grid, dim3(GN_THREADS), 0, s, a);
-  }
+  const int columns = gn_column_blocks(a);
+  const int64_t blocks = columns + (a.y ? (int64_t)a.n * a.groups : 0);
+  if (e == cudaSuccess)
+    e = launch_pdl(gn_join_sums_kernel, dim3((unsigned)blocks), dim3(GN_THREADS), 0, s, a, columns);
+  if (e == cudaSuccess && a.y) e = launch_pdl(gn_backward_kernel<VEC, LAST, 1>, grid, dim3(GN_THREADS), 0, s, a);
   return e;
 }
 
-// Floats of the workspace: two per channel and segment, and two per image and group.
+// Floats of the workspace, whichever kernels run: two per channel and segment, and two
+// per image and group.
 static int64_t gn_floats(const GnArgs& a) {
-  return 2 * a.segs_n * a.channels + 2 * (int64_t)a.n * a.groups;
+  int64_t rows = gn_plan_rows(a.n, a.pixels);
+  for (const bool last : {true, false}) {
+    GnArgs cut = a;
+    gn_cut(&cut, last);
+    rows = rows > cut.segs_n ? rows : cut.segs_n;
+  }
+  return 2 * rows * a.channels + 2 * (int64_t)a.n * a.groups;
 }
 
 static int gn_workspace(const char* who, const GnArgs& a, void** workspace, size_t bytes, Scratch* scratch,
@@ -562,8 +563,8 @@ extern "C" int mm_group_norm_workspace_size(int64_t n, int64_t channels, int64_t
   if (bytes == nullptr) return fail(MM_ERR_INVALID, "mm_group_norm_workspace_size: invalid argument");
   GnArgs a;
   const float* some = (const float*)16;
-  const int rc = gn_setup("mm_group_norm_workspace_size", some, 0, 0, n, channels, pixels, groups, nullptr, nullptr,
-                          nullptr, nullptr, 0, &a);
+  const int rc = gn_setup("mm_group_norm_workspace_size", some, 0, 0, n, channels, pixels, groups, true, nullptr,
+                          nullptr, nullptr, nullptr, 0, &a);
   if (rc == MM_OK) *bytes = (size_t)gn_floats(a) * sizeof(float);
   return rc;
 }
@@ -573,19 +574,26 @@ extern "C" int mm_group_norm(const float* x, int64_t x_image, int64_t x_row, int
                              double eps, int act, float* y, float* mean, float* rstd, void* workspace,
                              size_t workspace_bytes, void* stream) {
   GnArgs a;
-  int rc = gn_setup("mm_group_norm", x, x_image, x_row, n, channels, pixels, groups, weight, bias, mean, rstd, act, &a);
+  int rc = gn_setup("mm_group_norm", x, x_image, x_row, n, channels, pixels, groups, channels_last != 0, weight, bias,
+                    mean, rstd, act, &a);
   if (rc != MM_OK) return rc;
   if (n == 0 || channels == 0) return MM_OK;
   if (pixels == 0) return fail(MM_ERR_UNSUPPORTED, "mm_group_norm: images without pixels");
   if (!y || !mean || !rstd) return fail(MM_ERR_INVALID, "mm_group_norm: null data pointer");
   cudaStream_t s = resolve_stream(stream);
-  Scratch scratch;
-  if ((rc = gn_workspace("mm_group_norm", a, &workspace, workspace_bytes, &scratch, s)) != MM_OK) return rc;
   a.y = y;
   a.eps = (float)eps;
-  a.part = (float*)workspace;
   const bool last = channels_last != 0;
   const int vec = gn_vec(a, last);
+  const GnPlan plan = gn_plan(a, vec, last, false);
+  Scratch scratch;
+  if (workspace != nullptr || plan.ranks == 0)
+    if ((rc = gn_workspace("mm_group_norm", a, &workspace, workspace_bytes, &scratch, s)) != MM_OK) return rc;
+  a.part = (float*)workspace;
+  if (plan.ranks > 0) {
+    MM_CUDA(gn_resident_forward(a, plan, vec, last, s), "mm_group_norm launch");
+    return MM_OK;
+  }
   MM_CUDA(GN_BY_VEC(gn_walk_forward, a, s), "mm_group_norm launch");
   return MM_OK;
 }
@@ -596,7 +604,7 @@ extern "C" int mm_group_norm_backward(const float* dy, int64_t dy_image, int64_t
                                       const float* weight, const float* bias, int act, float* dx, float* dweight,
                                       float* dbias, void* workspace, size_t workspace_bytes, void* stream) {
   GnArgs a;
-  int rc = gn_setup("mm_group_norm_backward", x, x_image, x_row, n, channels, pixels, groups, weight, bias,
+  int rc = gn_setup("mm_group_norm_backward", x, x_image, x_row, n, channels, pixels, groups, channels_last != 0, weight, bias,
                     const_cast<float*>(mean), const_cast<float*>(rstd), act, &a);
   if (rc != MM_OK) return rc;
   if ((!dx && !dweight && !dbias) || channels == 0) return MM_OK;
@@ -609,16 +617,29 @@ extern "C" int mm_group_norm_backward(const float* dy, int64_t dy_image, int64_t
   if (!dy || dy_image < 0 || dy_row < 0) return fail(MM_ERR_INVALID, "mm_group_norm_backward: invalid gradient");
   if (!mean || !rstd) return fail(MM_ERR_INVALID, "mm_group_norm_backward: null statistics");
   cudaStream_t s = resolve_stream(stream);
-  Scratch scratch;
-  if ((rc = gn_workspace("mm_group_norm_backward", a, &workspace, workspace_bytes, &scratch, s)) != MM_OK) return rc;
   a.dy = dy;
   a.gi = dy_image;
   a.gr = dy_row;
   a.y = dx;
+  a.dw = dweight;
+  a.db = dbias;
+  const bool last = channels_last != 0, columns = dweight || dbias;
+  const int vec = gn_vec(a, last);
+  const GnPlan plan = gn_plan(a, vec, last, true);
+  Scratch scratch;
+  if (workspace != nullptr || plan.ranks == 0 || columns)
+    if ((rc = gn_workspace("mm_group_norm_backward", a, &workspace, workspace_bytes, &scratch, s)) != MM_OK) return rc;
+  if (plan.ranks > 0) {
+    a.part = columns ? (float*)workspace : nullptr;
+    a.segs_n = (int64_t)plan.blocks * plan.ranks;  // partial rows
+    MM_CUDA(gn_resident_backward(a, plan, vec, last, s), "mm_group_norm_backward launch");
+    if (columns)
+      MM_CUDA(launch_pdl(gn_join_sums_kernel, dim3(gn_column_blocks(a)), dim3(GN_THREADS), 0, s, a, gn_column_blocks(a)),
+              "mm_group_norm_backward columns launch");
+    return MM_OK;
+  }
   a.part = (float*)workspace;
   a.sums = a.part + 2 * a.segs_n * channels;
-  const bool last = channels_last != 0;
-  const int vec = gn_vec(a, last);
-  MM_CUDA(GN_BY_VEC(gn_walk_backward, a, dweight, dbias, s), "mm_group_norm_backward launch");
+  MM_CUDA(GN_BY_VEC(gn_walk_backward, a, s), "mm_group_norm_backward launch");
   return MM_OK;
 }
