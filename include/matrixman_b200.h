@@ -415,7 +415,7 @@ int mm_linear_workspace_size(int64_t m, int64_t n, int64_t k, int backward, size
  * x + i * x_image + s * x_row, and y is dense [n, pixels, channels]; otherwise
  * channel c holds its pixels densely at x + i * x_image + c * x_row, and y is dense
  * [n, channels, pixels].  weight and bias [channels] may be NULL.  mean and rstd
- * [n, groups] are kept for the backward pass.  workspace: device memory, 16-byte
+ * [n, groups] are kept for the backward pass; both may be NULL.  workspace: device memory, 16-byte
  * aligned, of mm_group_norm_workspace_size bytes, or NULL to take it from the scratch
  * pool.  No counterpart in the reference, whose only normalisation is eval BatchNorm. */
 int mm_group_norm(const float* x, int64_t x_image, int64_t x_row, int64_t n, int64_t channels, int64_t pixels,

@@ -579,7 +579,7 @@ extern "C" int mm_group_norm(const float* x, int64_t x_image, int64_t x_row, int
   if (rc != MM_OK) return rc;
   if (n == 0 || channels == 0) return MM_OK;
   if (pixels == 0) return fail(MM_ERR_UNSUPPORTED, "mm_group_norm: images without pixels");
-  if (!y || !mean || !rstd) return fail(MM_ERR_INVALID, "mm_group_norm: null data pointer");
+  if (!y || !mean != !rstd) return fail(MM_ERR_INVALID, "mm_group_norm: null data pointer");
   cudaStream_t s = resolve_stream(stream);
   a.y = y;
   a.eps = (float)eps;
@@ -590,6 +590,10 @@ extern "C" int mm_group_norm(const float* x, int64_t x_image, int64_t x_row, int
   if (workspace != nullptr || plan.ranks == 0)
     if ((rc = gn_workspace("mm_group_norm", a, &workspace, workspace_bytes, &scratch, s)) != MM_OK) return rc;
   a.part = (float*)workspace;
+  if (plan.ranks == 0 && !mean) {
+    a.mean = a.part + 2 * a.segs_n * channels;
+    a.rstd = a.mean + (int64_t)a.n * a.groups;
+  }
   if (plan.ranks > 0) {
     MM_CUDA(gn_resident_forward(a, plan, vec, last, s), "mm_group_norm launch");
     return MM_OK;

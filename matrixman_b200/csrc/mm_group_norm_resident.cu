@@ -308,7 +308,7 @@ __global__ void __launch_bounds__(GN_MOST_THREADS) gn_resident_kernel(const __gr
   }
   auto rstd_of = [&](float q) { return 1.f / sqrtf((q < 0.f ? 0.f : q) / all + a.eps); };  // (NaN stays)
   auto keep = [&](int image, int g, float mean, float rstd) {
-    if (t.rank == 0) {
+    if (t.rank == 0 && a.mean) {
       const int64_t at = (int64_t)image * a.groups + t.slab * k.slab + g;
       a.mean[at] = mean;
       a.rstd[at] = rstd;

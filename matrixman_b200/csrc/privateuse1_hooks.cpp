@@ -442,6 +442,119 @@ py::object layer_norm_backward(py::handle dy_, py::handle x_, int64_t width, py:
   return py::make_tuple(dx, dw, db);
 }
 
+using group_norm_fn = int (*)(const void*, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int, const void*,
+                              const void*, double, int, void*, void*, void*, void*, size_t, void*);
+using group_norm_back_fn = int (*)(const void*, int64_t, int64_t, const void*, int64_t, int64_t, int64_t, int64_t,
+                                   int64_t, int64_t, int, const void*, const void*, const void*, const void*, int,
+                                   void*, void*, void*, void*, size_t, void*);
+
+// Feature maps [n, channels, *spatial] as the group-norm kernels read them.
+struct Maps {
+  int64_t n = 0, channels = 0, pixels = 1, image = 0, row = 0;
+  bool last = true;
+  // False where the strides take a copy, or a dimension is empty.
+  bool of(const Operand& x) {
+    const int64_t d = x.dim();
+    if (d < 2) return false;
+    n = x.size(0);
+    channels = x.size(1);
+    int64_t pixel = 0;
+    for (int64_t i = d - 1; i >= 2; --i) {
+      if (x.size(i) == 1) continue;
+      if (pixels == 1) pixel = x.t->stride(i);
+      else if (x.t->stride(i) != pixel * pixels) return false;
+      pixels *= x.size(i);
+      if (pixels == 0) return false;
+    }
+    if (n == 0 || channels == 0) return false;
+    image = x.t->stride(0);
+    const int64_t channel = x.t->stride(1);
+    if (pixels > 1 && pixel == 1 && (channels == 1 || channel != 1)) {
+      last = false;
+      row = channel;
+      return true;
+    }
+    row = pixels > 1 ? pixel : channels;
+    return channels == 1 || channel == 1;
+  }
+  // Strides of dense maps in this order; x's own where they say the same.
+  std::vector<int64_t> strides(const Operand& x) const {
+    const int64_t d = x.dim();
+    std::vector<int64_t> s(d);
+    int64_t at = last ? channels : 1;
+    for (int64_t i = d; i-- > 2;) {
+      s[i] = at;
+      at *= x.size(i);
+    }
+    s[1] = last ? 1 : pixels;
+    s[0] = channels * pixels;
+    bool same = true;
+    for (int64_t i = 0; i < d; ++i) same = same && (x.size(i) == 1 || s[i] == x.t->stride(i));
+    return same ? x.t->strides().vec() : s;
+  }
+};
+
+py::object group_norm(py::handle x_, int64_t groups, py::handle w_, py::handle b_, double eps, int act, bool keep) {
+  Operand x, w, b;
+  Maps maps;
+  Target t;
+  if (!names().ready || !operand(x_, &x) || !operand(w_, &w) || !operand(b_, &b) || !x.given || !maps.of(x) ||
+      groups < 1 || maps.channels % groups != 0 || !is_vector(w, maps.channels) || !is_vector(b, maps.channels) ||
+      !t.of(x) || !t.owns(w) || !t.owns(b))
+    return py::none();
+  char *py_ = nullptr, *ps = nullptr;
+  py::object owner = new_storage(t, x.t->numel(), &py_), stats;
+  if (!owner) return py::none();
+  const int64_t rows = maps.n * groups;
+  // mean and rstd share a block, apart from y's: they are kept for the backward pass, y may go.
+  if (keep && !(stats = new_storage(t, 2 * rows, &ps))) return py::none();
+  const int status = unlocked(MM_SYMBOL(group_norm_fn, "mm_group_norm"), x.ptr, maps.image, maps.row, maps.n,
+                              maps.channels, maps.pixels, groups, (int)maps.last, w.ptr, b.ptr, eps, act, py_, ps,
+                              keep ? ps + 4 * rows : nullptr, nullptr, 0, t.stream);
+  if (status != 0) return py::int_(status);
+  py::object y = new_tensor(t, owner, int_tuple(x.t->sizes()), int_tuple(maps.strides(x)), 0);
+  if (!keep) return py::make_tuple(y, py::none(), py::none());
+  const int64_t shape[] = {maps.n, groups};
+  const py::tuple stat = int_tuple(at::IntArrayRef(shape, 2)), strides = dense_strides(at::IntArrayRef(shape, 2));
+  return py::make_tuple(y, new_tensor(t, stats, stat, strides, 0), new_tensor(t, stats, stat, strides, rows));
+}
+
+py::object group_norm_backward(py::handle dy_, py::handle x_, py::handle mean_, py::handle rstd_, py::handle w_,
+                               py::handle b_, int64_t groups, int act, bool need_x, bool need_w, bool need_b) {
+  Operand dy, x, mean, rstd, w, b;
+  Maps maps, grads;
+  Target t;
+  if (!names().ready || !operand(dy_, &dy) || !operand(x_, &x) || !operand(mean_, &mean) || !operand(rstd_, &rstd) ||
+      !operand(w_, &w) || !operand(b_, &b) || !dy.given || !x.given || !mean.given || !rstd.given || !maps.of(x) ||
+      !grads.of(dy) || dy.t->sizes() != x.t->sizes() || groups < 1 || maps.channels % groups != 0)
+    return py::none();
+  // (one pixel is in both orders)
+  if (grads.last != maps.last || !is_vector(w, maps.channels) || !is_vector(b, maps.channels) ||
+      !mean.t->is_contiguous() || !rstd.t->is_contiguous() || mean.t->numel() != maps.n * groups ||
+      rstd.t->numel() != maps.n * groups)
+    return py::none();
+  if (!t.of(x) || !t.owns(dy) || !t.owns(mean) || !t.owns(rstd) || !t.owns(w) || !t.owns(b)) return py::none();
+  char *px = nullptr, *pw = nullptr;
+  py::object dx = py::none(), dw = py::none(), db = py::none(), owner;
+  if (need_x) {
+    if (!(owner = new_storage(t, x.t->numel(), &px))) return py::none();
+    dx = new_tensor(t, owner, int_tuple(x.t->sizes()), int_tuple(maps.strides(x)), 0);
+  }
+  const int64_t each = (maps.channels + 63) / 64 * 64;  // dw and db share a block, each at a 256-byte boundary
+  if (need_w || need_b) {
+    if (!(owner = new_storage(t, 2 * each, &pw))) return py::none();
+    const py::tuple shape = py::make_tuple(maps.channels), one = py::make_tuple(1);
+    if (need_w) dw = new_tensor(t, owner, shape, one, 0);
+    if (need_b) db = new_tensor(t, owner, shape, one, each);
+  }
+  const int status = unlocked(MM_SYMBOL(group_norm_back_fn, "mm_group_norm_backward"), dy.ptr, grads.image, grads.row,
+                              x.ptr, maps.image, maps.row, maps.n, maps.channels, maps.pixels, groups, (int)maps.last,
+                              mean.ptr, rstd.ptr, w.ptr, b.ptr, act, px, need_w ? pw : nullptr,
+                              need_b ? pw + 4 * each : nullptr, nullptr, 0, t.stream);
+  if (status != 0) return py::int_(status);
+  return py::make_tuple(dx, dw, db);
+}
+
 // [..., k] as rows: their number and the two strides; false where that takes a copy.
 bool matrix(const Operand& x, int64_t* rows, int64_t* s0, int64_t* s1) {
   const int64_t d = x.dim();
@@ -541,7 +654,6 @@ bool holds_codes(const Operand& codes, const Operand& scales, const Operand& p) 
 // a tensor is not as usual.
 py::object adamw_step(const py::list& params, const py::list& states, int bits, double lr, double beta1, double beta2,
                       double eps, double decay, bool maximize, const py::handle& scale_) {
-  static const py::object& grad_name = *new py::object(name("grad"));
   static const py::object& step_name = *new py::object(name("step"));
   static const py::object* const wide = new py::object[2]{name("exp_avg"), name("exp_avg_sq")};
   static const py::object* const narrow = new py::object[4]{name("exp_avg_code"), name("exp_avg_sq_code"),
@@ -565,7 +677,7 @@ py::object adamw_step(const py::list& params, const py::list& states, int bits, 
     if (!operand(params[i], &p) || !p.given || !p.t->is_non_overlapping_and_dense()) return py::none();
     if (i == 0 ? !t.of(p) : !t.owns(p)) return py::none();
     held.push_back(params[i]);
-    held.push_back(attribute(params[i].ptr(), grad_name));
+    held.push_back(py::reinterpret_steal<py::object>(THPVariable_Wrap(p.t->grad())));
     if (!operand(held.back(), &g) || !g.given || !t.owns(g) || g.t->sizes() != p.t->sizes() ||
         g.t->strides() != p.t->strides())
       return py::none();
@@ -587,6 +699,48 @@ py::object adamw_step(const py::list& params, const py::list& states, int bits, 
   const int status = unlocked(MM_SYMBOL(adamw_fn, "mm_adamw_scaled"), table.data(), (int)count, bits, lr, beta1,
                               beta2, eps, decay, 1, maximize, 1, scale.ptr, nullptr, 0, t.stream);
   return status == 0 ? py::object(py::bool_(true)) : py::object(py::int_(status));
+}
+
+using grad_norm_fn = int (*)(const void*, int, int, double, void*, void*, void*, size_t, void*);
+using grad_clip_fn = int (*)(const void*, int, int, double, void*, void*, size_t, void*);
+
+// The norm of the parameters' gradients (those that have one), and the coefficient
+// that clips to max_norm; with `clip` they are scaled by it in place and the norm
+// alone is returned.  None where a gradient is not as usual, or there is none.
+py::object grad_norm(const py::list& params, int order, double max_norm, bool clip) {
+  if (!names().ready) return py::none();
+  std::vector<int64_t> table;
+  std::vector<at::Tensor> held;  // (the program may change the list or a gradient during the call)
+  Target t;
+  table.reserve(2 * params.size());
+  held.reserve(params.size());
+  for (const py::handle& p : params) {
+    if (!THPVariable_Check(p.ptr())) return py::none();
+    const at::Tensor& grad = THPVariable_Unpack(p.ptr()).grad();
+    if (!grad.defined()) continue;
+    const py::object g_ = py::reinterpret_steal<py::object>(THPVariable_Wrap(grad));
+    Operand g;
+    if (!operand(g_, &g) || !g.given || !g.t->is_non_overlapping_and_dense()) return py::none();
+    if (held.empty() ? !t.of(g) : !t.owns(g)) return py::none();
+    held.push_back(grad);
+    table.push_back((int64_t)(intptr_t)g.ptr);
+    table.push_back(grad.numel());
+  }
+  if (held.empty()) return py::none();
+  char* ptr = nullptr;
+  py::object owner = new_storage(t, 2, &ptr);
+  if (!owner) return py::none();
+  const int status =
+      clip ? unlocked(MM_SYMBOL(grad_clip_fn, "mm_grad_clip"), table.data(), (int)held.size(), order, max_norm, ptr,
+                      nullptr, 0, t.stream)
+           : unlocked(MM_SYMBOL(grad_norm_fn, "mm_grad_norm"), table.data(), (int)held.size(), order, max_norm, ptr,
+                      ptr + 4, nullptr, 0, t.stream);
+  if (status != 0) return py::int_(status);
+  const py::tuple none = py::tuple(0);
+  py::object norm = new_tensor(t, owner, none, none, 0);
+  if (!clip) return py::make_tuple(norm, new_tensor(t, owner, none, none, 1));
+  for (const at::Tensor& g : held) g.unsafeGetTensorImpl()->bump_version();
+  return norm;
 }
 
 // The float32 values of 8-bit states, of a parameter's shape and strides (the step
@@ -622,6 +776,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("bind_tensors", &bind_tensors, "Classes that the operators below make their results of");
   m.def("layer_norm", &layer_norm, "mm_layer_norm with its outputs, or None");
   m.def("layer_norm_backward", &layer_norm_backward, "mm_layer_norm_backward with its outputs, or None");
+  m.def("group_norm", &group_norm, "mm_group_norm with its outputs, or None");
+  m.def("group_norm_backward", &group_norm_backward, "mm_group_norm_backward with its outputs, or None");
+  m.def("grad_norm", &grad_norm, "mm_grad_norm or mm_grad_clip over parameters' gradients, or None");
   m.def("linear", &linear, "mm_linear with its outputs, or None");
   m.def("linear_ready", &linear_ready, "Whether linear would take these operands");
   m.def("adamw_step", &adamw_step, "mm_adamw over parameters and their states, or None", py::arg("params"),

@@ -49,9 +49,13 @@ def group_norm(x, num_groups: int, weight=None, bias=None, eps: float = 1e-5, *,
                          f"got {activation!r}")
     ops.require_mm(x, "group_norm")
     if torch.is_grad_enabled():
+        need = x.requires_grad
         for name, t in (("weight", weight), ("bias", bias)):
-            if isinstance(t, torch.Tensor) and t.requires_grad and not isinstance(t, MatrixManTensor):
-                raise RuntimeError(f"MatrixMan/CUDA: group_norm {name} needs a gradient and must be a MatrixMan tensor")
-        if x.requires_grad or any(t is not None and t.requires_grad for t in (weight, bias)):
+            if isinstance(t, torch.Tensor) and t.requires_grad:
+                need = True
+                if not isinstance(t, MatrixManTensor):
+                    raise RuntimeError(f"MatrixMan/CUDA: group_norm {name} needs a gradient and must be a MatrixMan "
+                                       "tensor")
+        if need:
             return _GroupNorm.apply(x, weight, bias, int(num_groups), float(eps), act)
-    return ops.group_norm(x, num_groups, weight, bias, float(eps), act)[0]
+    return ops.group_norm(x, num_groups, weight, bias, float(eps), act, keep=False)[0]

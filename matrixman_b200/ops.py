@@ -705,7 +705,7 @@ def _map_rows(x: MatrixManTensor) -> tuple[MatrixManTensor, bool, int, int]:
     where the strides force it."""
     shape, st = tuple(x.shape), x._logical_strides
     channels, pixels = shape[1], numel(shape[2:])
-    flat = view_strides(shape[2:], st[2:], (pixels,)) if len(shape) > 2 else (channels,)
+    flat = view_strides(shape[2:], st[2:], (pixels,)) if pixels > 1 else (channels,)
     if numel(shape) == 0:
         return x, True, 0, 0
     if flat is not None:
@@ -756,10 +756,13 @@ def _group_check(x, groups: int) -> tuple[int, ...]:
     return shape
 
 
-def group_norm(x, groups: int, weight=None, bias=None, eps=1e-5, act: int = 0):
+def group_norm(x, groups: int, weight=None, bias=None, eps=1e-5, act: int = 0, keep: bool = True):
     """(y, mean, rstd): act(group norm), in x's memory order, and the statistics
-    [N, groups]."""
+    [N, groups] (None unless kept)."""
     groups = int(groups)
+    done = native_call("group_norm", "mm_group_norm", x, groups, weight, bias, eps, act, keep)
+    if done is not None:
+        return done
     shape = _group_check(x, groups)
     rt = x.runtime
     w = _group_vector(rt, weight, shape[1], "weight")
@@ -767,10 +770,13 @@ def group_norm(x, groups: int, weight=None, bias=None, eps=1e-5, act: int = 0):
     xr, last, image, row = _map_rows(x)
     n, c, pixels = shape[0], shape[1], numel(shape[2:])
     y = _map_like(rt, shape, last, x._logical_strides)
-    owner = rt.new_storage(2 * n * groups)  # mean and rstd are kept for the backward pass, y may go
-    mean, rstd = (MatrixManTensor._wrap(owner, (n, groups), i * n * groups, (groups, 1)) for i in (0, 1))
+    mean = rstd = None
+    if keep:  # in a block apart from y's: they are kept for the backward pass, y may go
+        owner = rt.new_storage(2 * n * groups)
+        mean, rstd = (MatrixManTensor._wrap(owner, (n, groups), i * n * groups, (groups, 1)) for i in (0, 1))
     _launch("mm_group_norm", pointer(xr), image, row, n, c, pixels, groups, last, None if w is None else pointer(w),
-            None if b is None else pointer(b), eps, act, pointer(y), pointer(mean), pointer(rstd), None, 0, rt.stream)
+            None if b is None else pointer(b), eps, act, pointer(y),
+            *(None if t is None else pointer(t) for t in (mean, rstd)), None, 0, rt.stream)
     return y, mean, rstd
 
 
@@ -778,6 +784,10 @@ def group_norm_backward(dy, x, mean, rstd, weight, bias, groups: int, mask, act:
     """(dx, dweight, dbias) of group_norm; None where the mask is false.  bias is
     only read with an activation."""
     groups = int(groups)
+    done = native_call("group_norm_backward", "mm_group_norm_backward", dy, x, mean, rstd, weight,
+                       bias if act else None, groups, act, *mask)
+    if done is not None:
+        return done
     shape = _group_check(x, groups)
     for t in (dy, mean, rstd):
         require_f32(require_mm(t, "GroupNorm backward"), "GroupNorm backward")

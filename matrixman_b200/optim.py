@@ -54,10 +54,12 @@ def _norm_order(norm_type) -> int:
     return order
 
 
-def _grads_of(parameters) -> list:
-    """The gradients of an iterable of parameters, or of one; those without are left out."""
-    if isinstance(parameters, torch.Tensor):
-        parameters = [parameters]
+def _as_list(parameters) -> list:
+    """An iterable of parameters, or one."""
+    return [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
+
+
+def _grads_of(parameters: list) -> list:
     return [p.grad for p in parameters if p.grad is not None]
 
 
@@ -90,8 +92,12 @@ def _grad_table(grads: list) -> tuple[array.array, list]:
     return array.array("q", [v for g in held for v in (_pointer(g), numel(g.shape))]), held
 
 
-def _norm_and_coef(grads: list, order: int, max_norm: float) -> tuple[MatrixManTensor, MatrixManTensor]:
-    """The norm and the coefficient that clips to max_norm, on the device."""
+def _norm_of(parameters: list, order: int, max_norm: float) -> tuple[MatrixManTensor, MatrixManTensor]:
+    """The norm of the gradients and the coefficient that clips to max_norm, on the device."""
+    done = ops.native_call("grad_norm", "mm_grad_norm", parameters, order, max_norm, False)
+    if done is not None:
+        return done
+    grads = _grads_of(parameters)
     rt = _grad_runtime(grads)
     table, held = _grad_table(grads)
     owner = rt.new_storage(2)
@@ -105,8 +111,7 @@ def grad_norm(parameters, norm_type: float = 2.0) -> MatrixManTensor:
     """The norm of the gradients of `parameters` (an iterable, or one) as if they were
     one vector, on their device: order 1, 2 or inf, summed in 64 bits.  Parameters
     without a gradient are left out; of no gradients it is 0."""
-    order = _norm_order(norm_type)
-    return _norm_and_coef(_grads_of(parameters), order, 0.0)[0]
+    return _norm_of(_as_list(parameters), _norm_order(norm_type), 0.0)[0]
 
 
 @torch.no_grad()
@@ -122,15 +127,19 @@ def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0,
     max_norm = float(max_norm)
     if not max_norm >= 0.0:
         raise ValueError(f"MatrixMan/CUDA: clip_grad_norm_ max_norm must be non-negative, got {max_norm}")
-    grads = _grads_of(parameters)
-    rt = _grad_runtime(grads)
+    parameters = _as_list(parameters)
     if error_if_nonfinite:
-        if rt.capturing:
+        if _grad_runtime(_grads_of(parameters)).capturing:
             raise RuntimeError("MatrixMan/CUDA: clip_grad_norm_ cannot read the norm back during graph capture")
-        norm = _norm_and_coef(grads, order, 0.0)[0].cpu()
+        norm = _norm_of(parameters, order, 0.0)[0].cpu()
         if not torch.isfinite(norm):
             raise RuntimeError(f"MatrixMan/CUDA: the gradients' norm of order {norm_type} is {norm.item()}, so they are "
                                "not clipped (error_if_nonfinite)")
+    done = ops.native_call("grad_norm", "mm_grad_clip", parameters, order, max_norm, True)
+    if done is not None:
+        return done
+    grads = _grads_of(parameters)
+    rt = _grad_runtime(grads)
     for g in grads:
         if not _is_apart(g):
             raise NotImplementedError("MatrixMan/CUDA: clip_grad_norm_ needs gradients whose elements share no memory, "
@@ -320,8 +329,9 @@ class AdamW(torch.optim.Optimizer):
                 loss = closure()
         scale = None
         if self.max_grad_norm is not None:
-            grads = [p.grad for group in self.param_groups for p in group["params"] if p.grad is not None]
-            self.grad_norm, scale = _norm_and_coef(grads, _lib.NORM_ORDERS[2.0], float(self.max_grad_norm))
+            groups = self.param_groups
+            params = groups[0]["params"] if len(groups) == 1 else [p for group in groups for p in group["params"]]
+            self.grad_norm, scale = _norm_of(params, _lib.NORM_ORDERS[2.0], float(self.max_grad_norm))
         for group in self.param_groups:
             params = [p for p in group["params"] if p.grad is not None]
             if not params:

@@ -340,3 +340,23 @@ def test_a_refused_limit_and_checkpoints(mm):
     opt.step()
     loaded.step()
     assert all(torch.equal(p.detach().cpu(), q.detach().cpu()) for p, q in zip(params, other))
+
+
+@pytest.mark.parametrize("order", ORDERS)
+def test_one_step_calls_and_the_python_code_agree(mm, monkeypatch, order):
+    from matrixman_b200 import ops
+    grads = tensors([(784, 51), (51,), (), (0, 3), (7, 3, 5)], seed=2)
+
+    def both(params):
+        first = mm.optim.grad_norm(params, order)
+        return first, mm.optim.clip_grad_norm_(iter(params), 0.5, order), *(p.grad for p in params[1:])
+
+    def fresh():  # one without a gradient in front, one whose gradient is transposed
+        got = params_of(mm, grads[:1] + grads)
+        got[0].grad = None
+        got[1].grad = mm.to_device(grads[0].t().contiguous()).t()
+        return got
+
+    native = both(fresh())
+    monkeypatch.setattr(ops, "native_call", lambda *a: None)
+    assert all(torch.equal(a.cpu(), b.cpu()) and a.shape == b.shape for a, b in zip(native, both(fresh())))

@@ -18,7 +18,7 @@ def test_group_norm_checks():
         return f(a["x"], a["xi"], a["xr"], a["n"], a["c"], a["px"], a["g"], 1, FAKE, FAKE, 1e-5, a["act"], a["y"],
                  a["mean"], a["rstd"], a["work"], a["size"], None)
 
-    for name in ("x", "y", "mean", "rstd"):
+    for name in ("x", "y", "mean", "rstd"):  # (mean and rstd go together)
         assert call(**{name: None}) == _lib.MM_ERR_INVALID
     for name in ("xi", "xr", "n", "c", "px"):
         assert call(**{name: -1}) == _lib.MM_ERR_INVALID

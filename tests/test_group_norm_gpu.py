@@ -388,3 +388,34 @@ def test_the_backward_pass_keeps_the_statistics_but_not_the_output(mm):
     assert live() - start <= 4 * 64 * 32 * 32 + 3 * 512 + 2 * 4 * 64 * 8  # s, mean, rstd
     s.sum(dim=0).sum(dim=0).sum(dim=0).backward()
     assert x.grad.shape == x.shape
+
+
+@pytest.mark.parametrize("act", ["none", "silu"])
+def test_one_step_calls_and_the_python_code_agree(mm, monkeypatch, act):
+    """The same bits, shapes and strides through the C++ calls and without them."""
+    from matrixman_b200 import ops
+    host = randn(4, 12, 6, 5, seed=1)
+    nhwc = mm.to_device(host.permute(0, 2, 3, 1).contiguous())
+    w, b = mm.to_device(randn(12, seed=2)), mm.to_device(randn(12, seed=3))
+    wide = mm.to_device(randn(4, 6, 5, 20, seed=4)).permute(0, 3, 1, 2)
+    rows = mm.to_device(randn(9, 12, seed=5))
+    maps = [mm.to_device(host), nhwc.permute(0, 3, 1, 2), wide[:, 3:15], wide[:, 4:16, 1:], rows, rows[:, :, None],
+            mm.to_device(randn(3, 12, 7, seed=6)), mm.to_device(randn(2, 12, 3, 2, 4, seed=7)), rows[:1].expand(5, 12),
+            mm.to_device(randn(12, 9, seed=8)).t(), mm.to_device(randn(5, 12, 1, 8, seed=9)),
+            mm.to_device(randn(3, 12, 4, 5, seed=10)).transpose(2, 3)]
+
+    def all_of(x):
+        x = x.detach().requires_grad_(True)
+        p, q = w.detach().requires_grad_(True), b.detach().requires_grad_(True)
+        y = mm.group_norm(x, 3, p, q, EPS, activation=act)
+        with torch.no_grad():
+            plain = mm.group_norm(x, 3, p, q, EPS, activation=act)
+        dy = mm.to_device(randn(*x.shape, seed=20))
+        return (y, plain, *torch.autograd.grad(y, (x, p, q), dy))
+
+    native = [all_of(x) for x in maps]
+    monkeypatch.setattr(ops, "native_call", lambda *a: None)
+    for x, got in zip(maps, native):
+        for one, other in zip(got, all_of(x)):
+            assert one.shape == other.shape and one._logical_strides == other._logical_strides
+            assert torch.equal(one.detach().cpu(), other.detach().cpu())
