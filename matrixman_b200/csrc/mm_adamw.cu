@@ -162,13 +162,20 @@ __device__ __forceinline__ int aw_find(const AwTable<MOST>& tab, uint32_t chunk)
   return lo;
 }
 
+// The block's chunk: after a pass over the gradients from the last to the first, since
+// L2 still holds the last.
+__device__ __forceinline__ uint32_t aw_chunk(const AwScalars& a) {
+  return a.scale ? gridDim.x - 1 - blockIdx.x : blockIdx.x;
+}
+
 template <int MOST>
 __global__ void __launch_bounds__(AW_THREADS) adamw32_kernel(const __grid_constant__ AwTable<MOST> tab,
                                                              const float2* __restrict__ coefs, AwScalars a) {
-  const int k = aw_find(tab, blockIdx.x);
+  const uint32_t chunk = aw_chunk(a);
+  const int k = aw_find(tab, chunk);
   const AwTensor& t = tab.t[k];
   const float2 coef = coefs[k];
-  const int64_t base = (int64_t)(blockIdx.x - t.first) * AW_CHUNK;
+  const int64_t base = (int64_t)(chunk - t.first) * AW_CHUNK;
   float* p = t.p + base;
   const float* g = t.g + base;
   float* m = (float*)t.m + base;
@@ -275,12 +282,13 @@ __device__ __forceinline__ void aw_encode_block(const float* m, const float* r, 
 template <int MOST>
 __global__ void __launch_bounds__(AW_THREADS) adamw8_kernel(const __grid_constant__ AwTable<MOST> tab,
                                                             const float2* __restrict__ coefs, AwScalars a) {
-  const int k = aw_find(tab, blockIdx.x);
+  const uint32_t chunk = aw_chunk(a);
+  const int k = aw_find(tab, chunk);
   const AwTensor& t = tab.t[k];
   const float2 coef = coefs[k];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const bool vec = t.aligned != 0;
-  const int64_t base = (int64_t)(blockIdx.x - t.first) * AW_CHUNK8 + warp * AW_BLOCK;
+  const int64_t base = (int64_t)(chunk - t.first) * AW_CHUNK8 + warp * AW_BLOCK;
   if (base >= t.n) return;
   const int64_t block = base / AW_BLOCK;
   const int left = (int)min((int64_t)AW_BLOCK, t.n - base);

@@ -28,14 +28,13 @@ namespace mm {
 
 constexpr int GR_THREADS = 256;
 constexpr int GR_CHUNK = 4096;      // elements
-constexpr int GR_EACH = 8;          // float4 loads in flight per thread
+constexpr int GR_EACH = 8, GR_SCALE = 4;  // float4 loads in flight per thread: for the norm, to scale
 constexpr int GR_FEW = 16, GR_MANY = 1000;  // tensors of a launch; its parameters may hold up to 32,764 bytes
 
 struct GrTensor {
   float* p;
   int64_t n;
-  uint32_t first;    // first chunk
-  uint32_t aligned;  // 16-byte aligned
+  uint32_t first;  // first chunk
 };
 
 template <int MOST>
@@ -78,56 +77,63 @@ __device__ __forceinline__ double gr_block(double s, double* sm) {
   return s;
 }
 
-// Calls f(p, n, aligned) for each tensor's part of the block's range of chunks.
+// Calls f(p, n) for each tensor's part of the block's range of chunks, the last
+// part first where `back`.
 template <int MOST, class F>
-__device__ __forceinline__ void gr_walk(const GrTable<MOST>& tab, F f) {
+__device__ __forceinline__ void gr_walk(const GrTable<MOST>& tab, bool back, F f) {
   const uint32_t from = (uint32_t)((uint64_t)tab.chunks * blockIdx.x / gridDim.x);
   const uint32_t to = (uint32_t)((uint64_t)tab.chunks * (blockIdx.x + 1) / gridDim.x);
-  int lo = 0, hi = tab.count - 1;
+  if (from == to) return;
+  const uint32_t start = back ? to - 1 : from;
+  int lo = 0, hi = tab.count - 1;  // the last tensor whose first chunk is not behind `start`
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
-    if (tab.t[mid].first <= from) lo = mid;
+    if (tab.t[mid].first <= start) lo = mid;
     else hi = mid - 1;
   }
-  for (int k = lo; k < tab.count && tab.t[k].first < to; ++k) {
+  for (int k = lo; k >= 0 && k < tab.count; k += back ? -1 : 1) {
     const GrTensor& t = tab.t[k];
     const int64_t begin = (int64_t)(max(from, t.first) - t.first) * GR_CHUNK;
-    const int64_t end = min(t.n, (int64_t)(to - t.first) * GR_CHUNK);
-    if (begin < end) f(t.p + begin, end - begin, t.aligned != 0);
+    const int64_t end = min(t.n, (int64_t)(max(to, t.first) - t.first) * GR_CHUNK);
+    if (begin < end) f(t.p + begin, end - begin);
+    if (back ? t.first <= from : t.first >= to) break;
   }
 }
+
+// The part's elements in front of the first 16-byte boundary, and the vectors behind it.
+struct GrPart {
+  int64_t head, n4, tail;  // tail: where the rest begins
+  __device__ __forceinline__ GrPart(const float* p, int64_t n) {
+    head = min(n, (int64_t)((4 - ((uintptr_t)p >> 2 & 3)) & 3));
+    n4 = (n - head) / 4;
+    tail = head + 4 * n4;
+  }
+};
 
 template <int ORDER, int MOST>
 __global__ void __launch_bounds__(GR_THREADS) grad_norm_kernel(const __grid_constant__ GrTable<MOST> tab, double* part) {
   __shared__ double sm[GR_THREADS / 32];
   double s = 0.0;
-  gr_walk(tab, [&](const float* p, int64_t n, bool aligned) {
+  gr_walk(tab, false, [&](const float* p, int64_t n) {
+    const GrPart at(p, n);
+    const float4* p4 = reinterpret_cast<const float4*>(p + at.head);
     int64_t i = threadIdx.x;
-    if (aligned) {
-      const float4* p4 = reinterpret_cast<const float4*>(p);
-      const int64_t n4 = n / 4;
-      for (; i + (GR_EACH - 1) * GR_THREADS < n4; i += GR_EACH * GR_THREADS) {
-        float4 v[GR_EACH];
+    auto take = [&](const float4& v) {
+      gr_add<ORDER>(s, v.x);
+      gr_add<ORDER>(s, v.y);
+      gr_add<ORDER>(s, v.z);
+      gr_add<ORDER>(s, v.w);
+    };
+    for (; i + (GR_EACH - 1) * GR_THREADS < at.n4; i += GR_EACH * GR_THREADS) {
+      float4 v[GR_EACH];
 #pragma unroll
-        for (int e = 0; e < GR_EACH; ++e) v[e] = p4[i + e * GR_THREADS];
+      for (int e = 0; e < GR_EACH; ++e) v[e] = p4[i + e * GR_THREADS];
 #pragma unroll
-        for (int e = 0; e < GR_EACH; ++e) {
-          gr_add<ORDER>(s, v[e].x);
-          gr_add<ORDER>(s, v[e].y);
-          gr_add<ORDER>(s, v[e].z);
-          gr_add<ORDER>(s, v[e].w);
-        }
-      }
-      for (; i < n4; i += GR_THREADS) {
-        const float4 v = p4[i];
-        gr_add<ORDER>(s, v.x);
-        gr_add<ORDER>(s, v.y);
-        gr_add<ORDER>(s, v.z);
-        gr_add<ORDER>(s, v.w);
-      }
-      i = n4 * 4 + threadIdx.x;
+      for (int e = 0; e < GR_EACH; ++e) take(v[e]);
     }
-    for (; i < n; i += GR_THREADS) gr_add<ORDER>(s, p[i]);
+    for (; i < at.n4; i += GR_THREADS) take(p4[i]);
+    if (threadIdx.x < at.head) gr_add<ORDER>(s, p[threadIdx.x]);
+    if (threadIdx.x < n - at.tail) gr_add<ORDER>(s, p[at.tail + threadIdx.x]);
   });
   s = gr_block<ORDER, GR_THREADS>(s, sm);
   if (threadIdx.x == 0) part[blockIdx.x] = s;
@@ -171,26 +177,25 @@ __global__ void __launch_bounds__(GR_THREADS) grad_scale_kernel(const __grid_con
   const float total = gr_total<ORDER, GR_THREADS>(part, count, sm), c = gr_coef(total, max_norm);
   if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = total;
   if (c == 1.f) return;  // every value stays what it is
-  gr_walk(tab, [&](float* p, int64_t n, bool aligned) {
-    int64_t i = threadIdx.x;
-    if (aligned) {
-      float4* p4 = reinterpret_cast<float4*>(p);
-      const int64_t n4 = n / 4;
-      for (; i + 3 * GR_THREADS < n4; i += 4 * GR_THREADS) {
-        float4 v[4];
+  // (from the end, which the norm's pass read last: what L2 still holds of it comes from there)
+  gr_walk(tab, true, [&](float* p, int64_t n) {
+    const GrPart at(p, n);
+    float4* p4 = reinterpret_cast<float4*>(p + at.head);
+    int64_t left = at.n4;
+    for (; left >= GR_SCALE * GR_THREADS; left -= GR_SCALE * GR_THREADS) {
+      float4 v[GR_SCALE];
+      float4* q = p4 + left - GR_SCALE * GR_THREADS + threadIdx.x;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = p4[i + e * GR_THREADS];
+      for (int e = 0; e < GR_SCALE; ++e) v[e] = q[e * GR_THREADS];
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          p4[i + e * GR_THREADS] = make_float4(v[e].x * c, v[e].y * c, v[e].z * c, v[e].w * c);
-      }
-      for (; i < n4; i += GR_THREADS) {
-        const float4 v = p4[i];
-        p4[i] = make_float4(v.x * c, v.y * c, v.z * c, v.w * c);
-      }
-      i = n4 * 4 + threadIdx.x;
+      for (int e = 0; e < GR_SCALE; ++e) q[e * GR_THREADS] = make_float4(v[e].x * c, v[e].y * c, v[e].z * c, v[e].w * c);
     }
-    for (; i < n; i += GR_THREADS) p[i] *= c;
+    for (int64_t i = threadIdx.x; i < left; i += GR_THREADS) {
+      const float4 v = p4[i];
+      p4[i] = make_float4(v.x * c, v.y * c, v.z * c, v.w * c);
+    }
+    if (threadIdx.x < at.head) p[threadIdx.x] *= c;
+    if (threadIdx.x < n - at.tail) p[at.tail + threadIdx.x] *= c;
   });
 }
 
@@ -214,7 +219,7 @@ template <int MOST>
 static int gr_fill(const mm_grad_t* in, int count, GrTable<MOST>* tab) {
   int64_t chunks = 0;
   for (int i = 0; i < count; ++i) {
-    tab->t[i] = {in[i].data, in[i].numel, (uint32_t)chunks, (uintptr_t)in[i].data % 16 == 0};
+    tab->t[i] = {in[i].data, in[i].numel, (uint32_t)chunks};
     chunks += (in[i].numel + GR_CHUNK - 1) / GR_CHUNK;
     if (chunks > INT32_MAX) return fail(MM_ERR_UNSUPPORTED, "mm_grad_norm: too many elements in one call");
   }
