@@ -605,6 +605,25 @@ def _native_group_norm_backward(grad_out, x, mean, rstd, weight, N, C, HxW, grou
     return ops.group_norm_backward(grad_out, x, mean, rstd, weight, None, group, output_mask)
 
 
+# -- norms of whole tensors (torch.nn.utils.clip_grad_norm_) ------------------
+
+@_register(aten.linalg_vector_norm.default)
+def _linalg_vector_norm(x, ord=2, dim=None, keepdim=False, dtype=None):
+    from . import optim
+    rank = x.dim()
+    if dim is not None and {_norm_dim(d, rank) for d in dim} != set(range(rank)):
+        raise NotImplementedError("MatrixMan/CUDA: linalg_vector_norm over some dimensions is not implemented")
+    if dtype is not None and dtype != torch.float32:
+        raise NotImplementedError("MatrixMan/CUDA: linalg_vector_norm supports float32 only")
+    norm = optim.tensor_norm(x, ord)
+    return _view(norm, (1,) * rank, (1,) * rank) if keepdim else norm
+
+
+@_register(aten.reciprocal.default)
+def _reciprocal(x):
+    return ops.binary("div", 1.0, x)
+
+
 # -- torch.optim.AdamW / Adam with fused=True ---------------------------------
 
 @_register(aten._foreach_add_.Scalar)

@@ -92,12 +92,7 @@ def _grad_table(grads: list) -> tuple[array.array, list]:
     return array.array("q", [v for g in held for v in (_pointer(g), numel(g.shape))]), held
 
 
-def _norm_of(parameters: list, order: int, max_norm: float) -> tuple[MatrixManTensor, MatrixManTensor]:
-    """The norm of the gradients and the coefficient that clips to max_norm, on the device."""
-    done = ops.native_call("grad_norm", "mm_grad_norm", parameters, order, max_norm, False)
-    if done is not None:
-        return done
-    grads = _grads_of(parameters)
+def _norms(grads: list, order: int, max_norm: float) -> tuple[MatrixManTensor, MatrixManTensor]:
     rt = _grad_runtime(grads)
     table, held = _grad_table(grads)
     owner = rt.new_storage(2)
@@ -105,6 +100,19 @@ def _norm_of(parameters: list, order: int, max_norm: float) -> tuple[MatrixManTe
     ops._launch("mm_grad_norm", table.buffer_info()[0], len(held), order, max_norm, _pointer(norm), _pointer(coef),
                 None, 0, rt.stream)
     return norm, coef
+
+
+def tensor_norm(t: MatrixManTensor, norm_type: float = 2.0) -> MatrixManTensor:
+    """The norm of one tensor's elements."""
+    return _norms([t], _norm_order(norm_type), 0.0)[0]
+
+
+def _norm_of(parameters: list, order: int, max_norm: float) -> tuple[MatrixManTensor, MatrixManTensor]:
+    """The norm of the gradients and the coefficient that clips to max_norm, on the device."""
+    done = ops.native_call("grad_norm", "mm_grad_norm", parameters, order, max_norm, False)
+    if done is not None:
+        return done
+    return _norms(_grads_of(parameters), order, max_norm)
 
 
 def grad_norm(parameters, norm_type: float = 2.0) -> MatrixManTensor:

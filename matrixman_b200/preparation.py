@@ -25,7 +25,8 @@ What is new (B200 design):
   ``PreparedSPPF`` (one fused 5/9/13 pooling kernel into the concat buffer),
   ``PreparedDetect`` (box/class branches write one feature buffer per level;
   DFL + dist2bbox + sigmoid in one kernel), ``PreparedBasicBlock`` (ResNet),
-  ``PreparedLinear`` (GEMM + bias + ReLU).
+  ``PreparedLinear`` (GEMM + bias + ReLU), ``PreparedGroupNorm`` (group norm +
+  activation).
 * Weights are prepacked to KRSC (and to tf32 hi/lo planes for the tcgen05
   kernel) and uploaded once per device.
 * With ``config.cuda_graphs`` the prepared forward is captured into a CUDA
@@ -637,6 +638,44 @@ def _downsample_unit(ds):
     return None
 
 
+class PreparedGroupNorm(nn.Module):
+    """GroupNorm and the activation behind it in one call, in the order of the maps
+    (channels last behind a prepared convolution)."""
+
+    def __init__(self, norm: nn.GroupNorm, activation: str = "none", source=None):
+        super().__init__()
+        self.num_groups = int(norm.num_groups)
+        self.num_channels = int(norm.num_channels)
+        self.eps = float(norm.eps)
+        self.activation = activation
+        for name in ("weight", "bias"):
+            value = getattr(norm, name)
+            self.register_buffer(name, None if value is None else value.detach().to(torch.float32).contiguous())
+        self._device_parameters: dict[int, tuple] = {}
+        _copy_routing_attrs(self, source)
+
+    def device_parameters(self, rt) -> tuple:
+        entry = self._device_parameters.get(rt.index)
+        if entry is None:
+            entry = tuple(None if v is None else
+                          MatrixManTensor(rt.upload(v, kind=_lib.POOL_PARAMETER, sync=True), tuple(v.shape), 0, (1,))
+                          for v in (self.weight, self.bias))
+            self._device_parameters[rt.index] = entry
+        return entry
+
+    def forward(self, x):
+        weight, bias = self.device_parameters(ops.require_mm(x, "GroupNorm").runtime)
+        return ops.group_norm(x, self.num_groups, weight, bias, self.eps, _lib.LINEAR_ACTS[self.activation],
+                              keep=False)[0]
+
+
+def _norm_activation(module) -> str | None:
+    """The activation that a group norm in front of `module` takes over."""
+    if type(module) is nn.GELU:
+        return {"none": "gelu", "tanh": "gelu_tanh"}.get(module.approximate)
+    return {nn.SiLU: "silu", nn.ReLU: "relu", nn.Sigmoid: "sigmoid"}.get(type(module))
+
+
 # ---------------------------------------------------------------------------
 # Module replacement
 # ---------------------------------------------------------------------------
@@ -723,7 +762,7 @@ def _replace(parent: nn.Module, report: PreparationReport, aliases: Counter) -> 
             setattr(parent, name, prepared)
             continue
         _replace(module, report, aliases)
-    # Containers: fuse Conv2d/Linear with a following activation.
+    # Containers: fuse Conv2d/Linear/GroupNorm with a following activation.
     if isinstance(parent, nn.Sequential):
         keys = list(parent._modules.keys())
         i = 0
@@ -741,6 +780,14 @@ def _replace(parent: nn.Module, report: PreparationReport, aliases: Counter) -> 
                 parent._modules[keys[i]] = PreparedLinear(m, code if code is not None else _lib.ACT_NONE)
                 report.linear_units_prepared += 1
                 if code is not None:
+                    parent._modules[keys[i + 1]] = nn.Identity()
+                    i += 1
+            elif type(m) is nn.GroupNorm and aliases[id(m)] <= 1 and all(
+                    v is None or v.device.type == "cpu" for v in (m.weight, m.bias)):
+                act = _norm_activation(nxt)
+                parent._modules[keys[i]] = PreparedGroupNorm(m, act or "none")
+                report.block_units_prepared["GroupNorm"] += 1
+                if act is not None:
                     parent._modules[keys[i + 1]] = nn.Identity()
                     i += 1
             i += 1
