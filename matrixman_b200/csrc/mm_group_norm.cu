@@ -237,20 +237,22 @@ __global__ void __launch_bounds__(T) gn_join_moments_kernel(GnArgs a) {
   const int image = blockIdx.x / a.groups, group = blockIdx.x % a.groups;
   const float* pu = a.part + (int64_t)image * a.segs * a.channels + group * a.each;
   const float* pv = pu + a.segs_n * a.channels;
-  const int64_t count = (int64_t)a.segs * a.each;
+  const unsigned count = (unsigned)a.segs * a.each, each = a.each;
   const float m = (float)a.pixels * (float)a.each;
   float s = 0.f, q = 0.f;
-  for (int64_t i = threadIdx.x; i < count; i += T) {
-    const int seg = (int)(i / a.each);
+#pragma unroll 4
+  for (unsigned i = threadIdx.x; i < count; i += T) {
+    const int seg = (int)(i / each);
     const float n = (float)min(a.seg, a.pixels - seg * a.seg);
-    s += n * pu[(int64_t)seg * a.channels + i % a.each];
+    s += n * pu[(int64_t)seg * a.channels + (i - seg * each)];
   }
   gn_sum2<T>(s, q, sm);
   const float mean = s / m;  // (divided, so that a constant's own mean is exact wherever the sum is)
   s = q = 0.f;
-  for (int64_t i = threadIdx.x; i < count; i += T) {
-    const int seg = (int)(i / a.each);
-    const int64_t at = (int64_t)seg * a.channels + i % a.each;
+#pragma unroll 4
+  for (unsigned i = threadIdx.x; i < count; i += T) {
+    const int seg = (int)(i / each);
+    const int64_t at = (int64_t)seg * a.channels + (i - seg * each);
     const float n = (float)min(a.seg, a.pixels - seg * a.seg), d = pu[at] - mean;
     s += pv[at] + n * d * d;
   }
@@ -400,13 +402,14 @@ __global__ void __launch_bounds__(GN_THREADS) gn_join_sums_kernel(GnArgs a, int 
   const int id = blockIdx.x - columns, image = id / a.groups, group = id % a.groups;
   const float* pu = a.part + (int64_t)image * a.segs * a.channels + group * a.each;
   const float* pv = pu + a.segs_n * a.channels;
-  const int64_t count = (int64_t)a.segs * a.each;
+  const unsigned count = (unsigned)a.segs * a.each, each = a.each;
   const float inv = 1.f / ((float)a.pixels * (float)a.each);
   float s1 = 0.f, s2 = 0.f;
 #pragma unroll 4
-  for (int64_t i = threadIdx.x; i < count; i += GN_THREADS) {
-    const int64_t at = i / a.each * a.channels + i % a.each;
-    const float w = a.w ? a.w[group * a.each + i % a.each] : 1.f;
+  for (unsigned i = threadIdx.x; i < count; i += GN_THREADS) {
+    const unsigned seg = i / each, c = i - seg * each;
+    const int64_t at = (int64_t)seg * a.channels + c;
+    const float w = a.w ? a.w[group * a.each + c] : 1.f;
     s1 += w * pu[at];
     s2 += w * pv[at];
   }

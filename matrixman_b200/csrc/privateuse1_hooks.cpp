@@ -704,10 +704,12 @@ py::object adamw_step(const py::list& params, const py::list& states, int bits, 
 using grad_norm_fn = int (*)(const void*, int, int, double, void*, void*, void*, size_t, void*);
 using grad_clip_fn = int (*)(const void*, int, int, double, void*, void*, size_t, void*);
 
-// The norm of the parameters' gradients (those that have one), and the coefficient
-// that clips to max_norm; with `clip` they are scaled by it in place and the norm
-// alone is returned.  None where a gradient is not as usual, or there is none.
-py::object grad_norm(const py::list& params, int order, double max_norm, bool clip) {
+using norm_size_fn = int (*)(int, size_t*);
+
+// The norm of the parameters' gradients (those that have one), and, if wanted, the
+// coefficient that clips to max_norm (else None); with `clip` they are scaled by it in
+// place.  None where a gradient is not as usual, or there is none.
+py::object grad_norm(const py::list& params, int order, double max_norm, bool coef, bool clip) {
   if (!names().ready) return py::none();
   std::vector<int64_t> table;
   std::vector<at::Tensor> held;  // (the program may change the list or a gradient during the call)
@@ -727,20 +729,24 @@ py::object grad_norm(const py::list& params, int order, double max_norm, bool cl
     table.push_back(grad.numel());
   }
   if (held.empty()) return py::none();
+  // Norm, coefficient and workspace in one block.
+  constexpr size_t head = 256;
+  size_t size = 0;
+  if (MM_SYMBOL(norm_size_fn, "mm_grad_norm_workspace_size")((int)held.size(), &size) != 0) return py::none();
   char* ptr = nullptr;
-  py::object owner = new_storage(t, 2, &ptr);
+  py::object owner = new_storage(t, (int64_t)((head + size + 3) / 4), &ptr);
   if (!owner) return py::none();
   const int status =
       clip ? unlocked(MM_SYMBOL(grad_clip_fn, "mm_grad_clip"), table.data(), (int)held.size(), order, max_norm, ptr,
-                      nullptr, 0, t.stream)
+                      ptr + head, size, t.stream)
            : unlocked(MM_SYMBOL(grad_norm_fn, "mm_grad_norm"), table.data(), (int)held.size(), order, max_norm, ptr,
-                      ptr + 4, nullptr, 0, t.stream);
+                      coef ? ptr + 4 : nullptr, ptr + head, size, t.stream);
   if (status != 0) return py::int_(status);
+  if (clip)
+    for (const at::Tensor& g : held) g.unsafeGetTensorImpl()->bump_version();
   const py::tuple none = py::tuple(0);
   py::object norm = new_tensor(t, owner, none, none, 0);
-  if (!clip) return py::make_tuple(norm, new_tensor(t, owner, none, none, 1));
-  for (const at::Tensor& g : held) g.unsafeGetTensorImpl()->bump_version();
-  return norm;
+  return py::make_tuple(norm, coef ? new_tensor(t, owner, none, none, 1) : py::none());
 }
 
 // The float32 values of 8-bit states, of a parameter's shape and strides (the step

@@ -13,7 +13,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib, ops
-from .tensor import MatrixManTensor
+from .tensor import MatrixManTensor, numel
 
 
 class _GroupNorm(torch.autograd.Function):
@@ -30,6 +30,25 @@ class _GroupNorm(torch.autograd.Function):
         x, weight, bias, mean, rstd = ctx.saved_tensors
         mask = ctx.needs_input_grad[:3]
         return (*ops.group_norm_backward(dy, x, mean, rstd, weight, bias, ctx.groups, mask, ctx.act), None, None, None)
+
+
+def _torch_group_norm(x, num_groups, weight=None, bias=None, eps=1e-5, cudnn_enabled=True):
+    """torch.nn.functional.group_norm on MatrixMan tensors.  ATen's own composite
+    copies channels-last maps and gradients to channels first in its backward pass."""
+    ops.require_mm(x, "GroupNorm")
+    if torch.is_grad_enabled():
+        need = [t for t in (x, weight, bias) if t is not None and t.requires_grad]
+        if not all(isinstance(t, MatrixManTensor) for t in need):
+            # Parameters on the CPU: ATen's autograd knows which gradients are asked for.
+            shape = tuple(x.shape)
+            return torch.native_group_norm(x, weight, bias, *shape[:2], numel(shape[2:]), num_groups, eps)[0]
+        if need:
+            return _GroupNorm.apply(x, weight, bias, num_groups, eps, 0)
+    return ops.group_norm(x, num_groups, weight, bias, eps, keep=False)[0]
+
+
+_library = torch.library.Library("aten", "IMPL", "AutogradPrivateUse1")
+_library.impl("group_norm", _torch_group_norm)
 
 
 def group_norm(x, num_groups: int, weight=None, bias=None, eps: float = 1e-5, *,

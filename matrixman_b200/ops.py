@@ -799,6 +799,9 @@ def group_norm_backward(dy, x, mean, rstd, weight, bias, groups: int, mask, act:
         raise RuntimeError("MatrixMan/CUDA: GroupNorm backward statistics do not match the input's groups")
     mean, rstd = (t if is_contiguous(t.shape, t._logical_strides) else materialize(t) for t in (mean, rstd))
     need_x, need_w, need_b = mask
+    if (need_w and not isinstance(weight, MatrixManTensor)) or (
+            need_b and isinstance(bias, torch.Tensor) and not isinstance(bias, MatrixManTensor)):
+        raise RuntimeError("MatrixMan/CUDA: GroupNorm parameters that need a gradient must be MatrixMan tensors")
     w = _group_vector(rt, weight, c, "weight")
     b = _group_vector(rt, bias, c, "bias") if act else None
     xr, last, xi, xs = _map_rows(x)

@@ -107,9 +107,12 @@ def tensor_norm(t: MatrixManTensor, norm_type: float = 2.0) -> MatrixManTensor:
     return _norms([t], _norm_order(norm_type), 0.0)[0]
 
 
-def _norm_of(parameters: list, order: int, max_norm: float) -> tuple[MatrixManTensor, MatrixManTensor]:
-    """The norm of the gradients and the coefficient that clips to max_norm, on the device."""
-    done = ops.native_call("grad_norm", "mm_grad_norm", parameters, order, max_norm, False)
+def _norm_of(parameters: list, order: int, max_norm: float | None = None) -> tuple:
+    """The norm of the gradients and the coefficient that clips to max_norm (if given),
+    on the device."""
+    coef = max_norm is not None
+    max_norm = max_norm if coef else 0.0
+    done = ops.native_call("grad_norm", "mm_grad_norm", parameters, order, max_norm, coef, False)
     if done is not None:
         return done
     return _norms(_grads_of(parameters), order, max_norm)
@@ -119,7 +122,7 @@ def grad_norm(parameters, norm_type: float = 2.0) -> MatrixManTensor:
     """The norm of the gradients of `parameters` (an iterable, or one) as if they were
     one vector, on their device: order 1, 2 or inf, summed in 64 bits.  Parameters
     without a gradient are left out; of no gradients it is 0."""
-    return _norm_of(_as_list(parameters), _norm_order(norm_type), 0.0)[0]
+    return _norm_of(_as_list(parameters), _norm_order(norm_type))[0]
 
 
 @torch.no_grad()
@@ -139,13 +142,13 @@ def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0,
     if error_if_nonfinite:
         if _grad_runtime(_grads_of(parameters)).capturing:
             raise RuntimeError("MatrixMan/CUDA: clip_grad_norm_ cannot read the norm back during graph capture")
-        norm = _norm_of(parameters, order, 0.0)[0].cpu()
+        norm = _norm_of(parameters, order)[0].cpu()
         if not torch.isfinite(norm):
             raise RuntimeError(f"MatrixMan/CUDA: the gradients' norm of order {norm_type} is {norm.item()}, so they are "
                                "not clipped (error_if_nonfinite)")
-    done = ops.native_call("grad_norm", "mm_grad_clip", parameters, order, max_norm, True)
+    done = ops.native_call("grad_norm", "mm_grad_clip", parameters, order, max_norm, False, True)
     if done is not None:
-        return done
+        return done[0]
     grads = _grads_of(parameters)
     rt = _grad_runtime(grads)
     for g in grads:

@@ -419,3 +419,20 @@ def test_one_step_calls_and_the_python_code_agree(mm, monkeypatch, act):
         for one, other in zip(got, all_of(x)):
             assert one.shape == other.shape and one._logical_strides == other._logical_strides
             assert torch.equal(one.detach().cpu(), other.detach().cpu())
+
+
+def test_torch_functional_keeps_channels_last(mm):
+    """No copy to another order on the way, forward or backward."""
+    x, w, b, dy = inputs(2, 16, (9, 7), 4, "none")
+    dx = on_device(mm, x, True).detach().requires_grad_(True)
+    y = F.group_norm(dx, 4)
+    grad, = torch.autograd.grad(y, dx, on_device(mm, dy, True))
+    assert y._logical_strides == dx._logical_strides == grad._logical_strides
+    module = torch.nn.GroupNorm(4, 16)  # parameters on the CPU: forward and dx work, their own gradients do not
+    y = module(dx)
+    want = oracle(x, 4, torch.ones(16), torch.zeros(16), dy)
+    check("y", y.detach().cpu(), want["y"])
+    check("dx", torch.autograd.grad(y, dx, on_device(mm, dy, True), retain_graph=True)[0].cpu(), want["dx"])
+    for p in module.parameters():
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(y, p, on_device(mm, dy, True), retain_graph=True)
