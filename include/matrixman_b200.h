@@ -588,18 +588,20 @@ int mm_conv2d_tc_region(const mm_tensor_t* x, const float* w_hi, const float* w_
  * frees its tensor memory and returns, and the host reads the code here. */
 int mm_kernel_error(int device, int* code_out, int clear);
 
-/* A word of host memory that a kernel of mm_linear or mm_linear_backward sets to
- * its code (101 to 105) when it gives up a bounded wait, after which outputs of
- * that call are incomplete.  Readable without a call once the stream has been
+/* A word of host memory that a kernel of mm_linear or mm_linear_backward (codes 101
+ * to 105), mm_group_norm or mm_group_norm_backward (111) sets to its code when it
+ * gives up a bounded wait, after which outputs of that call are incomplete.  Readable without a call once the stream has been
  * waited for; mm_kernel_error reports it too, and clears it. */
 int mm_fault_word(int device, int** word_out);
 
-/* Test hook for the bounded-wait error path of mm_conv2d_tc, and of mm_linear and
- * mm_linear_backward where they run on the tensor cores (no counterpart in
+/* Test hook for the bounded-wait error path of mm_conv2d_tc, of mm_linear and
+ * mm_linear_backward where they run on the tensor cores, and of mm_group_norm and
+ * mm_group_norm_backward where clusters join their blocks' sums (no counterpart in
  * the reference): for later launches on `device`, the budget of every
- * device-side wait (wait_ns <= 0 restores the default 200 ms) and, when
- * drop_first_load != 0, CTA 0 leaves its first k-block's loads unissued so that
- * the waits for that stage run out: the kernel records an error code (read
+ * device-side wait (wait_ns <= 0 restores the defaults, 200 ms and at most 2 s) and, when
+ * drop_first_load != 0, CTA 0 leaves its first k-block's loads unissued (group norm:
+ * each cluster's first block gives the others nothing) so that
+ * the waits for it run out: the kernel records an error code (read
  * with mm_kernel_error), finishes its own in-flight copies and MMAs, frees its
  * tensor memory and returns.  Not for production use. */
 int mm_debug_tc_fault(int device, int64_t wait_ns, int drop_first_load);

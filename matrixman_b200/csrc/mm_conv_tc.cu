@@ -64,7 +64,9 @@
 namespace mm {
 
 __device__ int g_tc_error = 0;
-void lin_debug_fault(int device, int64_t wait_ns, int drop);  // mm_debug_tc_fault of the linear operator's kernel
+// mm_debug_tc_fault of the linear operator's kernel and of group norm's
+void lin_debug_fault(int device, int64_t wait_ns, int drop);
+void gn_debug_fault(int device, int64_t wait_ns, int drop);
 
 constexpr int TC_BM = 128;        // pixels per tile (MMA M)
 constexpr int TC_BK = 32;         // channels per k-block (128 bytes of fp32)
@@ -1761,9 +1763,10 @@ extern "C" int mm_conv2d_tc_region(const mm_tensor_t* x, const float* w_hi, cons
 }
 
 // Test hook for the bounded-wait error path (no counterpart in the
-// reference): sets the budget of the waits of this kernel and of the linear
-// operator's on `device` (wait_ns <= 0: the default 200 ms) and whether CTA 0
-// leaves its first k-block unissued, for every later launch on that device.
+// reference): sets the budget of the waits of this kernel, of the linear
+// operator's and of group norm's on `device` (wait_ns <= 0: the defaults) and
+// whether CTA 0 leaves its first k-block unissued (group norm: each cluster's
+// first block gives nothing), for every later launch on that device.
 extern "C" int mm_debug_tc_fault(int device, int64_t wait_ns, int drop_first_load) {
   int prev = 0;
   cudaGetDevice(&prev);
@@ -1775,6 +1778,7 @@ extern "C" int mm_debug_tc_fault(int device, int64_t wait_ns, int drop_first_loa
   if (prev != device) cudaSetDevice(prev);
   if (e != cudaSuccess) return cuda_fail(e, "mm_debug_tc_fault");
   lin_debug_fault(device, wait_ns, drop);
+  gn_debug_fault(device, wait_ns, drop);
   return MM_OK;
 }
 
@@ -1791,7 +1795,7 @@ extern "C" int mm_kernel_error(int device, int* code_out, int clear) {
   }
   if (prev != device) cudaSetDevice(prev);
   if (e != cudaSuccess) return cuda_fail(e, "mm_kernel_error");
-  if (volatile int* word = fault_word(device, false)) {  // the linear operator's kernel
+  if (volatile int* word = fault_word(device, false)) {  // of the linear operator's kernel and group norm's
     if (code == 0) code = *word;
     if (clear) *word = 0;
   }

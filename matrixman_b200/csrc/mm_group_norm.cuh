@@ -22,6 +22,7 @@ struct GnArgs {
   int act;
   float eps;
   int* fault;               // the device's fault word (clusters)
+  int tries, drop;          // of a wait; whether rank 0 gives nothing (see mm_debug_tc_fault)
 };
 
 template <int VEC>

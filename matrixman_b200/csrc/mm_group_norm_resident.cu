@@ -82,12 +82,12 @@ __device__ __forceinline__ void gn_give(float2* p, uint64_t* bar, uint32_t rank,
                : "memory");
 }
 
-// Waits until everything was given: at most 2 s (2000 tries that may sleep 1 ms each;
-// the cluster's blocks run at the same time), then leaves a code in the fault word and goes on.
-constexpr int GN_FAULT = 111;
-__device__ __forceinline__ void gn_given(uint64_t* bar, int* fault) {
+// Waits until everything was given: GN_TRIES tries that may sleep 1 ms each (the
+// cluster's blocks run at the same time), then leaves a code in the fault word and goes on.
+constexpr int GN_FAULT = 111, GN_TRIES = 2000;
+__device__ __forceinline__ void gn_given(uint64_t* bar, const GnArgs& a) {
   const uint32_t at = (uint32_t)__cvta_generic_to_shared(bar);
-  for (int i = 0; i < 2000; ++i) {
+  for (int i = 0; i < a.tries; ++i) {
     uint32_t done;
     asm volatile(
         "{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], 0, 1000000; selp.u32 %0, 1, 0, p; }"
@@ -96,7 +96,7 @@ __device__ __forceinline__ void gn_given(uint64_t* bar, int* fault) {
         : "memory");
     if (done) return;
   }
-  if (fault != nullptr && *(volatile int*)fault == 0) *(volatile int*)fault = GN_FAULT;
+  if (*(volatile int*)a.fault == 0) *(volatile int*)a.fault = GN_FAULT;
 }
 
 // i / d for 0 <= i < 2^20, by the float32 inverse of d: i + 0.5 is at least 0.5 / d
@@ -352,7 +352,7 @@ __global__ void __launch_bounds__(GN_MOST_THREADS) gn_resident_kernel(const __gr
       gn_lanes<3>(v, 1, span);
       const float inv = v[2] > 0.f ? 1.f / v[2] : 0.f, mean = first + v[0] * inv, away = v[1] - v[0] * v[0] * inv;
       if (k.ranks > 1) {
-        if (lane < k.ranks) gn_give(peer + i * GN_RANKS + t.rank, &bar, lane, make_float2(mean, away));
+        if (lane < k.ranks && (t.rank || !a.drop)) gn_give(peer + i * GN_RANKS + t.rank, &bar, lane, make_float2(mean, away));
       } else if (lane == 0) {
         const float rstd = rstd_of(away);
         stat[i] = make_float2(mean, rstd);
@@ -363,7 +363,7 @@ __global__ void __launch_bounds__(GN_MOST_THREADS) gn_resident_kernel(const __gr
     if (k.ranks > 1) {
       const int ranks = gn_span(k.ranks);
       const float held = lane < k.ranks ? t.count(a, max(0, min(k.rows, k.all - lane * k.rows))) : 0.f;
-      gn_given(&bar, a.fault);
+      gn_given(&bar, a);
       gn_groups(a, k, t, [&](int i, int u, int g) {
         const float first = peer[i * GN_RANKS].x;
         const float2 one = held > 0.f ? peer[i * GN_RANKS + lane] : make_float2(first, 0.f);
@@ -521,7 +521,7 @@ __global__ void __launch_bounds__(GN_MOST_THREADS) gn_resident_backward_kernel(c
       });
       gn_lanes<2>(v, 1, span);
       if (k.ranks > 1) {
-        if (lane < k.ranks) gn_give(peer + i * GN_RANKS + t.rank, &bar, lane, make_float2(v[0], v[1]));
+        if (lane < k.ranks && (t.rank || !a.drop)) gn_give(peer + i * GN_RANKS + t.rank, &bar, lane, make_float2(v[0], v[1]));
       } else if (lane == 0) {
         stat[i] = make_float2(v[0] * inv, v[1] * inv);
       }
@@ -543,7 +543,7 @@ __global__ void __launch_bounds__(GN_MOST_THREADS) gn_resident_backward_kernel(c
   }
   if (k.ranks > 1) {
     const int ranks = gn_span(k.ranks);
-    gn_given(&bar, a.fault);
+    gn_given(&bar, a);
     gn_groups(a, k, t, [&](int i, int, int) {
       const float2 one = lane < k.ranks ? peer[i * GN_RANKS + lane] : make_float2(0.f, 0.f);
       float v[2] = {one.x, one.y};
@@ -581,6 +581,15 @@ __global__ void __launch_bounds__(GN_MOST_THREADS) gn_resident_backward_kernel(c
 // ---------------------------------------------------------------------------
 // Host side.
 // ---------------------------------------------------------------------------
+
+// Set by mm_debug_tc_fault for a device's later launches (0 tries: GN_TRIES).
+static std::atomic<int> g_gn_tries[64], g_gn_drop[64];
+
+void gn_debug_fault(int device, int64_t wait_ns, int drop) {
+  if (device < 0 || device >= 64) return;
+  g_gn_tries[device] = wait_ns > 0 ? (int)std::min<int64_t>(std::max<int64_t>(wait_ns / 1000000, 1), GN_TRIES) : 0;
+  g_gn_drop[device] = drop;
+}
 
 constexpr int GN_SMEM = 227 * 1024;      // of an SM; a block's 1 KB and its static part come off it
 constexpr int GN_SMEM_FIXED = 1024 + GN_GROUPS * 8 + 16;
@@ -704,6 +713,9 @@ static cudaError_t gn_resident_launch(K kernel, std::atomic<bool>* ready, const 
   if (p.ranks == 1) return launch_pdl(kernel, grid, dim3(p.threads), p.smem, s, a, p);
   a.fault = fault_word(dev, true);
   if (a.fault == nullptr) return cudaErrorMemoryAllocation;
+  const int tries = g_gn_tries[dev];  // (a device with a fault word is below 64)
+  a.tries = tries ? tries : GN_TRIES;
+  a.drop = g_gn_drop[dev];
   return launch_pdl_cluster(kernel, grid, dim3(p.threads), p.ranks, p.smem, s, a, p);
 }
 

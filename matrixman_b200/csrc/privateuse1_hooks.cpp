@@ -75,7 +75,7 @@ void sync_runtime_stream(int device, const char* what) {
     int code = 0;
     MM_SYMBOL(kernel_error_fn, "mm_kernel_error")(device, &code, 1);
     TORCH_CHECK(code == 0, "matrixman guard: ", what, " of device ", device,
-                ": a tensor-core kernel stopped after a bounded wait (code ", code, ")");
+                ": a kernel stopped after a bounded wait (code ", code, ")");
     return;
   }
   char msg[512] = {0};

@@ -269,8 +269,8 @@ class DeviceRuntime:
         self.raise_fault()
 
     def raise_fault(self) -> None:
-        """After a wait for the device: raise if a linear kernel left its call
-        incomplete (reads host memory only)."""
+        """After a wait for the device: raise if a kernel of a linear layer or group
+        norm left its call incomplete (reads host memory only)."""
         if self._fault.value:
             self.check_kernel_error()
 
@@ -280,7 +280,7 @@ class DeviceRuntime:
         _lib.check(self.lib.mm_kernel_error(self.index, ctypes.byref(code), 1), "kernel status")
         if code.value:
             raise _lib.MatrixManNativeError(
-                f"MatrixMan/CUDA: a tensor-core kernel stopped after a bounded wait (code {code.value})")
+                f"MatrixMan/CUDA: a kernel stopped after a bounded wait (code {code.value})")
 
     # -- parameters ----------------------------------------------------------
     @staticmethod

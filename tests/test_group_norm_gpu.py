@@ -16,11 +16,14 @@ up the terms of their formulas; sums of columns take L + n S / 2048 additions.
 ReLU's slope jumps at 0: elements whose z is within its error of 0 may take
 either, and are moved away from it in the input."""
 
+import ctypes
 import math
 
 import pytest
 import torch
 import torch.nn.functional as F
+
+from matrixman_b200 import _lib
 
 pytestmark = pytest.mark.gpu
 
@@ -436,3 +439,31 @@ def test_torch_functional_keeps_channels_last(mm):
     for p in module.parameters():
         with pytest.raises(RuntimeError):
             torch.autograd.grad(y, p, on_device(mm, dy, True), retain_graph=True)
+
+
+@pytest.mark.parametrize("last", [True, False])
+def test_bounded_waits_run_out_and_recover(mm, last):
+    """With the test hook each cluster's first block gives the others nothing and the limit of a wait is one try of
+    1 ms, so their waits run out: the kernel leaves a code, every block goes on to its end, and the next wait of the
+    host raises.  Calls after that are whole."""
+    lib = _lib.load()
+    x, w, b, dy = inputs(2, 48, (64, 64), 8, "silu")
+    want = run(mm, x, 8, w, b, dy, "silu", last)
+    dx, g = (on_device(mm, t, last) for t in (x, dy))
+    leaf, dw, db = (t.detach().requires_grad_(True) for t in (dx, mm.to_device(w), mm.to_device(b)))
+    rt = dx.runtime
+    y = mm.group_norm(leaf, 8, dw, db, EPS, activation="silu")
+    rt.synchronize()
+    code = ctypes.c_int(-1)
+    for call in (lambda: mm.group_norm(dx, 8, w, b, EPS, activation="silu"),
+                 lambda: torch.autograd.grad(y, (leaf, dw, db), g, retain_graph=True)):
+        _lib.check(lib.mm_debug_tc_fault(rt.index, 1_000_000, 1))
+        try:
+            call()
+        finally:
+            _lib.check(lib.mm_debug_tc_fault(rt.index, 0, 0))
+        with pytest.raises(_lib.MatrixManNativeError, match="code 111"):
+            rt.synchronize(timeout_ms=30_000)
+        _lib.check(lib.mm_kernel_error(rt.index, ctypes.byref(code), 0))
+        assert code.value == 0  # reported once
+        assert all(torch.equal(p, q) for p, q in zip(run(mm, x, 8, w, b, dy, "silu", last), want))
