@@ -24,6 +24,7 @@
 #include <math.h>
 #include <stdint.h>
 
+#include <algorithm>
 #include <string>
 #include <type_traits>
 
@@ -432,25 +433,52 @@ static int gn_vec(const GnArgs& a, bool last) {
   return bits % 4 == 0 ? 4 : bits % 2 == 0 ? 2 : 1;
 }
 
-constexpr int64_t GN_BLOCKS = 148 * 16;  // walking blocks of a call of large maps: four on each SM, four times
-constexpr int GN_LEAST = 64;             // pixels of a segment, at least (a multiple of what a load takes);
-                                         // of few channels as many more as a block has rows under way
-
-// Segments of an image for the walking kernels: enough blocks (channels first: warps of
-// one channel) to fill the GPU, whatever the vector width is, so that the workspace's
-// size follows from the sizes alone.
-static int64_t gn_segments(int64_t n, int64_t channels, int64_t pixels, bool last) {
-  const int64_t walkers = last ? n * ((channels + 127) / 128) : (n * channels + GN_WARPS - 1) / GN_WARPS;
-  const int64_t least = last && channels < 128 ? GN_LEAST * 128 / channels : GN_LEAST;
-  const int64_t segs = (GN_BLOCKS + walkers - 1) / walkers, most = (pixels + least - 1) / least;
-  return segs < most ? segs : most;
+// Into how many slabs of columns the channels are cut (channels last): the fewest, unless
+// more leave a tenth less of a block's threads without a column (2 x 100 x 80 x 1280: four slabs
+// of 80 vectors in place of 256 and 64, 65 us to 59).
+static int gn_slabs(int channels, int vec) {
+  const int vectors = (channels + vec - 1) / vec, fewest = (vectors + GN_THREADS - 1) / GN_THREADS;
+  int best = fewest;
+  float most = 0.f;
+  for (int s = fewest; s < fewest + 8 && (s == fewest || vectors / s * vec >= 32); ++s) {
+    const int width = (vectors + s - 1) / s;
+    const float used = (float)(GN_THREADS / width * width) / GN_THREADS * vectors / ((float)width * s);
+    if (used > most + 0.1f) {
+      most = used;
+      best = s;
+    }
+  }
+  return best;
 }
 
+// Walking blocks of a call of large maps.  Channels last one wave of three per SM: with
+// five times as many 64 x 64 x 80 x 80 backward took 111 us in place of 102, 33 x 96 x 80 x
+// 50 64 in place of 55 (a block's first loads and its joins, and waves that end uneven).
+// Channels first segments are short, and several waves even out (2 x 128 x 512 x 512
+// forward: 136 us, with one wave 146 to 158).
+constexpr int64_t GN_BLOCKS_LAST = 148 * 3, GN_BLOCKS_FIRST = 148 * 16;
+constexpr int GN_LEAST = 64;  // pixels of a segment, at least; of few channels as many more as
+                              // a block has rows under way
+
+// Cuts images into segments: enough blocks (channels first: warps of one channel) to
+// fill the GPU, whatever the vector width is, so that the workspace's size follows from
+// the sizes alone.
 static void gn_cut(GnArgs* a, bool last) {
   if (a->n == 0 || a->channels == 0 || a->pixels == 0) return;
-  const int64_t segs = gn_segments(a->n, a->channels, a->pixels, last);
-  a->seg = (int)((((int64_t)a->pixels + segs - 1) / segs + GN_LEAST - 1) / GN_LEAST * GN_LEAST);
-  a->segs = (a->pixels - 1) / a->seg + 1;
+  const int64_t pixels = a->pixels, channels = a->channels;
+  int64_t segs, least = GN_LEAST, step = GN_LEAST;
+  if (last) {
+    const int64_t walkers = (int64_t)a->n * gn_slabs(a->channels, 4);
+    segs = std::max<int64_t>(GN_BLOCKS_LAST / walkers, 1);
+    if (channels < 128) least = GN_LEAST * 128 / channels;
+    step = 16;
+  } else {
+    const int64_t walkers = (a->n * channels + GN_WARPS - 1) / GN_WARPS;
+    segs = (GN_BLOCKS_FIRST + walkers - 1) / walkers;
+  }
+  segs = std::min(segs, (pixels + least - 1) / least);
+  a->seg = (int)(((pixels + segs - 1) / segs + step - 1) / step * step);
+  a->segs = (int)((pixels - 1) / a->seg + 1);
   a->segs_n = (int64_t)a->n * a->segs;
 }
 
@@ -490,7 +518,8 @@ static int gn_setup(const char* who, const float* x, int64_t xi, int64_t xr, int
 template <int VEC, bool LAST>
 static dim3 gn_grid(GnArgs& a) {
   if (!LAST) return dim3((unsigned)((a.segs_n * a.channels + GN_WARPS - 1) / GN_WARPS));
-  a.cols = a.channels < GN_THREADS * VEC ? a.channels : GN_THREADS * VEC;
+  const int slabs = gn_slabs(a.channels, VEC);
+  a.cols = (a.channels / VEC + slabs - 1) / slabs * VEC;
   return dim3((unsigned)a.segs_n, (unsigned)((a.channels + a.cols - 1) / a.cols));
 }
 
@@ -531,7 +560,7 @@ static int64_t gn_floats(const GnArgs& a) {
   for (const bool last : {true, false}) {
     GnArgs cut = a;
     gn_cut(&cut, last);
-    rows = rows > cut.segs_n ? rows : cut.segs_n;
+    rows = std::max(rows, cut.segs_n);
   }
   return 2 * rows * a.channels + 2 * (int64_t)a.n * a.groups;
 }

@@ -135,7 +135,7 @@ __device__ __forceinline__ void gn_act(float (&v)[N], int act) {
 
 // dz = dz act'(z).  One branch per activation: with the slope selected value by value all
 // of them were computed, and the backward pass's first kernel issued in 50 % of its cycles
-// instead of 40 % (16 x 160 x 160 x 128: 188 us, now 184; 2 x 512 x 512 x 128: 241, now 233).
+// instead of 40 % (16 x 128 x 160 x 160: 188 us in place of 184).
 template <int N>
 __device__ __forceinline__ void gn_times_slope(float (&dz)[N], const float (&z)[N], int act) {
   const float one[2] = {1.f, 1.f};

@@ -640,20 +640,21 @@ static bool gn_fit(GnPlan& p, const GnArgs& a, int vec, int part, bool last, boo
 
 // The plan of least estimated time, in us; none (ranks 0) where the walking kernels
 // take less.  The rates are those that maps larger than L2 were measured at, by the
-// blocks that an SM holds: forward 64 x 64 x 80 x 80 4.5 TB/s with four, 4.0 with two,
-// 3.6 with one (walking: 2.6), 16 x 128 x 160 x 160 3.3, 3.6, 3.3 (3.4: 32-byte rows, 64,
-// 64); backward 2.8, 2.8, 2.7 (2.8) and none, 2.0, 2.1 (3.3).
+// blocks that an SM holds: forward 64 x 64 x 80 x 80 4.4 TB/s with four, 3.9 with two,
+// 3.5 with one (walking: 2.9), 16 x 128 x 160 x 160 3.3, 3.6, 3.2 (3.4: 32-byte rows, 64,
+// 64); backward 32 x 256 x 40 x 40 3.1, 2.7, 2.1 (2.6), 16 x 128 x 160 x 160 none, 2.0, 2.1
+// (3.5).
 GnPlan gn_plan(const GnArgs& a, int vec, bool last, bool backward) {
   static const struct {
     int threads, blocks;
     double forward, backward;  // bytes per us
-  } shapes[] = {{256, 4, 4.5e6, 3.1e6}, {512, 2, 4.0e6, 2.9e6}, {1024, 1, 3.5e6, 2.1e6}};
+  } shapes[] = {{256, 4, 4.5e6, 3.4e6}, {512, 2, 4.0e6, 2.9e6}, {1024, 1, 3.5e6, 2.1e6}};
   const double bytes = (double)a.n * a.channels * a.pixels * (backward ? 12 : 8);  // in and out
   const int64_t most = std::min<int64_t>(GN_RANKS, (a.pixels + 63) / 64);
   // Values of one group in a vector.
   const int part = a.each % vec == 0 || !last ? vec : a.each % 2 == 0 && vec == 4 ? 2 : 1;
   GnPlan best;
-  double least = 12.0 + bytes / 3.3e6;
+  double least = backward ? 12.0 + bytes / 3.5e6 : 10.0 + bytes / 3.6e6;  // walking
   int slab = 1;  // the fewest groups that whole vectors hold, then twice as many up to rows of 256 bytes
   while (last && slab < a.groups && (int64_t)slab * a.each % vec != 0) slab *= 2;
   for (slab = std::min(slab, a.groups); slab <= GN_GROUPS; slab = std::min(2 * slab, a.groups)) {
@@ -676,9 +677,11 @@ GnPlan gn_plan(const GnArgs& a, int vec, bool last, bool backward) {
         if (!gn_fit(more, a, vec, part, last, backward, room) || ((more.rows - 1) >> more.p_log) >= 4) break;
         p = more;
       }
-      // Rows narrower than a line's half waste sectors, and so do lanes without a column.
+      // Rows narrower than a line's half waste sectors; lanes without a column copy nothing
+      // (8 x 320 x 64 x 64 in 32 groups, five of eight lanes: 3.7 and 2.8 TB/s).
       const double piece = last ? (double)std::min<int64_t>(width, a.channels) * 4 : 128;
-      const double waste = piece >= 64 ? 1.0 : piece >= 32 ? 1.3 : 2.2;
+      const double lanes = last ? 0.7 + 0.3 * (1 << p.q_log) / p.q : 1.0;
+      const double waste = (piece >= 64 ? 1.0 : piece >= 32 ? 1.3 : 2.2) * lanes;
       const double grid = (double)p.blocks * p.slabs * p.ranks, waves = grid / (148.0 * shape.blocks);
       const double rate = std::min(backward ? shape.backward : shape.forward, grid * 5e4);
       const double time = 5.0 + 0.1 * p.ranks + bytes / rate * waste * (0.5 + 0.5 * std::ceil(waves) / std::max(waves, 1.0));
