@@ -33,8 +33,17 @@
 namespace mm {
 
 // Rows (channels last) or vectors (first) that a thread of the walking kernels has under
-// way: x for the moments, x for the result, x and dy.
-constexpr int GN_ROWS = 8, GN_APPLY_ROWS = 4, GN_BACK_ROWS = 4;
+// way: x for the moments, x for the result, x and dy (channels last four of these spill, 16 x
+// 128 x 160 x 160 backward 182 us in place of 173; channels first three take 172, four 161).
+constexpr int GN_ROWS = 8, GN_APPLY_ROWS = 4, GN_BACK_LAST = 3, GN_BACK_FIRST = 4;
+
+// Blocks of the forward kernels that an SM holds.  Channels last three are the call's one
+// wave (see GN_BLOCKS_LAST), and the registers of four would spill (2 x 128 x 512 x 512:
+// 154 us in place of 145).
+template <bool LAST>
+constexpr int gn_held() {
+  return LAST ? 3 : 4;
+}
 
 // Joins (n2, mean2, m2) into (n, mean, m).
 __device__ __forceinline__ void gn_join(float& n, float& mean, float& m, float n2, float mean2, float m2) {
@@ -161,7 +170,7 @@ __device__ __forceinline__ void gn_leave(const GnArgs& a, const GnWalk<VEC, LAST
 }
 
 template <int VEC, bool LAST>
-__global__ void __launch_bounds__(GN_THREADS, 4) gn_moments_kernel(GnArgs a) {
+__global__ void __launch_bounds__(GN_THREADS, gn_held<LAST>()) gn_moments_kernel(GnArgs a) {
   const GnWalk<VEC, LAST> k(a);
   const float* x = a.x + k.offset(a.xi, a.xr);
   float n = 0.f, mean[VEC], m2[VEC];
@@ -265,7 +274,7 @@ __global__ void __launch_bounds__(T) gn_join_moments_kernel(GnArgs a) {
 }
 
 template <int VEC, bool LAST>
-__global__ void __launch_bounds__(GN_THREADS, 4) gn_apply_kernel(GnArgs a) {
+__global__ void __launch_bounds__(GN_THREADS, gn_held<LAST>()) gn_apply_kernel(GnArgs a) {
   const GnWalk<VEC, LAST> k(a, true);
   pdl_wait();
   if (k.c < 0) return;
@@ -350,9 +359,10 @@ __global__ void __launch_bounds__(GN_THREADS, 3) gn_backward_kernel(GnArgs a) {
         }
       }
     };
+    constexpr int ROWS = LAST ? GN_BACK_LAST : GN_BACK_FIRST;
     int px = k.at;
-    for (; px + (GN_BACK_ROWS - 1) * (int64_t)k.step < k.end; px += GN_BACK_ROWS * k.step)
-      step(std::integral_constant<int, GN_BACK_ROWS>{}, px);
+    for (; px + (ROWS - 1) * (int64_t)k.step < k.end; px += ROWS * k.step)
+      step(std::integral_constant<int, ROWS>{}, px);
     for (; px < k.end; px += k.step) step(std::integral_constant<int, 1>{}, px);
   }
   if (PASS == 0)

@@ -641,9 +641,9 @@ static bool gn_fit(GnPlan& p, const GnArgs& a, int vec, int part, bool last, boo
 // The plan of least estimated time, in us; none (ranks 0) where the walking kernels
 // take less.  The rates are those that maps larger than L2 were measured at, by the
 // blocks that an SM holds: forward 64 x 64 x 80 x 80 4.4 TB/s with four, 3.9 with two,
-// 3.5 with one (walking: 2.9), 16 x 128 x 160 x 160 3.3, 3.6, 3.2 (3.4: 32-byte rows, 64,
-// 64); backward 32 x 256 x 40 x 40 3.1, 2.7, 2.1 (2.6), 16 x 128 x 160 x 160 none, 2.0, 2.1
-// (3.5).
+// 3.5 with one (walking: 3.2), 16 x 128 x 160 x 160 3.3, 3.6, 3.2 (3.6: 32-byte rows, 64,
+// 64); backward 32 x 256 x 40 x 40 3.1, 2.7, 2.1 (2.7), 16 x 128 x 160 x 160 none, 2.0, 2.1
+// (3.6).
 GnPlan gn_plan(const GnArgs& a, int vec, bool last, bool backward) {
   static const struct {
     int threads, blocks;
@@ -654,7 +654,7 @@ GnPlan gn_plan(const GnArgs& a, int vec, bool last, bool backward) {
   // Values of one group in a vector.
   const int part = a.each % vec == 0 || !last ? vec : a.each % 2 == 0 && vec == 4 ? 2 : 1;
   GnPlan best;
-  double least = backward ? 12.0 + bytes / 3.5e6 : 10.0 + bytes / 3.6e6;  // walking
+  double least = backward ? 12.0 + bytes / 3.5e6 : 10.0 + bytes / 3.95e6;  // walking
   int slab = 1;  // the fewest groups that whole vectors hold, then twice as many up to rows of 256 bytes
   while (last && slab < a.groups && (int64_t)slab * a.each % vec != 0) slab *= 2;
   for (slab = std::min(slab, a.groups); slab <= GN_GROUPS; slab = std::min(2 * slab, a.groups)) {
