@@ -590,8 +590,9 @@ int mm_kernel_error(int device, int* code_out, int clear);
 
 /* A word of host memory that a kernel of mm_linear or mm_linear_backward (codes 101
  * to 105), mm_group_norm or mm_group_norm_backward (111) sets to its code when it
- * gives up a bounded wait, after which outputs of that call are incomplete.  Readable without a call once the stream has been
- * waited for; mm_kernel_error reports it too, and clears it. */
+ * gives up a bounded wait, after which outputs of that call are incomplete.
+ * Readable without a call once the stream has been waited for; mm_kernel_error
+ * reports it too, and clears it. */
 int mm_fault_word(int device, int** word_out);
 
 /* Test hook for the bounded-wait error path of mm_conv2d_tc, of mm_linear and
