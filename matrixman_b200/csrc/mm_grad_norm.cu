@@ -12,7 +12,7 @@
 // vanish.
 //
 // Bound by memory: 4 bytes per element for the norm, 12 to clip (read, then read
-// and written).  The norm of 12 tensors of 101 M elements takes 64 us (6.3 TB/s), to clip
+// and written).  The norm of 72 tensors of 101 M elements takes 64 us (6.3 TB/s), to clip
 // them 204 us (5.9 TB/s), of one tensor of 200 M 117 us (6.8 TB/s).
 #include <cuda_runtime.h>
 #include <math.h>
