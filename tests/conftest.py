@@ -15,6 +15,16 @@ def pytest_configure(config):
     config.addinivalue_line("markers", "gpu: needs a B200 (runs through libmatrixman_b200 on cuda:0)")
 
 
+@pytest.fixture(autouse=True)
+def no_device_behind_host_tests(request, monkeypatch):
+    """Tests without the gpu marker make tensors of made-up addresses and record
+    launches: the C++ extension, which GPU tests before them may have loaded, would
+    hand those addresses to a device."""
+    if request.node.get_closest_marker("gpu") is None:
+        from matrixman_b200 import privateuse
+        monkeypatch.setattr(privateuse, "_native", None)
+
+
 @pytest.fixture(scope="session")
 def golden():
     import numpy as np
