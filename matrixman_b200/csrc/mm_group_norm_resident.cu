@@ -87,13 +87,14 @@ __device__ __forceinline__ void gn_give(float2* p, uint64_t* bar, uint32_t rank,
 
 // Waits until everything was given: GN_TRIES tries that may sleep 1 ms each (the
 // cluster's blocks run at the same time), then leaves a code in the fault word and goes on.
+// The acquire has the cluster's scope, as the stores come from its other blocks.
 constexpr int GN_FAULT = 111, GN_TRIES = 2000;
 __device__ __forceinline__ void gn_given(uint64_t* bar, const GnArgs& a) {
   const uint32_t at = (uint32_t)__cvta_generic_to_shared(bar);
   for (int i = 0; i < a.tries; ++i) {
     uint32_t done;
     asm volatile(
-        "{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], 0, 1000000; selp.u32 %0, 1, 0, p; }"
+        "{ .reg .pred p; mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], 0, 1000000; selp.u32 %0, 1, 0, p; }"
         : "=r"(done)
         : "r"(at)
         : "memory");
