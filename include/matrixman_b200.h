@@ -435,6 +435,16 @@ int mm_group_norm_backward(const float* dy, int64_t dy_image, int64_t dy_row, co
                            size_t workspace_bytes, void* stream);
 int mm_group_norm_workspace_size(int64_t n, int64_t channels, int64_t pixels, int64_t groups, size_t* bytes);
 
+/* Test hooks (no counterpart in the reference).  mm_debug_group_norm_ranks: later calls of
+ * both on `device` divide an image's groups over clusters of at most `most` blocks, as on a
+ * device that can place no larger ones (0: no map is held on chip; below 0: the default).
+ * mm_debug_group_norm_plan: how a call of dense, aligned maps is divided where every cluster
+ * can be placed: blocks of a cluster (0: walking kernels) and images of a block, or
+ * an image's segments. */
+int mm_debug_group_norm_ranks(int device, int most);
+int mm_debug_group_norm_plan(int64_t n, int64_t channels, int64_t pixels, int64_t groups, int channels_last,
+                             int backward, int* ranks, int* images, int* segments);
+
 /* One tensor whose norm is taken: numel consecutive float32 elements. */
 typedef struct mm_grad {
   float* data;

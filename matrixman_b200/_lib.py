@@ -216,6 +216,9 @@ SIGNATURES = {
     "mm_group_norm_backward": [_fp, _i64, _i64, _fp, _i64, _i64, _i64, _i64, _i64, _i64, _i, _fp, _fp, _fp, _fp, _i,
                                _fp, _fp, _fp, _vp, _sz, _vp],
     "mm_group_norm_workspace_size": [_i64, _i64, _i64, _i64, ctypes.POINTER(_sz)],
+    "mm_debug_group_norm_ranks": [_i, _i],
+    "mm_debug_group_norm_plan": [_i64, _i64, _i64, _i64, _i, _i, ctypes.POINTER(_i), ctypes.POINTER(_i),
+                                 ctypes.POINTER(_i)],
     "mm_grad_norm": [_vp, _i, _i, _d, _fp, _fp, _vp, _sz, _vp],
     "mm_grad_clip": [_vp, _i, _i, _d, _fp, _vp, _sz, _vp],
     "mm_grad_norm_workspace_size": [_i, ctypes.POINTER(_sz)],

@@ -467,7 +467,7 @@ static int gn_slabs(int channels, int vec) {
 // 50 64 in place of 55 (a block's first loads and its joins, and waves that end uneven).
 // Channels first segments are short, and several waves even out (2 x 128 x 512 x 512
 // forward: 136 us, with one wave 146 to 158).
-constexpr int64_t GN_BLOCKS_LAST = 148 * 3, GN_BLOCKS_FIRST = 148 * 16;
+constexpr int64_t GN_BLOCKS_LAST = 3, GN_BLOCKS_FIRST = 16;  // per SM
 constexpr int GN_LEAST = 64;  // pixels of a segment, at least; of few channels as many more as
                               // a block has rows under way
 
@@ -480,12 +480,12 @@ static void gn_cut(GnArgs* a, bool last) {
   int64_t segs, least = GN_LEAST, step = GN_LEAST;
   if (last) {
     const int64_t walkers = (int64_t)a->n * gn_slabs(a->channels, 4);
-    segs = std::max<int64_t>(GN_BLOCKS_LAST / walkers, 1);
+    segs = std::max<int64_t>(sm_count() * GN_BLOCKS_LAST / walkers, 1);
     if (channels < 128) least = GN_LEAST * 128 / channels;
     step = 16;
   } else {
     const int64_t walkers = (a->n * channels + GN_WARPS - 1) / GN_WARPS;
-    segs = (GN_BLOCKS_FIRST + walkers - 1) / walkers;
+    segs = (sm_count() * GN_BLOCKS_FIRST + walkers - 1) / walkers;
   }
   segs = std::min(segs, (pixels + least - 1) / least);
   a->seg = (int)(((pixels + segs - 1) / segs + step - 1) / step * step);
@@ -610,6 +610,26 @@ extern "C" int mm_group_norm_workspace_size(int64_t n, int64_t channels, int64_t
                           nullptr, nullptr, nullptr, 0, &a);
   if (rc == MM_OK) *bytes = (size_t)gn_floats(a) * sizeof(float);
   return rc;
+}
+
+extern "C" int mm_debug_group_norm_ranks(int device, int most) { return gn_debug_ranks(device, most); }
+
+extern "C" int mm_debug_group_norm_plan(int64_t n, int64_t channels, int64_t pixels, int64_t groups, int channels_last,
+                                        int backward, int* ranks, int* images, int* segments) {
+  GnArgs a;
+  const bool last = channels_last != 0;
+  const float* some = (const float*)16;
+  if (!ranks || !images || !segments) return fail(MM_ERR_INVALID, "mm_debug_group_norm_plan: invalid argument");
+  if (const int rc = gn_setup("mm_debug_group_norm_plan", some, 0, 0, n, channels, pixels, groups, last, nullptr,
+                              nullptr, nullptr, nullptr, 0, &a))
+    return rc;
+  if (n == 0 || channels == 0 || pixels == 0)
+    return fail(MM_ERR_INVALID, "mm_debug_group_norm_plan: maps without elements");
+  const GnPlan p = gn_plan_of(a, gn_vec(a, last), last, backward != 0, GN_RANKS);
+  *ranks = p.ranks;
+  *images = p.ranks ? p.units : 0;
+  *segments = p.ranks ? 0 : a.segs;
+  return MM_OK;
 }
 
 extern "C" int mm_group_norm(const float* x, int64_t x_image, int64_t x_row, int64_t n, int64_t channels,

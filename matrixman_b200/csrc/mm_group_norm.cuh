@@ -201,7 +201,13 @@ struct GnPlan {
 constexpr int GN_RANKS = 16;    // blocks of a cluster, at most
 constexpr int GN_GROUPS = 128;  // groups of a block, at most
 
+// The way of a call on the current device: with clusters only where the device can place
+// them.
 GnPlan gn_plan(const GnArgs& a, int vec, bool last, bool backward);
+// The same with clusters of at most `most` blocks (0: none is held on chip), wherever they
+// can be placed.
+GnPlan gn_plan_of(const GnArgs& a, int vec, bool last, bool backward, int most);
+int gn_debug_ranks(int device, int most);
 int64_t gn_plan_rows(int64_t n, int64_t pixels);  // partial rows that dw and db may take
 // (the backward pass leaves p.blocks * p.ranks partial rows of dw and db)
 cudaError_t gn_resident_forward(const GnArgs& a, const GnPlan& p, int vec, bool last, cudaStream_t s);

@@ -648,13 +648,17 @@ static bool gn_fit(GnPlan& p, const GnArgs& a, int vec, int part, bool last, boo
 // 3.5 with one (walking: 3.2), 16 x 128 x 160 x 160 3.3, 3.6, 3.2 (3.6: 32-byte rows, 64,
 // 64); backward 32 x 256 x 40 x 40 3.1, 2.7, 2.1 (2.7), 16 x 128 x 160 x 160 none, 2.0, 2.1
 // (3.6).
-GnPlan gn_plan(const GnArgs& a, int vec, bool last, bool backward) {
-  static const struct {
-    int threads, blocks;
-    double forward, backward;  // bytes per us
-  } shapes[] = {{256, 4, 4.5e6, 3.4e6}, {512, 2, 4.0e6, 2.9e6}, {1024, 1, 3.5e6, 2.1e6}};
+static const struct GnShape {
+  int threads, blocks;
+  double forward, backward;  // bytes per us
+} gn_shapes[] = {{256, 4, 4.5e6, 3.4e6}, {512, 2, 4.0e6, 2.9e6}, {1024, 1, 3.5e6, 2.1e6}};
+
+static int gn_room(const GnShape& shape) { return GN_SMEM / shape.blocks - GN_SMEM_FIXED; }
+
+GnPlan gn_plan_of(const GnArgs& a, int vec, bool last, bool backward, int most_ranks) {
+  if (most_ranks < 1) return GnPlan();
   const double bytes = (double)a.n * a.channels * a.pixels * (backward ? 12 : 8);  // in and out
-  const int64_t most = std::min<int64_t>(GN_RANKS, (a.pixels + 63) / 64);
+  const int64_t most = std::min<int64_t>(most_ranks, (a.pixels + 63) / 64), sms = sm_count();
   // Values of one group in a vector.
   const int part = a.each % vec == 0 || !last ? vec : a.each % 2 == 0 && vec == 4 ? 2 : 1;
   GnPlan best;
@@ -663,19 +667,19 @@ GnPlan gn_plan(const GnArgs& a, int vec, bool last, bool backward) {
   while (last && slab < a.groups && (int64_t)slab * a.each % vec != 0) slab *= 2;
   for (slab = std::min(slab, a.groups); slab <= GN_GROUPS; slab = std::min(2 * slab, a.groups)) {
     const int64_t width = (int64_t)slab * a.each;
-    for (const auto& shape : shapes) {
+    for (const GnShape& shape : gn_shapes) {
       GnPlan p;
       p.slab = slab;
       p.units = 1;
       p.threads = shape.threads;
-      const int room = GN_SMEM / shape.blocks - GN_SMEM_FIXED;
+      const int room = gn_room(shape);
       const int64_t share = width * a.pixels * (backward ? 8 : 4) / room;
       if (share > most) continue;
       bool fits = false;
       for (p.ranks = (int)std::max<int64_t>(share, 1); p.ranks <= most; ++p.ranks)
         if ((fits = gn_fit(p, a, vec, part, last, backward, room))) break;
       if (!fits) continue;
-      while (p.ranks == 1 && 2 * p.units * p.slab <= GN_GROUPS && (int64_t)p.blocks * p.slabs >= 2 * 148 * 4) {
+      while (p.ranks == 1 && 2 * p.units * p.slab <= GN_GROUPS && (int64_t)p.blocks * p.slabs >= 2 * sms * 4) {
         GnPlan more = p;  // several small images' units in a block, while its threads have few vectors
         more.units *= 2;
         if (!gn_fit(more, a, vec, part, last, backward, room) || ((more.rows - 1) >> more.p_log) >= 4) break;
@@ -686,7 +690,7 @@ GnPlan gn_plan(const GnArgs& a, int vec, bool last, bool backward) {
       const double piece = last ? (double)std::min<int64_t>(width, a.channels) * 4 : 128;
       const double lanes = last ? 0.7 + 0.3 * (1 << p.q_log) / p.q : 1.0;
       const double waste = (piece >= 64 ? 1.0 : piece >= 32 ? 1.3 : 2.2) * lanes;
-      const double grid = (double)p.blocks * p.slabs * p.ranks, waves = grid / (148.0 * shape.blocks);
+      const double grid = (double)p.blocks * p.slabs * p.ranks, waves = grid / ((double)sms * shape.blocks);
       const double rate = std::min(backward ? shape.backward : shape.forward, grid * 5e4);
       const double time = 5.0 + 0.1 * p.ranks + bytes / rate * waste * (0.5 + 0.5 * std::ceil(waves) / std::max(waves, 1.0));
       if (time < least) {
@@ -701,19 +705,60 @@ GnPlan gn_plan(const GnArgs& a, int vec, bool last, bool backward) {
   return best;
 }
 
+// What is known of a kernel on a device.  Host threads may race here, which only repeats
+// the calls.
+struct GnKnown {
+  std::atomic<bool> ready;                           // its attributes are set
+  std::atomic<int8_t> places[3][GN_RANKS + 1];       // by shape and ranks: 1 a cluster has room, 2 it has not
+};
+
 template <class K>
-static cudaError_t gn_resident_launch(K kernel, std::atomic<bool>* ready, const GnArgs& args, const GnPlan& p,
-                                      cudaStream_t s) {
+static cudaError_t gn_ready(K kernel, GnKnown* known, int dev) {
+  if (dev >= 0 && dev < 64 && known[dev].ready.load(std::memory_order_acquire)) return cudaSuccess;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, GN_SMEM - GN_SMEM_FIXED);
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  if (e == cudaSuccess && dev >= 0 && dev < 64) known[dev].ready.store(true, std::memory_order_release);
+  return e;
+}
+
+// Whether the device can place a cluster of the plan's blocks, each with all of the shared
+// memory that its shape may take.
+template <class K>
+static bool gn_places(K kernel, GnKnown* known, const GnPlan& p, int dev) {
+  int shape = 0;
+  while (gn_shapes[shape].threads != p.threads) ++shape;
+  std::atomic<int8_t>* at = dev >= 0 && dev < 64 ? &known[dev].places[shape][p.ranks] : nullptr;
+  if (at)
+    if (const int8_t v = at->load(std::memory_order_relaxed)) return v == 1;
+  int clusters = 0;
+  cudaError_t e = gn_ready(kernel, known, dev);
+  if (e == cudaSuccess) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)p.ranks);
+    cfg.blockDim = dim3(p.threads);
+    cfg.dynamicSmemBytes = gn_room(gn_shapes[shape]);
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)p.ranks;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    e = cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg);
+  }
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return false;
+  }
+  if (at) at->store(clusters > 0 ? 1 : 2, std::memory_order_relaxed);
+  return clusters > 0;
+}
+
+template <class K>
+static cudaError_t gn_resident_launch(K kernel, GnKnown* known, const GnArgs& args, const GnPlan& p, cudaStream_t s) {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess) e = gn_ready(kernel, known, dev);
   if (e != cudaSuccess) return e;
-  // Once per device; host threads may race here, which only repeats the call.
-  if (dev < 0 || dev >= 256 || !ready[dev].load(std::memory_order_acquire)) {
-    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, GN_SMEM - GN_SMEM_FIXED);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-    if (e != cudaSuccess) return e;
-    if (dev >= 0 && dev < 256) ready[dev].store(true, std::memory_order_release);
-  }
   GnArgs a = args;
   const unsigned z = (unsigned)((p.blocks + 65534) / 65535), y = (unsigned)((p.blocks + z - 1) / z);
   const dim3 grid((unsigned)(p.slabs * p.ranks), y, z);
@@ -726,31 +771,67 @@ static cudaError_t gn_resident_launch(K kernel, std::atomic<bool>* ready, const 
   return launch_pdl_cluster(kernel, grid, dim3(p.threads), p.ranks, p.smem, s, a, p);
 }
 
-template <int VEC, int PARTS, bool LAST>
-static cudaError_t gn_forward(const GnArgs& a, const GnPlan& p, cudaStream_t s) {
-  static std::atomic<bool> ready[256];
-  return gn_resident_launch(gn_resident_kernel<VEC, PARTS, LAST>, ready, a, p, s);
-}
+template <int VEC, int PARTS, bool LAST, bool BACKWARD>
+struct GnResident {
+  static inline GnKnown known[64];
+  static constexpr auto kernel() {
+    if constexpr (BACKWARD) return gn_resident_backward_kernel<VEC, PARTS, LAST>;
+    else return gn_resident_kernel<VEC, PARTS, LAST>;
+  }
+  static cudaError_t launch(const GnArgs& a, const GnPlan& p, cudaStream_t s) {
+    return gn_resident_launch(kernel(), known, a, p, s);
+  }
+  static bool places(const GnPlan& p, int dev) { return gn_places(kernel(), known, p, dev); }
+};
 
-template <int VEC, int PARTS, bool LAST>
-static cudaError_t gn_backward(const GnArgs& a, const GnPlan& p, cudaStream_t s) {
-  static std::atomic<bool> ready[256];
-  return gn_resident_launch(gn_resident_backward_kernel<VEC, PARTS, LAST>, ready, a, p, s);
+// Calls f with the kernel of a call.
+template <bool BACKWARD, class F>
+static auto gn_resident_of(const GnArgs& a, int vec, bool last, F f) {
+  if (!last) {
+    if (vec == 4) return f(GnResident<4, 1, false, BACKWARD>());
+    if (vec == 2) return f(GnResident<2, 1, false, BACKWARD>());
+    return f(GnResident<1, 1, false, BACKWARD>());
+  }
+  if (vec == 4) {
+    if (a.each % 4 == 0) return f(GnResident<4, 1, true, BACKWARD>());
+    if (a.each % 2 == 0) return f(GnResident<4, 2, true, BACKWARD>());
+    return f(GnResident<4, 4, true, BACKWARD>());
+  }
+  if (vec == 2) {
+    if (a.each % 2 == 0) return f(GnResident<2, 1, true, BACKWARD>());
+    return f(GnResident<2, 2, true, BACKWARD>());
+  }
+  return f(GnResident<1, 1, true, BACKWARD>());
 }
-
-#define GN_RESIDENT(FN)                                                                             \
-  if (!last) return vec == 4 ? FN<4, 1, false>(a, p, s) : vec == 2 ? FN<2, 1, false>(a, p, s) : FN<1, 1, false>(a, p, s); \
-  if (vec == 4)                                                                                     \
-    return a.each % 4 == 0 ? FN<4, 1, true>(a, p, s) : a.each % 2 == 0 ? FN<4, 2, true>(a, p, s) : FN<4, 4, true>(a, p, s); \
-  if (vec == 2) return a.each % 2 == 0 ? FN<2, 1, true>(a, p, s) : FN<2, 2, true>(a, p, s);         \
-  return FN<1, 1, true>(a, p, s);
 
 cudaError_t gn_resident_forward(const GnArgs& a, const GnPlan& p, int vec, bool last, cudaStream_t s) {
-  GN_RESIDENT(gn_forward)
+  return gn_resident_of<false>(a, vec, last, [&](auto k) { return k.launch(a, p, s); });
 }
 
 cudaError_t gn_resident_backward(const GnArgs& a, const GnPlan& p, int vec, bool last, cudaStream_t s) {
-  GN_RESIDENT(gn_backward)
+  return gn_resident_of<true>(a, vec, last, [&](auto k) { return k.launch(a, p, s); });
+}
+
+// Set by mm_debug_group_norm_ranks for a device's later calls, plus one (0: GN_RANKS).
+static std::atomic<int> g_gn_most[64];
+
+int gn_debug_ranks(int device, int most) {
+  if (device < 0 || device >= 64) return fail(MM_ERR_INVALID, "mm_debug_group_norm_ranks: invalid device");
+  g_gn_most[device] = most < 0 ? 0 : std::min(most, GN_RANKS) + 1;
+  return MM_OK;
+}
+
+GnPlan gn_plan(const GnArgs& a, int vec, bool last, bool backward) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) cudaGetLastError();
+  const int set = dev >= 0 && dev < 64 ? g_gn_most[dev].load(std::memory_order_relaxed) : 0;
+  for (int most = set ? set - 1 : GN_RANKS;;) {
+    const GnPlan p = gn_plan_of(a, vec, last, backward, most);
+    if (p.ranks <= 1) return p;
+    const auto places = [&](auto k) { return k.places(p, dev); };
+    if (backward ? gn_resident_of<true>(a, vec, last, places) : gn_resident_of<false>(a, vec, last, places)) return p;
+    most = p.ranks - 1;
+  }
 }
 
 }  // namespace mm
