@@ -46,13 +46,14 @@ constexpr int gn_held() {
   return LAST ? 3 : 4;
 }
 
-// Joins (n2, mean2, m2) into (n, mean, m).
+// Joins (n2, mean2, m2) into (n, mean, m).  d is all of the mean where n is 0, and its
+// square may overflow: it meets n first.
 __device__ __forceinline__ void gn_join(float& n, float& mean, float& m, float n2, float mean2, float m2) {
   const float all = n + n2;
   if (n2 == 0.f) return;
   const float d = mean2 - mean, share = n2 / all;
   mean += d * share;
-  m += m2 + d * d * n * share;
+  m += m2 + d * n * (d * share);
   n = all;
 }
 
@@ -201,7 +202,7 @@ __global__ void __launch_bounds__(GN_THREADS, gn_held<LAST>()) gn_moments_kernel
       for (int e = 0; e < VEC; ++e) {
         const float d = -less[e] + sum[e] * inv - mean[e];
         mean[e] += d * share;
-        m2[e] += squares[e] - sum[e] * sum[e] * inv + d * d * n * share;
+        m2[e] += squares[e] - sum[e] * sum[e] * inv + d * n * (d * share);  // (as gn_join)
       }
       n += nb;
     };
