@@ -19,8 +19,8 @@
 // Moments are held as a mean and a sum of squared distances from it and joined
 // by d^2 n1 n2 / (n1 + n2) (Chan, Golub, LeVeque 1979), so large offsets do not
 // cancel; those of GN_ROWS rows are taken around the first row's values (see
-// mm_group_norm_resident.cu).  All sums are float32 in a fixed order, without atomics: the same
-// inputs give the same bits.
+// mm_group_norm_resident.cu).  Sums are float32, and float64 where the moments of segments are
+// joined, all in a fixed order, without atomics: the same inputs give the same bits.
 #include <cuda_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -221,8 +221,8 @@ __global__ void __launch_bounds__(GN_THREADS, gn_held<LAST>()) gn_moments_kernel
 }
 
 // Sums of two values over a block of T threads; every thread gets them.
-template <int T>
-__device__ __forceinline__ void gn_sum2(float& u, float& v, float2* sm) {
+template <int T, class V, class V2>
+__device__ __forceinline__ void gn_sum2(V& u, V& v, V2* sm) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     u += __shfl_xor_sync(0xffffffffu, u, o);
@@ -230,9 +230,9 @@ __device__ __forceinline__ void gn_sum2(float& u, float& v, float2* sm) {
   }
   if (T == 32) return;
   __syncthreads();
-  if ((threadIdx.x & 31) == 0) sm[threadIdx.x >> 5] = make_float2(u, v);
+  if ((threadIdx.x & 31) == 0) sm[threadIdx.x >> 5] = {u, v};
   __syncthreads();
-  u = v = 0.f;
+  u = v = 0;
 #pragma unroll
   for (int i = 0; i < T / 32; ++i) {
     u += sm[i].x;
@@ -241,37 +241,39 @@ __device__ __forceinline__ void gn_sum2(float& u, float& v, float2* sm) {
 }
 
 // mean and rstd of one image and group per block of T threads, from the channels'
-// segments.
+// segments.  Their means are weighted and added in 64 bits: the sum of all values neither
+// rounds (a constant is its own mean) nor overflows, however many segments there are.
 template <int T>
 __global__ void __launch_bounds__(T) gn_join_moments_kernel(GnArgs a) {
-  __shared__ float2 sm[T / 32];
+  __shared__ double2 sm[T / 32];
   pdl_wait();
   const int image = blockIdx.x / a.groups, group = blockIdx.x % a.groups;
   const float* pu = a.part + (int64_t)image * a.segs * a.channels + group * a.each;
   const float* pv = pu + a.segs_n * a.channels;
   const unsigned count = (unsigned)a.segs * a.each, each = a.each;
-  const float m = (float)a.pixels * (float)a.each;
-  float s = 0.f, q = 0.f;
+  const double m = (double)a.pixels * (double)a.each;
+  double s = 0, q = 0;
 #pragma unroll 4
   for (unsigned i = threadIdx.x; i < count; i += T) {
     const int seg = (int)(i / each);
-    const float n = (float)min(a.seg, a.pixels - seg * a.seg);
-    s += n * pu[(int64_t)seg * a.channels + (i - seg * each)];
+    const int n = min(a.seg, a.pixels - seg * a.seg);
+    s += (double)n * (double)pu[(int64_t)seg * a.channels + (i - seg * each)];
   }
   gn_sum2<T>(s, q, sm);
-  const float mean = s / m;  // (divided, so that a constant's own mean is exact wherever the sum is)
-  s = q = 0.f;
+  const double mean = s / m;
+  s = q = 0;
 #pragma unroll 4
   for (unsigned i = threadIdx.x; i < count; i += T) {
     const int seg = (int)(i / each);
     const int64_t at = (int64_t)seg * a.channels + (i - seg * each);
-    const float n = (float)min(a.seg, a.pixels - seg * a.seg), d = pu[at] - mean;
-    s += pv[at] + n * d * d;
+    const int n = min(a.seg, a.pixels - seg * a.seg);
+    const double d = (double)pu[at] - mean;
+    s += (double)pv[at] + (double)n * d * d;
   }
   gn_sum2<T>(s, q, sm);
   if (threadIdx.x == 0) {
-    a.mean[blockIdx.x] = mean;
-    a.rstd[blockIdx.x] = 1.f / sqrtf(s / m + a.eps);
+    a.mean[blockIdx.x] = (float)mean;
+    a.rstd[blockIdx.x] = 1.f / sqrtf((float)(s / m) + a.eps);
   }
 }
 

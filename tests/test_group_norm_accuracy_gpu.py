@@ -4,7 +4,7 @@ maps held on chip and of the walking kernels alike.  u = 2^-24."""
 import pytest
 import torch
 
-from .test_group_norm_gpu import randn, run
+from .test_group_norm_gpu import EPS, on_device, randn, run
 from .test_group_norm_plan import plan
 from .test_group_norm_ways_gpu import pixels
 
@@ -17,6 +17,17 @@ WALKING = [(1, 16, (300, 300), 1), (1, 18, (302, 301), 1), (1, 15, (305, 303), 1
 @pytest.mark.parametrize("n,c,spatial,groups", WALKING)
 def test_these_walk(n, c, spatial, groups):
     assert all(plan(n, c, pixels(spatial), groups, last, back)[0] == 0 for last in (0, 1) for back in (0, 1))
+
+
+@pytest.mark.parametrize("last", [True, False])
+@pytest.mark.parametrize("n,c,spatial,groups", [(2, 48, (64, 64), 8), *WALKING])
+@pytest.mark.parametrize("value", [0.1, 1000.1, -3.3e7, 1e34])
+def test_a_constant_is_its_own_mean(mm, n, c, spatial, groups, last, value):
+    """No spread: y is the bias, whatever the value's bits."""
+    b = randn(c, seed=1)
+    y = mm.group_norm(on_device(mm, torch.full((n, c, *spatial), value), last), groups, mm.to_device(torch.ones(c)),
+                      mm.to_device(b), EPS)
+    assert torch.equal(y.cpu(), b.reshape(1, c, 1, 1).expand(n, c, *spatial))
 
 
 @pytest.mark.parametrize("last", [True, False])
