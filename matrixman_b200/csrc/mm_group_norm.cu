@@ -19,8 +19,9 @@
 // Moments are held as a mean and a sum of squared distances from it and joined
 // by d^2 n1 n2 / (n1 + n2) (Chan, Golub, LeVeque 1979), so large offsets do not
 // cancel; those of GN_ROWS rows are taken around the first row's values (see
-// mm_group_norm_resident.cu).  Sums are float32, and float64 where the moments of segments are
-// joined, all in a fixed order, without atomics: the same inputs give the same bits.
+// mm_group_norm_resident.cu).  A thread adds at most 128 values in float32, a block joins its
+// threads in float32 (13 additions), what is added behind that takes float64 every 4 or 8
+// values; all in a fixed order, without atomics: the same inputs give the same bits.
 #include <cuda_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -240,9 +241,29 @@ __device__ __forceinline__ void gn_sum2(V& u, V& v, V2* sm) {
   }
 }
 
+// The sums of both values of term(0 .. count - 1) over a thread's share of them, in float64
+// every four.
+template <int T, class F>
+__device__ __forceinline__ double2 gn_share(unsigned count, F term) {
+  double2 s = make_double2(0, 0);
+  unsigned i = threadIdx.x;
+  for (; i + 3 * T < count; i += 4 * T) {
+    const float2 p = term(i), q = term(i + T), r = term(i + 2 * T), t = term(i + 3 * T);
+    s.x += (double)((p.x + q.x) + (r.x + t.x));
+    s.y += (double)((p.y + q.y) + (r.y + t.y));
+  }
+  float2 rest = make_float2(0.f, 0.f);
+  for (; i < count; i += T) {
+    const float2 p = term(i);
+    rest.x += p.x;
+    rest.y += p.y;
+  }
+  return make_double2(s.x + (double)rest.x, s.y + (double)rest.y);
+}
+
 // mean and rstd of one image and group per block of T threads, from the channels'
-// segments.  Their means are weighted and added in 64 bits: the sum of all values neither
-// rounds (a constant is its own mean) nor overflows, however many segments there are.
+// segments.  Their means are weighted and added as distances from the first one's: a constant
+// is its own mean, and the sum of all values overflows nowhere.
 template <int T>
 __global__ void __launch_bounds__(T) gn_join_moments_kernel(GnArgs a) {
   __shared__ double2 sm[T / 32];
@@ -252,28 +273,24 @@ __global__ void __launch_bounds__(T) gn_join_moments_kernel(GnArgs a) {
   const float* pv = pu + a.segs_n * a.channels;
   const unsigned count = (unsigned)a.segs * a.each, each = a.each;
   const double m = (double)a.pixels * (double)a.each;
-  double s = 0, q = 0;
-#pragma unroll 4
-  for (unsigned i = threadIdx.x; i < count; i += T) {
-    const int seg = (int)(i / each);
-    const int n = min(a.seg, a.pixels - seg * a.seg);
-    s += (double)n * (double)pu[(int64_t)seg * a.channels + (i - seg * each)];
-  }
-  gn_sum2<T>(s, q, sm);
-  const double mean = s / m;
-  s = q = 0;
-#pragma unroll 4
-  for (unsigned i = threadIdx.x; i < count; i += T) {
-    const int seg = (int)(i / each);
-    const int64_t at = (int64_t)seg * a.channels + (i - seg * each);
-    const int n = min(a.seg, a.pixels - seg * a.seg);
-    const double d = (double)pu[at] - mean;
-    s += (double)pv[at] + (double)n * d * d;
-  }
-  gn_sum2<T>(s, q, sm);
+  const float first = pu[0];
+  auto walk = [&](auto f) {
+    return gn_share<T>(count, [&](unsigned i) {
+      const int seg = (int)(i / each);
+      return make_float2(f((int64_t)seg * a.channels + (i - seg * each), (float)min(a.seg, a.pixels - seg * a.seg)), 0.f);
+    });
+  };
+  double2 s = walk([&](int64_t at, float n) { return n * (pu[at] - first); });
+  gn_sum2<T>(s.x, s.y, sm);
+  const float away = (float)(s.x / m);
+  s = walk([&](int64_t at, float n) {
+    const float d = pu[at] - first - away;
+    return pv[at] + n * d * d;
+  });
+  gn_sum2<T>(s.x, s.y, sm);
   if (threadIdx.x == 0) {
-    a.mean[blockIdx.x] = (float)mean;
-    a.rstd[blockIdx.x] = 1.f / sqrtf((float)(s / m) + a.eps);
+    a.mean[blockIdx.x] = first + away;
+    a.rstd[blockIdx.x] = 1.f / sqrtf((float)(s.x / m) + a.eps);
   }
 }
 
@@ -310,6 +327,11 @@ __global__ void __launch_bounds__(GN_THREADS, gn_held<LAST>()) gn_apply_kernel(G
     apply(std::integral_constant<int, GN_APPLY_ROWS>{}, px);
   for (; px < k.end; px += k.step) apply(std::integral_constant<int, 1>{}, px);
 }
+
+// Rows that a thread adds in float32; it adds the sums of more rows in float64, in its own
+// place in shared memory.  (Of values of one sign every addition rounds the same way, and
+// a thread may have thousands of rows; one of 16 x 128 x 160 x 160 has 120.)
+constexpr int GN_FOLD = 128;
 
 // PASS 0: each channel's sums of dz and dz xh; 1: dx.
 template <int VEC, bool LAST, int PASS>
@@ -364,10 +386,31 @@ __global__ void __launch_bounds__(GN_THREADS, 3) gn_backward_kernel(GnArgs a) {
       }
     };
     constexpr int ROWS = LAST ? GN_BACK_LAST : GN_BACK_FIRST;
-    int px = k.at;
-    for (; px + (ROWS - 1) * (int64_t)k.step < k.end; px += ROWS * k.step)
-      step(std::integral_constant<int, ROWS>{}, px);
-    for (; px < k.end; px += k.step) step(std::integral_constant<int, 1>{}, px);
+    auto walk = [&](int px, int end) {
+      for (; px + (ROWS - 1) * (int64_t)k.step < end; px += ROWS * k.step)
+        step(std::integral_constant<int, ROWS>{}, px);
+      for (; px < end; px += k.step) step(std::integral_constant<int, 1>{}, px);
+    };
+    if (PASS == 1) {
+      walk(k.at, k.end);
+    } else {
+      __shared__ double sums[2][VEC][GN_THREADS];  // (a thread's own)
+      const int fold = GN_FOLD / ROWS * ROWS * k.step;
+      for (int px = k.at; px < k.end; px += fold) {
+        const bool first = px == k.at, more = px + fold < k.end;
+        walk(px, more ? px + fold : k.end);
+        if (first && !more) break;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          const double su = (first ? 0 : sums[0][e][threadIdx.x]) + (double)u[e];
+          const double sv = (first ? 0 : sums[1][e][threadIdx.x]) + (double)v[e];
+          sums[0][e][threadIdx.x] = su;
+          sums[1][e][threadIdx.x] = sv;
+          u[e] = more ? 0.f : (float)su;
+          v[e] = more ? 0.f : (float)sv;
+        }
+      }
+    }
   }
   if (PASS == 0)
     gn_leave<VEC, LAST>(a, k, 0.f, u, v, [](float&, float& au, float& av, float, float bu, float bv) {
@@ -380,19 +423,35 @@ constexpr int GN_COLUMNS = 4;  // channels of a block that adds partial rows
 constexpr int GN_COLUMN_THREADS = GN_THREADS / GN_COLUMNS;
 
 // db and dw of a block's channels: 64 threads per channel add the partial rows k, k +
-// 64, ..., then their sums are added in order.
-__device__ __forceinline__ void gn_add_rows(const GnArgs& a, int block, float2 (*acc)[GN_COLUMNS + 1]) {
+// 64, ... (in float64 every eight, as there may be as many rows as images), then their sums
+// are added in order.
+__device__ __forceinline__ void gn_add_rows(const GnArgs& a, int block, double2 (*acc)[GN_COLUMNS + 1]) {
   const int lane = threadIdx.x % GN_COLUMNS, k = threadIdx.x / GN_COLUMNS;
   const int c = block * GN_COLUMNS + lane;
   const float* pu = a.part + c;
   const float* pv = pu + a.segs_n * a.channels;
-  float2 s = make_float2(0.f, 0.f);
-  if (c < a.channels)
-#pragma unroll 8
-    for (int64_t r = k; r < a.segs_n; r += GN_COLUMN_THREADS) {
-      s.x += pu[r * a.channels];
-      s.y += pv[r * a.channels];
+  double2 s = make_double2(0, 0);
+  if (c < a.channels) {
+    constexpr int EACH = 8;
+    int64_t r = k;
+    for (; r + (EACH - 1) * GN_COLUMN_THREADS < a.segs_n; r += EACH * GN_COLUMN_THREADS) {
+      float u = 0.f, v = 0.f;
+#pragma unroll
+      for (int e = 0; e < EACH; ++e) {
+        u += pu[(r + e * GN_COLUMN_THREADS) * a.channels];
+        v += pv[(r + e * GN_COLUMN_THREADS) * a.channels];
+      }
+      s.x += (double)u;
+      s.y += (double)v;
     }
+    float u = 0.f, v = 0.f;
+    for (; r < a.segs_n; r += GN_COLUMN_THREADS) {
+      u += pu[r * a.channels];
+      v += pv[r * a.channels];
+    }
+    s.x += (double)u;
+    s.y += (double)v;
+  }
   acc[k][lane] = s;
   __syncthreads();
   if (k == 0 && c < a.channels) {
@@ -400,15 +459,15 @@ __device__ __forceinline__ void gn_add_rows(const GnArgs& a, int block, float2 (
       s.x += acc[j][lane].x;
       s.y += acc[j][lane].y;
     }
-    if (a.db) a.db[c] = s.x;
-    if (a.dw) a.dw[c] = s.y;
+    if (a.db) a.db[c] = (float)s.x;
+    if (a.dw) a.dw[c] = (float)s.y;
   }
 }
 
 // Means of g and g xh of one image and group per block; the first `columns` blocks add
 // the partial rows.
 __global__ void __launch_bounds__(GN_THREADS) gn_join_sums_kernel(GnArgs a, int columns) {
-  __shared__ float2 acc[GN_COLUMN_THREADS][GN_COLUMNS + 1];
+  __shared__ double2 acc[GN_COLUMN_THREADS][GN_COLUMNS + 1];
   pdl_wait();
   if ((int)blockIdx.x < columns) {
     gn_add_rows(a, blockIdx.x, acc);
@@ -418,20 +477,17 @@ __global__ void __launch_bounds__(GN_THREADS) gn_join_sums_kernel(GnArgs a, int 
   const float* pu = a.part + (int64_t)image * a.segs * a.channels + group * a.each;
   const float* pv = pu + a.segs_n * a.channels;
   const unsigned count = (unsigned)a.segs * a.each, each = a.each;
-  const float inv = 1.f / ((float)a.pixels * (float)a.each);
-  float s1 = 0.f, s2 = 0.f;
-#pragma unroll 4
-  for (unsigned i = threadIdx.x; i < count; i += GN_THREADS) {
+  const double inv = 1 / ((double)a.pixels * (double)a.each);
+  double2 s = gn_share<GN_THREADS>(count, [&](unsigned i) {
     const unsigned seg = i / each, c = i - seg * each;
     const int64_t at = (int64_t)seg * a.channels + c;
     const float w = a.w ? a.w[group * a.each + c] : 1.f;
-    s1 += w * pu[at];
-    s2 += w * pv[at];
-  }
-  gn_sum2<GN_THREADS>(s1, s2, &acc[0][0]);
+    return make_float2(w * pu[at], w * pv[at]);
+  });
+  gn_sum2<GN_THREADS>(s.x, s.y, &acc[0][0]);
   if (threadIdx.x == 0) {
-    a.sums[id] = s1 * inv;
-    a.sums[(int64_t)a.n * a.groups + id] = s2 * inv;
+    a.sums[id] = (float)(s.x * inv);
+    a.sums[(int64_t)a.n * a.groups + id] = (float)(s.y * inv);
   }
 }
 

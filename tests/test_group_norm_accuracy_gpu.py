@@ -4,7 +4,9 @@ maps held on chip and of the walking kernels alike.  u = 2^-24."""
 import pytest
 import torch
 
-from .test_group_norm_gpu import EPS, on_device, randn, run
+from matrixman_b200 import ops
+
+from .test_group_norm_gpu import EPS, U, check, on_device, randn, run
 from .test_group_norm_plan import plan
 from .test_group_norm_ways_gpu import pixels
 
@@ -39,3 +41,47 @@ def test_means_whose_squares_overflow(mm, n, c, spatial, groups, last):
     assert x.unique().numel() > 5
     got = run(mm, x, groups, torch.ones(c), torch.zeros(c), randn(n, c, *spatial, seed=3), "none", last)
     assert all(torch.isfinite(t).all() for t in got)
+
+
+# One segment per image, and a thread takes 2000 and 1000 of its values; the images are all the
+# same, so that they take little memory.  A thread's sum goes through at most 128 additions,
+# the block's through 13 more, and what is added behind that takes 64 bits every eight: 150 u,
+# of values of one sign.
+@pytest.mark.parametrize("n,c,size,last", [(230, 2, 512000, True), (19000, 1, 32001, False)])
+def test_sums_of_one_sign_over_long_segments(mm, n, c, size, last):
+    assert plan(n, c, size, c, last, True)[::2] == (0, 1)
+    one, grad = randn(1, c, size, seed=1), torch.full((1, c, size), 0.1)
+    x, dy = (on_device(mm, t, last).expand(n, c, size) for t in (one, grad))
+    assert x._logical_strides[0] == 0
+    m64 = one.double().mean(2, keepdim=True)
+    r64 = 1 / torch.sqrt(((one.double() - m64) ** 2).mean(2, keepdim=True) + EPS)
+    xh = (one.double() - m64) * r64
+    exh = r64 * U * m64.abs() + 4 * U * xh.abs()  # mean and rstd are given in float32
+    mean, rstd = (mm.to_device(t.float().reshape(1, c)).expand(n, c).contiguous() for t in (m64, r64))
+    dx, dw, db = ops.group_norm_backward(dy, x, mean, rstd, mm.to_device(torch.ones(c)), None, c, (True, True, True))
+    g = grad.double()
+    check("db", db.cpu(), (n * g.sum((0, 2)), n * 150 * U * g.sum((0, 2))))
+    check("dw", dw.cpu(), (n * (g * xh).sum((0, 2)), n * (151 * U * (g * xh).abs() + g * exh).sum((0, 2))))
+    s1, s2 = g.mean(2, keepdim=True), (g * xh).mean(2, keepdim=True)
+    es1, es2 = 151 * U * s1, (152 * U * (g * xh).abs() + g * exh).mean(2, keepdim=True)
+    want = r64 * (g - s1 - xh * s2)
+    bound = r64 * (4 * U * (g + s1 + (xh * s2).abs()) + es1 + xh.abs() * es2 + exh * s2.abs()) + 4 * U * want.abs()
+    for image in (0, n - 1):
+        check("dx", dx[image:image + 1].cpu(), (want, bound))
+
+
+def test_means_of_one_sign_over_many_channels(mm):
+    """A group of 262,144 channels of nine pixels: its mean is the sum of as many partial
+    sums, of nine additions each, in 64 bits every four."""
+    n, c, size = 1, 1 << 18, 9
+    one, grad = randn(n, c, size, seed=1), torch.full((n, c, size), 0.1)
+    for last in (True, False):
+        assert plan(n, c, size, 1, last, True)[0] == 0
+        y, dx, _, _ = run(mm, one, 1, torch.ones(c), torch.zeros(c), grad, "none", last)
+        m64 = one.double().mean()
+        r64 = 1 / torch.sqrt(((one.double() - m64) ** 2).mean() + EPS)
+        # g is constant, so dx = rstd (g - mean(g) - xh mean(g xh)) is what sums round to, and
+        # mean(g xh) is g times the mean of xh, whose own mean is off by 50 roundings at most
+        xh = ((one.double() - m64) * r64).abs()
+        bound = r64 * 0.1 * (24 * U + 4 * U + xh * (64 * U * xh.mean()))
+        check("dx", dx.cpu(), (torch.zeros(n, c, size, dtype=torch.float64), bound))
