@@ -337,14 +337,14 @@ constexpr int GN_FOLD = 128;
 template <int VEC, bool LAST, int PASS>
 __global__ void __launch_bounds__(GN_THREADS, 3) gn_backward_kernel(GnArgs a) {
   const GnWalk<VEC, LAST> k(a, PASS == 1);
-  float u[VEC], v[VEC], less[VEC], rstd[VEC], w[VEC], b[VEC];  // less: -mean
+  float u[VEC], v[VEC], less[VEC], rstd[VEC], wr[VEC], b[VEC];  // less: -mean; wr: w rstd
 #pragma unroll
   for (int e = 0; e < VEC; ++e) u[e] = v[e] = 0.f;
   if (PASS == 1) pdl_wait();
   if (k.c >= 0) {
     gn_of_groups<VEC, LAST>(a, k, a.mean, less);
     gn_of_groups<VEC, LAST>(a, k, a.rstd, rstd);
-    gn_of_channels<VEC, LAST>(a.w, k.c, 1.f, w);
+    gn_of_channels<VEC, LAST>(a.w, k.c, 1.f, wr);
     gn_of_channels<VEC, LAST>(a.b, k.c, 0.f, b);
     if (PASS == 1) {
       gn_of_groups<VEC, LAST>(a, k, a.sums, u);
@@ -353,6 +353,7 @@ __global__ void __launch_bounds__(GN_THREADS, 3) gn_backward_kernel(GnArgs a) {
 #pragma unroll
     for (int e = 0; e < VEC; ++e) {
       less[e] = -less[e];
+      wr[e] *= rstd[e];
       if (PASS == 1) {
         u[e] *= -rstd[e];
         v[e] *= -rstd[e];
@@ -373,14 +374,13 @@ __global__ void __launch_bounds__(GN_THREADS, 3) gn_backward_kernel(GnArgs a) {
       for (int r = 0; r < N; r += VEC) {  // (a vector at a time, for the registers)
         float(&h)[VEC] = *reinterpret_cast<float(*)[VEC]>(xh + r);
         float(&z)[VEC] = *reinterpret_cast<float(*)[VEC]>(dz + r);
-        gn_slopes<VEC>(h, z, less, rstd, w, b, a.act);
+        gn_slopes<VEC>(h, z, less, rstd, wr, b, a.act);
         if (PASS == 0) {
           gn_add<VEC, VEC>(u, u, z);
           gn_fma<VEC, VEC, VEC>(v, z, h, v);
         } else {  // dx = rstd w dz - (rstd s2 xh + rstd s1)
           gn_fma<VEC, VEC, VEC>(h, h, v, u);
-          gn_mul<VEC, VEC>(z, z, w);
-          gn_fma<VEC, VEC, VEC>(z, z, rstd, h);
+          gn_fma<VEC, VEC, VEC>(z, z, wr, h);
           gn_store<VEC>(dx + k.pixel(px + r / VEC * k.step, a.channels), z);
         }
       }

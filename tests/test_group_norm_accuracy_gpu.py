@@ -6,9 +6,9 @@ import torch
 
 from matrixman_b200 import ops
 
-from .test_group_norm_gpu import EPS, U, check, on_device, randn, run
+from .test_group_norm_gpu import EPS, U, check, inputs, on_device, randn, run
 from .test_group_norm_plan import plan
-from .test_group_norm_ways_gpu import pixels
+from .test_group_norm_ways_gpu import at_most, pixels  # noqa: F401 - a fixture
 
 pytestmark = pytest.mark.gpu
 
@@ -41,6 +41,23 @@ def test_means_whose_squares_overflow(mm, n, c, spatial, groups, last):
     assert x.unique().numel() > 5
     got = run(mm, x, groups, torch.ones(c), torch.zeros(c), randn(n, c, *spatial, seed=3), "none", last)
     assert all(torch.isfinite(t).all() for t in got)
+
+
+@pytest.mark.parametrize("last", [True, False])
+@pytest.mark.parametrize("walking", [True, False])
+def test_relu_passes_the_gradients_of_what_it_let_through(mm, at_most, last, walking):  # noqa: F811
+    """Each channel's bias cancels its first pixel to within a rounding of 0."""
+    if walking:
+        at_most(0)
+    n, c, groups = 1, 1024, 32
+    x, w, _, _ = inputs(n, c, (8, 8), groups, "none")
+    first = mm.group_norm(on_device(mm, x, last), groups, mm.to_device(w), None, EPS).cpu()[0, :, 0, 0]
+    dy = torch.zeros(n, c, 8, 8)
+    dy[0, :, 0, 0] = 1.0
+    y, _, _, db = run(mm, x, groups, w, -first, dy, "relu", last)
+    let = y[0, :, 0, 0] > 0
+    assert 100 < let.sum() < 924
+    assert torch.equal(db > 0, let)
 
 
 # One segment per image, and a thread takes 2000 and 1000 of its values; the images are all the
