@@ -16,10 +16,30 @@ from . import _lib, ops
 from .tensor import MatrixManTensor, numel
 
 
+aten = torch.ops.aten
+
+
+def _dispatched(x, act: int) -> tuple | None:
+    """The sizes that ATen's operators take, where a dispatch mode is on (counters, tracing,
+    selective checkpoints): it has to see the norm, so the call goes through the dispatcher
+    instead of straight to the native one.  ATen has no form with an activation."""
+    if act or not torch._C._len_torch_dispatch_stack():
+        return None
+    shape = tuple(x.shape)
+    return (*shape[:2], numel(shape[2:])) if len(shape) >= 2 else None
+
+
+def _forward(x, groups, weight, bias, eps, act, keep=True):
+    sizes = _dispatched(x, act)
+    if sizes is not None:
+        return aten.native_group_norm.default(x, weight, bias, *sizes, groups, eps)
+    return ops.group_norm(x, groups, weight, bias, eps, act, keep)
+
+
 class _GroupNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, groups, eps, act):
-        y, mean, rstd = ops.group_norm(x, groups, weight, bias, eps, act)
+        y, mean, rstd = _forward(x, groups, weight, bias, eps, act)
         ctx.groups, ctx.act = groups, act
         ctx.save_for_backward(x, weight, bias, mean, rstd)
         return y
@@ -29,7 +49,12 @@ class _GroupNorm(torch.autograd.Function):
     def backward(ctx, dy):
         x, weight, bias, mean, rstd = ctx.saved_tensors
         mask = ctx.needs_input_grad[:3]
-        return (*ops.group_norm_backward(dy, x, mean, rstd, weight, bias, ctx.groups, mask, ctx.act), None, None, None)
+        sizes = _dispatched(x, ctx.act)
+        if sizes is not None:
+            got = aten.native_group_norm_backward.default(dy, x, mean, rstd, weight, *sizes, ctx.groups, mask)
+        else:
+            got = ops.group_norm_backward(dy, x, mean, rstd, weight, bias, ctx.groups, mask, ctx.act)
+        return (*got, None, None, None)
 
 
 def _torch_group_norm(x, num_groups, weight=None, bias=None, eps=1e-5, cudnn_enabled=True):
@@ -44,7 +69,7 @@ def _torch_group_norm(x, num_groups, weight=None, bias=None, eps=1e-5, cudnn_ena
             return torch.native_group_norm(x, weight, bias, *shape[:2], numel(shape[2:]), num_groups, eps)[0]
         if need:
             return _GroupNorm.apply(x, weight, bias, num_groups, eps, 0)
-    return ops.group_norm(x, num_groups, weight, bias, eps, keep=False)[0]
+    return _forward(x, num_groups, weight, bias, eps, 0, keep=False)[0]
 
 
 _library = torch.library.Library("aten", "IMPL", "AutogradPrivateUse1")
@@ -77,4 +102,4 @@ def group_norm(x, num_groups: int, weight=None, bias=None, eps: float = 1e-5, *,
                                        "tensor")
         if need:
             return _GroupNorm.apply(x, weight, bias, int(num_groups), float(eps), act)
-    return ops.group_norm(x, num_groups, weight, bias, float(eps), act, keep=False)[0]
+    return _forward(x, int(num_groups), weight, bias, float(eps), act, keep=False)[0]
