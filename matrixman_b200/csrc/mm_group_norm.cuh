@@ -97,20 +97,23 @@ __device__ __forceinline__ float gn_inverse(float x) {
   return y;
 }
 
-// Sigmoids of N values, as 1 / (1 + 2^(-z log2 e)): the exponent's rounding moves
-// them by |z| 2^-24 relative, the two approximations by 2^-22 each.  With expf and a
+// Sigmoids of N values, as 2^-2 / (2^-2 + 2^(-z log2 e - 2)): the exponent's rounding moves
+// them by (|z| + 2) 2^-24 relative, the two approximations by 2^-22 each.  With expf and a
 // division in their place SiLU took half of the forward pass's instructions (64 x 80 x
-// 80 x 64: 62 us).  Infinity and NaN go through: the exponential overflows to
+// 80 x 64: 62 us).  The 2^-2 keeps the inverse a normal number wherever 2^(-z log2 e) is below
+// infinity, as the approximation returns 0 for others: without it sigmoids below 2^-126, and so
+// SiLU from z = -87.3 on, were 0.  Infinity and NaN go through: the exponential overflows to
 // infinity, whose inverse is 0.
 template <int N>
 __device__ __forceinline__ void gn_sigmoid(float* s, const float* z) {
-  const float scale[2] = {-1.44269504f, -1.44269504f}, one[2] = {1.f, 1.f};
-  gn_mul<N, 2>(s, z, scale);
+  const float scale[2] = {-1.44269504f, -1.44269504f}, less[2] = {-2.f, -2.f}, quarter[2] = {0.25f, 0.25f};
+  gn_fma<N, 2, 2>(s, z, scale, less);
 #pragma unroll
   for (int i = 0; i < N; ++i) s[i] = gn_exp2(s[i]);
-  gn_add<N, 2>(s, s, one);
+  gn_add<N, 2>(s, s, quarter);
 #pragma unroll
   for (int i = 0; i < N; ++i) s[i] = gn_inverse(s[i]);
+  gn_mul<N, 2>(s, s, quarter);
 }
 
 // v = act(v).

@@ -60,6 +60,30 @@ def test_relu_passes_the_gradients_of_what_it_let_through(mm, at_most, last, wal
     assert torch.equal(db > 0, let)
 
 
+@pytest.mark.parametrize("act", ["silu", "sigmoid", "gelu_tanh"])
+@pytest.mark.parametrize("walking", [True, False])
+def test_activations_far_below_zero(mm, at_most, act, walking):  # noqa: F811
+    """Relative accuracy down to the smallest sigmoid of a finite exponential, 2^-128.  The
+    weight is 0, so z is the bias.  The exponent is one product and one rounding (its error is
+    (|t| + 2) u, relative to the exponential), the exponential and the inverse are off by 2^-22 each,
+    five roundings follow, and results below 2^-126 are multiples of 2^-149."""
+    if walking:
+        at_most(0)
+    c = 4096
+    b = torch.linspace(-88.7, 20.0, c) if act != "gelu_tanh" else torch.linspace(-10.4, 5.0, c)
+    t = (2 * (2 / torch.pi) ** 0.5 * (b.double() + 0.044715 * b.double() ** 3)) if act == "gelu_tanh" else b.double()
+    b, t = b[t > -88.72], t[t > -88.72]
+    b, t = b[:b.numel() // 64 * 64], t[:t.numel() // 64 * 64]
+    s = 1 / (1 + torch.exp(-t))
+    want = s if act == "sigmoid" else b.double() * s
+    x = randn(1, b.numel(), 3, seed=1)
+    y = mm.group_norm(mm.to_device(x), 2, mm.to_device(torch.zeros(b.numel())), mm.to_device(b), EPS, activation=act)
+    got = y.cpu()[0, :, 0].double()
+    inner = 3 if act == "gelu_tanh" else 0  # roundings of t itself
+    bound = want.abs() * ((1.5 + inner) * (t.abs() + 2) * U + 2 * 2.0 ** -22 + 8 * U) + 2.0 ** -148 * (1 + b.double().abs())
+    assert ((got - want).abs() <= bound).all(), ((got - want).abs() - bound).max()
+
+
 # One segment per image, and a thread takes 2000 and 1000 of its values; the images are all the
 # same, so that they take little memory.  A thread's sum goes through at most 128 additions,
 # the block's through 13 more, and what is added behind that takes 64 bits every eight: 150 u,
