@@ -328,23 +328,23 @@ __global__ void __launch_bounds__(GN_THREADS, gn_held<LAST>()) gn_apply_kernel(G
   for (; px < k.end; px += k.step) apply(std::integral_constant<int, 1>{}, px);
 }
 
-// Rows that a thread adds in float32; it adds the sums of more rows in float64, in its own
-// place in shared memory.  (Of values of one sign every addition rounds the same way, and
-// a thread may have thousands of rows; one of 16 x 128 x 160 x 160 has 120.)
-constexpr int GN_FOLD = 128;
+// Batches of rows that a thread adds in float32; it adds the sums of more of them in float64,
+// in its own place in shared memory.  (Of values of one sign every addition rounds the same
+// way, and a thread may have thousands of rows; one of 16 x 128 x 160 x 160 has 120.)
+constexpr int GN_FOLD = 32;
 
 // PASS 0: each channel's sums of dz and dz xh; 1: dx.
 template <int VEC, bool LAST, int PASS>
 __global__ void __launch_bounds__(GN_THREADS, 3) gn_backward_kernel(GnArgs a) {
   const GnWalk<VEC, LAST> k(a, PASS == 1);
-  float u[VEC], v[VEC], less[VEC], rstd[VEC], wr[VEC], b[VEC];  // less: -mean; wr: w rstd
+  float u[VEC], v[VEC], less[VEC], rstd[VEC], w[VEC], b[VEC];  // less: -mean
 #pragma unroll
   for (int e = 0; e < VEC; ++e) u[e] = v[e] = 0.f;
   if (PASS == 1) pdl_wait();
   if (k.c >= 0) {
     gn_of_groups<VEC, LAST>(a, k, a.mean, less);
     gn_of_groups<VEC, LAST>(a, k, a.rstd, rstd);
-    gn_of_channels<VEC, LAST>(a.w, k.c, 1.f, wr);
+    gn_of_channels<VEC, LAST>(a.w, k.c, 1.f, w);
     gn_of_channels<VEC, LAST>(a.b, k.c, 0.f, b);
     if (PASS == 1) {
       gn_of_groups<VEC, LAST>(a, k, a.sums, u);
@@ -353,7 +353,6 @@ __global__ void __launch_bounds__(GN_THREADS, 3) gn_backward_kernel(GnArgs a) {
 #pragma unroll
     for (int e = 0; e < VEC; ++e) {
       less[e] = -less[e];
-      wr[e] *= rstd[e];
       if (PASS == 1) {
         u[e] *= -rstd[e];
         v[e] *= -rstd[e];
@@ -374,43 +373,43 @@ __global__ void __launch_bounds__(GN_THREADS, 3) gn_backward_kernel(GnArgs a) {
       for (int r = 0; r < N; r += VEC) {  // (a vector at a time, for the registers)
         float(&h)[VEC] = *reinterpret_cast<float(*)[VEC]>(xh + r);
         float(&z)[VEC] = *reinterpret_cast<float(*)[VEC]>(dz + r);
-        gn_slopes<VEC>(h, z, less, rstd, wr, b, a.act);
+        gn_slopes<VEC>(h, z, less, rstd, w, b, a.act);
         if (PASS == 0) {
           gn_add<VEC, VEC>(u, u, z);
           gn_fma<VEC, VEC, VEC>(v, z, h, v);
         } else {  // dx = rstd w dz - (rstd s2 xh + rstd s1)
           gn_fma<VEC, VEC, VEC>(h, h, v, u);
-          gn_fma<VEC, VEC, VEC>(z, z, wr, h);
+          gn_mul<VEC, VEC>(z, z, w);
+          gn_fma<VEC, VEC, VEC>(z, z, rstd, h);
           gn_store<VEC>(dx + k.pixel(px + r / VEC * k.step, a.channels), z);
         }
       }
     };
     constexpr int ROWS = LAST ? GN_BACK_LAST : GN_BACK_FIRST;
-    auto walk = [&](int px, int end) {
-      for (; px + (ROWS - 1) * (int64_t)k.step < end; px += ROWS * k.step)
-        step(std::integral_constant<int, ROWS>{}, px);
-      for (; px < end; px += k.step) step(std::integral_constant<int, 1>{}, px);
-    };
-    if (PASS == 1) {
-      walk(k.at, k.end);
-    } else {
-      __shared__ double sums[2][VEC][GN_THREADS];  // (a thread's own)
-      const int fold = GN_FOLD / ROWS * ROWS * k.step;
-      for (int px = k.at; px < k.end; px += fold) {
-        const bool first = px == k.at, more = px + fold < k.end;
-        walk(px, more ? px + fold : k.end);
-        if (first && !more) break;
+    __shared__ double sums[2][VEC][PASS == 0 ? GN_THREADS : 1];  // (a thread's own)
+    int batches = 0;
+    auto fold = [&] {
+      const bool first = batches == GN_FOLD;
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-          const double su = (first ? 0 : sums[0][e][threadIdx.x]) + (double)u[e];
-          const double sv = (first ? 0 : sums[1][e][threadIdx.x]) + (double)v[e];
-          sums[0][e][threadIdx.x] = su;
-          sums[1][e][threadIdx.x] = sv;
-          u[e] = more ? 0.f : (float)su;
-          v[e] = more ? 0.f : (float)sv;
-        }
+      for (int e = 0; e < VEC; ++e) {
+        double &su = sums[0][e][threadIdx.x], &sv = sums[1][e][threadIdx.x];
+        su = (first ? 0 : su) + (double)u[e];
+        sv = (first ? 0 : sv) + (double)v[e];
+        u[e] = v[e] = 0.f;
       }
+    };
+    int px = k.at;
+    for (; px + (ROWS - 1) * (int64_t)k.step < k.end; px += ROWS * k.step) {
+      step(std::integral_constant<int, ROWS>{}, px);
+      if (PASS == 0 && ++batches % GN_FOLD == 0) fold();
     }
+    for (; px < k.end; px += k.step) step(std::integral_constant<int, 1>{}, px);
+    if (PASS == 0 && batches >= GN_FOLD)
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        u[e] = (float)(sums[0][e][threadIdx.x] + (double)u[e]);
+        v[e] = (float)(sums[1][e][threadIdx.x] + (double)v[e]);
+      }
   }
   if (PASS == 0)
     gn_leave<VEC, LAST>(a, k, 0.f, u, v, [](float&, float& au, float& av, float, float bu, float bv) {

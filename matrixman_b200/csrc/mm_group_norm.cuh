@@ -169,20 +169,26 @@ __device__ __forceinline__ void gn_times_slope(float (&dz)[N], const float (&z)[
   }
 }
 
-// xh and dz of N / VEC vectors of x (in `xh` on entry) and dy (in `dz`); less is -mean, wr is
-// w rstd.  z takes the forward pass's own operations, (x - mean) wr + b, so that ReLU's slope
-// selects what its values were selected by: with xh w + b a value within a rounding of 0 could
-// pass its gradient though it was off, or the other way round.
+// xh and dz of N / VEC vectors of x (in `xh` on entry) and dy (in `dz`); less is -mean.  ReLU
+// takes the forward pass's own z, (x - mean) (w rstd) + b, so that its slope selects what its
+// values were selected by: with xh w + b a value within a rounding of 0 could pass its gradient
+// though it was off, or the other way round.
 template <int VEC, int N>
 __device__ __forceinline__ void gn_slopes(float (&xh)[N], float (&dz)[N], const float* less, const float* rstd,
-                                          const float* wr, const float* b, int act) {
+                                          const float* w, const float* b, int act) {
   gn_add<N, VEC>(xh, xh, less);
-  if (act != MM_LINEAR_NONE) {
-    float z[N];
-    gn_fma<N, VEC, VEC>(z, xh, wr, b);
-    gn_times_slope<N>(dz, z, act);
+  if (act == MM_LINEAR_RELU) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float z = fmaf(xh[i], w[i % VEC] * rstd[i % VEC], b[i % VEC]);
+      dz[i] = lin_grad_t<MM_LINEAR_RELU>(dz[i], z);
+    }
   }
   gn_mul<N, VEC>(xh, xh, rstd);
+  if (act == MM_LINEAR_NONE || act == MM_LINEAR_RELU) return;
+  float z[N];
+  gn_fma<N, VEC, VEC>(z, xh, w, b);
+  gn_times_slope<N>(dz, z, act);
 }
 
 // How the resident kernels divide a call: a unit is one image's `slab` groups (all

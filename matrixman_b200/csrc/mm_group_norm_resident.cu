@@ -443,7 +443,7 @@ __global__ void __launch_bounds__(GN_MOST_THREADS) gn_resident_backward_kernel(c
       gn_copy<VEC>(ds + i * t.step, dy);
     }
   }
-  float less[VEC], rstd[VEC], w[VEC], wr[VEC], da[2 * CH];  // less: -mean; wr: w rstd
+  float less[VEC], rstd[VEC], w[VEC], da[2 * CH];  // less: -mean
   int group[PARTS];
 #pragma unroll
   for (int h = 0; h < PARTS; ++h) group[h] = t.group(k, h);
@@ -457,7 +457,6 @@ __global__ void __launch_bounds__(GN_MOST_THREADS) gn_resident_backward_kernel(c
       rstd[e] = t.n ? a.rstd[g] : 0.f;
       w[e] = a.w && t.n ? a.w[c] : 1.f;
       b[e] = a.b && t.n ? a.b[c] : 0.f;
-      wr[e] = w[e] * rstd[e];
     }
 #pragma unroll
     for (int e = 0; e < 2 * CH; ++e) da[e] = 0.f;
@@ -474,7 +473,7 @@ __global__ void __launch_bounds__(GN_MOST_THREADS) gn_resident_backward_kernel(c
       for (int r = 0; r < N; ++r) {  // (a vector at a time, for the registers)
         float(&h)[VEC] = *reinterpret_cast<float(*)[VEC]>(xh + r * VEC);
         float(&z)[VEC] = *reinterpret_cast<float(*)[VEC]>(dz + r * VEC);
-        gn_slopes<VEC>(h, z, less, rstd, wr, b, a.act);
+        gn_slopes<VEC>(h, z, less, rstd, w, b, a.act);
 #pragma unroll
         for (int e = 0; e < VEC; e += CH) {
           gn_add<CH, CH>(da, da, z + e);
@@ -564,6 +563,7 @@ __global__ void __launch_bounds__(GN_MOST_THREADS) gn_resident_backward_kernel(c
 #pragma unroll
     for (int e = 0; e < VEC; ++e) {
       const float2 v = direct ? make_float2(s[e / PER] * inv, s[PARTS + e / PER] * inv) : stat[group[e / PER]];
+      w[e] *= rstd[e];
       s1[e] = -rstd[e] * v.x;
       s2[e] = -rstd[e] * v.y;
     }
@@ -575,7 +575,7 @@ __global__ void __launch_bounds__(GN_MOST_THREADS) gn_resident_backward_kernel(c
       gn_load<VEC>(xs + i * t.step, xh);
       gn_load<VEC>(ds + i * t.step, dz);
       gn_fma<VEC, VEC, VEC>(xh, xh, s2, s1);
-      gn_fma<VEC, VEC, VEC>(dz, dz, wr, xh);
+      gn_fma<VEC, VEC, VEC>(dz, dz, w, xh);
       gn_store<VEC>(dx, dz);
     }
   }
