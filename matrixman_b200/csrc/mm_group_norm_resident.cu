@@ -85,22 +85,35 @@ __device__ __forceinline__ void gn_give(float2* p, uint64_t* bar, uint32_t rank,
                : "memory");
 }
 
-// Waits until everything was given: GN_TRIES tries that may sleep 1 ms each (the
-// cluster's blocks run at the same time), then leaves a code in the fault word and goes on.
-// The acquire has the cluster's scope, as the stores come from its other blocks.
-constexpr int GN_FAULT = 111, GN_TRIES = 2000;
-__device__ __forceinline__ void gn_given(uint64_t* bar, const GnArgs& a) {
+// One try, which may sleep 1 ms.  The acquire has the cluster's scope, as the stores come from
+// its other blocks.
+__device__ __forceinline__ bool gn_try(uint64_t* bar) {
   const uint32_t at = (uint32_t)__cvta_generic_to_shared(bar);
-  for (int i = 0; i < a.tries; ++i) {
-    uint32_t done;
-    asm volatile(
-        "{ .reg .pred p; mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], 0, 1000000; selp.u32 %0, 1, 0, p; }"
-        : "=r"(done)
-        : "r"(at)
-        : "memory");
-    if (done) return;
-  }
+  uint32_t done;
+  asm volatile(
+      "{ .reg .pred p; mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], 0, 1000000; selp.u32 %0, 1, 0, p; }"
+      : "=r"(done)
+      : "r"(at)
+      : "memory");
+  return done;
+}
+
+// Waits until everything was given: GN_TRIES tries (the cluster's blocks run at the same
+// time), then leaves a code in the fault word and goes on.
+constexpr int GN_FAULT = 111, GN_TRIES = 2000;
+__device__ __forceinline__ bool gn_given(uint64_t* bar, const GnArgs& a) {
+  for (int i = 0; i < a.tries; ++i)
+    if (gn_try(bar)) return true;
   if (*(volatile int*)a.fault == 0) *(volatile int*)a.fault = GN_FAULT;
+  return false;
+}
+
+// The end of a cluster's block: none leaves while one may give to it.  Where it gave up its
+// wait, what the others have given since then is still on its way: one more try (a store of
+// theirs takes a microsecond).
+__device__ __forceinline__ void gn_leave_cluster(uint64_t* bar, bool given) {
+  gn_wait();
+  if (!given) gn_try(bar);
 }
 
 // i / d for 0 <= i < 2^20, by the float32 inverse of d: i + 0.5 is at least 0.5 / d
@@ -224,6 +237,7 @@ __global__ void __launch_bounds__(GN_MOST_THREADS) gn_resident_kernel(const __gr
   extern __shared__ float4 gn_smem[];
   __shared__ float2 stat[GN_GROUPS];
   __shared__ uint64_t bar;
+  bool given = true;
   GnPlace<VEC, PARTS, LAST> t(a, k);
   if (k.ranks > 1) {
     if (threadIdx.x == 0) gn_expect(&bar, gn_block() < k.blocks ? k.ranks * t.kk * 8 : 0);
@@ -367,7 +381,7 @@ __global__ void __launch_bounds__(GN_MOST_THREADS) gn_resident_kernel(const __gr
     if (k.ranks > 1) {
       const int ranks = gn_span(k.ranks);
       const float held = lane < k.ranks ? t.count(a, max(0, min(k.rows, k.all - lane * k.rows))) : 0.f;
-      gn_given(&bar, a);
+      given = gn_given(&bar, a);
       gn_groups(a, k, t, [&](int i, int u, int g) {
         const float first = peer[i * GN_RANKS].x;
         const float2 one = held > 0.f ? peer[i * GN_RANKS + lane] : make_float2(first, 0.f);
@@ -411,7 +425,7 @@ __global__ void __launch_bounds__(GN_MOST_THREADS) gn_resident_kernel(const __gr
     for (; i + 1 < t.n; i += 2) apply(std::integral_constant<int, 2>{});
     if (i < t.n) apply(std::integral_constant<int, 1>{});
   }
-  if (k.ranks > 1) gn_wait();  // (no block leaves while one may give to it)
+  if (k.ranks > 1) gn_leave_cluster(&bar, given);
 }
 
 template <int VEC, int PARTS, bool LAST>
@@ -421,6 +435,7 @@ __global__ void __launch_bounds__(GN_MOST_THREADS) gn_resident_backward_kernel(c
   __shared__ float2 stat[GN_GROUPS];
   __shared__ uint64_t bar;
   constexpr int PER = VEC / PARTS, CH = LAST ? VEC : 1;  // CH: channels of a thread
+  bool given = true;
   GnPlace<VEC, PARTS, LAST> t(a, k);
   if (k.ranks > 1) {
     if (threadIdx.x == 0) gn_expect(&bar, gn_block() < k.blocks ? k.ranks * t.kk * 8 : 0);
@@ -547,7 +562,7 @@ __global__ void __launch_bounds__(GN_MOST_THREADS) gn_resident_backward_kernel(c
   }
   if (k.ranks > 1) {
     const int ranks = gn_span(k.ranks);
-    gn_given(&bar, a);
+    given = gn_given(&bar, a);
     gn_groups(a, k, t, [&](int i, int, int) {
       const float2 one = lane < k.ranks ? peer[i * GN_RANKS + lane] : make_float2(0.f, 0.f);
       float v[2] = {one.x, one.y};
@@ -579,7 +594,7 @@ __global__ void __launch_bounds__(GN_MOST_THREADS) gn_resident_backward_kernel(c
       gn_store<VEC>(dx, dz);
     }
   }
-  if (k.ranks > 1) gn_wait();  // (no block leaves while one may give to it)
+  if (k.ranks > 1) gn_leave_cluster(&bar, given);
 }
 
 // ---------------------------------------------------------------------------

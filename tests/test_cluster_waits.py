@@ -21,3 +21,14 @@ def test_group_norm_waits_at_the_clusters_scope():
     assert "st.async" in text  # blocks give each other their results
     waits = re.findall(r"mbarrier\.(?:try|test)_wait[\w.:]*", text)
     assert waits and all(".acquire.cluster." in w for w in waits), waits
+
+
+def test_a_block_that_gave_up_waits_for_late_stores_before_it_leaves():
+    text = code("mm_group_norm_resident.cu")
+    kernels = re.findall(r"\n__global__ void.*?\n}\n", text, re.S)
+    assert len(kernels) == 2
+    for kernel in kernels:
+        assert "given = gn_given(" in kernel
+        assert kernel.rstrip().endswith("if (k.ranks > 1) gn_leave_cluster(&bar, given);\n}")
+    leave = re.search(r"void gn_leave_cluster\(.*?\n}\n", text, re.S)[0]
+    assert re.search(r"gn_wait\(\);\s*if \(!given\) gn_try\(bar\);", leave)
