@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import array
 import copy
+import math
 
 import torch
 
@@ -85,6 +86,61 @@ def _is_apart(t: MatrixManTensor) -> bool:
     return True
 
 
+def _share_memory(a: MatrixManTensor, b: MatrixManTensor) -> bool:
+    """Whether an element of a is one of b's: whether the distance of their first elements
+    is a sum of multiples of the strides that their sizes allow."""
+    away = (_pointer(b) - _pointer(a)) // 4
+    ranges: dict[int, list] = {}
+    for t, side in ((a, 1), (b, 0)):
+        for n, stride in zip(t.shape, t._logical_strides):
+            if n == 0:
+                return False
+            ranges.setdefault(stride, [0, 0])[side] += (n - 1) * (1 if side else -1)
+    terms = sorted(((stride, *r) for stride, r in ranges.items() if stride and r != [0, 0]), reverse=True)
+    rest = [(0, 0, 0)]  # what the terms behind reach, and what divides it
+    for stride, lo, hi in reversed(terms):
+        low, high, common = rest[-1]
+        rest.append((low + stride * lo, high + stride * hi, math.gcd(common, stride)))
+    rest.reverse()
+
+    def reached(i: int, d: int) -> bool:
+        low, high, common = rest[i]
+        if not low <= d <= high or (d % common if common else d):
+            return False
+        if i == len(terms):
+            return True
+        stride, lo, hi = terms[i]
+        low, high, _ = rest[i + 1]
+        return any(reached(i + 1, d - stride * c)
+                   for c in range(max(lo, -((high - d) // stride)), min(hi, (d - low) // stride) + 1))
+
+    return reached(0, away)
+
+
+def _check_apart(grads: list) -> None:
+    """Refuses gradients that overlap, themselves or each other, where one of them does not
+    fill its storage span (of those that do, the native call looks at the spans)."""
+    spans = []
+    for g in grads:
+        if not _is_apart(g):
+            raise NotImplementedError("MatrixMan/CUDA: clip_grad_norm_ needs gradients whose elements share no memory, "
+                                      f"got strides {g._logical_strides}")
+        if numel(g.shape):
+            reach = 1 + sum((n - 1) * s for n, s in zip(g.shape, g._logical_strides))
+            spans.append((_pointer(g), _pointer(g) + 4 * reach, is_dense(g.shape, g._logical_strides), g))
+    if all(dense for _, _, dense, _ in spans):
+        return
+    spans.sort(key=lambda s: s[0])
+    before: list = []
+    for span in spans:
+        before = [s for s in before if s[1] > span[0]]
+        for other in before:
+            if not (span[2] and other[2]) and _share_memory(other[3], span[3]):
+                raise ValueError("MatrixMan/CUDA: clip_grad_norm_ got a gradient that is given twice or shares memory "
+                                 "with another")
+        before.append(span)
+
+
 def _grad_table(grads: list) -> tuple[array.array, list]:
     """mm_grad_t rows, and the tensors that they point into: the gradients, or dense
     copies of those that do not fill their storage span."""
@@ -151,10 +207,7 @@ def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0,
         return done[0]
     grads = _grads_of(parameters)
     rt = _grad_runtime(grads)
-    for g in grads:
-        if not _is_apart(g):
-            raise NotImplementedError("MatrixMan/CUDA: clip_grad_norm_ needs gradients whose elements share no memory, "
-                                      f"got strides {g._logical_strides}")
+    _check_apart(grads)
     table, held = _grad_table(grads)
     norm = ops.new_dense(rt, ())
     ops._launch("mm_grad_clip", table.buffer_info()[0], len(held), order, max_norm, _pointer(norm), None, 0, rt.stream)
