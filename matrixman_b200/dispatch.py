@@ -611,10 +611,12 @@ def _native_group_norm_backward(grad_out, x, mean, rstd, weight, N, C, HxW, grou
 def _linalg_vector_norm(x, ord=2, dim=None, keepdim=False, dtype=None):
     from . import optim
     rank = x.dim()
-    if dim is not None and {_norm_dim(d, rank) for d in dim} != set(range(rank)):
+    if dim and {_norm_dim(d, rank) for d in dim} != set(range(rank)):  # (no dimensions are all of them)
         raise NotImplementedError("MatrixMan/CUDA: linalg_vector_norm over some dimensions is not implemented")
     if dtype is not None and dtype != torch.float32:
         raise NotImplementedError("MatrixMan/CUDA: linalg_vector_norm supports float32 only")
+    if ord == float("inf") and x.numel() == 0:
+        raise RuntimeError("MatrixMan/CUDA: linalg_vector_norm of order inf has no value for an empty tensor")
     norm = optim.tensor_norm(x, ord)
     return _view(norm, (1,) * rank, (1,) * rank) if keepdim else norm
 
