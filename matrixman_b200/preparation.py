@@ -669,6 +669,11 @@ class PreparedGroupNorm(nn.Module):
                               keep=False)[0]
 
 
+def _hooked(module) -> bool:
+    """Whether a call of `module` does more than its forward."""
+    return module is not None and bool(module._forward_hooks or module._forward_pre_hooks)
+
+
 def _norm_activation(module) -> str | None:
     """The activation that a group norm in front of `module` takes over."""
     if type(module) is nn.GELU:
@@ -782,9 +787,11 @@ def _replace(parent: nn.Module, report: PreparationReport, aliases: Counter) -> 
                 if code is not None:
                     parent._modules[keys[i + 1]] = nn.Identity()
                     i += 1
-            elif type(m) is nn.GroupNorm and aliases[id(m)] <= 1 and all(
+            elif type(m) is nn.GroupNorm and aliases[id(m)] <= 1 and not _hooked(m) and all(
                     v is None or v.device.type == "cpu" for v in (m.weight, m.bias)):
-                act = _norm_activation(nxt)
+                # (a container with a forward of its own may use what lies between the two)
+                behind = getattr(parent.forward, "__func__", None) is nn.Sequential.forward and not _hooked(nxt)
+                act = _norm_activation(nxt) if behind else None
                 parent._modules[keys[i]] = PreparedGroupNorm(m, act or "none")
                 report.block_units_prepared["GroupNorm"] += 1
                 if act is not None:
