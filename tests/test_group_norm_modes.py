@@ -72,6 +72,20 @@ def test_a_mode_sees_the_gradient(mm):
         check(name, got.cpu(), want[name])
 
 
+@pytest.mark.gpu
+def test_parameters_on_the_cpu_under_a_mode(mm):
+    from .test_group_norm_gpu import EPS, check, inputs, on_device, oracle
+    x, w, b, dy = inputs(2, 8, (3, 5), 4, "none")
+    want = oracle(x, 4, w, b, dy)
+    leaf = on_device(mm, x, True).detach().requires_grad_(True)
+    with Seen() as seen:
+        y = F.group_norm(leaf, 4, w, b, EPS)
+        dx, = torch.autograd.grad(y, leaf, on_device(mm, dy, True))
+    assert aten.native_group_norm_backward.default in seen.calls
+    check("y", y.detach().cpu(), want["y"])
+    check("dx", dx.cpu(), want["dx"])
+
+
 def test_without_a_mode_nothing_is_dispatched(maps, launches, monkeypatch):  # noqa: F811
     from matrixman_b200 import dispatch
     monkeypatch.delitem(dispatch._HANDLERS, aten.native_group_norm.default)

@@ -2,6 +2,10 @@
 one block, in clusters of any size, several images in a block, walking kernels.  The
 bounds are those of test_group_norm_gpu.py."""
 
+import subprocess
+import sys
+from pathlib import Path
+
 import pytest
 import torch
 
@@ -146,3 +150,27 @@ def test_small_spread_far_from_zero(mm, at_most, n, c, spatial, groups, offset, 
     bound = e + adds * base.U * xh.abs().mean(2, keepdim=True) + (2 * e + 2 * e * e + (adds / 2 + 8) * base.U) * xh.abs()
     assert bound.max() < (0.1 if offset == 100.0 else 1.0)
     check("y", y.reshape(t.shape), (xh, bound))
+
+
+FIRST_CALL = """
+import torch, matrixman_b200 as mm
+mm.init()
+x = mm.to_device(torch.randn(2, 48, 64, 64))
+rt = x.runtime
+rt.synchronize()
+rt.capture_begin()
+y = mm.group_norm(x, 8, activation="silu")
+graph = rt.capture_end()
+graph.replay()
+got = y.cpu()
+assert torch.equal(got, mm.group_norm(x, 8, activation="silu").cpu()) and torch.isfinite(got).all()
+print("ok")
+"""
+
+
+def test_a_process_whose_first_call_is_captured():
+    """Whether a cluster can be placed is asked during the capture."""
+    assert plan(2, 48, 4096, 8, False, False)[0] > 1
+    done = subprocess.run([sys.executable, "-c", FIRST_CALL], capture_output=True, text=True, timeout=300,
+                          cwd=Path(__file__).resolve().parents[1])
+    assert done.returncode == 0 and done.stdout.strip().endswith("ok"), done.stderr
