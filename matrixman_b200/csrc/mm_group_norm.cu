@@ -14,7 +14,7 @@
 // walks a segment of an image's pixels and leaves each channel's moments (or sums) in
 // the workspace, a second kernel joins them by group, a third reads the map again and
 // writes y (or dx): 12 (20) bytes per element.  2 x 128 x 512 x 512 with SiLU takes 145 us
-// (5.6 TB/s) forward and 218 us (6.2 TB/s) backward.
+// (5.6 TB/s) forward and 219 us (6.1 TB/s) backward.
 //
 // Moments are held as a mean and a sum of squared distances from it and joined
 // by d^2 n1 n2 / (n1 + n2) (Chan, Golub, LeVeque 1979), so large offsets do not

@@ -16,7 +16,7 @@
 // of its two places).
 //
 // 64 x 64 x 80 x 80 with SiLU takes 48 us channels last (4.4 TB/s; a bare copy in the same
-// pieces of 64 bytes 36), 32 x 256 x 40 x 40 27 us and backward 52 us (3.0 TB/s).
+// pieces of 64 bytes 36), 32 x 256 x 40 x 40 27 us and backward 49 us (3.2 TB/s).
 //
 // Channels last, the slab of groups is wide enough that a row's piece fills whole
 // sectors.
