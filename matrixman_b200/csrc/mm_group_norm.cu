@@ -263,7 +263,8 @@ __device__ __forceinline__ double2 gn_share(unsigned count, F term) {
 
 // mean and rstd of one image and group per block of T threads, from the channels'
 // segments.  Their means are weighted and added as distances from the first one's: a constant
-// is its own mean, and the sum of all values overflows nowhere.
+// is its own mean, and the sum of all values overflows nowhere.  (The mean itself is rounded
+// once, at its own scale: the first part may be far from the others.)
 template <int T>
 __global__ void __launch_bounds__(T) gn_join_moments_kernel(GnArgs a) {
   __shared__ double2 sm[T / 32];
@@ -282,14 +283,14 @@ __global__ void __launch_bounds__(T) gn_join_moments_kernel(GnArgs a) {
   };
   double2 s = walk([&](int64_t at, float n) { return n * (pu[at] - first); });
   gn_sum2<T>(s.x, s.y, sm);
-  const float away = (float)(s.x / m);
+  const float mean = (float)((double)first + s.x / m);
   s = walk([&](int64_t at, float n) {
-    const float d = pu[at] - first - away;
+    const float d = pu[at] - mean;
     return pv[at] + n * d * d;
   });
   gn_sum2<T>(s.x, s.y, sm);
   if (threadIdx.x == 0) {
-    a.mean[blockIdx.x] = first + away;
+    a.mean[blockIdx.x] = mean;
     a.rstd[blockIdx.x] = 1.f / sqrtf((float)(s.x / m) + a.eps);
   }
 }

@@ -126,3 +126,24 @@ def test_means_of_one_sign_over_many_channels(mm):
         xh = ((one.double() - m64) * r64).abs()
         bound = r64 * 0.1 * (24 * U + 4 * U + xh * (64 * U * xh.mean()))
         check("dx", dx.cpu(), (torch.zeros(n, c, size, dtype=torch.float64), bound))
+
+
+@pytest.mark.parametrize("last", [True, False])
+@pytest.mark.parametrize("far", [1e6, -3e6, 1e7])
+def test_a_first_part_far_from_the_others(mm, far, last):
+    """The join adds distances from the first part's mean, here of 262,144 channels around 0 of which
+    the first is far.  In units of far u, a distance is rounded by 1 at most, its product with the
+    part's nine values by 1 of nine, and the k-th sum of eight products by k: as independent
+    roundings of up to these sizes, (1 + 1 + (4 + 9 + ... + 64) / 8) / 3 = 3.0^2 per part, and 3.0 /
+    sqrt(262144) of their mean.  8 of those, and 64 u of the mean magnitude for the mean's own rounding and
+    everything else."""
+    n, c, size = 1, 1 << 18, 9
+    assert plan(n, c, size, 1, last, False)[0] == 0
+    x = randn(n, c, size, seed=1)
+    x[:, 0] = far
+    y = mm.group_norm(on_device(mm, x, last), 1, None, None, EPS).cpu().double()
+    x = x.double()
+    rstd = 1 / torch.sqrt(((x - x.mean()) ** 2).mean() + EPS)
+    want = (x - x.mean()) * rstd
+    shift = (24 / c ** 0.5 * abs(far) + 64 * x.abs().mean()) * U * rstd
+    check("y", y, (want, shift + 200 * U * want.abs()))
